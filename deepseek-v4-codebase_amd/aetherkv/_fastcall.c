@@ -274,7 +274,123 @@ static PyObject* f_prefill_counts(PyObject* self, PyObject* const* args, Py_ssiz
                                              (int32_t*)sel, (int32_t*)ws, (int32_t*)wl, st));
 }
 
+/* aekv_kv_append(k, v, dtype, k_token, k_head, v_token, v_head, n_tokens, cu, B, start, d, bits, diag, k_codes, k_scale,
+ * v_codes, v_scale, pages, heads, page_size, table, max_pages, weights, tokens, capacity, token, stream) */
+static PyObject* f_kv_append(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 28, "aekv_kv_append")) return NULL;
+  void* k = ptr_arg(A(0));
+  void* v = ptr_arg(A(1));
+  const int32_t dt = i32_arg(A(2));
+  const int64_t kt = i64_arg(A(3)), kh = i64_arg(A(4)), vt = i64_arg(A(5)), vh = i64_arg(A(6)), n = i64_arg(A(7));
+  void* cu = ptr_arg(A(8));
+  const int64_t B = i64_arg(A(9));
+  void* start = ptr_arg(A(10));
+  const int32_t d = i32_arg(A(11)), bits = i32_arg(A(12));
+  void* p[5];
+  for (int i = 0; i < 5; ++i) p[i] = ptr_arg(A(13 + i));
+  const int64_t pages = i64_arg(A(18)), heads = i64_arg(A(19));
+  const int32_t ps = i32_arg(A(20));
+  void* table = ptr_arg(A(21));
+  const int64_t mp = i64_arg(A(22));
+  void* w = ptr_arg(A(23));
+  void* tok = ptr_arg(A(24));
+  const int64_t cap = i64_arg(A(25));
+  void* first = ptr_arg(A(26));
+  void* st = ptr_arg(A(27));
+  RETURN_STATUS_UNLOCKED(aekv_kv_append(k, v, dt, kt, kh, vt, vh, n, (const int32_t*)cu, B, (const int32_t*)start, d,
+                                        bits, (const float*)p[0], p[1], (float*)p[2], p[3], (float*)p[4], pages, heads,
+                                        ps, (const int32_t*)table, mp, (float*)w, (int32_t*)tok, cap,
+                                        (const int32_t*)first, st));
+}
+
+/* aekv_paged_attention(q, dtype, q_batch, q_token, q_head, B, T, H, d, bits, diag, k_codes, k_scale, v_codes, v_scale,
+ * pages, heads, page_size, table, max_pages, lengths, sink, weights, capacity, scale, ws, ws_bytes, out, stream) */
+static PyObject* f_paged_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 29, "aekv_paged_attention")) return NULL;
+  void* q = ptr_arg(A(0));
+  const int32_t dt = i32_arg(A(1));
+  const int64_t qb = i64_arg(A(2)), qt = i64_arg(A(3)), qh = i64_arg(A(4));
+  const int64_t B = i64_arg(A(5)), T = i64_arg(A(6)), H = i64_arg(A(7));
+  const int32_t d = i32_arg(A(8)), bits = i32_arg(A(9));
+  void* p[5];
+  for (int i = 0; i < 5; ++i) p[i] = ptr_arg(A(10 + i));
+  const int64_t pages = i64_arg(A(15)), heads = i64_arg(A(16));
+  const int32_t ps = i32_arg(A(17));
+  void* table = ptr_arg(A(18));
+  const int64_t mp = i64_arg(A(19));
+  void* len = ptr_arg(A(20));
+  void* sink = ptr_arg(A(21));
+  void* w = ptr_arg(A(22));
+  const int64_t cap = i64_arg(A(23));
+  const float sm = f32_arg(A(24));
+  void* ws = ptr_arg(A(25));
+  const size_t wsb = (size_t)i64_arg(A(26));
+  void* out = ptr_arg(A(27));
+  void* st = ptr_arg(A(28));
+  RETURN_STATUS(aekv_paged_attention(q, dt, qb, qt, qh, B, T, H, d, bits, (const float*)p[0], p[1], (const float*)p[2],
+                                     p[3], (const float*)p[4], pages, heads, ps, (const int32_t*)table, mp,
+                                     (const int32_t*)len, (const float*)sink, (float*)w, cap, sm, ws, wsb, out, st));
+}
+
+/* aekv_kv_evict(d, bits, k_codes, k_scale, v_codes, v_scale, pages, heads, page_size, table, max_pages, B, lengths,
+ * weights, tokens, capacity, seen, keep, first, recent, ws, ws_bytes, stream) */
+static PyObject* f_kv_evict(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 23, "aekv_kv_evict")) return NULL;
+  const int32_t d = i32_arg(A(0)), bits = i32_arg(A(1));
+  void* p[4];
+  for (int i = 0; i < 4; ++i) p[i] = ptr_arg(A(2 + i));
+  const int64_t pages = i64_arg(A(6)), heads = i64_arg(A(7));
+  const int32_t ps = i32_arg(A(8));
+  void* table = ptr_arg(A(9));
+  const int64_t mp = i64_arg(A(10)), B = i64_arg(A(11));
+  void* len = ptr_arg(A(12));
+  void* w = ptr_arg(A(13));
+  void* tok = ptr_arg(A(14));
+  const int64_t cap = i64_arg(A(15));
+  void* seen = ptr_arg(A(16));
+  const int64_t keep = i64_arg(A(17)), first = i64_arg(A(18)), recent = i64_arg(A(19));
+  void* ws = ptr_arg(A(20));
+  const size_t wsb = (size_t)i64_arg(A(21));
+  void* st = ptr_arg(A(22));
+  RETURN_STATUS(aekv_kv_evict(d, bits, p[0], (float*)p[1], p[2], (float*)p[3], pages, heads, ps, (const int32_t*)table,
+                              mp, B, (const int32_t*)len, (float*)w, (int32_t*)tok, cap, (const int32_t*)seen, keep,
+                              first, recent, ws, wsb, st));
+}
+
+/* aekv_prompt_attention(q, k, v, dtype, q_token, q_head, k_token, k_head, v_token, v_head, cu_q, cu_k, B, n_q, n_k, H,
+ * heads, d, sink, scale, out, lse, clear_rest, stream) */
+static PyObject* f_prompt_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 24, "aekv_prompt_attention")) return NULL;
+  void* q = ptr_arg(A(0));
+  void* k = ptr_arg(A(1));
+  void* v = ptr_arg(A(2));
+  const int32_t dt = i32_arg(A(3));
+  int64_t n[6];
+  for (int i = 0; i < 6; ++i) n[i] = i64_arg(A(4 + i));
+  void* cq = ptr_arg(A(10));
+  void* ck = ptr_arg(A(11));
+  const int64_t B = i64_arg(A(12)), nq = i64_arg(A(13)), nk = i64_arg(A(14)), H = i64_arg(A(15)), hk = i64_arg(A(16));
+  const int32_t d = i32_arg(A(17));
+  void* sink = ptr_arg(A(18));
+  const float sm = f32_arg(A(19));
+  void* out = ptr_arg(A(20));
+  void* lse = ptr_arg(A(21));
+  const int32_t clear = i32_arg(A(22));
+  void* st = ptr_arg(A(23));
+  RETURN_STATUS_UNLOCKED(aekv_prompt_attention(q, k, v, dt, n[0], n[1], n[2], n[3], n[4], n[5], (const int32_t*)cq,
+                                               (const int32_t*)ck, B, nq, nk, H, hk, d, (const float*)sink, sm, out,
+                                               (float*)lse, clear, st));
+}
+
 static PyMethodDef methods[] = {
+    {"aekv_kv_append", (PyCFunction)(void (*)(void))f_kv_append, METH_FASTCALL, NULL},
+    {"aekv_paged_attention", (PyCFunction)(void (*)(void))f_paged_attention, METH_FASTCALL, NULL},
+    {"aekv_kv_evict", (PyCFunction)(void (*)(void))f_kv_evict, METH_FASTCALL, NULL},
+    {"aekv_prompt_attention", (PyCFunction)(void (*)(void))f_prompt_attention, METH_FASTCALL, NULL},
     {"aekv_tq_encode", (PyCFunction)(void (*)(void))f_tq_encode, METH_FASTCALL, NULL},
     {"aekv_tq_decode", (PyCFunction)(void (*)(void))f_tq_decode, METH_FASTCALL, NULL},
     {"aekv_hca_compress", (PyCFunction)(void (*)(void))f_hca_compress, METH_FASTCALL, NULL},

@@ -37,6 +37,8 @@ SYMBOLS = (
     "aekv_quant_prefill_attention", "aekv_rope_rmsnorm", "aekv_csa_indexer_topk_quant_noalloc",
     "aekv_csa_decode_workspace_size", "aekv_csa_decode_quant", "aekv_sparse_sink_attention_ws",
     "aekv_tiled_prefill_attention_ws", "aekv_sink_attention_workspace_size", "aekv_prefill_counts",
+    "aekv_kv_append", "aekv_paged_attention_workspace_size", "aekv_paged_attention", "aekv_kv_evict_workspace_size",
+    "aekv_kv_evict", "aekv_prompt_attention",
 )
 
 # size of the static device scratch behind aekv_csa_indexer_topk_quant_noalloc (AEKV_STATIC_SCRATCH_BYTES)
@@ -103,6 +105,15 @@ def lib() -> ctypes.CDLL:
         "aekv_tiled_prefill_attention_ws": (
             [P, P, P, I64_, I32_, I64_, I64_, I64_, I64_, I64_, F, I32_, P, SZ, P, P], ctypes.c_int),
         "aekv_prefill_counts": ([I64_] * 8 + [P, P, P, P, P], ctypes.c_int),
+        "aekv_kv_append": ([P, P, I32_] + [I64_] * 5 + [P, I64_, P, I32_, I32_] + [P] * 5 + [I64_, I64_, I32_, P, I64_, P, P, I64_,
+                            P, P], ctypes.c_int),
+        "aekv_paged_attention_workspace_size": ([I64_] * 4 + [I32_, I64_, I32_], SZ),
+        "aekv_paged_attention": ([P, I32_] + [I64_] * 6 + [I32_, I32_] + [P] * 5 + [I64_, I64_, I32_, P, I64_, P, P, P, I64_, F,
+                                  P, SZ, P, P], ctypes.c_int),
+        "aekv_kv_evict_workspace_size": ([I64_] * 4, SZ),
+        "aekv_kv_evict": ([I32_, I32_, P, P, P, P, I64_, I64_, I32_, P, I64_, I64_, P, P, P, I64_, P, I64_, I64_, I64_, P, SZ, P],
+                          ctypes.c_int),
+        "aekv_prompt_attention": ([P, P, P, I32_] + [I64_] * 6 + [P, P] + [I64_] * 5 + [I32_, P, F, P, P, I32_, P], ctypes.c_int),
         "aekv_sink_attention_workspace_size": ([I32_, I64_, I64_, I64_, I64_, I64_, I64_], SZ),
     }
     for name, (argtypes, restype) in sig.items():
@@ -218,6 +229,16 @@ def attention_ws_bytes(B: int, H: int, D: int, n_comp: int, W: int) -> int:
 @functools.lru_cache(maxsize=1024)
 def decode_ws_bytes(B: int, S: int, k: int, H: int, D: int, W: int) -> int:
     return lib().aekv_csa_decode_workspace_size(B, S, k, H, D, W)
+
+
+@functools.lru_cache(maxsize=1024)
+def paged_ws_bytes(B: int, T: int, H: int, heads: int, d: int, slots: int, tracked: int) -> int:
+    return lib().aekv_paged_attention_workspace_size(B, T, H, heads, d, slots, tracked)
+
+
+@functools.lru_cache(maxsize=1024)
+def evict_ws_bytes(B: int, heads: int, keep: int, slots: int) -> int:
+    return lib().aekv_kv_evict_workspace_size(B, heads, keep, slots)
 
 
 def require_device(name: str, *tensors: Optional[torch.Tensor]) -> None:

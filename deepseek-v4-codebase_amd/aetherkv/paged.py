@@ -1,0 +1,285 @@
+"""A paged per-head KV cache held in TurboQuant codes: filled, attended and kept within a budget in place.
+
+PolarQuant codes K and V entries of any attention (one vector per token and KV head); here they live in pages that
+sequences share through page tables, and nothing is ever decoded to memory:
+
+  append_tokens     codes the K and V of new tokens straight into their slots (bit for bit PolarQuant.encode)
+  paged_attention   the newest tokens' attention over their sequence's slots, heads grouped over KV heads, optionally
+                    adding every slot's attention weight to a tracker
+  evict_by_weight   brings sequences back to a budget of slots by accumulated weight
+
+A PagedKVCache is one layer's pool; page table int32 [B, max_pages], lengths and the like int32 [B] are shared by the
+layers and only read here: after a step the caller adds the new tokens to `lengths`, after an eviction of every layer it
+clamps them to `keep`.  Slot p of sequence b is row p % page_size of page table[b, p // page_size].  The tables and counts
+are device data that no host check can see, so a slot outside the table or a page outside the pool is skipped, never
+accessed.  Pages may be shared between sequences as long as nothing writes to them: append_tokens and evict_by_weight
+write to the pages of the slots they fill.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .decode import _check_out, _f32, _i32, _iptr, _sink_f32
+from .turbo_quant import PolarQuant
+
+
+class PagedKVCache:
+    """One layer's pool of pages: codes [pages, kv_heads, page_size, row] and fp32 scales [pages, kv_heads, page_size],
+    for K and for V.  head dim 64 or 128, page_size a power of two from 16 to 4096."""
+
+    def __init__(self, quant: PolarQuant, pages: int, kv_heads: int, dim: int, *, page_size: int = 64,
+                 device: Optional[torch.device] = None):
+        if dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: head dim must be 64 or 128, got {dim}")
+        if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError(f"PagedKVCache: page_size must be a power of two from 16 to 4096, got {page_size}")
+        if pages < 1 or kv_heads < 1:
+            raise ValueError(f"PagedKVCache needs pages, kv_heads >= 1, got {pages}, {kv_heads}")
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        rows = (int(pages), int(kv_heads), int(page_size))
+        dtype = torch.int8 if quant.bits == 8 else torch.uint8
+        row = dim * quant.bits // 8
+        self._set(quant, *(torch.zeros(rows + (row,), dtype=dtype, device=dev) if i % 2 == 0 else
+                           torch.zeros(rows, dtype=torch.float32, device=dev) for i in range(4)))
+
+    def _set(self, quant, k_codes, k_scale, v_codes, v_scale) -> None:
+        self.quant, self.bits = quant, quant.bits
+        self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
+        self.pages, self.kv_heads, self.page_size = k_scale.shape
+        self.dim = k_codes.size(3) * (1 if quant.bits == 8 else 2)
+        self.device = k_codes.device
+
+    @classmethod
+    def from_tensors(cls, quant: PolarQuant, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
+                     v_scale: torch.Tensor) -> "PagedKVCache":
+        """A cache over existing pools (used in place: contiguous, on one device)."""
+        _lib.require_device("k_codes", k_codes, k_scale, v_codes, v_scale)
+        want = torch.int8 if quant.bits == 8 else torch.uint8
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+            raise RuntimeError(f"codes must be [pages, kv_heads, page_size, row], got {tuple(k_codes.shape)} and "
+                               f"{tuple(v_codes.shape)}")
+        if k_codes.dtype != want or v_codes.dtype != want:
+            raise RuntimeError(f"{quant.bits}-bit codes must be {want}, got {k_codes.dtype} and {v_codes.dtype}")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or t.shape != k_codes.shape[:3]:
+                raise RuntimeError(f"{name} must be float32 {tuple(k_codes.shape[:3])}, got {t.dtype} {tuple(t.shape)}")
+        for t in (k_codes, k_scale, v_codes, v_scale):
+            if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k_codes.device:
+                raise RuntimeError("codes and scales must be contiguous, 16-byte aligned and on one device")
+        self = cls.__new__(cls)
+        self._set(quant, k_codes, k_scale, v_codes, v_scale)
+        if self.dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: head dim must be 64 or 128, got {self.dim}")
+        if self.page_size < 16 or self.page_size > 4096 or self.page_size & (self.page_size - 1):
+            raise ValueError(f"PagedKVCache: page_size must be a power of two from 16 to 4096, got {self.page_size}")
+        return self
+
+    def decode(self, page_table: torch.Tensor, length: int, out_dtype: torch.dtype = torch.bfloat16):
+        """(K, V) [kv_heads, length, dim] of one sequence's first slots, decoded (page_table [max_pages])."""
+        slots = torch.arange(int(length), device=self.device)
+        page, row = page_table.long()[slots // self.page_size], slots % self.page_size
+        return tuple(self.quant.decode(c[page, :, row], s[page, :, row].unsqueeze(-1), out_dtype).transpose(0, 1)
+                     for c, s in ((self.k_codes, self.k_scale), (self.v_codes, self.v_scale)))
+
+
+class SlotTracker:
+    """Per sequence, KV head and slot of one layer: `weights` fp32, the attention weight accumulated since the slot was
+    filled, and `tokens` int32, the token index that it holds ([B, kv_heads, capacity], views of one int32 tensor)."""
+
+    def __init__(self, batch: int, kv_heads: int, capacity: int, *, device: Optional[torch.device] = None):
+        if batch < 1 or kv_heads < 1 or capacity < 1:
+            raise ValueError(f"SlotTracker needs batch, kv_heads, capacity >= 1, got {batch}, {kv_heads}, {capacity}")
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self._set(torch.zeros((2, int(batch), int(kv_heads), int(capacity)), dtype=torch.int32, device=dev))
+
+    def _set(self, storage: torch.Tensor) -> None:
+        self.storage = storage
+        self.weights, self.tokens = storage[0].view(torch.float32), storage[1]
+        self.batch, self.kv_heads, self.capacity = storage.shape[1:]
+
+    @classmethod
+    def from_tensor(cls, storage: torch.Tensor) -> "SlotTracker":
+        """A tracker over an existing int32 [2, B, kv_heads, capacity] (used in place)."""
+        _lib.require_device("storage", storage)
+        if storage.dtype != torch.int32 or storage.dim() != 4 or storage.size(0) != 2 or not storage.is_contiguous():
+            raise RuntimeError(f"storage must be contiguous int32 [2, B, kv_heads, capacity], got {storage.dtype} "
+                               f"{tuple(storage.shape)}")
+        self = cls.__new__(cls)
+        self._set(storage)
+        return self
+
+
+def _counts(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
+    """A per-sequence count as contiguous int32 [B]."""
+    if t.dim() != 1 or t.size(0) != B or t.is_floating_point():
+        raise RuntimeError(f"{name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+    return _i32(t)
+
+
+def _table(page_table: torch.Tensor) -> torch.Tensor:
+    if page_table.dim() != 2 or page_table.is_floating_point():
+        raise RuntimeError(f"page_table must be int32 [B, max_pages], got {page_table.dtype} {tuple(page_table.shape)}")
+    return _i32(page_table)
+
+
+def _one_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels get raw pointers: every tensor of a call must be on the cache's device."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"every tensor of the call must be on {device}, got one on {t.device}")
+
+
+def _check_tracker(tracker: SlotTracker, cache: PagedKVCache, B: int) -> None:
+    if tracker.batch != B or tracker.kv_heads != cache.kv_heads:
+        raise RuntimeError(f"tracker of {tracker.batch} sequences x {tracker.kv_heads} heads does not match {B} x "
+                           f"{cache.kv_heads}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [.., heads, D] with rows the kernels can read in place: contiguous in D, 16-byte aligned; else a copy."""
+    e = 16 // t.element_size()
+    st = t.stride()
+    if st[-1] != 1 or t.data_ptr() % 16 or any(s % e for s in st[:-1]):
+        return _lib.aligned(t, 16)
+    return t
+
+
+def _flat_tokens(t: torch.Tensor) -> torch.Tensor:
+    """[B, T, heads, D] -> [B * T, heads, D], a view where the strides allow it."""
+    B, T, H, D = t.shape
+    if B == 1 or T == 1 or t.stride(0) == T * t.stride(1):
+        n, s = B * T, (t.stride(1) if T > 1 else t.stride(0))
+        return t.as_strided((n, H, D), (s, t.stride(2), t.stride(3)))
+    return t.reshape(B * T, H, D)
+
+
+def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
+                  start: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                  tracker: Optional[SlotTracker] = None, token: Optional[torch.Tensor] = None) -> None:
+    """Code the K and V of new tokens into slots start[b], start[b] + 1, ... of their sequences.
+
+    k, v [B, T, kv_heads, D] (T tokens of every sequence), or packed [N, kv_heads, D] with cu_seqlens int32 [B + 1]
+    (sequence b's tokens are cu_seqlens[b] .. cu_seqlens[b + 1]; rows outside are skipped); bf16, fp16 or fp32, strided
+    views are read in place.  The codes are PolarQuant.encode's, bit for bit.  With a tracker, the slots' weights start at
+    0 and their token indices at token[b] (int32 [B]: the sequence's tokens before this call)."""
+    B = page_table.size(0)
+    want = 4 if cu_seqlens is None else 3
+    if k.dim() != want or v.dim() != want or k.shape != v.shape or k.shape[-2:] != (cache.kv_heads, cache.dim):
+        shape = "[B, T" if cu_seqlens is None else "[N"
+        raise RuntimeError(f"append_tokens expects k and v {shape}, {cache.kv_heads}, {cache.dim}], got {tuple(k.shape)} "
+                           f"and {tuple(v.shape)}")
+    if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError(f"k and v must be bfloat16, float16 or float32 alike, got {k.dtype} and {v.dtype}")
+    if cu_seqlens is None and k.size(0) != B:
+        raise RuntimeError(f"k holds {k.size(0)} sequences, page_table {B}")
+    if (tracker is None) != (token is None):
+        raise RuntimeError("append_tokens: a tracker and the sequences' token counts come together")
+    _one_device(cache.device, k, v, page_table, start, cu_seqlens, token, None if tracker is None else tracker.storage)
+    table, start = _table(page_table), _counts("start", start, B)
+    cu = None if cu_seqlens is None else _counts("cu_seqlens", cu_seqlens, B + 1)
+    if tracker is not None:
+        _check_tracker(tracker, cache, B)
+        token = _counts("token", token, B)
+    kr, vr = _rows(k if cu is not None else _flat_tokens(k)), _rows(v if cu is not None else _flat_tokens(v))
+    dev = cache.device
+    diag = cache.quant._diag(cache.dim, dev)
+    with _lib.on_device(dev):
+        rc = _lib.hot("aekv_kv_append")(
+            kr.data_ptr(), vr.data_ptr(), _lib.TORCH_TO_AEKV[k.dtype], kr.stride(0), kr.stride(1), vr.stride(0),
+            vr.stride(1), kr.size(0), _iptr(cu), B, start.data_ptr(), cache.dim, cache.bits, diag.data_ptr(),
+            cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(), cache.v_scale.data_ptr(),
+            cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1),
+            None if tracker is None else tracker.weights.data_ptr(),
+            None if tracker is None else tracker.tokens.data_ptr(), 0 if tracker is None else tracker.capacity,
+            _iptr(token), _lib.raw_stream(dev))
+    _lib.check(rc, "aekv_kv_append")
+
+
+def paged_attention_workspace(B: int, T: int, H: int, kv_heads: int, dim: int, slots: int, device, *,
+                              tracked: bool = False) -> torch.Tensor:
+    """Workspace of paged_attention; slots = page_table.size(1) * page_size."""
+    n = _lib.paged_ws_bytes(int(B), int(T), int(H), int(kv_heads), int(dim), int(slots), int(tracked))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                    softmax_scale: float, *, sink: Optional[torch.Tensor] = None,
+                    tracker: Optional[SlotTracker] = None, workspace: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the newest T tokens of every sequence, its last T slots, over its slots [0, lengths[b]).
+
+    q [B, T, H, D] bf16 or fp16 (strided views are read in place), H a multiple of the cache's KV heads: query head h
+    reads KV head h // (H // kv_heads).  Token t sees slots j < lengths[b] - T + 1 + t.  sink [H] (or a scalar): a logit
+    counted once in the normaliser.  A row that sees nothing gives 0.  With a tracker, weights[b, kv head, j] grows by
+    the attention weight of slot j, summed over the group's heads and the T tokens.  Returns [B, T, H, D] like q."""
+    if q.dim() != 4 or q.size(3) != cache.dim:
+        raise RuntimeError(f"q must be [B, T, H, {cache.dim}], got {tuple(q.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"q must be bfloat16 or float16, got {q.dtype}")
+    B, T, H, D = q.shape
+    if H % cache.kv_heads:
+        raise RuntimeError(f"{H} query heads are no multiple of {cache.kv_heads} KV heads")
+    if page_table.size(0) != B:
+        raise RuntimeError(f"q holds {B} sequences, page_table {page_table.size(0)}")
+    _one_device(cache.device, q, page_table, lengths, sink, workspace, out, None if tracker is None else tracker.storage)
+    table, lengths = _table(page_table), _counts("lengths", lengths, B)
+    if tracker is not None:
+        _check_tracker(tracker, cache, B)
+    qr = _rows(q)
+    sk = None if sink is None else _sink_f32(sink, H)
+    dev = cache.device
+    diag = cache.quant._diag(D, dev)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _check_out("out", out, q.dtype, q.numel(), dev)
+    need = _lib.paged_ws_bytes(B, T, H, cache.kv_heads, D, table.size(1) * cache.page_size, 0 if tracker is None else 1)
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
+        rc = _lib.hot("aekv_paged_attention")(
+            qr.data_ptr(), _lib.TORCH_TO_AEKV[q.dtype], qr.stride(0), qr.stride(1), qr.stride(2), B, T, H, D, cache.bits,
+            diag.data_ptr(), cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(),
+            cache.v_scale.data_ptr(), cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1),
+            lengths.data_ptr(), _iptr(sk), None if tracker is None else tracker.weights.data_ptr(),
+            0 if tracker is None else tracker.capacity, float(softmax_scale), _iptr(ws), 0 if ws is None else ws.numel(),
+            out.data_ptr(), stream)
+    _lib.check(rc, "aekv_paged_attention")
+    return out if out.dim() == 4 else out.view(q.shape)
+
+
+def evict_workspace(B: int, kv_heads: int, keep: int, slots: int, device) -> torch.Tensor:
+    """Workspace of evict_by_weight; slots = min(page_table.size(1) * page_size, tracker.capacity)."""
+    return torch.empty(_lib.evict_ws_bytes(int(B), int(kv_heads), int(keep), int(slots)), dtype=torch.uint8, device=device)
+
+
+def evict_by_weight(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor, tracker: SlotTracker,
+                    seen: torch.Tensor, keep: int, *, first: int = 0, recent: int = 0,
+                    workspace: Optional[torch.Tensor] = None) -> None:
+    """Bring every (sequence, KV head) with more than `keep` slots back to `keep`, in place.
+
+    The slots that stay are those of the first `first` tokens and of the last `recent` of the seen[b] tokens (by the
+    tracker's token indices), then the ones with the largest accumulated weight (equal ones: the lower slot; NaN above
+    every number).  Kept slots below `keep` stay where they are; the evicted ones below `keep`, in order, take the kept
+    slots from `keep` on, in order, with their weight and token index: cached keys carry their rotation, so attention
+    does not depend on the order of the slots.  `lengths` is only read: clamp it to `keep` once every layer is done."""
+    B = page_table.size(0)
+    _one_device(cache.device, page_table, lengths, seen, workspace, tracker.storage)
+    table, lengths, seen = _table(page_table), _counts("lengths", lengths, B), _counts("seen", seen, B)
+    _check_tracker(tracker, cache, B)
+    keep, first, recent = int(keep), int(first), int(recent)
+    dev = cache.device
+    need = _lib.evict_ws_bytes(B, cache.kv_heads, keep, min(table.size(1) * cache.page_size, tracker.capacity))
+    with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
+        rc = _lib.hot("aekv_kv_evict")(
+            cache.dim, cache.bits, cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(),
+            cache.v_scale.data_ptr(), cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1), B,
+            lengths.data_ptr(), tracker.weights.data_ptr(), tracker.tokens.data_ptr(), tracker.capacity,
+            seen.data_ptr(), keep, first, recent, _iptr(ws), 0 if ws is None else ws.numel(), stream)
+    _lib.check(rc, "aekv_kv_evict")

@@ -1,0 +1,65 @@
+"""Causal attention over whole prompts: sequences of different lengths packed into one buffer, heads grouped over KV
+heads.  The attention of the prefill that fills a paged cache (aetherkv.paged), beside the chunked prefill over
+compressed blocks (aetherkv.prefill) and the dense drop-in (aetherkv.sparse_attention.tiled_prefill_attention), which
+attend every source from every target."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .decode import _check_out, _iptr, _sink_f32
+from .paged import _counts, _one_device, _rows
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, *,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None,
+                     return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """out_i = sum_j p_ij v_j over the keys j <= i + (keys - queries) of query i's sequence.
+
+    q [N, H, D], k and v [M, kv_heads, D], bf16 or fp16, D 64 or 128, H a multiple of kv_heads (query head h reads KV head
+    h // (H // kv_heads)); strided views, such as parts of one projection's rows, are read in place.  cu_seqlens int32
+    [B + 1]: sequence b's queries are rows cu_seqlens[b] .. cu_seqlens[b + 1]; cu_seqlens_k likewise for the keys (None:
+    the same), so that a later chunk of a prompt comes with the keys before it.  sink [H] (or a scalar): a logit counted
+    once in the normaliser.  A query that sees nothing gives 0.  Rows of q in no sequence: a given `out` keeps them, a new
+    one holds 0.  Returns out [N, H, D], with return_lse (out, lse fp32 [N, H]): the log of every row's sum of
+    exponentials, the sink's among them (-inf for rows in no sequence)."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.size(2) != q.size(2):
+        raise RuntimeError(f"prompt_attention expects q [N, H, D] and k, v [M, kv_heads, D], got {tuple(q.shape)}, "
+                           f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError(f"q, k and v must be bfloat16 or float16 alike, got {q.dtype}, {k.dtype} and {v.dtype}")
+    _lib.require_device("q", q, k, v, cu_seqlens, cu_seqlens_k, sink, out)
+    N, H, D = q.shape
+    M, hk, _ = k.shape
+    if hk < 1 or H % hk:
+        raise RuntimeError(f"{H} query heads are no multiple of {hk} KV heads")
+    if cu_seqlens.dim() != 1 or cu_seqlens.size(0) < 2:
+        raise RuntimeError(f"cu_seqlens must be int32 [B + 1], got {tuple(cu_seqlens.shape)}")
+    B = cu_seqlens.size(0) - 1
+    dev = q.device
+    _one_device(dev, k, v, cu_seqlens, cu_seqlens_k, sink, out)
+    cq = _counts("cu_seqlens", cu_seqlens, B + 1)
+    if cu_seqlens_k is None:
+        if M != N:
+            raise RuntimeError(f"{N} queries and {M} keys: cu_seqlens_k is needed")
+        ck = cq
+    else:
+        ck = _counts("cu_seqlens_k", cu_seqlens_k, B + 1)
+    qr, kr, vr = _rows(q), _rows(k), _rows(v)
+    sk = None if sink is None else _sink_f32(sink, H)
+    clear = 0
+    if out is None:
+        out, clear = torch.empty(q.shape, dtype=q.dtype, device=dev), 1
+    else:
+        _check_out("out", out, q.dtype, q.numel(), dev)
+    lse = torch.empty((N, H), dtype=torch.float32, device=dev) if return_lse else None
+    with _lib.on_device(dev):
+        rc = _lib.hot("aekv_prompt_attention")(
+            qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), _lib.TORCH_TO_AEKV[q.dtype], qr.stride(0), qr.stride(1),
+            kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1), cq.data_ptr(), ck.data_ptr(), B, N, M, H, hk, D,
+            _iptr(sk), float(softmax_scale), out.data_ptr(), _iptr(lse), clear, _lib.raw_stream(dev))
+    _lib.check(rc, "aekv_prompt_attention")
+    out = out if out.dim() == 3 else out.view(q.shape)
+    return (out, lse) if return_lse else out

@@ -300,6 +300,72 @@ int aekv_tiled_prefill_attention_ws(const void* q, const void* kv, const void* s
                                     float softmax_scale, int32_t tile_size, void* ws, size_t ws_bytes, void* out,
                                     void* stream);
 
+/* ---- paged per-head KV cache in TurboQuant codes -------------------------------------------------
+ * A pool of `pages` pages for K and for V: codes [pages, heads, page_size, d bits/8] (bytes as
+ * aekv_tq_encode writes them) and scales fp32 [pages, heads, page_size]; page_size a power of two from
+ * 16 to 4096, d = 64 or 128, codes and scales 16-byte aligned.  Slot p of sequence b lies in row
+ * p % page_size of page page_table[b, p / page_size] (int32 [B, max_pages]).  Tables, lengths and starts
+ * are device data: a slot outside the table or a page outside the pool is skipped, never accessed.
+ * A tracker holds, per sequence, KV head and slot, the accumulated attention weight (fp32) and the token
+ * index of the slot (int32), both [B, heads, capacity]. */
+
+/* Codes the K and V vectors of n_tokens new tokens (F32/F16/BF16; rows of d contiguous elements, token and
+ * head strides in elements, rows 16-byte aligned) into slots start[b], start[b] + 1, ... of their sequences:
+ * token n belongs to sequence n / (n_tokens / B), or, with cu_seqlens int32 [B + 1], to the b with
+ * cu_seqlens[b] <= n < cu_seqlens[b + 1] (tokens outside every sequence are skipped).  Bit for bit
+ * aekv_tq_encode's codes and scales.  weights / tokens / token (all or none): the slot's weight is set to 0
+ * and its token index to token[b] + its place among the sequence's new tokens. */
+int aekv_kv_append(const void* k, const void* v, int32_t dtype, int64_t k_token_stride, int64_t k_head_stride,
+                   int64_t v_token_stride, int64_t v_head_stride, int64_t n_tokens, const int32_t* cu_seqlens,
+                   int64_t B, const int32_t* start, int32_t d, int32_t bits, const float* diag, void* k_codes,
+                   float* k_scale, void* v_codes, float* v_scale, int64_t pages, int64_t heads, int32_t page_size,
+                   const int32_t* page_table, int64_t max_pages, float* weights, int32_t* tokens, int64_t capacity,
+                   const int32_t* token, void* stream);
+
+/* Attention of the newest T tokens of each sequence (its last T slots) over the cache: q [B, T, H, d] bf16 or
+ * fp16 (strides in elements), H a multiple of heads, query head h reads KV head h / (H / heads); token t sees
+ * slots j < lengths[b] - T + 1 + t; l = softmax_scale q . decode(K_j), p = exp(l) / (sum exp(l) + exp(sink[h]))
+ * (sink fp32 [H] or NULL), out [B, T, H, d] = sum p decode(V_j), contiguous, in q's type; 0 where nothing is
+ * seen.  weights (nullable): weights[b, head, j] += the sum of p_j over the head's query heads and the T
+ * tokens.  Workspace: aekv_paged_attention_workspace_size(B, T, H, heads, d, max_pages * page_size,
+ * weights != NULL) bytes, 16-byte aligned; its contents never matter. */
+size_t aekv_paged_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t heads, int32_t d,
+                                           int64_t slots, int32_t tracked);
+int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batch_stride, int64_t q_token_stride,
+                         int64_t q_head_stride, int64_t B, int64_t T, int64_t H, int32_t d, int32_t bits,
+                         const float* diag, const void* k_codes, const float* k_scale, const void* v_codes,
+                         const float* v_scale, int64_t pages, int64_t heads, int32_t page_size,
+                         const int32_t* page_table, int64_t max_pages, const int32_t* lengths, const float* sink,
+                         float* weights, int64_t capacity, float softmax_scale, void* ws, size_t ws_bytes, void* out,
+                         void* stream);
+
+/* Brings every (sequence, head) with n = lengths[b] > keep slots back to `keep`, in place: kept are the highest
+ * ranked slots, first those with token index < first or >= seen[b] - recent, then by weight (larger first, NaN
+ * above every number), equal ranks by slot.  Kept slots below keep stay; the evicted ones below keep, in
+ * increasing order, take the kept slots from keep on, in increasing order (codes, scales, weight, token).
+ * Slots from keep on are left as they are; lengths are only read (the caller clamps them to keep once every
+ * layer is done).  first + recent <= keep.  Workspace: aekv_kv_evict_workspace_size(B, heads, keep,
+ * min(max_pages * page_size, capacity)) bytes, 16-byte aligned. */
+size_t aekv_kv_evict_workspace_size(int64_t B, int64_t heads, int64_t keep, int64_t slots);
+int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_scale, void* v_codes, float* v_scale,
+                  int64_t pages, int64_t heads, int32_t page_size, const int32_t* page_table, int64_t max_pages,
+                  int64_t B, const int32_t* lengths, float* weights, int32_t* tokens, int64_t capacity,
+                  const int32_t* seen, int64_t keep, int64_t first, int64_t recent, void* ws, size_t ws_bytes,
+                  void* stream);
+
+/* Causal attention over whole prompts packed into one buffer: q [n_q, H, d], k and v [n_k, heads, d] bf16 or
+ * fp16 (token and head strides in elements, rows 16-byte aligned), sequence b holding queries cu_seqlens_q[b]
+ * .. cu_seqlens_q[b + 1] and keys cu_seqlens_k[b] .. (int32 [B + 1], non-decreasing); its i-th query sees keys
+ * j <= i + (keys - queries).  out [n_q, H, d] contiguous; lse fp32 [n_q, H] (nullable): log of the row's sum of
+ * exponentials, the sink's (fp32 [H] or NULL) among them.  A query that sees nothing gives 0.  Rows in no
+ * sequence: out is left as it is (clear_rest 0) or 0 (1), lse is -inf.  d = 64 or 128. */
+int aekv_prompt_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
+                          int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens_q,
+                          const int32_t* cu_seqlens_k, int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads,
+                          int32_t d, const float* sink, float softmax_scale, void* out, float* lse,
+                          int32_t clear_rest, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

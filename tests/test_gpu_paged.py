@@ -1,0 +1,559 @@
+"""Paged cache in TurboQuant codes on the GPU against plain 64-bit forms (paged_ref.py): append, attention, eviction, and
+a run of them together."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from aetherkv import PolarQuant
+from aetherkv.paged import (PagedKVCache, SlotTracker, append_tokens, evict_by_weight, evict_workspace, paged_attention,
+                            paged_attention_workspace)
+from conftest import randn_outliers
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _fill(dev, seed, bits, dim, heads, page, pages):
+    """A pool of coded Gaussian entries, with NaN scales nowhere."""
+    pq = PolarQuant(bits)
+    x = torch.randn(2, pages, heads, page, dim, device=dev, generator=_gen(dev, seed)).to(torch.bfloat16)
+    kc, ks = pq.encode(x[0])
+    vc, vs = pq.encode(x[1])
+    return PagedKVCache.from_tensors(pq, kc, ks[..., 0].contiguous(), vc, vs[..., 0].contiguous())
+
+
+def _cache(dev, seed, bits, dim, heads, page, lengths, spare=3):
+    per = max(1, -(-max(max(lengths), 1) // page))
+    pages = per * len(lengths) + spare
+    cache = _fill(dev, seed, bits, dim, heads, page, pages)
+    table = torch.randperm(pages, device=dev, generator=_gen(dev, seed + 1))[:per * len(lengths)].to(torch.int32).view(len(lengths), per)
+    return cache, table, torch.tensor(lengths, dtype=torch.int32, device=dev)
+
+
+def _poison(cache, table, lengths):
+    """NaN scales in every slot past a sequence's length and in every page of no sequence: they must not matter."""
+    used = torch.zeros(cache.pages, cache.page_size, dtype=torch.bool, device=table.device)
+    for b, n in enumerate(lengths.tolist()):
+        slot = torch.arange(max(0, n), device=table.device)
+        used[table[b].long()[slot // cache.page_size], slot % cache.page_size] = True
+    for s in (cache.k_scale, cache.v_scale):
+        s.masked_fill_(~used[:, None, :], NAN)
+
+
+def _check_attention(dev, bits, dim, dtype, page, heads, group, T, lengths, sink, track, seed=0, scale=None, gain=1.0):
+    cache, table, n = _cache(dev, seed, bits, dim, heads, page, lengths)
+    _poison(cache, table, n)
+    B, H = len(lengths), heads * group
+    q = (torch.randn(B, T, H, dim, device=dev, generator=_gen(dev, seed + 2)) * gain).to(dtype)
+    sk = torch.randn(H, device=dev, generator=_gen(dev, seed + 3)) if sink else None
+    tracker = before = None
+    if track:
+        tracker = SlotTracker(B, heads, table.size(1) * page, device=dev)
+        tracker.weights.uniform_(0, 3, generator=_gen(dev, seed + 4))
+        before = tracker.weights.double().cpu()
+    scale = dim ** -0.5 if scale is None else scale
+    got = paged_attention(q, cache, table, n, scale, sink=sk, tracker=tracker)
+    want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, table), q.cpu(), lengths, scale, None if sk is None else sk.cpu(), tracker.capacity if track else None)
+    R.within(got, want, bound, "out")
+    if track:
+        R.within(tracker.weights, before + w, wb + 2.0 ** -23 * (before + w), "weights")
+        assert torch.equal(tracker.weights.cpu()[w == 0], before.float()[w == 0]), "weights of slots that nothing sees"
+
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 127, 129, 257, 300]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_every_type_and_length(dev, bits, dim, dtype):
+    _check_attention(dev, bits, dim, dtype, 16, 2, 3, 1, LENGTHS, False, True, seed=bits + dim)
+
+
+@pytest.mark.parametrize("heads,group", [(1, 1), (1, 12), (12, 1), (3, 4), (2, 16), (1, 17), (1, 40)])
+def test_attention_head_layouts(dev, heads, group):
+    _check_attention(dev, 4, 128, torch.bfloat16, 32, heads, group, 1, [70, 1, 333], True, True, seed=group)
+
+
+@pytest.mark.parametrize("T,heads,group", [(2, 2, 3), (5, 1, 4), (16, 2, 8), (7, 3, 1), (33, 1, 2)])
+def test_attention_several_tokens(dev, T, heads, group):
+    # (a sequence shorter than T: its first tokens see nothing)
+    _check_attention(dev, 8, 64, torch.float16, 16, heads, group, T, [T, T + 1, 200, 3, 0], False, True, seed=T)
+
+
+@pytest.mark.parametrize("page", [16, 64, 256, 1024])
+def test_attention_page_sizes(dev, page):
+    _check_attention(dev, 4, 64, torch.bfloat16, page, 2, 2, 2, [5, page, page + 1, 3 * page - 7], True, True, seed=page)
+
+
+@pytest.mark.parametrize("length", [1000, 4097, 20011])
+def test_attention_long(dev, length):
+    _check_attention(dev, 4, 128, torch.bfloat16, 64, 1, 3, 1, [length, length // 3], False, True, seed=length)
+
+
+def test_attention_peaked_and_flat(dev):
+    _check_attention(dev, 8, 128, torch.float16, 16, 2, 2, 1, [200, 90], False, True, gain=30.0)
+    _check_attention(dev, 4, 128, torch.bfloat16, 16, 2, 2, 1, [200, 90], True, True, scale=0.0)
+    _check_attention(dev, 4, 64, torch.bfloat16, 16, 2, 2, 1, [200, 90], True, False, scale=-0.2)
+
+
+def test_attention_scales_of_many_sizes(dev):
+    """V scales over twelve decades, the largest where the weight is small, and queries near the type's ends."""
+    cache, table, n = _cache(dev, 5, 4, 128, 1, 16, [150])
+    cache.v_scale.mul_(10 ** (12 * torch.rand(cache.v_scale.shape, device=dev, generator=_gen(dev, 6)) - 6))
+    q = torch.randn(1, 1, 3, 128, device=dev, generator=_gen(dev, 7)).to(torch.bfloat16)
+    for f in (1.0, 2.0 ** 60, 2.0 ** -60):
+        qq = q * f
+        got = paged_attention(qq, cache, table, n, 128 ** -0.5 / f)
+        want, bound, _, _ = R.paged_attention_ref(R.HostCache(cache, table), qq.cpu(), [150], 128 ** -0.5 / f)
+        R.within(got, want, bound, f"q times {f}")
+
+
+def test_attention_sinks_at_the_ends(dev):
+    cache, table, n = _cache(dev, 8, 4, 128, 1, 16, [40, 0, 1])
+    q = torch.randn(3, 1, 2, 128, device=dev, generator=_gen(dev, 9)).to(torch.bfloat16)
+    sink = torch.tensor([-math.inf, 200.0], device=dev)
+    got = paged_attention(q, cache, table, n, 0.09, sink=sink)
+    want, bound, _, _ = R.paged_attention_ref(R.HostCache(cache, table), q.cpu(), [40, 0, 1], 0.09, sink.cpu())
+    R.within(got, want, bound, "out")
+    assert not got[1].any()
+    plain = paged_attention(q[:, :, :1], cache, table, n, 0.09)
+    assert torch.equal(plain, got[:, :, :1])  # a sink of -inf is none
+
+
+def test_attention_nan_stays_in_its_rows(dev):
+    cache, table, n = _cache(dev, 10, 8, 64, 2, 16, [50, 60])
+    q = torch.randn(2, 3, 4, 64, device=dev, generator=_gen(dev, 11)).to(torch.float16)
+    clean = paged_attention(q, cache, table, n, 0.125)
+    q2 = q.clone()
+    q2[1, 2, 3] = NAN
+    got = paged_attention(q2, cache, table, n, 0.125)
+    assert got[1, 2, 3].isnan().all()
+    keep = torch.ones(2, 3, 4, dtype=torch.bool, device=dev)
+    keep[1, 2, 3] = False
+    assert torch.equal(got[keep], clean[keep])
+    # a NaN entry in the newest slot: the earlier tokens do not see it
+    cache.v_scale[table[0, 49 // 16].long(), 0, 49 % 16] = NAN
+    got = paged_attention(q, cache, table, n, 0.125)
+    assert got[0, 2, :2].isnan().all() and torch.equal(got[0, :2], clean[0, :2]) and torch.equal(got[1], clean[1])
+
+
+def test_attention_skips_bad_pages_and_clamps_lengths(dev):
+    cache, table, n = _cache(dev, 12, 4, 128, 2, 16, [100, 100, 100])
+    table[0, 2], table[1, 0], table[1, 6] = -1, cache.pages, 0x7fffffff
+    n = torch.tensor([100, 100, 5000], dtype=torch.int32, device=dev)
+    q = torch.randn(3, 1, 4, 128, device=dev, generator=_gen(dev, 13)).to(torch.bfloat16)
+    tracker = SlotTracker(3, 2, 112, device=dev)
+    got = paged_attention(q, cache, table, n, 0.09, tracker=tracker)
+    want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, table), q.cpu(), [100, 100, 5000], 0.09, capacity=112)
+    R.within(got, want, bound, "out")
+    R.within(tracker.weights, w, wb, "weights")
+    neg = paged_attention(q, cache, table, torch.tensor([-5, 0, -(2 ** 31)], dtype=torch.int32, device=dev), 0.09)
+    assert not neg.any()
+    assert not paged_attention(q, cache, torch.full_like(table, -1), n, 0.09).any()
+    assert not paged_attention(q, cache, table[:, :0], n, 0.09, tracker=tracker).any()
+
+
+def test_attention_tracker_smaller_than_the_table(dev):
+    """Slots behind the tracker's last have nowhere to be counted: a tracked call ends at its capacity."""
+    cache, table, n = _cache(dev, 14, 4, 64, 1, 16, [90])
+    q = torch.randn(1, 1, 2, 64, device=dev, generator=_gen(dev, 15)).to(torch.bfloat16)
+    storage = torch.zeros(2, 1, 1, 70, dtype=torch.int32, device=dev)
+    tracker = SlotTracker.from_tensor(storage)
+    got = paged_attention(q, cache, table, n, 0.125, tracker=tracker)
+    want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, table), q.cpu(), [90], 0.125, capacity=70)
+    R.within(got, want, bound, "out")
+    R.within(tracker.weights, w, wb, "weights")
+
+
+def test_attention_strided_query_given_output_and_workspace(dev):
+    cache, table, n = _cache(dev, 16, 4, 128, 2, 32, [77, 200])
+    wide = torch.randn(2, 3, 9, 128, device=dev, generator=_gen(dev, 17)).to(torch.bfloat16)
+    q = wide[:, :, 1:5]
+    want = paged_attention(q.contiguous(), cache, table, n, 0.09)
+    out = torch.empty(2, 3, 4, 128, dtype=torch.bfloat16, device=dev)
+    ws = paged_attention_workspace(2, 3, 4, 2, 128, table.size(1) * 32, dev)
+    ws.fill_(255)
+    assert paged_attention(q, cache, table, n, 0.09, out=out, workspace=ws).data_ptr() == out.data_ptr()
+    assert torch.equal(out, want)
+    odd = torch.empty(2 * 3 * 4 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(2, 3, 4, 128).copy_(q)
+    assert torch.equal(paged_attention(odd, cache, table, n.long(), 0.09), want)  # misaligned: copied
+    back = torch.empty(2, 4, 128, 3, dtype=torch.bfloat16, device=dev).copy_(q.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
+    assert torch.equal(paged_attention(back, cache, table.long(), n, 0.09), want)  # strided in D: copied
+
+
+def test_attention_repeats_and_streams(dev):
+    """The same call gives the same bits, on its own stream or another, beside a call on a second stream."""
+    cache, table, n = _cache(dev, 18, 4, 128, 4, 64, [3000, 1500, 64, 5])
+    q = torch.randn(4, 1, 12, 128, device=dev, generator=_gen(dev, 19)).to(torch.bfloat16)
+    want = paged_attention(q, cache, table, n, 0.09)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(paged_attention(q, cache, table, n, 0.09))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, want)
+
+
+def test_attention_tracked_repeats_bit_for_bit(dev):
+    cache, table, n = _cache(dev, 20, 4, 128, 2, 64, [5000, 700])
+    q = torch.randn(2, 4, 6, 128, device=dev, generator=_gen(dev, 21)).to(torch.bfloat16)
+    got = []
+    for _ in range(3):
+        tracker = SlotTracker(2, 2, table.size(1) * 64, device=dev)
+        got.append((paged_attention(q, cache, table, n, 0.09, tracker=tracker), tracker.weights))
+    for o, w in got[1:]:
+        assert torch.equal(o, got[0][0]) and torch.equal(w, got[0][1])
+
+
+def test_attention_offsets_past_31_bits(dev):
+    """A pool of more than 2 GiB of codes, the sequence in its last pages."""
+    pq = PolarQuant(8)
+    pages, page = 4200, 4096
+    codes = torch.zeros(pages, 1, page, 128, dtype=torch.int8, device=dev)  # 2.2 GB
+    scale = torch.zeros(pages, 1, page, device=dev)
+    x = torch.randn(2, page, 128, device=dev, generator=_gen(dev, 22)).to(torch.bfloat16)
+    c, s = pq.encode(x)
+    codes[-2:, 0], scale[-2:, 0] = c, s[..., 0]
+    cache = PagedKVCache.from_tensors(pq, codes, scale, codes, scale)
+    table = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device=dev)
+    q = torch.randn(1, 1, 2, 128, device=dev, generator=_gen(dev, 23)).to(torch.bfloat16)
+    got = paged_attention(q, cache, table, torch.tensor([4500], dtype=torch.int32, device=dev), 0.09)
+    small = PagedKVCache.from_tensors(pq, codes[-2:].clone(), scale[-2:].clone(), codes[-2:].clone(), scale[-2:].clone())
+    st = torch.tensor([[1, 0]], dtype=torch.int32, device=dev)
+    want, bound, _, _ = R.paged_attention_ref(R.HostCache(small, st), q.cpu(), [4500], 0.09)
+    R.within(got, want, bound, "out")
+
+
+def test_refusals(dev):
+    cache, table, n = _cache(dev, 24, 4, 128, 2, 16, [20, 30])
+    q = torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16, device=dev)
+    tracker = SlotTracker(2, 2, 32, device=dev)
+    for bad in (q.float(), q[..., :64], q[:, :, :3], q[:1], q[0]):
+        with pytest.raises(RuntimeError):
+            paged_attention(bad, cache, table, n, 0.1)
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n[:1], 0.1)
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n.cpu(), 0.1)
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n, 0.1, sink=torch.zeros(3, device=dev))
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n, 0.1, tracker=SlotTracker(2, 3, 32, device=dev))
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n, 0.1, out=torch.empty_like(q, dtype=torch.float16))
+    with pytest.raises(RuntimeError):
+        paged_attention(q, cache, table, n, 0.1, tracker=tracker, workspace=torch.empty(16, dtype=torch.uint8, device=dev))
+    k = torch.zeros(2, 1, 2, 128, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError):
+        append_tokens(cache, k, k.half(), table, n)
+    with pytest.raises(RuntimeError):
+        append_tokens(cache, k, k[:, :, :1], table, n)
+    with pytest.raises(RuntimeError):
+        append_tokens(cache, k, k, table, n, tracker=tracker)  # without token
+    with pytest.raises(RuntimeError):
+        append_tokens(cache, k[:, 0], k[:, 0], table, n, cu_seqlens=n)  # [B + 1] wanted
+    with pytest.raises(ValueError):
+        evict_by_weight(cache, table, n, tracker, n, 8, first=5, recent=4)
+    with pytest.raises(RuntimeError):
+        evict_by_weight(cache, table, n, tracker, n, 8, workspace=torch.empty(16, dtype=torch.uint8, device=dev))
+    with pytest.raises(RuntimeError):
+        PagedKVCache.from_tensors(cache.quant, cache.k_codes, cache.k_scale[:1], cache.v_codes, cache.v_scale)
+    with pytest.raises(RuntimeError):
+        PagedKVCache.from_tensors(PolarQuant(8), cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale)
+
+
+# ---- append ----------------------------------------------------------------------------------------------------
+
+def _expect_append(cache, k, v, table, start, cu):
+    """The pools after the append, by PolarQuant.encode and plain indexing."""
+    pools = [cache.k_codes.clone(), cache.k_scale.clone(), cache.v_codes.clone(), cache.v_scale.clone()]
+    for x, pc, ps in ((k, pools[0], pools[1]), (v, pools[2], pools[3])):
+        codes, scale = cache.quant.encode(x.contiguous())
+        for b in range(table.size(0)):
+            for i, r in enumerate(range(max(0, cu[b]), min(cu[b + 1], x.size(0)))):
+                p = start[b] + i
+                page = int(table[b, p // cache.page_size]) if 0 <= p < table.size(1) * cache.page_size else -1
+                if 0 <= page < cache.pages:
+                    pc[page, :, p % cache.page_size] = codes[r]
+                    ps[page, :, p % cache.page_size] = scale[r, :, 0]
+    return pools
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_append_bit_exact(dev, bits, dim, dtype):
+    heads, B, T, page = 3, 4, 5, 16
+    cache, table, _ = _cache(dev, 30, bits, dim, heads, page, [40] * B)
+    kv = randn_outliers((B, T, 2 * heads, dim), seed=31).to(dev).to(dtype)
+    k, v = kv[:, :, :heads], kv[:, :, heads:]  # views of one projection
+    start = [0, 14, 30, 46]  # the last one runs past its table
+    want = _expect_append(cache, k.reshape(B * T, heads, dim), v.reshape(B * T, heads, dim), table.cpu(), start, [T * b for b in range(B + 1)])
+    tracker = SlotTracker(B, heads, 48, device=dev)
+    tracker.weights.fill_(9.0)
+    tracker.tokens.fill_(-7)
+    append_tokens(cache, k, v, table, torch.tensor(start, dtype=torch.int32, device=dev), tracker=tracker, token=torch.tensor([0, 100, 200, 300], dtype=torch.int32, device=dev))
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        assert torch.equal(got, w)
+    for b in range(B):
+        for p in range(48):
+            i = p - start[b]
+            assert (tracker.weights[b, :, p] == (0.0 if 0 <= i < T else 9.0)).all()
+            assert (tracker.tokens[b, :, p] == (100 * b + i if 0 <= i < T else -7)).all()
+
+
+@pytest.mark.parametrize("lens", [[1], [0, 3, 0, 40, 1], [257, 64, 0]])
+def test_append_packed(dev, lens):
+    heads, dim, page = 2, 128, 16
+    B = len(lens)
+    cache, table, _ = _cache(dev, 32, 4, dim, heads, page, [max(lens) + 20] * B)
+    N = sum(lens) + 5  # rows behind the last sequence
+    k, v = (randn_outliers((N, heads, dim), seed=33 + i).to(dev) for i in range(2))
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    start = [3 * b for b in range(B)]
+    want = _expect_append(cache, k, v, table.cpu(), start, cu)
+    append_tokens(cache, k, v, table, torch.tensor(start, dtype=torch.int32, device=dev), cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev))
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        assert torch.equal(got, w)
+
+
+def test_append_special_values_and_many_sequences(dev):
+    """Zeros, infinities and NaN code as PolarQuant codes them; 300 sequences of one packed token each."""
+    cache, table, _ = _cache(dev, 34, 4, 64, 1, 16, [16] * 300)
+    k = torch.randn(300, 1, 64, device=dev, generator=_gen(dev, 35)).to(torch.bfloat16)
+    k[0], k[1, 0, 3], k[2, 0, 5], k[3] = 0, math.inf, NAN, 1e-30
+    v = k.flip(0)
+    cu = torch.arange(301, dtype=torch.int32, device=dev)
+    start = torch.arange(300, dtype=torch.int32, device=dev) % 16
+    want = _expect_append(cache, k, v, table.cpu(), start.tolist(), cu.tolist())
+    append_tokens(cache, k, v, table, start, cu_seqlens=cu)
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        fine = ~torch.isnan(w) if w.is_floating_point() else torch.ones_like(w, dtype=torch.bool)
+        assert torch.equal(got[fine], w[fine])
+        assert not w.is_floating_point() or got[~fine].isnan().all()
+
+
+def test_append_skips_bad_pages_and_counts(dev):
+    cache, table, _ = _cache(dev, 36, 8, 64, 2, 16, [64, 64, 64])
+    table[0, 1], table[1, 0] = -3, cache.pages
+    k, v = (torch.randn(3, 4, 2, 64, device=dev, generator=_gen(dev, 37 + i)).to(torch.bfloat16) for i in range(2))
+    start = [14, 14, -2]  # a negative start: the first two have no slot
+    want = _expect_append(cache, k.flatten(0, 1), v.flatten(0, 1), table.cpu(), start, [0, 4, 8, 12])
+    append_tokens(cache, k, v, table, torch.tensor(start, dtype=torch.int32, device=dev))
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        assert torch.equal(got, w)
+    before = cache.k_codes.clone()
+    append_tokens(cache, k[:, :0], v[:, :0], table, torch.tensor(start, dtype=torch.int32, device=dev))
+    assert torch.equal(cache.k_codes, before)
+
+
+# ---- eviction --------------------------------------------------------------------------------------------------
+
+def _check_evict(dev, bits, dim, heads, page, lengths, keep, first, recent, weights=None, seed=0, capacity=None):
+    cache, table, n = _cache(dev, seed, bits, dim, heads, page, lengths)
+    B = len(lengths)
+    cap = capacity if capacity is not None else table.size(1) * page
+    tracker = SlotTracker(B, heads, cap, device=dev)
+    w = torch.randn(B, heads, cap, generator=torch.Generator().manual_seed(seed + 5)).exp() if weights is None else weights(B, heads, cap)
+    tracker.weights.copy_(w)
+    tok = torch.stack([torch.randperm(cap, generator=torch.Generator().manual_seed(seed + i)) for i in range(B * heads)]).view(B, heads, cap)
+    tracker.tokens.copy_(tok)
+    seen = torch.tensor([max(x, 0) for x in lengths], dtype=torch.int32, device=dev)
+    pools = [x.clone() for x in (cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale)]
+    ww, tt, tc = w.clone(), tok.clone(), table.cpu().long()
+    w = tracker.weights.cpu()
+    for b in range(B):
+        for h in range(heads):
+            m = min(lengths[b], cap, table.size(1) * page)
+            for src, dst in R.evict_ref(w[b, h].tolist(), tok[b, h].tolist(), m, int(seen[b]), keep, first, recent):
+                ps, pd = int(tc[b, src // page]), int(tc[b, dst // page])
+                if 0 <= ps < cache.pages and 0 <= pd < cache.pages:
+                    for x, y in zip(pools, (cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale)):
+                        x[pd, h, dst % page] = y[ps, h, src % page]
+                ww[b, h, dst], tt[b, h, dst] = w[b, h, src], tok[b, h, src]
+    evict_by_weight(cache, table, n, tracker, seen, keep, first=first, recent=recent)
+    assert torch.equal(tracker.tokens.cpu().long(), tt)
+    assert torch.equal(tracker.weights.cpu().view(torch.int32), ww.float().view(torch.int32))
+    for got, want in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), pools):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 64), (4, 128), (8, 64), (8, 128)])
+def test_evict_moves_whole_rows(dev, bits, dim):
+    _check_evict(dev, bits, dim, 2, 16, [0, 1, 39, 40, 41, 64, 100, 200], 40, 4, 10, seed=bits + dim)
+
+
+@pytest.mark.parametrize("keep,first,recent", [(1, 0, 0), (1, 1, 0), (7, 0, 7), (500, 2, 100), (999, 0, 0), (1024, 4, 128), (1025, 0, 1)])
+def test_evict_budgets(dev, keep, first, recent):
+    _check_evict(dev, 4, 64, 1, 64, [1500, 1025, 300], keep, first, recent, seed=keep)
+
+
+@pytest.mark.parametrize("length", [1023, 1024, 1025, 2049, 5000, 9000, 33000])
+def test_evict_long_rows(dev, length):
+    _check_evict(dev, 4, 64, 2, 256, [length, length - 1], length // 3, 4, 64, seed=length)
+
+
+def test_evict_keeps_nothing(dev):
+    _check_evict(dev, 4, 64, 1, 16, [50], 0, 0, 0)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few", "zeros", "tiny", "special"])
+def test_evict_ties_and_special_weights(dev, kind):
+    def weights(B, heads, cap):
+        g = torch.Generator().manual_seed(3)
+        if kind == "equal":
+            return torch.ones(B, heads, cap)
+        if kind == "few":
+            return torch.randint(0, 3, (B, heads, cap), generator=g).float()
+        if kind == "zeros":  # both zeros are one weight
+            return torch.where(torch.rand(B, heads, cap, generator=g) < 0.5, 0.0, -0.0)
+        if kind == "tiny":
+            return torch.randint(0, 5, (B, heads, cap), generator=g).float() * 2.0 ** -149
+        w = torch.randn(B, heads, cap, generator=g)
+        w[..., 3::17], w[..., 5::19], w[..., 7::23], w[..., 8::29] = NAN, math.inf, -math.inf, -NAN
+        return w
+    _check_evict(dev, 4, 64, 2, 32, [700, 2500], 300, 2, 20, weights=weights)
+
+
+def test_evict_bad_pages_short_tracker_and_given_workspace(dev):
+    _check_evict(dev, 8, 64, 1, 16, [300, 200], 100, 0, 0, capacity=250)
+    cache, table, n = _cache(dev, 40, 4, 64, 2, 16, [120, 120])
+    table[0, 0], table[1, 6] = -1, cache.pages + 5
+    tracker = SlotTracker(2, 2, 128, device=dev)
+    tracker.weights.uniform_(generator=_gen(dev, 41))
+    tracker.tokens.copy_(torch.arange(128, device=dev).expand(2, 2, 128))
+    kc, w = cache.k_codes.clone(), tracker.weights.cpu()
+    ws = evict_workspace(2, 2, 64, 128, dev)
+    ws.fill_(255)
+    seen = n.clone()
+    evict_by_weight(cache, table, n, tracker, seen, 64, workspace=ws)
+    tc = table.cpu().long()
+    for b in range(2):
+        for h in range(2):
+            for src, dst in R.evict_ref(w[b, h].tolist(), list(range(128)), 120, 120, 64, 0, 0):
+                ps, pd = int(tc[b, src // 16]), int(tc[b, dst // 16])
+                if 0 <= ps < cache.pages and 0 <= pd < cache.pages:
+                    kc[pd, h, dst % 16] = cache.k_codes[ps, h, src % 16]
+    assert torch.equal(cache.k_codes, kc)
+
+
+# ---- together --------------------------------------------------------------------------------------------------
+
+def test_prompt_decode_evict_together(dev):
+    """Prompts attended and coded into the cache, decode steps with weights, an eviction, more steps: every attention
+    against the plain form over the cache as it is, and the cache against what PolarQuant and the rules say."""
+    from aetherkv.prompt import prompt_attention
+
+    heads, group, dim, page, keep = 2, 3, 128, 16, 48
+    H, lens, steps = heads * group, [90, 33, 61], 4
+    pq = PolarQuant(4)
+    gen = _gen(dev, 50)
+    table = torch.randperm(27, device=dev, generator=gen)[:24].to(torch.int32).view(3, 8)
+    cache = PagedKVCache(pq, 27, heads, dim, page_size=page, device=dev)
+    tracker = SlotTracker(3, heads, 128, device=dev)
+    lengths = torch.zeros(3, dtype=torch.int32, device=dev)
+    seen = torch.zeros(3, dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 90, 123, 184], dtype=torch.int32, device=dev)
+    qkv = torch.randn(184, H + 2 * heads, dim, device=dev, generator=gen).to(torch.bfloat16)
+    q, k, v = qkv[:, :H], qkv[:, H:H + heads], qkv[:, H + heads:]
+    out = prompt_attention(q, k, v, cu, dim ** -0.5)
+    want, bound, _, _ = R.prompt_attention_ref(q.cpu(), k.cpu(), v.cpu(), cu.tolist(), cu.tolist(), dim ** -0.5)
+    R.within(out, want, bound, "prompt")
+    append_tokens(cache, k, v, table, lengths, cu_seqlens=cu, tracker=tracker, token=seen)
+    new = torch.tensor(lens, dtype=torch.int32, device=dev)
+    lengths += new
+    seen += new
+    kk, vv = cache.decode(table[0], 90, torch.float32)
+    for got, x in ((kk, k), (vv, v)):
+        assert torch.equal(got, pq.decode(*pq.encode(x[:90].contiguous()), out_dtype=torch.float32).transpose(0, 1))
+
+    def step():
+        qkv = torch.randn(3, 1, H + 2 * heads, dim, device=dev, generator=gen).to(torch.bfloat16)
+        append_tokens(cache, qkv[:, :, H:H + heads], qkv[:, :, H + heads:], table, lengths, tracker=tracker, token=seen)
+        lengths.add_(1)
+        seen.add_(1)
+        before = tracker.weights.double().cpu()
+        out = paged_attention(qkv[:, :, :H], cache, table, lengths, dim ** -0.5, tracker=tracker)
+        want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, table), qkv[:, :, :H].cpu(), lengths.tolist(), dim ** -0.5, capacity=128)
+        R.within(out, want, bound, "step")
+        R.within(tracker.weights, before + w, wb + 2.0 ** -23 * (before + w), "weights")
+
+    for _ in range(steps):
+        step()
+    kept = []
+    for b, n in enumerate(lengths.tolist()):
+        for h in range(heads):
+            w, t = tracker.weights[b, h].tolist(), tracker.tokens[b, h].tolist()
+            slots = list(range(min(n, keep)))
+            for src, dst in R.evict_ref(w, t, n, int(seen[b]), keep, 4, 8):
+                slots[dst] = src
+            kept.append([t[i] for i in slots])
+    evict_by_weight(cache, table, lengths, tracker, seen, keep, first=4, recent=8)
+    lengths.clamp_(max=keep)
+    for b, n in enumerate(lengths.tolist()):
+        for h in range(heads):
+            assert tracker.tokens[b, h, :n].tolist() == kept[b * heads + h]
+            assert set(range(4)) | set(range(int(seen[b]) - 8, int(seen[b]))) <= set(kept[b * heads + h])
+    for _ in range(steps):
+        step()
+
+
+def test_step_captured_and_replayed(dev):
+    """One captured graph of a whole step (append, attention with weights, eviction), replayed among eager work and equal
+    to the eager calls on copies every time."""
+    heads, H, dim, page, keep = 2, 6, 128, 16, 64
+    cache, table, n = _cache(dev, 60, 4, dim, heads, page, [64, 40])
+    table = torch.arange(12, dtype=torch.int32, device=dev).view(2, 6)[:, :5].contiguous()
+    tracker = SlotTracker(2, heads, 80, device=dev)
+    tracker.weights.uniform_(generator=_gen(dev, 61))
+    tracker.tokens.copy_(torch.arange(80, device=dev).expand(2, heads, 80))
+    lengths, seen = n.clone(), n.clone()
+    qkv = torch.randn(2, 1, H + 2 * heads, dim, device=dev, generator=_gen(dev, 62)).to(torch.bfloat16)
+
+    def step(c, t, ln, sn):
+        append_tokens(c, qkv[:, :, H:H + heads], qkv[:, :, H + heads:], table, ln, tracker=t, token=sn)
+        ln.add_(1)
+        sn.add_(1)
+        out = paged_attention(qkv[:, :, :H], c, table, ln, dim ** -0.5, tracker=t)
+        evict_by_weight(c, table, ln, t, sn, keep, first=2, recent=4)
+        ln.clamp_(max=keep)
+        return out
+
+    def copy():
+        c = PagedKVCache.from_tensors(cache.quant, *(x.clone() for x in (cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale)))
+        return c, SlotTracker.from_tensor(tracker.storage.clone()), lengths.clone(), seen.clone()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*copy())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(cache, tracker, lengths, seen)
+    for rep in range(4):
+        qkv.copy_(torch.randn(qkv.shape, device=dev, generator=_gen(dev, 70 + rep)))
+        c, t, ln, sn = copy()
+        want = step(c, t, ln, sn)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), f"replay {rep}"
+        assert torch.equal(tracker.storage, t.storage) and torch.equal(lengths, ln)
+        for x, y in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), (c.k_codes, c.k_scale, c.v_codes, c.v_scale)):
+            assert torch.equal(x, y)

@@ -1,0 +1,199 @@
+"""Causal prompt attention over packed sequences on the GPU against the plain 64-bit form (paged_ref.py)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from aetherkv.prompt import prompt_attention
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _cu(lens):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+def _inputs(dev, seed, dtype, dim, H, hk, lq, lk, pad=0, gain=1.0):
+    nq, nk = sum(lq) + pad, sum(lk) + pad
+    if lq == lk:  # one projection's rows
+        qkv = torch.randn(nq, H + 2 * hk, dim, device=dev, generator=_gen(dev, seed))
+        qkv[:, :H] *= gain
+        qkv = qkv.to(dtype)
+        return qkv[:, :H], qkv[:, H:H + hk], qkv[:, H + hk:]
+    q = (torch.randn(nq, H, dim, device=dev, generator=_gen(dev, seed)) * gain).to(dtype)
+    kv = torch.randn(nk, 2, hk, dim, device=dev, generator=_gen(dev, seed + 1)).to(dtype)
+    return q, kv[:, 0], kv[:, 1]
+
+
+def _check(dev, dtype, dim, H, hk, lq, lk=None, sink=False, pad=0, seed=0, gain=1.0, scale=None):
+    lk = lq if lk is None else lk
+    q, k, v = _inputs(dev, seed, dtype, dim, H, hk, lq, lk, pad, gain)
+    cq, ck = _cu(lq), _cu(lk)
+    sk = torch.randn(H, device=dev, generator=_gen(dev, seed + 2)) if sink else None
+    scale = dim ** -0.5 if scale is None else scale
+    out, lse = prompt_attention(q, k, v, torch.tensor(cq, dtype=torch.int32, device=dev), scale,
+                                cu_seqlens_k=None if lq == lk else torch.tensor(ck, dtype=torch.int32, device=dev), sink=sk, return_lse=True)
+    want, bound, wl, lb = R.prompt_attention_ref(q.cpu(), k.cpu(), v.cpu(), cq, ck, scale, None if sk is None else sk.cpu())
+    R.within(out, want, bound, "out")
+    got = lse.double().cpu()
+    none = wl == -math.inf
+    assert torch.equal(got == -math.inf, none)
+    R.within(got[~none], wl[~none], lb[~none], "lse")
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 15, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200])
+def test_prompt_lengths(dev, dtype, dim, n):
+    _check(dev, dtype, dim, 2, 1, [n], seed=n)
+
+
+@pytest.mark.parametrize("H,hk", [(1, 1), (3, 3), (12, 4), (12, 1), (16, 2), (10, 2)])
+def test_prompt_head_layouts(dev, H, hk):
+    _check(dev, torch.bfloat16, 128, H, hk, [70, 33], sink=True, seed=H)
+
+
+@pytest.mark.parametrize("lens", [[0], [0, 5, 0, 0, 130, 1], [1] * 70, [300, 1, 64, 65], [17, 200, 129]])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_prompt_packed(dev, lens, pad):
+    if sum(lens) + pad == 0:
+        out = prompt_attention(*(torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev) for _ in range(3)), torch.zeros(2, dtype=torch.int32, device=dev), 0.1)
+        assert out.shape == (0, 2, 64)
+        return
+    out, lse = _check(dev, torch.bfloat16, 64, 4, 2, lens, pad=pad, seed=len(lens))
+    if pad:
+        assert not out[-pad:].any() and (lse[-pad:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("lq,lk", [([1], [200]), ([5, 64, 1], [6, 300, 129]), ([130], [131]), ([64], [64 + 1000]), ([40, 7], [20, 0]), ([100, 3], [30, 3])])
+@pytest.mark.parametrize("sink", [False, True])
+def test_prompt_chunks(dev, lq, lk, sink):
+    """More keys than queries, and fewer: the first queries then see nothing."""
+    out, _ = _check(dev, torch.float16, 128, 4, 2, lq, lk, sink=sink, seed=sum(lk))
+    if lq == [40, 7]:
+        assert not out[:20].any() and not out[40:].any()
+
+
+def test_prompt_long(dev):
+    _check(dev, torch.bfloat16, 128, 1, 1, [1300], seed=5)
+    _check(dev, torch.float16, 64, 2, 1, [900, 513], seed=6)
+
+
+def test_prompt_peaked_flat_and_negative_scale(dev):
+    _check(dev, torch.float16, 64, 2, 2, [150], gain=20.0)
+    _check(dev, torch.bfloat16, 128, 2, 2, [150], scale=0.0)
+    _check(dev, torch.bfloat16, 64, 2, 2, [150], scale=-0.3, sink=True)
+
+
+def test_prompt_rows_behind_the_last_are_left(dev):
+    q, k, v = _inputs(dev, 8, torch.bfloat16, 64, 4, 2, [60], [60], pad=10)
+    cu = torch.tensor([0, 60], dtype=torch.int32, device=dev)
+    out = torch.full((70, 4, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    assert prompt_attention(q, k, v, cu, 0.125, out=out).data_ptr() == out.data_ptr()
+    assert (out[60:] == 7).all()
+    assert torch.equal(out[:60], prompt_attention(q[:60], k[:60], v[:60], cu, 0.125))
+    mid = torch.tensor([5, 20, 20, 50], dtype=torch.int32, device=dev)  # rows before the first too
+    out.fill_(7.0)
+    prompt_attention(q, k, v, mid, 0.125, out=out)
+    assert (out[:5] == 7).all() and (out[50:] == 7).all()
+    want, bound, _, _ = R.prompt_attention_ref(q.cpu(), k.cpu(), v.cpu(), [5, 20, 20, 50], [5, 20, 20, 50], 0.125)
+    R.within(out[5:50], want[5:50], bound[5:50], "out")
+
+
+@pytest.mark.parametrize("bad", [NAN, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_masked_places_do_not_matter(dev, bad, dtype):
+    """Entries that a row does not see may hold anything: later tokens, other sequences, rows behind the last."""
+    q, k, v = (x.clone() for x in _inputs(dev, 9, dtype, 128, 2, 1, [100, 90], [100, 90], pad=20))
+    cu = torch.tensor([0, 100, 190], dtype=torch.int32, device=dev)
+    clean, clean_lse = prompt_attention(q, k, v, cu, 0.09, return_lse=True)
+    for x in (k, v):
+        x[190:] = bad
+        x[60, 0, ::7] = bad
+        x[180] = bad
+    got, lse = prompt_attention(q, k, v, cu, 0.09, return_lse=True)
+    for rows in (slice(0, 60), slice(100, 180)):
+        assert torch.equal(got[rows], clean[rows]) and torch.equal(lse[rows], clean_lse[rows])
+    if bad != bad:
+        assert got[60:100].isnan().any(-1).all() and got[180:190].isnan().all()
+
+
+def test_prompt_infinite_value_reaches_the_rows_that_see_it(dev):
+    q, k, v = (x.clone() for x in _inputs(dev, 10, torch.bfloat16, 128, 2, 1, [100], [100]))
+    cu = torch.tensor([0, 100], dtype=torch.int32, device=dev)
+    clean = prompt_attention(q, k, v, cu, 0.09)
+    v[70, 0, 5], v[40, 0, 6] = math.inf, -math.inf
+    got = prompt_attention(q, k, v, cu, 0.09)
+    assert (got[70:, :, 5] == math.inf).all() and (got[40:, :, 6] == -math.inf).all()
+    got[70:, :, 5], got[40:, :, 6] = clean[70:, :, 5], clean[40:, :, 6]
+    assert torch.equal(got, clean)
+
+
+def test_prompt_strides_streams_and_devices(dev):
+    q, k, v = _inputs(dev, 11, torch.bfloat16, 128, 4, 2, [130, 40], [130, 40])
+    cu = torch.tensor([0, 130, 170], dtype=torch.int32, device=dev)
+    want = prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, 0.09)
+    assert torch.equal(prompt_attention(q, k, v, cu.long(), 0.09), want)
+    heads_first = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    assert torch.equal(prompt_attention(*heads_first, cu, 0.09), want)
+    odd = [torch.empty(x.numel() + 1, dtype=x.dtype, device=dev)[1:].view(x.shape).copy_(x) for x in (q, k, v)]
+    assert torch.equal(prompt_attention(*odd, cu, 0.09), want)
+    shared = k[:, :1].expand(-1, 2, -1)  # one head under two names
+    assert torch.equal(prompt_attention(q, shared, v, cu, 0.09), prompt_attention(q, shared.contiguous(), v, cu, 0.09))
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(s[i % 2]):
+            outs.append(prompt_attention(q, k, v, cu, 0.09))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_prompt_captured_and_replayed(dev):
+    q, k, v = (x.clone() for x in _inputs(dev, 12, torch.bfloat16, 128, 6, 2, [100, 60], [100, 60], pad=8))
+    cu = torch.tensor([0, 100, 160], dtype=torch.int32, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        prompt_attention(q, k, v, cu, 0.09, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = prompt_attention(q, k, v, cu, 0.09, return_lse=True)
+    for rep, lens in enumerate(([0, 100, 160], [0, 7, 168], [0, 168, 168], [3, 3, 90])):
+        q.copy_(torch.randn(q.shape, device=dev, generator=_gen(dev, rep)))
+        cu.copy_(torch.tensor(lens, dtype=torch.int32))
+        want, wl = prompt_attention(q, k, v, cu, 0.09, return_lse=True)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, wl), f"replay {rep}"
+
+
+def test_prompt_refusals(dev):
+    q, k, v = _inputs(dev, 13, torch.bfloat16, 128, 4, 2, [50], [50])
+    cu = torch.tensor([0, 50], dtype=torch.int32, device=dev)
+    for args in ((q.float(), k, v, cu), (q, k.half(), v, cu), (q[:, :3], k, v, cu), (q, k, v[:, :1], cu), (q[:40], k, v, cu), (q, k, v, cu[:1]), (q, k, v, cu.cpu()),
+                 (q, k, v, cu.float()), (q[..., :96], k[..., :96], v[..., :96], cu), (q[0], k, v, cu)):
+        with pytest.raises(RuntimeError):
+            prompt_attention(*args, 0.09)
+    with pytest.raises(RuntimeError):
+        prompt_attention(q, k, v, cu, 0.09, sink=torch.zeros(3, device=dev))
+    with pytest.raises(RuntimeError):
+        prompt_attention(q, k, v, cu, 0.09, out=torch.empty(50, 4, 64, dtype=torch.bfloat16, device=dev))
+    with pytest.raises(RuntimeError):
+        prompt_attention(q, k, v, cu, 0.09, cu_seqlens_k=torch.zeros(3, dtype=torch.int32, device=dev))
