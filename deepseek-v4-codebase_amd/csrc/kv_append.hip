@@ -96,7 +96,7 @@ int check_pool(const char* who, void* k_codes, float* k_scale, void* v_codes, fl
   if (B < 0 || heads < 1 || pages < 0 || max_pages < 0)
     return fail(AEKV_ERR_SHAPE, "%s: B=%lld heads=%lld pages=%lld max_pages=%lld", who, (long long)B, (long long)heads,
                 (long long)pages, (long long)max_pages);
-  if (pages > 0x7fffffff || heads > 65535 || max_pages * page_size > 0x7fffffff || B > 0x7fffffff)
+  if (pages > 0x7fffffff || heads > 65535 || max_pages * page_size > 0x7fff0000 || B > 0x7fffffff)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: pages=%lld heads=%lld slots=%lld B=%lld exceed 31 bits (65535 heads)", who,
                 (long long)pages, (long long)heads, (long long)(max_pages * page_size), (long long)B);
   if (pages > 0 && (!k_codes || !k_scale || !v_codes || !v_scale)) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);

@@ -4,8 +4,28 @@
 // h / (H / heads):  l_j = scale q . K_j,  p_j = exp(l_j) / (sum exp(l) + exp(sink_h)),  out = sum_j p_j V_j.
 // With the codec's orthogonal rotation R = c Had diag (K_j = s_j R^T codes_j) both products stay in the rotated domain:
 //   q . K_j = s_j (R q) . codes_j        sum_j p_j V_j = R^T sum_j p_j s_j codes_j
-// so a query is rotated once, an output is rotated back once, and a cached row costs its codes and one scale.
-// weights[b, KV head, j] += the sum of p_j over the group's heads and the T tokens.
+// so a query is rotated once, an output is rotated back once, and a cached row costs its codes and one scale: the kernel
+// is bound by reading them, 2 (D bits / 8 + 4) bytes per slot and KV head.
+//
+// Work split.  The T tokens x G heads of a KV head's group are rows; a workgroup takes 16 MT of them and one piece of the
+// sequence, its four waves alternate over steps of 32 slots, and their states are merged through LDS.  Where a launch has
+// too few workgroups the sequence is split over n_split pieces, merged by a second kernel.
+//
+// Matrix layout (v_mfma_f32_16x16x32: A lane l holds A[l % 16][8 (l / 16) + j], B lane l holds B[8 (l / 16) + j][l % 16],
+// D lane l register i holds D[4 (l / 16) + i][l % 16]), g = l / 16:
+//   S^T = K Q^T: m = slot, n = row.  The order of the dims within a product is free, so a lane reads the D / 4 contiguous
+//     codes [g D / 4, (g + 1) D / 4) of its slot and product c takes 8 of them; the query has them in the same places.
+//     The codes are exact in fp16; the rotated query, scaled to the top of fp16's range, goes in as two fp16 parts (22
+//     bits), so that a logit has fp32's accuracy, which the accumulated weights need.
+//   O^T += V^T P^T: m = dim, n = row, k = slot: lane g holds slots 4 g + i and 16 + 4 g + i, exactly the slots of its own
+//     scores, so the weights need no data movement.  A lane reads the D / 16 codes of dims [n D / 16, ..) of those eight
+//     slots, and product e takes one dim of each: the transpose is within the lane.  The weights, times their slots'
+//     scales, go in as two bf16 parts (17 bits; the scales' range is fp32's, which fp16 has not), the codes as bf16 with
+//     an offset that makes them one bit operation each; a product with ones gives the sum that takes the offset out.
+//   A lane ends with D / 4 contiguous dims of one row, so both rotations are D / 4-point butterflies in the lane and two
+//   exchanges between lanes.
+#include <type_traits>
+
 #include "paged_cache.h"
 #include "tq_device.h"
 
@@ -13,6 +33,13 @@ namespace aekv {
 namespace {
 
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kStep = 32, kRound = kStep * kWaves;
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 struct PagedArgs {
   PagePool pool;
@@ -22,138 +49,644 @@ struct PagedArgs {
   const float* diag;
   const float* sink;                 // [H] or null
   float* weights;                    // [B, heads, capacity] or null
-  float* rot;                        // [B, T, H, D]: rotated queries (with weights)
-  float* lse;                        // [B, T, H] (with weights)
+  float* lse;                        // [B, T, H], log2 units, inf for a sum of 0 (with weights)
+  float* part;                       // [B, T, H, n_split, D + 4]: max, sum (log2 units), 2 pad, rotated output
   void* out;                         // [B, T, H, D]
+  int32_t reach;                     // slots of a sequence that can be seen: the table's, or the tracker's capacity
   int64_t capacity;
-  int32_t T, H;
-  float scale, wscale;
+  int32_t T, H, G, rows, row_blocks, n_split;
+  float scale2, wscale;              // softmax scale * log2(e), fp32(D^-1/2)
 };
 
+// Slots of sequence b that its last token sees.
+__device__ __forceinline__ int32_t newest_sees(const PagedArgs& a, int64_t b) { return max(min(a.lengths[b], a.reach), 0); }
+// The piece length of a sequence of n slots: whole rounds of the workgroup's waves.
+__device__ __forceinline__ int32_t piece_slots(int32_t n, int32_t n_split) {
+  const int32_t per = (n + n_split - 1) / n_split;
+  return max((per + kRound - 1) / kRound * kRound, kRound);
+}
+
+// Butterflies of a vector whose dims [g D / 4, (g + 1) D / 4) this lane holds (g = lane / 16).
+template <int N>
+__device__ __forceinline__ void rotate_lane(float (&a)[N], int lane) {
+#pragma unroll
+  for (int h = 1; h < N; h <<= 1)
+#pragma unroll
+    for (int blk = 0; blk < N; blk += 2 * h)
+#pragma unroll
+      for (int i = 0; i < h; ++i) {
+        const float x = a[blk + i], y = a[blk + h + i];
+        a[blk + i] = x + y;
+        a[blk + h + i] = x - y;
+      }
+  const float s16 = (lane & 16) ? -1.0f : 1.0f, s32 = (lane & 32) ? -1.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = fmaf(a[i], s16, xor_lane<16>(a[i]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = fmaf(a[i], s32, xor_lane<32>(a[i]));
+}
+
+// Place of element j of a product's operand among its 8 codes: the order in which unpacking a word of nibbles leaves them
+// (halves of a register hold nibbles i and i + 4), or that of the bytes.
 template <int BITS>
-__device__ __forceinline__ float code_at(const uint8_t* row, int d) {
-  if constexpr (BITS == 8) return static_cast<float>(static_cast<int8_t>(row[d]));
-  const int x = (row[d >> 1] >> (4 * (d & 1))) & 15;
-  return static_cast<float>((x ^ 8) - 8);
+constexpr int code_place(int j) {
+  return BITS == 4 ? (j & 1) * 4 + (j >> 1) : j;
 }
 
-__device__ __forceinline__ int32_t visible_slots(const PagedArgs& a, int64_t b, int32_t t) {
-  const int64_t cap = a.weights ? min<int64_t>(table_slots(a.pool), a.capacity) : table_slots(a.pool);
-  const int64_t n = min<int64_t>(a.lengths[b], cap);
-  return static_cast<int32_t>(max<int64_t>(n - a.T + 1 + t, 0));
-}
-
-// y[d] = c sum_e (-1)^popcount(d & e) x[e]
-template <int D>
-__device__ __forceinline__ float wht_at(const float* x, int d, float c) {
-  float s = 0.0f;
-  for (int e = 0; e < D; ++e) s += (__popc(d & e) & 1) ? -x[e] : x[e];
-  return s * c;
-}
-
-template <int DT, int D, int BITS>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
-  __shared__ float xs[D], qr[D], ps[4][64], acc[4][D], ml[4][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int32_t h = blockIdx.x, t = blockIdx.y;
-  const int64_t b = blockIdx.z;
-  const int32_t kh = h / (a.H / a.pool.heads);
-  if (tid < D) {
-    const int64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + tid;
-    const uint16_t u = static_cast<const uint16_t*>(a.q)[at];
-    xs[tid] = (DT == AEKV_BF16 ? bf16_to_f32(u) : f16_to_f32(u)) * a.diag[tid];
+// 8 codes as exact fp16.  Nibbles in two's complement: xor 8 makes them 0 .. 15, 0x6400 | u is 1024 + u and 0x6400 | 16 u
+// is 1024 + 16 u in fp16; bytes likewise, offset by 128.
+template <int BITS>
+__device__ __forceinline__ f16x8_t codes_f16(const uint32_t* w) {
+  uint4 r;
+  if constexpr (BITS == 4) {
+    const f16x2_t off = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+    const f16x2_t off16 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+    const f16x2_t s16 = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    const uint32_t v = w[0], u = w[0] >> 8;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, (v & 0x000F000Fu) ^ 0x64086408u) + off);
+    r.y = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (v & 0x00F000F0u) ^ 0x64806480u), s16, off16));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, (u & 0x000F000Fu) ^ 0x64086408u) + off);
+    r.w = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (u & 0x00F000F0u) ^ 0x64806480u), s16, off16));
+  } else {
+    const f16x2_t off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const uint32_t v = w[0] ^ 0x80808080u, u = w[1] ^ 0x80808080u;
+    auto two = [&](uint32_t x, uint32_t sel) {  // bytes (b, 0x64, b', 0x64)
+      return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, sel)) + off);
+    };
+    r.x = two(v, 0x07010700u);
+    r.y = two(v, 0x07030702u);
+    r.z = two(u, 0x07010700u);
+    r.w = two(u, 0x07030702u);
   }
-  __syncthreads();
-  if (tid < D) qr[tid] = wht_at<D>(xs, tid, a.wscale);
-  __syncthreads();
-  const int64_t orow = (b * a.T + t) * a.H + h;
-  if (a.weights && tid < D) a.rot[orow * D + tid] = qr[tid];
-  const int32_t n = visible_slots(a, b, t);
-  float m = kNegInf, l = 0.0f, o[D / 64];
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
-  for (int base = 64 * wave; base < n; base += 256) {
-    const int j = base + lane;
-    const int64_t row = j < n ? cache_row(a.pool, b, kh, j) : -1;
-    float s = kNegInf, vs = 0.0f;
-    if (row >= 0) {
-      const uint8_t* kr = a.pool.k_codes + row * (D * BITS / 8);
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot += qr[d] * code_at<BITS>(kr, d);
-      s = dot * a.pool.k_scale[row] * a.scale;
-      vs = a.pool.v_scale[row];
-    }
-    const float m2 = fmaxf(m, wave_max(s));
-    const float r = m2 == kNegInf ? 1.0f : expf(m - m2);
-    const float p = s == kNegInf ? 0.0f : expf(s - m2);
-    l = l * r + wave_sum(p);
-    m = m2;
-    ps[wave][lane] = row >= 0 ? p * vs : 0.0f;
-    __builtin_amdgcn_wave_barrier();
-    for (int i = 0; i < D / 64; ++i) o[i] *= r;
-    for (int k = 0; k < 64; ++k) {
-      const int64_t vrow = __shfl(row, k);
-      if (vrow < 0) continue;
-      for (int i = 0; i < D / 64; ++i) o[i] += ps[wave][k] * code_at<BITS>(a.pool.v_codes + vrow * (D * BITS / 8), lane + 64 * i);
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-  for (int i = 0; i < D / 64; ++i) acc[wave][lane + 64 * i] = o[i];
-  if (lane == 0) ml[wave][0] = m, ml[wave][1] = l;
-  __syncthreads();
-  float M = a.sink ? a.sink[h] : kNegInf, L = M == kNegInf ? 0.0f : 1.0f;
-  float x = 0.0f;
-  for (int w = 0; w < 4; ++w) {
-    if (ml[w][1] == 0.0f) continue;  // (NaN alone leaves a maximum of -inf, and a sum that says so)
-    const float M2 = fmaxf(M, ml[w][0]);
-    const float r = M == kNegInf ? 0.0f : expf(M - M2), f = expf(ml[w][0] - M2);
-    L = L * r + ml[w][1] * f;
-    x = x * r + (tid < D ? acc[w][tid] : 0.0f) * f;
-    M = M2;
-  }
-  __syncthreads();
-  if (tid < D) xs[tid] = L > 0.0f ? x / L : (L == 0.0f ? 0.0f : L);
-  __syncthreads();
-  if (tid < D) {
-    const float y = wht_at<D>(xs, tid, a.wscale) * a.diag[tid];
-    static_cast<uint16_t*>(a.out)[orow * D + tid] = DT == AEKV_BF16 ? static_cast<uint16_t>(pack_bf16x2(y, 0.0f)) : static_cast<uint16_t>(f32_to_f16_bits(y));
-  }
-  if (a.weights && tid == 0) a.lse[orow] = M + logf(L);
+  return __builtin_bit_cast(f16x8_t, r);
 }
 
 template <int D, int BITS>
-__global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int32_t kh = blockIdx.y, g = a.H / a.pool.heads;
-  const int64_t b = blockIdx.z;
-  if (j >= visible_slots(a, b, a.T - 1)) return;
-  const int64_t row = cache_row(a.pool, b, kh, j);
-  if (row < 0) return;
-  const uint8_t* kr = a.pool.k_codes + row * (D * BITS / 8);
-  float sum = 0.0f;
-  for (int32_t t = 0; t < a.T; ++t) {
-    if (j >= visible_slots(a, b, t)) continue;
-    for (int32_t i = 0; i < g; ++i) {
-      const int64_t orow = (b * a.T + t) * a.H + kh * g + i;
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot += a.rot[orow * D + d] * code_at<BITS>(kr, d);
-      sum += expf(dot * a.pool.k_scale[row] * a.scale - a.lse[orow]);
+struct PagedGeom {
+  static constexpr int kRowBytes = D * BITS / 8;
+  static constexpr int kKB = kRowBytes / 4;   // bytes of a slot's K row per lane
+  static constexpr int kKW = kKB / 4;         // words
+  static constexpr int kVB = kRowBytes / 16;  // bytes of a slot's V row per lane (2, 4 or 8)
+  static constexpr int kNC = D / 32;          // K products per 16 slots
+  static constexpr int kNE = D / 16;          // V products per 32 slots: codes per lane and slot
+  static constexpr int kWords = kVB > 4 ? 2 : 1;
+  // what the bf16 form of a code is more than the code: 16 + 8 for nibbles (0x4180 | 8 u is 16 + u), 128 for bytes
+  static constexpr float kBias = BITS == 4 ? 24.0f : 128.0f;
+};
+
+// What a step of 32 slots loads.
+template <int D, int BITS>
+struct StepData {
+  using G = PagedGeom<D, BITS>;
+  uint32_t k[2][G::kKW];
+  f32x4_t ks[2], vs[2];
+  uint32_t v[8][G::kWords];
+};
+
+// The wave's page ids: lane 2 i + k holds that of tile k (16 slots) of its i-th step from `first`; -1 where a tile has none.
+__device__ __forceinline__ int32_t load_pages(const PagedArgs& a, int64_t b, int32_t first, int32_t end, int lane) {
+  const int64_t slot = static_cast<int64_t>(first) + kRound * (lane >> 1) + 16 * (lane & 1);
+  int32_t page = -1;
+  if (slot < end) page = a.pool.table[b * a.pool.max_pages + (slot >> a.pool.page_shift)];
+  return page >= 0 && page < a.pool.pages ? page : -1;
+}
+
+template <int D, int BITS, bool WITH_V>
+__device__ __forceinline__ void load_step(const PagedArgs& a, int32_t kh, int32_t slot, int32_t p0, int32_t p1, int lane,
+                                          StepData<D, BITS>& s) {
+  using G = PagedGeom<D, BITS>;
+  const int n = lane & 15, g = lane >> 4;
+  const int32_t in_page = (1 << a.pool.page_shift) - 1;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int32_t page = k ? p1 : p0;  // wave-uniform
+    // (a tile without a page reads the pool's first row, and is masked)
+    const int64_t row = page < 0 ? 0 : ((static_cast<int64_t>(page) * a.pool.heads + kh) << a.pool.page_shift) + ((slot + 16 * k) & in_page);
+    const uint8_t* kr = a.pool.k_codes + row * G::kRowBytes + (n * G::kRowBytes + g * G::kKB);
+    if constexpr (G::kKW == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(kr);
+      s.k[k][0] = w.x, s.k[k][1] = w.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < G::kKW / 4; ++i) {
+        const uint4 w = reinterpret_cast<const uint4*>(kr)[i];
+        s.k[k][4 * i] = w.x, s.k[k][4 * i + 1] = w.y, s.k[k][4 * i + 2] = w.z, s.k[k][4 * i + 3] = w.w;
+      }
+    }
+    s.ks[k] = *reinterpret_cast<const f32x4_t*>(a.pool.k_scale + row + 4 * g);
+    if constexpr (WITH_V) {
+      s.vs[k] = *reinterpret_cast<const f32x4_t*>(a.pool.v_scale + row + 4 * g);
+      const uint8_t* vr = a.pool.v_codes + row * G::kRowBytes + (4 * g * G::kRowBytes + n * G::kVB);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (G::kVB == 2) s.v[4 * k + i][0] = *reinterpret_cast<const uint16_t*>(vr + i * G::kRowBytes);
+        else if constexpr (G::kVB == 4) s.v[4 * k + i][0] = *reinterpret_cast<const uint32_t*>(vr + i * G::kRowBytes);
+        else {
+          const uint2 w = *reinterpret_cast<const uint2*>(vr + i * G::kRowBytes);
+          s.v[4 * k + i][0] = w.x, s.v[4 * k + i][1] = w.y;
+        }
+      }
     }
   }
-  a.weights[(b * a.pool.heads + kh) * a.capacity + j] += sum;
+}
+
+// Dim e of the eight slots as bf16 with the offset kBias.
+template <int D, int BITS>
+__device__ __forceinline__ bf16x8_t values_bf16(const uint32_t (&v)[8][PagedGeom<D, BITS>::kWords], int e) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BITS == 4) {
+      // half-words of two slots side by side, then the nibble moved to the mantissa's top bits
+      const uint32_t t = __builtin_amdgcn_perm(v[2 * i + 1][0], v[2 * i][0], (e & 4) ? 0x07060302u : 0x05040100u);
+      const int place = 4 * (e & 3);
+      const uint32_t m = place == 0 ? t << 3 : t >> (place - 3);
+      r[i] = (m & 0x00780078u) ^ 0x41C041C0u;  // 0x4180 | (n ^ 8) << 3
+    } else {
+      const uint32_t x = v[2 * i][e >> 2], y = v[2 * i + 1][e >> 2];
+      const int sh = 8 * (e & 3);
+      r[i] = pack_bf16x2(static_cast<float>((x >> sh) & 255u), static_cast<float>((y >> sh) & 255u));
+    }
+  }
+  return __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// A row's query, rotated, in two fp16 parts in the products' order; *factor takes a score to a logit in log2 units.
+template <int DT, int D, int BITS>
+__device__ __forceinline__ void query_parts(const PagedArgs& a, int64_t b, int32_t kh, int32_t row, bool in, int lane,
+                                            f16x8_t (&hi)[D / 32], f16x8_t (&lo)[D / 32], float* factor) {
+  constexpr int N = D / 4;
+  const int g = lane >> 4;
+  float x[N];
+  const int32_t t = in ? row / a.G : 0, h = kh * a.G + (in ? row - t * a.G : 0);
+  const int64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + g * N;
+  const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    const uint4 w = qp[i];
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[8 * i + 2 * j] = DT == AEKV_BF16 ? bf16_to_f32(u[j] & 0xffffu) : f16_to_f32(u[j] & 0xffffu);
+      x[8 * i + 2 * j + 1] = DT == AEKV_BF16 ? bf16_to_f32(u[j] >> 16) : f16_to_f32(u[j] >> 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    const f32x4_t d = *reinterpret_cast<const f32x4_t*>(a.diag + g * N + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] = in ? x[4 * i + j] * d[j] : 0.0f;
+  }
+  rotate_lane<N>(x, lane);
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+  m = fmaxf(m, xor_lane<16>(m));
+  m = fmaxf(m, xor_lane<32>(m));
+  // the largest to [2^13, 2^14): the second part of an element above 2^-27 of it is then a normal fp16 number
+  const int e = m > 0.0f && m < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(m) : 0;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = __builtin_amdgcn_ldexpf(x[8 * c + code_place<BITS>(j)], e);
+      hi[c][j] = static_cast<_Float16>(y);
+      lo[c][j] = static_cast<_Float16>(y - static_cast<float>(hi[c][j]));
+    }
+  *factor = __builtin_amdgcn_ldexpf(a.wscale * a.scale2, -e);
+}
+
+// Scores of the step's 2 x 16 slots against 16 rows, in log2 units: slot 16 k + 4 g + i, row lane % 16.
+template <int D, int BITS>
+__device__ __forceinline__ void score_step(const f16x8_t (&kc)[2][D / 32], const f32x4_t (&ks)[2], const f16x8_t (&hi)[D / 32],
+                                           const f16x8_t (&lo)[D / 32], float factor, f32x4_t (&x)[2]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[k][c], lo[c], s, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[k][c], hi[c], s, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[k][i] = s[i] * (ks[k][i] * factor);
+  }
+}
+
+template <int DT, int N>
+__device__ __forceinline__ void store_row(void* out, int64_t at, const float (&y)[N]) {
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i)
+    w[i] = DT == AEKV_BF16 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : (f32_to_f16_bits(y[2 * i]) | (f32_to_f16_bits(y[2 * i + 1]) << 16));
+  uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) p[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+template <int DT, int D, int BITS, int MT>
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs a) {
+  using G = PagedGeom<D, BITS>;
+  constexpr int N = D / 4;
+  __shared__ __align__(16) float s_o[kWaves - 1][MT * N][64];
+  __shared__ float s_ml[kWaves - 1][MT][2][64];
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroups: pieces innermost, then row blocks, then KV heads, then sequences
+  uint32_t wg = blockIdx.x;
+  const int32_t split = static_cast<int32_t>(wg % a.n_split);
+  wg /= a.n_split;
+  const int32_t rb = static_cast<int32_t>(wg % a.row_blocks);
+  wg /= a.row_blocks;
+  const int32_t kh = static_cast<int32_t>(wg % a.pool.heads);
+  const int64_t b = wg / a.pool.heads;
+
+  const int32_t n = newest_sees(a, b);
+  const int32_t piece = piece_slots(n, a.n_split);
+  const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
+  if (split > 0 && p0 >= p1) return;  // (the merge knows how many pieces a sequence has)
+
+  f16x8_t qhi[MT][D / 32], qlo[MT][D / 32];
+  float factor[MT], m[MT], l[MT];
+  int32_t row[MT], sees[MT], sees_all = 0x7fffffff;
+  f32x4_t o[MT][G::kNE], ones_sum[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    row[t] = (rb * MT + t) * 16 + (lane & 15);
+    const bool in = row[t] < a.rows;
+    query_parts<DT, D, BITS>(a, b, kh, row[t], in, lane, qhi[t], qlo[t], &factor[t]);
+    sees[t] = in ? max(n - a.T + 1 + row[t] / a.G, 0) : n;
+    m[t] = kNegInf, l[t] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < G::kNE; ++e) o[t][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    ones_sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  sees_all = max(n - a.T + 1 + rb * MT * 16 / a.G, 0);  // the fewest that a row of the block sees
+
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
+  int32_t pages = -1;
+  StepData<D, BITS> buf[2];
+  const int32_t first = p0 + kStep * wave;
+  const int n_steps = first < p1 ? (p1 - first + kRound - 1) / kRound : 0;
+  uint32_t bad[2] = {0, 0};  // bit k: tile k of the buffered step has no page
+  auto load = [&](int i, auto which) {
+    constexpr int w = decltype(which)::value;
+    if (i >= n_steps) return;
+    if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+    const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
+    bad[w] = (g0 < 0 ? 1u : 0u) | (g1 < 0 ? 2u : 0u);
+    load_step<D, BITS, true>(a, kh, first + kRound * i, g0, g1, lane, buf[w]);
+  };
+  auto compute = [&](int i, auto which) {
+    constexpr int w = decltype(which)::value;
+    const StepData<D, BITS>& s = buf[w];
+    const int32_t base = first + kRound * i;
+    f16x8_t kc[2][D / 32];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) kc[k][c] = codes_f16<BITS>(&s.k[k][c * BITS / 4]);
+    bf16x8_t phi[MT], plo[MT];
+    const bool whole = bad[w] == 0 && base + kStep <= sees_all;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      f32x4_t x[2];
+      score_step<D, BITS>(kc, s.ks, qhi[t], qlo[t], factor[t], x);
+      bool hide[2][4] = {};
+      if (!whole)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hide[k][j] = ((bad[w] >> k) & 1u) || base + 16 * k + 4 * g + j >= sees[t];
+            x[k][j] = hide[k][j] ? kNegInf : x[k][j];
+          }
+      float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+      top = fmaxf(top, xor_lane<16>(top));
+      top = fmaxf(top, xor_lane<32>(top));
+      if (__builtin_amdgcn_ballot_w64(top > m[t])) {
+        const float up = fmaxf(m[t], top);
+        const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[t] - up);
+        l[t] *= r;
+#pragma unroll
+        for (int e = 0; e < G::kNE; ++e) o[t][e] *= r;
+        ones_sum[t] *= r;
+        m[t] = up;
+      }
+      const float nm = m[t] == kNegInf ? 0.0f : -m[t];
+      float c[2][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = __builtin_amdgcn_exp2f(x[k][j] + nm);
+          l[t] += p;
+          c[k][j] = p * s.vs[k][j];
+          if (!whole) c[k][j] = hide[k][j] ? 0.0f : c[k][j];  // (whatever a hidden slot's scale is)
+        }
+      uint32_t h[4], r[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float c0 = c[k][2 * j], c1 = c[k][2 * j + 1];
+          const uint32_t u = pack_bf16x2(c0, c1);
+          h[2 * k + j] = u;
+          r[2 * k + j] = pack_bf16x2(c0 - bf16_to_f32(u), c1 - __builtin_bit_cast(float, u & 0xffff0000u));
+        }
+      phi[t] = __builtin_bit_cast(bf16x8_t, make_uint4(h[0], h[1], h[2], h[3]));
+      plo[t] = __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
+      ones_sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, phi[t], ones_sum[t], 0, 0, 0);
+      ones_sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, plo[t], ones_sum[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < G::kNE; ++e) {
+      // (a step's codes are flipped once: xor 0x80 makes bytes 0 .. 255)
+      uint32_t v[8][G::kWords];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int q = 0; q < G::kWords; ++q) v[j][q] = BITS == 8 ? s.v[j][q] ^ 0x80808080u : s.v[j][q];
+      const bf16x8_t va = values_bf16<D, BITS>(v, e);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, phi[t], o[t][e], 0, 0, 0);
+        o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, plo[t], o[t][e], 0, 0, 0);
+      }
+    }
+  };
+  load(0, std::integral_constant<int, 0>{});
+#pragma unroll 1
+  for (int i = 0; i < n_steps; i += 2) {
+    load(i + 1, std::integral_constant<int, 1>{});
+    compute(i, std::integral_constant<int, 0>{});
+    if (i + 1 < n_steps) {
+      load(i + 2, std::integral_constant<int, 0>{});
+      compute(i + 1, std::integral_constant<int, 1>{});
+    }
+  }
+
+  // the wave's rows in order of their dims, the offset out; then the waves' states into the first one's
+  float y[MT][N];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    l[t] += xor_lane<16>(l[t]);
+    l[t] += xor_lane<32>(l[t]);
+#pragma unroll
+    for (int e = 0; e < G::kNE; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[t][G::kNE * i + e] = o[t][e][i] - G::kBias * ones_sum[t][i];
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s_o[wave - 1][t * N + i][lane] = y[t][i];
+      s_ml[wave - 1][t][0][lane] = m[t];
+      s_ml[wave - 1][t][1][lane] = l[t];
+    }
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    float top = m[t];
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) top = fmaxf(top, s_ml[w][t][0][lane]);
+    // (a state of nothing has a sum of 0; NaN alone leaves a maximum of -inf, and a sum that says so)
+    const float f = l[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
+    l[t] = l[t] == 0.0f ? 0.0f : l[t] * f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[t][i] *= f;
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) {
+      const float lw = s_ml[w][t][1][lane];
+      const float fw = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][t][0][lane] - top);
+      l[t] += lw == 0.0f ? 0.0f : lw * fw;
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[t][i] = fmaf(s_o[w][t * N + i][lane], fw, y[t][i]);
+    }
+    m[t] = top;
+    if (row[t] >= a.rows) continue;
+    const int32_t tok = row[t] / a.G, h = kh * a.G + (row[t] - tok * a.G);
+    const int64_t orow = (b * a.T + tok) * a.H + h;
+    if (a.n_split > 1) {
+      float* p = a.part + (orow * a.n_split + split) * (D + 4);
+      if (g == 0) p[0] = m[t], p[1] = l[t];
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i)
+        *reinterpret_cast<f32x4_t*>(p + 4 + g * N + 4 * i) = f32x4_t{y[t][4 * i], y[t][4 * i + 1], y[t][4 * i + 2], y[t][4 * i + 3]};
+    }
+  }
+  if (a.n_split > 1) return;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const bool in = row[t] < a.rows;
+    const int32_t tok = in ? row[t] / a.G : 0, h = in ? kh * a.G + (row[t] - tok * a.G) : 0;
+    const int64_t orow = (b * a.T + tok) * a.H + h;
+    const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+    const float top = fmaxf(m[t], sk);
+    const float f = l[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
+    const float sum = l[t] * f + (sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - top));
+    const float r = sum == 0.0f ? 0.0f : f / sum * a.wscale;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[t][i] *= r;
+    rotate_lane<N>(y[t], lane);
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[t][i] *= a.diag[g * N + i];
+    if (in) {
+      store_row<DT, N>(a.out, orow * D + g * N, y[t]);
+      if (a.lse && g == 0) a.lse[orow] = sum == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(sum);
+    }
+  }
+}
+
+// Merges the pieces of one row and rotates it back: the workgroup's waves take every fourth piece each.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
+  constexpr int PER = D / 64;
+  __shared__ float s_o[kWaves][D], s_ml[kWaves][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t orow = blockIdx.x;
+  const int64_t b = orow / (static_cast<int64_t>(a.T) * a.H);
+  const int32_t h = static_cast<int32_t>(orow % a.H);
+  const int32_t n = newest_sees(a, b);
+  const int32_t piece = piece_slots(n, a.n_split);
+  const int pieces = max((n + piece - 1) / piece, 1);
+  const float* p = a.part + orow * a.n_split * (D + 4);
+  float m = kNegInf, l = 0.0f, x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = 0.0f;
+#pragma unroll 4
+  for (int s = wave; s < pieces; s += kWaves) {
+    const float* ps = p + static_cast<int64_t>(s) * (D + 4);
+    const float pm = ps[0], pl = ps[1];
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = ps[4 + PER * lane + i];
+    const float top = fmaxf(m, pm);
+    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top), fp = pl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm - top);
+    l = (l == 0.0f ? 0.0f : l * f) + (pl == 0.0f ? 0.0f : pl * fp);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = x[i] * f + v[i] * fp;
+    m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) s_o[wave][PER * lane + i] = x[i];
+  if (lane == 0) s_ml[wave][0] = m, s_ml[wave][1] = l;
+  __syncthreads();
+  if (wave > 0) return;
+  const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+  float top = sk;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_ml[w][0]);
+  float sum = sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - top);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float lw = s_ml[w][1], f = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][0] - top);
+    sum += lw == 0.0f ? 0.0f : lw * f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = fmaf(s_o[w][PER * lane + i], f, x[i]);
+  }
+  const float r = sum == 0.0f ? 0.0f : a.wscale / sum;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] *= r;
+  wht_butterflies<D, PER>(x, lane);
+  uint32_t w[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const float y = x[i] * a.diag[PER * lane + i];
+    w[i] = DT == AEKV_BF16 ? (pack_bf16x2(y, 0.0f) & 0xffffu) : f32_to_f16_bits(y);
+  }
+  uint16_t* out = static_cast<uint16_t*>(a.out) + orow * D + PER * lane;
+  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = w[0] | (w[1] << 16);
+  else out[0] = static_cast<uint16_t>(w[0]);
+  if (a.lse && lane == 0) a.lse[orow] = sum == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(sum);
+}
+
+// The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
+// row of the KV head's group, 16 at a time (their query parts in LDS), and adds the sums over the rows.
+constexpr int kWeightTiles = 4;  // row tiles whose parts LDS holds at a time
+
+template <int DT, int D, int BITS>
+__global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
+  constexpr int NC = D / 32;
+  __shared__ __align__(16) f16x8_t s_hi[kWeightTiles][NC][64], s_lo[kWeightTiles][NC][64];
+  __shared__ float s_f[kWeightTiles][16], s_lse[kWeightTiles][16];
+  __shared__ int32_t s_sees[kWeightTiles][16];
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t wg = blockIdx.x;
+  const int32_t split = static_cast<int32_t>(wg % a.n_split);
+  wg /= a.n_split;
+  const int32_t kh = static_cast<int32_t>(wg % a.pool.heads);
+  const int64_t b = wg / a.pool.heads;
+  const int32_t n = newest_sees(a, b);
+  const int32_t piece = piece_slots(n, a.n_split);
+  const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
+  if (p0 >= p1) return;  // (the whole workgroup)
+  float* weights = a.weights + (b * a.pool.heads + kh) * a.capacity;
+  const int32_t first = p0 + kStep * wave;
+  const int n_steps = first < p1 ? (p1 - first + kRound - 1) / kRound : 0;
+  const int tiles = (a.rows + 15) / 16;
+  for (int t0 = 0; t0 < tiles; t0 += kWeightTiles) {
+    const int nt = min(tiles - t0, kWeightTiles);
+    if (t0 > 0) __syncthreads();
+    for (int t = wave; t < nt; t += kWaves) {
+      const int32_t row = (t0 + t) * 16 + (lane & 15);
+      const bool in = row < a.rows;
+      f16x8_t hi[NC], lo[NC];
+      float factor;
+      query_parts<DT, D, BITS>(a, b, kh, row, in, lane, hi, lo, &factor);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s_hi[t][c][lane] = hi[c], s_lo[t][c][lane] = lo[c];
+      if (g == 0) {
+        const int32_t tok = in ? row / a.G : 0, h = in ? kh * a.G + (row - tok * a.G) : 0;
+        s_f[t][lane] = factor;
+        s_lse[t][lane] = a.lse[(b * a.T + tok) * a.H + h];
+        s_sees[t][lane] = in ? max(n - a.T + 1 + tok, 0) : 0;
+      }
+    }
+    __syncthreads();
+    int32_t pages = -1;
+#pragma unroll 1
+    for (int i = 0; i < n_steps; ++i) {
+      if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+      const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
+      const int32_t base = first + kRound * i;
+      StepData<D, BITS> s;
+      load_step<D, BITS, false>(a, kh, base, g0, g1, lane, s);
+      f16x8_t kc[2][NC];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kc[k][c] = codes_f16<BITS>(&s.k[k][c * BITS / 4]);
+      f32x4_t sum[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+      for (int t = 0; t < nt; ++t) {
+        f16x8_t hi[NC], lo[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) hi[c] = s_hi[t][c][lane], lo[c] = s_lo[t][c][lane];
+        f32x4_t x[2];
+        score_step<D, BITS>(kc, s.ks, hi, lo, s_f[t][lane & 15], x);
+        const float lse = s_lse[t][lane & 15];
+        const int32_t sees = s_sees[t][lane & 15];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool hide = (k ? g1 : g0) < 0 || base + 16 * k + 4 * g + j >= sees;
+            sum[k][j] += hide ? 0.0f : __builtin_amdgcn_exp2f(x[k][j] - lse);
+          }
+      }
+      // over the 16 rows
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v = sum[k][j];
+          v += xor_lane<1>(v);
+          v += xor_lane<2>(v);
+          v += xor_lane<4>(v);
+          v += xor_lane<8>(v);
+          sum[k][j] = v;
+        }
+        const int j = lane & 15;
+        const int32_t slot = base + 16 * k + 4 * g + j;
+        if (j < 4 && slot < p1 && (k ? g1 : g0) >= 0) {
+          const float v = j == 0 ? sum[k][0] : j == 1 ? sum[k][1] : j == 2 ? sum[k][2] : sum[k][3];
+          if (v != 0.0f) weights[slot] += v;
+        }
+      }
+    }
+  }
 }
 
 using paged_fn = void (*)(PagedArgs);
 
 template <int DT>
-paged_fn pick_paged(int d, int bits) {
-  if (d == 64) return bits == 8 ? paged_attention_kernel<DT, 64, 8> : paged_attention_kernel<DT, 64, 4>;
-  return bits == 8 ? paged_attention_kernel<DT, 128, 8> : paged_attention_kernel<DT, 128, 4>;
+paged_fn pick_paged(int d, int bits, int mt) {
+  if (mt == 2) return bits == 8 ? paged_attention_kernel<DT, 64, 8, 2> : paged_attention_kernel<DT, 64, 4, 2>;
+  if (d == 64) return bits == 8 ? paged_attention_kernel<DT, 64, 8, 1> : paged_attention_kernel<DT, 64, 4, 1>;
+  return bits == 8 ? paged_attention_kernel<DT, 128, 8, 1> : paged_attention_kernel<DT, 128, 4, 1>;
 }
 
+template <int DT>
 paged_fn pick_weights(int d, int bits) {
-  if (d == 64) return bits == 8 ? paged_weights_kernel<64, 8> : paged_weights_kernel<64, 4>;
-  return bits == 8 ? paged_weights_kernel<128, 8> : paged_weights_kernel<128, 4>;
+  if (d == 64) return bits == 8 ? paged_weights_kernel<DT, 64, 8> : paged_weights_kernel<DT, 64, 4>;
+  return bits == 8 ? paged_weights_kernel<DT, 128, 8> : paged_weights_kernel<DT, 128, 4>;
 }
+
+// Pieces of a sequence: enough workgroups for the chip (2048: two per CU, four times over, which evens out sequences of
+// different lengths), none without a whole round of slots.
+int64_t paged_pieces(int64_t groups, int64_t slots) {
+  const int64_t want = ceil_div(2048, groups), most = ceil_div(slots, kRound);
+  const int64_t n = want < most ? want : most;
+  return n < 1 ? 1 : n;
+}
+
+// Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.
+int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 : 1; }
 
 }  // namespace
 }  // namespace aekv
@@ -162,8 +695,11 @@ using namespace aekv;
 
 extern "C" size_t aekv_paged_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t heads, int32_t d,
                                                       int64_t slots, int32_t tracked) {
-  if (B <= 0 || T <= 0 || H <= 0 || heads <= 0 || d <= 0 || slots <= 0 || !tracked) return 0;
-  return align_up(static_cast<size_t>(B * T * H) * 4, 16) + static_cast<size_t>(B * T * H) * d * 4;
+  if (B <= 0 || T <= 0 || H <= 0 || heads <= 0 || d <= 0 || slots <= 0) return 0;
+  const int64_t rows = T * (H / heads), blocks = ceil_div(rows, 16 * paged_row_tiles(rows, d));
+  const int64_t n = paged_pieces(B * heads * blocks, slots);
+  return (tracked ? align_up(static_cast<size_t>(B * T * H) * 4, 16) : 0) +
+         (n > 1 ? static_cast<size_t>(B * T * H) * static_cast<size_t>(n) * (d + 4) * 4 : 0);
 }
 
 extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batch_stride, int64_t q_token_stride,
@@ -186,13 +722,18 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   if (weights && capacity < 0) return fail(AEKV_ERR_SHAPE, "%s: capacity=%lld", who, (long long)capacity);
   if (B == 0 || T == 0) return AEKV_OK;
   if (!q || !lengths || !diag || !out) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
-  if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) || (q_batch_stride % 8) || (q_token_stride % 8) ||
-      (q_head_stride % 8))
-    return fail(AEKV_ERR_ALIGN, "%s: q rows, out and workspace must be 16-byte aligned", who);
-  if (B > 65535 || T > 65535 || H > 65535) return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld T=%lld H=%lld exceed the grid", who, (long long)B, (long long)T, (long long)H);
-  const int64_t slots = max_pages * page_size;
+  if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) || !is_aligned(diag, 16) || (q_batch_stride % 8) ||
+      (q_token_stride % 8) || (q_head_stride % 8))
+    return fail(AEKV_ERR_ALIGN, "%s: q rows, out, diag and workspace must be 16-byte aligned", who);
+  const int64_t slots = max_pages * page_size, rows = T * (H / heads);
+  const int mt = paged_row_tiles(rows, d);
+  const int64_t blocks = ceil_div(rows, 16 * mt);
+  if (H > 65535 || T > 0x7fffff || rows > 0x3fffffff || B * heads * blocks > kMaxGridThreads / kThreads / 4 || B * T * H > kMaxGridThreads / kThreads)
+    return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld T=%lld H=%lld exceed the grid", who, (long long)B, (long long)T, (long long)H);
   const size_t want = aekv_paged_attention_workspace_size(B, T, H, heads, d, slots, weights != nullptr);
   if (want && (!ws || ws_bytes < want)) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
+  int64_t reach = pages > 0 ? slots : 0;
+  if (weights && capacity < reach) reach = capacity;
   a.q = q;
   a.q_batch = q_batch_stride;
   a.q_token = q_token_stride;
@@ -200,22 +741,33 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   a.lengths = lengths;
   a.diag = diag;
   a.sink = sink;
-  a.weights = slots > 0 ? weights : nullptr;
-  a.lse = static_cast<float*>(ws);
-  a.rot = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align_up(static_cast<size_t>(B * T * H) * 4, 16));
+  a.weights = reach > 0 ? weights : nullptr;
+  a.lse = a.weights ? static_cast<float*>(ws) : nullptr;
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (weights ? align_up(static_cast<size_t>(B * T * H) * 4, 16) : 0));
   a.out = out;
+  a.reach = static_cast<int32_t>(reach);
   a.capacity = capacity;
   a.T = static_cast<int32_t>(T);
   a.H = static_cast<int32_t>(H);
-  a.scale = softmax_scale;
+  a.G = static_cast<int32_t>(H / heads);
+  a.rows = static_cast<int32_t>(rows);
+  a.row_blocks = static_cast<int32_t>(blocks);
+  a.n_split = static_cast<int32_t>(paged_pieces(B * heads * blocks, slots));
+  a.scale2 = softmax_scale * kLog2e;
   a.wscale = wht_scale(d);
   const hipStream_t st = as_stream(stream);
-  auto fn = dtype == AEKV_F16 ? pick_paged<AEKV_F16>(d, bits) : pick_paged<AEKV_BF16>(d, bits);
-  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(H), static_cast<uint32_t>(T), static_cast<uint32_t>(B)), dim3(256), 0, st, a);
+  auto fn = dtype == AEKV_F16 ? pick_paged<AEKV_F16>(d, bits, mt) : pick_paged<AEKV_BF16>(d, bits, mt);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(B * heads * blocks * a.n_split)), dim3(kThreads), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
+  if (a.n_split > 1) {
+    auto mg = dtype == AEKV_F16 ? (d == 64 ? paged_merge_kernel<AEKV_F16, 64> : paged_merge_kernel<AEKV_F16, 128>)
+                                : (d == 64 ? paged_merge_kernel<AEKV_BF16, 64> : paged_merge_kernel<AEKV_BF16, 128>);
+    hipLaunchKernelGGL(mg, dim3(static_cast<uint32_t>(B * T * H)), dim3(kThreads), 0, st, a);
+    if (const int rc = check_launch(who)) return rc;
+  }
   if (!a.weights) return AEKV_OK;
-  const int64_t reach = slots < capacity ? slots : capacity;
-  if (reach == 0) return AEKV_OK;
-  hipLaunchKernelGGL(pick_weights(d, bits), dim3(static_cast<uint32_t>(ceil_div(reach, 256)), static_cast<uint32_t>(heads), static_cast<uint32_t>(B)), dim3(256), 0, st, a);
+  a.n_split = static_cast<int32_t>(paged_pieces(B * heads, slots));
+  auto wf = dtype == AEKV_F16 ? pick_weights<AEKV_F16>(d, bits) : pick_weights<AEKV_BF16>(d, bits);
+  hipLaunchKernelGGL(wf, dim3(static_cast<uint32_t>(B * heads * a.n_split)), dim3(kThreads), 0, st, a);
   return check_launch(who);
 }
