@@ -4,95 +4,424 @@
 // j <= i + (keys - queries), so that the last query sees every key (a chunk of a prompt comes with the keys before it).
 //   out_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j) / (sum exp(scale q_i . k) + exp(sink)),  lse_i = log of that sum.
 // A query that sees nothing gives 0 and a log sum of the sink's, or -inf.
+//
+// Work split.  The G heads of a KV head's group share its keys: the rows of a sequence and KV head are (query, head),
+// query-major, and a workgroup takes 32 RB WR consecutive ones, 32 RB per wave.  Tiles of 64 keys and values stream through
+// two LDS buffers, loaded one tile ahead straight into LDS; with KS = 2 two waves share a row group and take half of every
+// tile each, merged at the end.  One pass: running maximum and sum, the output rescaled only where a maximum moved by more
+// than kMargin (weights up to 2^kMargin are as exact in 16 bits as those up to 1, and the sums are fp32).
+//
+// Matrix layout (v_mfma_f32_32x32x16: A lane l holds A[l % 32][8 (l / 32) + j], B lane l holds B[8 (l / 32) + j][l % 32],
+// D lane l register v holds D[8 (v / 4) + 4 (l / 32) + v % 4][l % 32]), h = l / 32:
+//   S^T = K Q^T: m = key, n = row; a lane reads 16-byte chunks of its key's row.
+//   O^T += V^T P^T: m = dim, n = row, k = key; lane h holds keys 16 c + 4 h + j and 16 c + 8 + 4 h + j of a 16-key chunk c,
+//   its own scores, and V^T comes from the row-major tile through the transposing LDS load.
+// LDS rows keep their 16-byte chunks XOR-swizzled by their key, so that both reads touch all banks once.
+#include <type_traits>
+
 #include "aekv_common.h"
 
 namespace aekv {
 namespace {
 
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kMargin = 8.0f;        // log2 units
+constexpr int kTile = 64;              // keys of a tile
+constexpr int kBufWord3 = 0x00020000;  // buffer resource word 3: raw 32-bit data, range-checked
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) short i16x4_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+typedef __attribute__((address_space(3))) void lds_void_t;
 
 struct PromptArgs {
-  const void* q;
-  const void* k;
-  const void* v;
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
   const int32_t* cu_q;  // [B + 1]
   const int32_t* cu_k;  // [B + 1]
   const float* sink;    // [H] or null
-  void* out;            // [n_q, H, D]
+  uint16_t* out;        // [n_q, H, D]
   float* lse;           // [n_q, H] or null
-  int32_t n_q, n_k, B, H, heads;
-  int32_t clear;        // rows behind the last sequence: 0 to leave out as it is, 1 to write zeros
-  float scale;
+  int32_t n_q, n_k, B, H, heads, G;
+  int32_t clear;        // rows in no sequence: 0 to leave out as it is, 1 to write zeros
+  float scale2;         // softmax scale * log2(e)
 };
 
 template <int DT>
-__device__ __forceinline__ float elem(const void* p, int64_t i) {
-  const uint16_t u = static_cast<const uint16_t*>(p)[i];
-  return DT == AEKV_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
+struct Elem;
+template <>
+struct Elem<AEKV_BF16> {
+  typedef bf16x8_t v8;
+  static constexpr uint32_t kExp = 0x7F807F80u;  // the exponents of a pair
+  __device__ static f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  __device__ static uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  __device__ static float value(uint32_t u) { return bf16_to_f32(u); }
+};
+template <>
+struct Elem<AEKV_F16> {
+  typedef f16x8_t v8;
+  static constexpr uint32_t kExp = 0x7C007C00u;
+  __device__ static f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  __device__ static uint32_t pack(float lo, float hi) { return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16); }
+  __device__ static float value(uint32_t u) { return f16_to_f32(u); }
+};
+
+template <int D>
+struct PromptGeom {
+  static constexpr int kRow = 2 * D;             // bytes of a tile row
+  static constexpr int kChunks = kRow / 16;      // 16-byte chunks of a row
+  static constexpr int kTileBytes = kTile * kRow;
+};
+
+// Chunk c of key r lies at c ^ swizzle(r) of its row.  256-byte rows: 16 keys' equal chunks fall on 16 places, and 4 keys
+// (4 i ..) x 4 chunks as well; 128-byte rows, two of which share the 256 bytes of all banks, likewise.
+template <int D>
+__device__ __forceinline__ int swizzle(int r) {
+  return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
 }
 
-// One wave per (query, head): 64 keys at a time, a lane each for the logits, then a lane for D / 64 dims each.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void prompt_attention_kernel(PromptArgs a) {
-  __shared__ float qs[4][D], ps[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (w >= static_cast<int64_t>(a.n_q) * a.H) return;
-  const int32_t n = static_cast<int32_t>(w / a.H), h = static_cast<int32_t>(w - static_cast<int64_t>(n) * a.H);
-  const int32_t kh = h / (a.H / a.heads);
-  uint16_t* out = static_cast<uint16_t*>(a.out) + w * D;
-  int lo = 0, hi = a.B;
-  const bool in = n >= a.cu_q[0] && n < a.cu_q[a.B];
-  while (in && hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= n) lo = mid;
-    else hi = mid;
-  }
-  if (!in) {
-    if (a.clear)
-      for (int i = 0; i < D / 64; ++i) out[lane + 64 * i] = 0;
-    if (a.lse && lane == 0) a.lse[w] = kNegInf;
-    return;
-  }
-  const int64_t k0 = max(a.cu_k[lo], 0), k1 = min(a.cu_k[lo + 1], a.n_k);
-  const int64_t seen = min<int64_t>(k1 - k0, n - a.cu_q[lo] + 1 + (k1 - k0) - (a.cu_q[lo + 1] - a.cu_q[lo]));
-  for (int i = 0; i < D / 64; ++i) qs[wave][lane + 64 * i] = elem<DT>(a.q, n * a.q_token + h * a.q_head + lane + 64 * i);
-  __builtin_amdgcn_wave_barrier();
-  float m = kNegInf, l = 0.0f, o[D / 64];
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
-  for (int64_t base = 0; base < seen; base += 64) {
-    const int64_t j = base + lane;
-    float s = kNegInf;
-    if (j < seen) {
-      const int64_t at = (k0 + j) * a.k_token + kh * a.k_head;
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot += qs[wave][d] * elem<DT>(a.k, at + d);
-      s = dot * a.scale;
+__device__ __forceinline__ i16x4_t read_tr16(const uint8_t* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p)); }
+
+// The sequence and row tile of the workgroup's `t`-th tile (tiles of `rows` rows of G per query, in the sequences' order;
+// a sequence's last rows, which see the most keys, come first).  False past the last tile.
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, int64_t t, int rows, int lane, int32_t* seq, int32_t* first) {
+  int64_t before = 0;
+  for (int32_t base = 0; base < a.B; base += 64) {
+    const int32_t b = base + lane;
+    int64_t n = 0;
+    if (b < a.B) {
+      const int32_t q0 = min(max(a.cu_q[b], 0), a.n_q), q1 = min(max(a.cu_q[b + 1], q0), a.n_q);
+      n = ((q1 - q0) * a.G + rows - 1) / rows;  // (n_q H, with a tile's rows, fits 31 bits)
     }
-    const float m2 = fmaxf(m, wave_max(s));
-    const float r = m2 == kNegInf ? 1.0f : expf(m - m2);
-    const float p = s == kNegInf ? 0.0f : expf(s - m2);
-    l = l * r + wave_sum(p);
-    m = m2;
-    ps[wave][lane] = p;
-    __builtin_amdgcn_wave_barrier();
-    for (int i = 0; i < D / 64; ++i) o[i] *= r;
-    const int cnt = static_cast<int>(min<int64_t>(64, seen - base));
-    for (int k = 0; k < cnt; ++k)
-      for (int i = 0; i < D / 64; ++i) o[i] += ps[wave][k] * elem<DT>(a.v, (k0 + base + k) * a.v_token + kh * a.v_head + lane + 64 * i);
-    __builtin_amdgcn_wave_barrier();
+    int64_t s = n;  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t o = __shfl_up(s, d);
+      if (lane >= d) s += o;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > t);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int64_t upto = before + __shfl(s, at);  // the tiles up to the sequence's last
+      *seq = base + at;
+      *first = static_cast<int32_t>(upto - 1 - t) * rows;
+      return true;
+    }
+    before += __shfl(s, 63);
   }
-  const float sk = a.sink ? a.sink[h] : kNegInf;
-  const float M = fmaxf(m, sk);
-  // (NaN alone leaves a maximum of -inf, and a sum that says so)
-  const float f = l == 0.0f ? 0.0f : expf(m - M);
-  const float L = (l == 0.0f ? 0.0f : l * f) + (sk == kNegInf ? 0.0f : expf(sk - M));
-  for (int i = 0; i < D / 64; ++i) {
-    const float y = L == 0.0f ? 0.0f : o[i] * f / L;
-    out[lane + 64 * i] = DT == AEKV_BF16 ? static_cast<uint16_t>(pack_bf16x2(y, 0.0f)) : static_cast<uint16_t>(f32_to_f16_bits(y));
+  return false;
+}
+
+template <int DT, int D, int RB, int WR, int KS>
+__global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB == 2 ? 1 : 2))) void prompt_attention_kernel(PromptArgs a) {
+  using E = Elem<DT>;
+  using Gm = PromptGeom<D>;
+  using v8 = typename E::v8;
+  constexpr int kWaves = WR * KS, kRows = 32 * RB * WR, kRow = Gm::kRow;
+  constexpr int kKB = 2 / KS;                              // 32-key blocks of a tile per wave
+  constexpr int kPass = 1024 * kWaves;                     // bytes that the workgroup stages at a time
+  constexpr int kPasses = Gm::kTileBytes / kPass;
+  constexpr int kMB = D / 32, kKSteps = D / 16;
+  static_assert(KS == 1 || KS == 2, "a tile is two 32-key blocks");
+  static_assert(Gm::kTileBytes % kPass == 0 && kPass % kRow == 0, "whole rows per pass");
+  // [buffer][K, V][key][swizzled chunks]: separate arrays, so that the compiler sees that loads into one buffer do not
+  // write what is read from the other
+  __shared__ __align__(16) uint8_t L0[2 * Gm::kTileBytes];
+  __shared__ __align__(16) uint8_t L1[2 * Gm::kTileBytes];
+  __shared__ uint16_t s_p[kWaves][32][32];  // a block's weights by key and row (values that are no numbers)
+
+  const int lane = threadIdx.x & 63, rl = lane & 31, hh = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wv % WR, kh = wv / WR;
+  const int32_t head = static_cast<int32_t>(blockIdx.x % a.heads);
+
+  // rows in no sequence: shared out over the workgroups
+  {
+    const int32_t q0 = min(max(a.cu_q[0], 0), a.n_q), q1 = min(max(a.cu_q[a.B], q0), a.n_q);
+    const int64_t words = static_cast<int64_t>(q0 + a.n_q - q1) * a.H * (D / 2);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (64 * kWaves) + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * (64 * kWaves)) {
+      const int64_t r = i / (D / 2), row = r < static_cast<int64_t>(q0) * a.H ? r : r + static_cast<int64_t>(q1 - q0) * a.H;
+      if (a.clear) reinterpret_cast<uint32_t*>(a.out)[row * (D / 2) + i % (D / 2)] = 0;
+      if (a.lse && i % (D / 2) == 0) a.lse[row] = kNegInf;
+    }
   }
-  if (a.lse && lane == 0) a.lse[w] = L == 0.0f ? kNegInf : M + logf(L);
+  int32_t seq;
+  int32_t row0;
+  if (!find_tile(a, blockIdx.x / a.heads, kRows, lane, &seq, &row0)) return;  // (the whole workgroup)
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  const int32_t q0 = min(max(a.cu_q[seq], 0), a.n_q), lq = min(max(a.cu_q[seq + 1], q0), a.n_q) - q0;
+  const int32_t k0 = min(max(a.cu_k[seq], 0), a.n_k), lk = min(max(a.cu_k[seq + 1], k0), a.n_k) - k0;
+  const int32_t n_rows = lq * a.G;
+  auto sees_of = [&](int32_t row) {  // keys that a row sees
+    const int64_t s = static_cast<int64_t>(row / a.G) + 1 + lk - lq;
+    return static_cast<int32_t>(s < 0 ? 0 : s > lk ? lk : s);
+  };
+  const int32_t last_row = (row0 + kRows < n_rows ? row0 + kRows : n_rows) - 1;
+  const int32_t n_keys = __builtin_amdgcn_readfirstlane(sees_of(last_row));
+  const int n_tiles = (n_keys + kTile - 1) / kTile;
+
+  // rows past the last are computed as copies of it
+  int32_t row[RB];
+  int32_t sees[RB];
+  v8 qb[RB][kKSteps];
+  const int32_t w0 = row0 + 32 * RB * wr;  // the wave's first row
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    row[rb] = w0 + 32 * rb + rl;
+    const int32_t r = row[rb] < n_rows ? row[rb] : n_rows - 1;
+    sees[rb] = sees_of(r);
+    const int32_t qi = r / a.G;
+    const uint16_t* qp = a.q + static_cast<int64_t>(q0 + qi) * a.q_token + static_cast<int64_t>(head * a.G + (r - qi * a.G)) * a.q_head + 8 * hh;
+#pragma unroll
+    for (int ks = 0; ks < kKSteps; ++ks) qb[rb][ks] = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
+  }
+  const int32_t wave_least = __builtin_amdgcn_readfirstlane(sees_of(w0 < n_rows ? w0 : n_rows - 1));
+  const int32_t wl = w0 + 32 * RB - 1;
+  const int32_t wave_most = __builtin_amdgcn_readfirstlane(sees_of(wl < n_rows ? wl : n_rows - 1));
+
+  // staging: pass c of wave wv writes bytes [kPass c + 1024 wv, + 1024) of a tile, lane l at + 16 l, so lane l loads the
+  // chunk that the swizzle puts there.  A pass is a multiple of 16 rows or half of one, so the swizzle repeats.
+  const int lin = 1024 * wv + 16 * lane;
+  const int key_in = lin / kRow, place = (lin % kRow) / 16;
+  static_assert(kPass / kRow % 8 == 0, "the swizzle repeats after two passes");
+  int koff[2], voff[2];
+  const int k_stride = static_cast<int>(a.k_token) * 2, v_stride = static_cast<int>(a.v_token) * 2;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int c = place ^ swizzle<D>((kPass / kRow * p + key_in) & 15);
+    koff[p] = key_in * k_stride + 16 * c;
+    voff[p] = key_in * v_stride + 16 * c;
+  }
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + k0 * a.k_token + head * a.k_head);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + k0 * a.v_token + head * a.v_head);
+  // Tile `it`, read through buffer resources whose range ends at the sequence's last key that the workgroup sees: rows
+  // past it are zero and touch no memory; past the last tile the range is empty.
+  auto load_tile = [&, n_keys, k_stride, v_stride, kbase, vbase](int it, auto buf_c) __attribute__((always_inline)) {
+    uint8_t* const dst = decltype(buf_c)::value ? L1 : L0;
+    const int left = n_keys - it * kTile, n = left < 0 ? 0 : left < kTile ? left : kTile;
+    const int64_t base = n > 0 ? static_cast<int64_t>(it) * kTile : 0;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kbase + base * k_stride), 0, n > 0 ? (n - 1) * k_stride + kRow : 0, kBufWord3);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vbase + base * v_stride), 0, n > 0 ? (n - 1) * v_stride + kRow : 0, kBufWord3);
+#pragma unroll
+    for (int c = 0; c < kPasses; ++c)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void_t*)(dst + kPass * c + 1024 * wv), 16, koff[c & 1], kPass / kRow * c * k_stride, 0, 0);
+#pragma unroll
+    for (int c = 0; c < kPasses; ++c)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void_t*)(dst + Gm::kTileBytes + kPass * c + 1024 * wv), 16, voff[c & 1], kPass / kRow * c * v_stride, 0, 0);
+  };
+
+  // LDS byte offsets.  Row-chunk reads (K): key 32 kb + rl, chunk (2 ks + hh) ^ swizzle(rl): sA ^ 32 ks.  Transposing reads
+  // (V, 16-lane group G = lane / 16, s = lane % 16): key 16 c + 8 e + 4 hh + s / 4, dims 32 mb + 16 (G % 2) + 4 (s % 4) ..,
+  // i.e. chunk 4 mb + x with x = 2 (G % 2) + (s % 4) / 2, xor the swizzle of the key.
+  const int sA = (32 * kKB * kh + rl) * kRow + ((hh ^ swizzle<D>(rl & 15)) << 4);
+  int tA[2];
+  {
+    const int s16 = lane & 15, x = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int key = 8 * e + 4 * hh + (s16 >> 2);
+      tA[e] = (32 * kKB * kh + key) * kRow + ((x ^ swizzle<D>(key)) << 4) + ((s16 & 1) << 3);
+    }
+  }
+
+  float m[RB], l[RB];
+  f32x16_t O[RB][kMB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    m[rb] = kNegInf, l[rb] = 0.0f;
+#pragma unroll
+    for (int mb = 0; mb < kMB; ++mb) O[rb][mb] = f32x16_t{};
+  }
+
+  // one tile; `masked`: some row of the wave does not see all of it
+  auto tile = [&](int it, const uint8_t* kt, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(masked_c)::value;
+    const uint8_t* vt = kt + Gm::kTileBytes;
+    const int base = it * kTile + 32 * kKB * kh;
+#pragma unroll masked ? 1 : kKB
+    for (int kb = 0; kb < kKB; ++kb) {
+      f32x16_t s[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16_t{};
+#pragma unroll
+      for (int ks = 0; ks < kKSteps; ++ks) {
+        const v8 ka = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(kt + 32 * kRow * kb + (sA ^ (ks << 5))));
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) s[rb] = E::mma(ka, qb[rb][ks], s[rb]);
+      }
+      v8 pb[RB][2];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float top = kNegInf;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          if constexpr (masked) {
+            const int key = base + 32 * kb + 8 * (v >> 2) + 4 * hh + (v & 3);
+            s[rb][v] = key < sees[rb] ? s[rb][v] * a.scale2 : kNegInf;
+            top = fmaxf(top, s[rb][v]);
+          } else {
+            s[rb][v] *= a.scale2;
+            top = fmaxf(top, s[rb][v]);
+          }
+        }
+        top = fmaxf(top, xor_lane<32>(top));
+        // (nothing yet: any maximum counts as moved)
+        if (__builtin_amdgcn_ballot_w64(top > m[rb] + kMargin)) {
+          const float up = fmaxf(m[rb], top);
+          const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - up);
+          l[rb] *= r;
+#pragma unroll
+          for (int mb = 0; mb < kMB; ++mb) O[rb][mb] *= r;
+          m[rb] = up;
+        }
+        const float nm = m[rb] == kNegInf ? 0.0f : -m[rb];
+        float p[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          p[v] = __builtin_amdgcn_exp2f(s[rb][v] + nm);
+          l[rb] += p[v];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          pb[rb][c] = __builtin_bit_cast(v8, make_uint4(E::pack(p[8 * c], p[8 * c + 1]), E::pack(p[8 * c + 2], p[8 * c + 3]),
+                                                        E::pack(p[8 * c + 4], p[8 * c + 5]), E::pack(p[8 * c + 6], p[8 * c + 7])));
+      }
+      bool odd = false;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint8_t* vc = vt + (32 * kb + 16 * c) * kRow;
+#pragma unroll
+        for (int mb = 0; mb < kMB; ++mb) {
+          const i16x4_t lo = read_tr16(vc + (tA[0] ^ (mb << 6))), hi = read_tr16(vc + (tA[1] ^ (mb << 6)));
+          u32x4_t w = __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (masked) {
+            // a value that is no finite number must not reach rows that do not see it (0 times it is no 0): it goes in
+            // as 0, and is added below to the rows that do
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool b0 = (w[i] & E::kExp & 0xffffu) == (E::kExp & 0xffffu), b1 = (w[i] & E::kExp & 0xffff0000u) == (E::kExp & 0xffff0000u);
+              odd = odd || b0 || b1;
+              w[i] = (b0 ? 0u : w[i] & 0xffffu) | (b1 ? 0u : w[i] & 0xffff0000u);
+            }
+          }
+          const v8 va = __builtin_bit_cast(v8, w);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) O[rb][mb] = E::mma(va, pb[rb][c], O[rb][mb]);
+        }
+      }
+      if constexpr (masked) {
+        if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // element j of lane half h is key 16 c + 4 h + j, or 16 c + 8 + 4 h + j - 4
+              const u32x4_t u = __builtin_bit_cast(u32x4_t, pb[rb][c]);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                s_p[wv][16 * c + 8 * (j >> 2) + 4 * hh + (j & 3)][rl] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int key = 0; key < 32; ++key) {
+              const float p = E::value(s_p[wv][key][rl]);
+              const bool in = base + 32 * kb + key < sees[rb];
+              const int kr = 32 * kKB * kh + 32 * kb + key;
+#pragma unroll
+              for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                  const int d = 32 * mb + 8 * (v >> 2) + 4 * hh + (v & 3);
+                  const uint32_t x = *reinterpret_cast<const uint16_t*>(vt + kr * kRow + (((d >> 3) ^ swizzle<D>(kr & 15)) << 4) + 2 * (d & 7));
+                  if (in && (x & (E::kExp & 0xffffu)) == (E::kExp & 0xffffu)) O[rb][mb][v] += p * E::value(x);
+                }
+            }
+          }
+        }
+      }
+    }
+  };
+  auto step = [&](int it, auto buf_c) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_c)::value;
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's part of tile `it` has landed (the compiler does not track these loads)
+    __syncthreads();                // every wave's, and the other buffer's readers are done
+    if (it + 1 < n_tiles) load_tile(it + 1, std::integral_constant<int, buf ^ 1>{});
+    const uint8_t* kt = buf ? L1 : L0;
+    const int end = (it + 1) * kTile;
+    if (end <= wave_least) tile(it, kt, std::false_type{});
+    else if (it * kTile < wave_most) tile(it, kt, std::true_type{});
+  };
+  if (n_tiles > 0) load_tile(0, std::integral_constant<int, 0>{});
+#pragma unroll 1
+  for (int it = 0; it < n_tiles; it += 2) {
+    step(it, std::integral_constant<int, 0>{});
+    if (it + 1 < n_tiles) step(it + 1, std::integral_constant<int, 1>{});
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) l[rb] += xor_lane<32>(l[rb]);  // both halves' keys
+
+  if constexpr (KS == 2) {  // the second key half's states into the first's, through the tile buffers
+    static_assert(RB == 1 && WR * kMB * 16 * 64 * 4 + WR * 2 * 64 * 4 <= 4 * Gm::kTileBytes, "the states fit both buffers");
+    __syncthreads();
+    constexpr int kPer = kMB * 16 * 64, kFit = 2 * Gm::kTileBytes / 4;  // floats
+    auto slot = [&](int i) -> float* { return i < kFit ? reinterpret_cast<float*>(L0) + i : reinterpret_cast<float*>(L1) + (i - kFit); };
+    static_assert(kFit % 64 == 0, "a run of 64 floats lies in one buffer");
+    const int at = wr * (kPer + 128);
+    if (kh == 1) {
+#pragma unroll
+      for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) slot(at + (mb * 16 + v) * 64)[lane] = O[0][mb][v];
+      slot(at + kPer)[lane] = m[0];
+      slot(at + kPer + 64)[lane] = l[0];
+    }
+    __syncthreads();
+    if (kh == 1) return;
+    const float m1 = slot(at + kPer)[lane], l1 = slot(at + kPer + 64)[lane];
+    const float up = fmaxf(m[0], m1);
+    // (a state of nothing has a sum of 0; NaN alone leaves a maximum of -inf, and a sum that says so)
+    const float f0 = l[0] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[0] - up), f1 = l1 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m1 - up);
+    l[0] = (l[0] == 0.0f ? 0.0f : l[0] * f0) + (l1 == 0.0f ? 0.0f : l1 * f1);
+    m[0] = up;
+#pragma unroll
+    for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) O[0][mb][v] = O[0][mb][v] * f0 + slot(at + (mb * 16 + v) * 64)[lane] * f1;
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    if (row[rb] >= n_rows) continue;
+    const int32_t qi = row[rb] / a.G;
+    const int32_t h = head * a.G + (row[rb] - qi * a.G);
+    const int64_t orow = static_cast<int64_t>(q0 + qi) * a.H + h;
+    const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+    const float up = fmaxf(m[rb], sk);
+    const float f = l[rb] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[rb] - up);
+    const float sum = (l[rb] == 0.0f ? 0.0f : l[rb] * f) + (sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - up));
+    const float r = sum == 0.0f ? 0.0f : f / sum;
+    uint16_t* op = a.out + orow * D + 4 * hh;
+#pragma unroll
+    for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(op + 32 * mb + 8 * i) = make_uint2(E::pack(O[rb][mb][4 * i] * r, O[rb][mb][4 * i + 1] * r),
+                                                                     E::pack(O[rb][mb][4 * i + 2] * r, O[rb][mb][4 * i + 3] * r));
+    if (a.lse && hh == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
+  }
+}
+
+using prompt_fn = void (*)(PromptArgs);
+template <int RB, int WR, int KS>
+prompt_fn pick_prompt(int32_t dtype, int32_t d) {
+  if (dtype == AEKV_F16) return d == 64 ? prompt_attention_kernel<AEKV_F16, 64, RB, WR, KS> : prompt_attention_kernel<AEKV_F16, 128, RB, WR, KS>;
+  return d == 64 ? prompt_attention_kernel<AEKV_BF16, 64, RB, WR, KS> : prompt_attention_kernel<AEKV_BF16, 128, RB, WR, KS>;
 }
 
 }  // namespace
@@ -119,14 +448,25 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
   if (!is_aligned(q, 16) || !is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(out, 16) || (q_token_stride % 8) ||
       (q_head_stride % 8) || (k_token_stride % 8) || (k_head_stride % 8) || (v_token_stride % 8) || (v_head_stride % 8))
     return fail(AEKV_ERR_ALIGN, "%s: q, k and v rows and out must be 16-byte aligned", who);
-  if (n_q > 0x7fffffff || n_k > 0x7fffffff || B > 0x7ffffffe || H > 65535 || n_q * H > kMaxGridThreads / 64 - 4)
+  if (n_q > 0x7fffffff || n_k > 0x7fffffff || B > 0x7ffffffe || H > 65535 || n_q * H > 0x7fff0000)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld n_k=%lld H=%lld exceed the grid", who, (long long)B,
                 (long long)n_q, (long long)n_k, (long long)H);
-  PromptArgs a{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
-               cu_seqlens_q, cu_seqlens_k, sink, out, lse, static_cast<int32_t>(n_q), static_cast<int32_t>(n_k),
-               static_cast<int32_t>(B), static_cast<int32_t>(H), static_cast<int32_t>(heads), clear_rest, softmax_scale};
-  auto fn = dtype == AEKV_F16 ? (d == 64 ? prompt_attention_kernel<AEKV_F16, 64> : prompt_attention_kernel<AEKV_F16, 128>)
-                              : (d == 64 ? prompt_attention_kernel<AEKV_BF16, 64> : prompt_attention_kernel<AEKV_BF16, 128>);
-  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(ceil_div(n_q * H, 4))), dim3(256), 0, as_stream(stream), a);
+  if (k_token_stride * 2 * kTile > 0x3fffffff || v_token_stride * 2 * kTile > 0x3fffffff || k_token_stride < 0 || v_token_stride < 0)
+    return fail(AEKV_ERR_UNSUPPORTED, "%s: token strides of %lld and %lld elements", who, (long long)k_token_stride,
+                (long long)v_token_stride);
+  PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), q_token_stride,
+               q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q, cu_seqlens_k, sink,
+               static_cast<uint16_t*>(out), lse, static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B),
+               static_cast<int32_t>(H), static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
+               softmax_scale * kLog2e};
+  // large launches take 256 rows per workgroup, the others 64
+  const int64_t rows = n_q * (H / heads);
+  const bool large = heads * (rows / 256) >= 512;
+  const int per = large ? 256 : 64;
+  const int64_t tiles = rows / per + B;  // at least every sequence's, whatever their lengths
+  if (tiles * heads > kMaxGridThreads / 256)
+    return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld H=%lld exceed the grid", who, (long long)B, (long long)n_q, (long long)H);
+  auto fn = large ? pick_prompt<2, 4, 1>(dtype, d) : pick_prompt<1, 2, 2>(dtype, d);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(tiles * heads)), dim3(256), 0, as_stream(stream), a);
   return check_launch(who);
 }
