@@ -34,113 +34,201 @@ __device__ __forceinline__ uint32_t evict_key(float w, int32_t token, int32_t fi
   return order_key(w + 0.0f);
 }
 
-// Exclusive sum of v over the workgroup's threads in order; *total its whole.  `part`: one word per wave.
-__device__ __forceinline__ int block_scan(int v, int* part, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(s, d);
-    if (lane >= d) s += o;
-  }
-  __syncthreads();  // part's readers of the call before are done
-  if (lane == 63) part[wave] = s;
+// One workgroup per (sequence, head).  Its waves own consecutive runs of slots, 64 kRegRows or fewer each, whose keys stay in
+// registers while the threshold is found; longer rows go through in rounds of kRound slots, read again for each pass.
+//
+// The threshold: the keep-th largest key by 11, 11 and 10 bits from the top, each level a histogram in LDS of the keys that
+// share the bits above, searched from its largest bin by all waves.  A level whose bin is kept whole ends it.
+// The order: ballots rank a wave's ties, holes and movers by slot; one word per wave carries the counts between waves.
+constexpr int kWaves = kSelThreads / 64, kRegRows = 16, kRound = kSelThreads * kRegRows, kBins = 2048;
+
+// The waves' counts before this one's, and their total, for two counters (the first below 2^32, packed with the second).
+__device__ __forceinline__ uint64_t wave_prefix(uint64_t mine, uint64_t* part, int lane, int wave, uint64_t* total) {
+  __syncthreads();  // the readers of the call before are done
+  if (lane == 0) part[wave] = mine;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelThreads / 64; ++w) {
-    before += w < wave ? part[w] : 0;
-    all += part[w];
+  uint64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const uint64_t p = part[w];
+    before += w < wave ? p : 0;
+    all += p;
   }
   *total = all;
-  return before + s - v;
+  return before;
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ int part[kSelThreads / 64];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t s_sum[kWaves];
+  __shared__ uint64_t s_part[kWaves];
+  __shared__ int s_found[3];  // bin, keys of it that stay, keys in it
   const int64_t bh = blockIdx.x;
   const int64_t b = bh / a.pool.heads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t cap = static_cast<int32_t>(min<int64_t>(table_slots(a.pool), a.capacity));
   const int32_t n = min(a.lengths[b], cap);
-  const int tid = threadIdx.x;
+  const int64_t recent_from = static_cast<int64_t>(a.seen[b]) - a.recent;
   if (n <= a.keep) {  // (the whole workgroup)
     if (tid == 0) a.counts[bh] = 0;
     return;
   }
   const float* w = a.weights + bh * a.capacity;
   const int32_t* tok = a.tokens + bh * a.capacity;
-  const int64_t recent_from = static_cast<int64_t>(a.seen[b]) - a.recent;
-  // the keep-th largest key, 8 bits at a time: `prefix` its leading bits, `need` how many of the keys with that prefix stay
+  // the waves' runs in a round that starts at `base`: `rows` rows of 64 slots each
+  uint32_t key[kRegRows];
+  int rows = 0, run = 0;
+  auto load_round = [&](int base) __attribute__((always_inline)) {
+    const int left = min(n - base, kRound);
+    rows = (left + kSelThreads - 1) / kSelThreads;
+    run = base + wave * rows * 64;
+    float wt[kRegRows];
+    int32_t tk[kRegRows];
+#pragma unroll
+    for (int r = 0; r < kRegRows; ++r) {
+      const int i = run + 64 * r + lane;
+      if (r < rows && i < n) wt[r] = w[i], tk[r] = tok[i];
+    }
+#pragma unroll
+    for (int r = 0; r < kRegRows; ++r)
+      key[r] = r < rows && run + 64 * r + lane < n ? evict_key(wt[r], tk[r], a.first, recent_from) : 0u;
+  };
+  const bool one_round = n <= kRound;
+  if (one_round) load_round(0);
   uint32_t prefix = 0;
-  int need = a.keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+  int need = a.keep, shift = 21;
+  for (;;) {
+    const int width = shift == 0 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
-      const uint32_t key = evict_key(w[i], tok[i], a.first, recent_from);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+    for (int base = 0; base < n; base += kRound) {
+      if (!one_round) load_round(base);
+#pragma unroll
+      for (int r = 0; r < kRegRows; ++r)
+        if (r < rows && run + 64 * r + lane < n && (shift == 21 || (key[r] >> (shift + width)) == (prefix >> (shift + width))))
+          atomicAdd(&hist[(key[r] >> shift) & ((1u << width) - 1)], 1u);
     }
     __syncthreads();
-    if (tid == 0) {
-      int left = need, bin = 255;
-      while (bin > 0 && left > static_cast<int>(hist[bin])) left -= static_cast<int>(hist[bin--]);
-      s_prefix = prefix | (static_cast<uint32_t>(bin) << shift);
-      s_need = left;
+    // bins from the top: thread t holds bins 2047 - 2 t and the one below
+    const uint32_t h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
+    uint32_t s = h0 + h1;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(s, d);
+      if (lane >= d) s += o;
     }
+    if (lane == 63) s_sum[wave] = s;
     __syncthreads();
-    prefix = s_prefix;
-    need = s_need;
+    uint32_t above = 0;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) above += v < wave ? s_sum[v] : 0;
+    above += s - h0 - h1;  // keys in higher bins than this thread's
+    const uint32_t want = static_cast<uint32_t>(need);
+    if (above < want && above + h0 >= want) s_found[0] = kBins - 1 - 2 * tid, s_found[1] = want - above, s_found[2] = h0;
+    else if (above + h0 < want && above + h0 + h1 >= want) s_found[0] = kBins - 2 - 2 * tid, s_found[1] = want - above - h0, s_found[2] = h1;
+    if (need == 0 && tid == 0) s_found[0] = kBins - 1, s_found[1] = 0, s_found[2] = -1;
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(s_found[0]) << shift;
+    need = s_found[1];
+    if (need == s_found[2] || shift == 0 || a.keep == 0) break;
+    shift = shift == 21 ? 10 : 0;
   }
-  // in slot order: the first `need` of the keys equal to the threshold stay; holes and movers by their ranks
-  int ties = 0, holes = 0, movers = 0;
+  // in slot order: of the keys that share the threshold's bits the first `need` stay; holes and movers by their ranks
+  uint64_t ties = 0, moved = 0;  // of the rounds before; holes low, movers high
   int2* mv = a.moves + bh * a.most;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + tid;
-    const uint32_t key = i < n ? evict_key(w[i], tok[i], a.first, recent_from) : 0u;
-    const bool tie = i < n && key == prefix;
-    int total;
-    const int rank = ties + block_scan(tie, part, &total);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int base = 0; base < n; base += kRound) {
+    if (!one_round) load_round(base);
+    uint64_t mine = 0, total;
+#pragma unroll
+    for (int r = 0; r < kRegRows; ++r) {
+      const bool in = r < rows && run + 64 * r + lane < n;
+      mine += __popcll(__builtin_amdgcn_ballot_w64(in && (key[r] >> shift) == (prefix >> shift)));
+    }
+    uint64_t rank = ties + wave_prefix(mine, s_part, lane, wave, &total);
     ties += total;
-    const bool kept = i < n && (key > prefix || (tie && rank < need));
-    const bool hole = i < n && !kept && i < a.keep, mover = kept && i >= a.keep;
-    const int hr = holes + block_scan(hole, part, &total);
-    holes += total;
-    const int mr = movers + block_scan(mover, part, &total);
-    movers += total;
-    if (hole) mv[hr].y = i;
-    if (mover) mv[mr].x = i;
+    uint32_t hole = 0, mover = 0;  // bit r: the slot of row r
+    uint64_t count = 0;
+#pragma unroll
+    for (int r = 0; r < kRegRows; ++r) {
+      const int i = run + 64 * r + lane;
+      const bool in = r < rows && i < n;
+      const bool tie = in && (key[r] >> shift) == (prefix >> shift);
+      const uint64_t tm = __builtin_amdgcn_ballot_w64(tie);
+      const bool kept = in && ((key[r] >> shift) > (prefix >> shift) || (tie && rank + __popcll(tm & below) < static_cast<uint64_t>(need)));
+      rank += __popcll(tm);
+      const bool h = in && !kept && i < a.keep, m = kept && i >= a.keep;
+      hole |= (h ? 1u : 0u) << r;
+      mover |= (m ? 1u : 0u) << r;
+      count += __popcll(__builtin_amdgcn_ballot_w64(h)) + (static_cast<uint64_t>(__popcll(__builtin_amdgcn_ballot_w64(m))) << 32);
+    }
+    uint64_t at = moved + wave_prefix(count, s_part, lane, wave, &total);
+    moved += total;
+#pragma unroll
+    for (int r = 0; r < kRegRows; ++r) {
+      const int i = run + 64 * r + lane;
+      const bool h = (hole >> r) & 1u, m = (mover >> r) & 1u;
+      const uint64_t hm = __builtin_amdgcn_ballot_w64(h), mm = __builtin_amdgcn_ballot_w64(m);
+      if (h) mv[(at & 0xffffffffu) + __popcll(hm & below)].y = i;
+      if (m) mv[(at >> 32) + __popcll(mm & below)].x = i;
+      at += __popcll(hm) + (static_cast<uint64_t>(__popcll(mm)) << 32);
+    }
   }
-  if (tid == 0) a.counts[bh] = holes;  // (as many movers: keep slots stay)
+  if (tid == 0) a.counts[bh] = static_cast<int32_t>(moved & 0xffffffffu);  // (as many movers: keep slots stay)
 }
 
-// 16 lanes move one slot: its code rows, scales, weight and token.
+// 16 lanes move one slot: its code rows, scales, weight and token.  kMoves slots at a time, so that their dependent loads
+// (the move, the pages, the rows) overlap.
+constexpr int kMoves = 4;
+
 template <int ROW>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
+  constexpr int NB = ROW / 16;
+  struct alignas(NB) W { uint8_t x[NB]; };
   const int64_t bh = blockIdx.y;
   const int64_t b = bh / a.pool.heads;
   const int32_t h = static_cast<int32_t>(bh - b * a.pool.heads);
   const int count = a.counts[bh];
   const int sub = threadIdx.x & 15;
-  for (int m = blockIdx.x * 16 + (threadIdx.x >> 4); m < count; m += gridDim.x * 16) {
-    const int2 mv = a.moves[bh * a.most + m];
-    const int64_t src = cache_row(a.pool, b, h, mv.x), dst = cache_row(a.pool, b, h, mv.y);
-    if (src >= 0 && dst >= 0) {
-      constexpr int NB = ROW / 16;
-      struct alignas(NB) W { uint8_t x[NB]; };
-      const W kc = *reinterpret_cast<const W*>(a.pool.k_codes + src * ROW + sub * NB);
-      const W vc = *reinterpret_cast<const W*>(a.pool.v_codes + src * ROW + sub * NB);
-      *reinterpret_cast<W*>(a.pool.k_codes + dst * ROW + sub * NB) = kc;
-      *reinterpret_cast<W*>(a.pool.v_codes + dst * ROW + sub * NB) = vc;
-      if (sub == 0) {
-        a.pool.k_scale[dst] = a.pool.k_scale[src];
-        a.pool.v_scale[dst] = a.pool.v_scale[src];
-      }
+  const int2* moves = a.moves + bh * a.most;
+  for (int first = (blockIdx.x * 16 + (threadIdx.x >> 4)) * kMoves; first < count; first += gridDim.x * 16 * kMoves) {
+    int2 mv[kMoves];
+    int64_t src[kMoves], dst[kMoves];
+    W kc[kMoves], vc[kMoves];
+    uint32_t extra[kMoves];
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) mv[i] = moves[min(first + i, count - 1)];  // (the last again past the end: not stored)
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      src[i] = cache_row(a.pool, b, h, mv[i].x);
+      dst[i] = cache_row(a.pool, b, h, mv[i].y);
     }
-    if (sub == 1) {
-      a.weights[bh * a.capacity + mv.y] = a.weights[bh * a.capacity + mv.x];
-      a.tokens[bh * a.capacity + mv.y] = a.tokens[bh * a.capacity + mv.x];
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int64_t r = src[i] < 0 ? 0 : src[i];  // (a pool has a first row)
+      kc[i] = *reinterpret_cast<const W*>(a.pool.k_codes + r * ROW + sub * NB);
+      vc[i] = *reinterpret_cast<const W*>(a.pool.v_codes + r * ROW + sub * NB);
+      // lanes 0 .. 3: K scale, V scale, weight, token
+      const int64_t slot = bh * a.capacity + mv[i].x;
+      const uint32_t* from = sub == 0   ? reinterpret_cast<const uint32_t*>(a.pool.k_scale) + r
+                             : sub == 1 ? reinterpret_cast<const uint32_t*>(a.pool.v_scale) + r
+                             : sub == 2 ? reinterpret_cast<const uint32_t*>(a.weights) + slot
+                                        : reinterpret_cast<const uint32_t*>(a.tokens) + slot;
+      extra[i] = *from;
+    }
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      if (first + i >= count) break;
+      const bool there = src[i] >= 0 && dst[i] >= 0;
+      if (there) {
+        *reinterpret_cast<W*>(a.pool.k_codes + dst[i] * ROW + sub * NB) = kc[i];
+        *reinterpret_cast<W*>(a.pool.v_codes + dst[i] * ROW + sub * NB) = vc[i];
+      }
+      const int64_t slot = bh * a.capacity + mv[i].y;
+      if (sub == 0 && there) reinterpret_cast<uint32_t*>(a.pool.k_scale)[dst[i]] = extra[i];
+      if (sub == 1 && there) reinterpret_cast<uint32_t*>(a.pool.v_scale)[dst[i]] = extra[i];
+      if (sub == 2) reinterpret_cast<uint32_t*>(a.weights)[slot] = extra[i];
+      if (sub == 3) a.tokens[slot] = static_cast<int32_t>(extra[i]);
     }
   }
 }
@@ -178,6 +266,7 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   if (!ws || ws_bytes < want) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
   if (!is_aligned(ws, 16) || !is_aligned(weights, 4) || !is_aligned(tokens, 4))
     return fail(AEKV_ERR_ALIGN, "%s: misaligned pointer", who);
+  if (pages == 0) return AEKV_OK;  // nothing is there
   if (B * heads > 65535) return fail(AEKV_ERR_UNSUPPORTED, "%s: %lld (sequence, head) rows exceed the grid", who, (long long)(B * heads));
   a.lengths = lengths;
   a.weights = weights;
@@ -194,7 +283,7 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<uint32_t>(B * heads)), dim3(kSelThreads), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
   if (a.most == 0) return AEKV_OK;  // keep = 0: nothing stays, nothing moves
-  const int64_t per = ceil_div(a.most, 16);
+  const int64_t per = ceil_div(a.most, 16 * kMoves);
   const dim3 grid(static_cast<uint32_t>(per < 64 ? per : 64), static_cast<uint32_t>(B * heads));
   const int row = d * bits / 8;
   auto fn = row == 32 ? evict_move_kernel<32> : row == 64 ? evict_move_kernel<64> : evict_move_kernel<128>;

@@ -50,10 +50,11 @@ struct PagedArgs {
   const float* sink;                 // [H] or null
   float* weights;                    // [B, heads, capacity] or null
   float* lse;                        // [B, T, H], log2 units, inf for a sum of 0 (with weights)
+  float* logits;                     // [B, heads, rows, logit_slots], log2 units, -inf where hidden; or null
   float* part;                       // [B, T, H, n_split, D + 4]: max, sum (log2 units), 2 pad, rotated output
   void* out;                         // [B, T, H, D]
   int32_t reach;                     // slots of a sequence that can be seen: the table's, or the tracker's capacity
-  int64_t capacity;
+  int64_t capacity, logit_slots;
   int32_t T, H, G, rows, row_blocks, n_split;
   float scale2, wscale;              // softmax scale * log2(e), fp32(D^-1/2)
 };
@@ -360,6 +361,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
             hide[k][j] = ((bad[w] >> k) & 1u) || base + 16 * k + 4 * g + j >= sees[t];
             x[k][j] = hide[k][j] ? kNegInf : x[k][j];
           }
+      if (a.logits && row[t] < a.rows) {
+        float* lg = a.logits + ((b * a.pool.heads + kh) * a.rows + row[t]) * a.logit_slots + base + 4 * g;
+        *reinterpret_cast<f32x4_t*>(lg) = x[0];
+        *reinterpret_cast<f32x4_t*>(lg + 16) = x[1];
+      }
       float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
       top = fmaxf(top, xor_lane<16>(top));
       top = fmaxf(top, xor_lane<32>(top));
@@ -565,6 +571,22 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   if (a.lse && lane == 0) a.lse[orow] = sum == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(sum);
 }
 
+// The weights of a sequence's slots from the logits that the attention left and the rows' log sums: a thread per slot.
+__global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blocks) {
+  const int32_t j = static_cast<int32_t>(blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int64_t bk = blockIdx.x / blocks, b = bk / a.pool.heads;
+  const int32_t kh = static_cast<int32_t>(bk - b * a.pool.heads);
+  if (j >= newest_sees(a, b)) return;
+  const float* lg = a.logits + bk * a.rows * a.logit_slots + j;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int32_t r = 0; r < a.rows; ++r) {
+    const int32_t t = r / a.G;
+    sum += __builtin_amdgcn_exp2f(lg[r * a.logit_slots] - a.lse[(b * a.T + t) * a.H + kh * a.G + (r - t * a.G)]);
+  }
+  if (sum != 0.0f) a.weights[bk * a.capacity + j] += sum;
+}
+
 // The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
 // row of the KV head's group, 16 at a time (their query parts in LDS), and adds the sums over the rows.
 constexpr int kWeightTiles = 4;  // row tiles whose parts LDS holds at a time
@@ -609,19 +631,25 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
       }
     }
     __syncthreads();
-    int32_t pages = -1;
+    int32_t pages = -1, g0 = -1, g1 = -1;
+    StepData<D, BITS> s, next;
+    auto load = [&](int i) __attribute__((always_inline)) {
+      if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+      g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
+      load_step<D, BITS, false>(a, kh, first + kRound * i, g0, g1, lane, next);
+    };
+    if (n_steps > 0) load(0);
 #pragma unroll 1
     for (int i = 0; i < n_steps; ++i) {
-      if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
-      const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
       const int32_t base = first + kRound * i;
-      StepData<D, BITS> s;
-      load_step<D, BITS, false>(a, kh, base, g0, g1, lane, s);
+      s = next;
+      const uint32_t bad = (g0 < 0 ? 1u : 0u) | (g1 < 0 ? 2u : 0u);
       f16x8_t kc[2][NC];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int c = 0; c < NC; ++c) kc[k][c] = codes_f16<BITS>(&s.k[k][c * BITS / 4]);
+      if (i + 1 < n_steps) load(i + 1);
       f32x4_t sum[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
       for (int t = 0; t < nt; ++t) {
         f16x8_t hi[NC], lo[NC];
@@ -635,7 +663,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool hide = (k ? g1 : g0) < 0 || base + 16 * k + 4 * g + j >= sees;
+            const bool hide = ((bad >> k) & 1u) || base + 16 * k + 4 * g + j >= sees;
             sum[k][j] += hide ? 0.0f : __builtin_amdgcn_exp2f(x[k][j] - lse);
           }
       }
@@ -653,7 +681,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
         }
         const int j = lane & 15;
         const int32_t slot = base + 16 * k + 4 * g + j;
-        if (j < 4 && slot < p1 && (k ? g1 : g0) >= 0) {
+        if (j < 4 && slot < p1 && !((bad >> k) & 1u)) {
           const float v = j == 0 ? sum[k][0] : j == 1 ? sum[k][1] : j == 2 ? sum[k][2] : sum[k][3];
           if (v != 0.0f) weights[slot] += v;
         }
@@ -688,6 +716,14 @@ int64_t paged_pieces(int64_t groups, int64_t slots) {
 // Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.
 int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 : 1; }
 
+// Tracked calls of few rows keep their logits and sum them afterwards; of many rows the scores are computed again, which
+// reads a slot's K codes instead of 8 bytes a row.
+size_t paged_logit_bytes(int64_t B, int64_t heads, int64_t rows, int64_t slots) {
+  if (rows > 16) return 0;
+  const double bytes = 4.0 * static_cast<double>(B) * heads * rows * static_cast<double>(slots + 32);
+  return bytes > 2147483648.0 ? 0 : static_cast<size_t>(B * heads * rows) * align_up(static_cast<size_t>(slots), 32) * 4;
+}
+
 }  // namespace
 }  // namespace aekv
 
@@ -698,7 +734,7 @@ extern "C" size_t aekv_paged_attention_workspace_size(int64_t B, int64_t T, int6
   if (B <= 0 || T <= 0 || H <= 0 || heads <= 0 || d <= 0 || slots <= 0) return 0;
   const int64_t rows = T * (H / heads), blocks = ceil_div(rows, 16 * paged_row_tiles(rows, d));
   const int64_t n = paged_pieces(B * heads * blocks, slots);
-  return (tracked ? align_up(static_cast<size_t>(B * T * H) * 4, 16) : 0) +
+  return (tracked ? align_up(static_cast<size_t>(B * T * H) * 4, 16) + paged_logit_bytes(B, heads, rows, slots) : 0) +
          (n > 1 ? static_cast<size_t>(B * T * H) * static_cast<size_t>(n) * (d + 4) * 4 : 0);
 }
 
@@ -743,7 +779,12 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   a.sink = sink;
   a.weights = reach > 0 ? weights : nullptr;
   a.lse = a.weights ? static_cast<float*>(ws) : nullptr;
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (weights ? align_up(static_cast<size_t>(B * T * H) * 4, 16) : 0));
+  // the workspace: the rows' log sums, the logits, the pieces
+  const size_t lse_bytes = weights ? align_up(static_cast<size_t>(B * T * H) * 4, 16) : 0;
+  const size_t logit_bytes = weights ? paged_logit_bytes(B, heads, rows, slots) : 0;
+  a.logits = a.weights && logit_bytes ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + lse_bytes) : nullptr;
+  a.logit_slots = static_cast<int64_t>(align_up(static_cast<size_t>(slots), 32));
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + lse_bytes + logit_bytes);
   a.out = out;
   a.reach = static_cast<int32_t>(reach);
   a.capacity = capacity;
@@ -766,6 +807,11 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
     if (const int rc = check_launch(who)) return rc;
   }
   if (!a.weights) return AEKV_OK;
+  if (a.logits) {
+    const int32_t per = static_cast<int32_t>(ceil_div(reach, 256));
+    hipLaunchKernelGGL(paged_add_kernel, dim3(static_cast<uint32_t>(B * heads * per)), dim3(256), 0, st, a, per);
+    return check_launch(who);
+  }
   a.n_split = static_cast<int32_t>(paged_pieces(B * heads, slots));
   auto wf = dtype == AEKV_F16 ? pick_weights<AEKV_F16>(d, bits) : pick_weights<AEKV_BF16>(d, bits);
   hipLaunchKernelGGL(wf, dim3(static_cast<uint32_t>(B * heads * a.n_split)), dim3(kThreads), 0, st, a);
