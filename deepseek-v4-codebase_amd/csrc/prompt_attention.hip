@@ -6,7 +6,7 @@
 // A query that sees nothing gives 0 and a log sum of the sink's, or -inf.
 //
 // Work split.  The G heads of a KV head's group share its keys: the rows of a sequence and KV head are (query, head),
-// query-major, and a workgroup takes 32 RB WR consecutive ones, 32 RB per wave.  Tiles of 64 keys and values stream through
+// query-major, and a workgroup takes 32 WR consecutive ones, 32 per wave.  Tiles of 64 keys and values stream through
 // two LDS buffers, loaded one tile ahead straight into LDS; with KS = 2 two waves share a row group and take half of every
 // tile each, merged at the end.  One pass: running maximum and sum, the output rescaled only where a maximum moved by more
 // than kMargin (weights up to 2^kMargin are as exact in 16 bits as those up to 1, and the sums are fp32).
@@ -36,6 +36,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short i16x4_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 typedef __attribute__((address_space(3))) void lds_void_t;
 
@@ -51,7 +52,8 @@ struct PromptArgs {
   float* lse;           // [n_q, H] or null
   int32_t n_q, n_k, B, H, heads, G;
   int32_t clear;        // rows in no sequence: 0 to leave out as it is, 1 to write zeros
-  float scale2;         // softmax scale * log2(e)
+  float scale2;         // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
+  int32_t flip;         // scale is negative the queries' signs are flipped: a row's largest product is its largest logit
 };
 
 template <int DT>
@@ -59,7 +61,7 @@ struct Elem;
 template <>
 struct Elem<AEKV_BF16> {
   typedef bf16x8_t v8;
-  static constexpr uint32_t kExp = 0x7F807F80u;  // the exponents of a pair
+  static constexpr uint32_t kExp = 0x7F80u;  // infinity; NaN above it
   __device__ static f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   __device__ static float value(uint32_t u) { return bf16_to_f32(u); }
@@ -67,7 +69,7 @@ struct Elem<AEKV_BF16> {
 template <>
 struct Elem<AEKV_F16> {
   typedef f16x8_t v8;
-  static constexpr uint32_t kExp = 0x7C007C00u;
+  static constexpr uint32_t kExp = 0x7C00u;
   __device__ static f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16); }
   __device__ static float value(uint32_t u) { return f16_to_f32(u); }
@@ -119,12 +121,12 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int64_t t, int ro
   return false;
 }
 
-template <int DT, int D, int RB, int WR, int KS>
-__global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB == 2 ? 1 : 2))) void prompt_attention_kernel(PromptArgs a) {
+template <int DT, int D, int WR, int KS>
+__global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2))) void prompt_attention_kernel(PromptArgs a) {
   using E = Elem<DT>;
   using Gm = PromptGeom<D>;
   using v8 = typename E::v8;
-  constexpr int kWaves = WR * KS, kRows = 32 * RB * WR, kRow = Gm::kRow;
+  constexpr int kWaves = WR * KS, kRows = 32 * WR, kRow = Gm::kRow;
   constexpr int kKB = 2 / KS;                              // 32-key blocks of a tile per wave
   constexpr int kPass = 1024 * kWaves;                     // bytes that the workgroup stages at a time
   constexpr int kPasses = Gm::kTileBytes / kPass;
@@ -168,22 +170,19 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB
   const int n_tiles = (n_keys + kTile - 1) / kTile;
 
   // rows past the last are computed as copies of it
-  int32_t row[RB];
-  int32_t sees[RB];
-  v8 qb[RB][kKSteps];
-  const int32_t w0 = row0 + 32 * RB * wr;  // the wave's first row
+  const int32_t w0 = row0 + 32 * wr;  // the wave's first row
+  v8 qb[kKSteps];
+  const int32_t row = w0 + rl, own = row < n_rows ? row : n_rows - 1;
+  const int32_t sees = sees_of(own), qi = own / a.G, h = head * a.G + (own - qi * a.G);
+  const uint16_t* qp = a.q + static_cast<int64_t>(q0 + qi) * a.q_token + h * a.q_head + 8 * hh;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    row[rb] = w0 + 32 * rb + rl;
-    const int32_t r = row[rb] < n_rows ? row[rb] : n_rows - 1;
-    sees[rb] = sees_of(r);
-    const int32_t qi = r / a.G;
-    const uint16_t* qp = a.q + static_cast<int64_t>(q0 + qi) * a.q_token + static_cast<int64_t>(head * a.G + (r - qi * a.G)) * a.q_head + 8 * hh;
-#pragma unroll
-    for (int ks = 0; ks < kKSteps; ++ks) qb[rb][ks] = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
+  for (int ks = 0; ks < kKSteps; ++ks) {
+    uint4 w = *reinterpret_cast<const uint4*>(qp + 16 * ks);
+    if (a.flip) w.x ^= 0x80008000u, w.y ^= 0x80008000u, w.z ^= 0x80008000u, w.w ^= 0x80008000u;
+    qb[ks] = __builtin_bit_cast(v8, w);
   }
   const int32_t wave_least = __builtin_amdgcn_readfirstlane(sees_of(w0 < n_rows ? w0 : n_rows - 1));
-  const int32_t wl = w0 + 32 * RB - 1;
+  const int32_t wl = w0 + 31;
   const int32_t wave_most = __builtin_amdgcn_readfirstlane(sees_of(wl < n_rows ? wl : n_rows - 1));
 
   // staging: pass c of wave wv writes bytes [kPass c + 1024 wv, + 1024) of a tile, lane l at + 16 l, so lane l loads the
@@ -231,118 +230,120 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB
     }
   }
 
-  float m[RB], l[RB];
-  f32x16_t O[RB][kMB];
+  float m = kNegInf, l = 0.0f;
+  f32x16_t O[kMB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m[rb] = kNegInf, l[rb] = 0.0f;
-#pragma unroll
-    for (int mb = 0; mb < kMB; ++mb) O[rb][mb] = f32x16_t{};
-  }
+  for (int mb = 0; mb < kMB; ++mb) O[mb] = f32x16_t{};
 
   // one tile; `masked`: some row of the wave does not see all of it
   auto tile = [&](int it, const uint8_t* kt, auto masked_c) __attribute__((always_inline)) {
     constexpr bool masked = decltype(masked_c)::value;
     const uint8_t* vt = kt + Gm::kTileBytes;
     const int base = it * kTile + 32 * kKB * kh;
-#pragma unroll masked ? 1 : kKB
-    for (int kb = 0; kb < kKB; ++kb) {
-      f32x16_t s[RB];
+    f32x16_t s[kKB];
+    float top = kNegInf;
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16_t{};
+    for (int kb = 0; kb < kKB; ++kb) {
+      s[kb] = f32x16_t{};
 #pragma unroll
       for (int ks = 0; ks < kKSteps; ++ks) {
         const v8 ka = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(kt + 32 * kRow * kb + (sA ^ (ks << 5))));
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb] = E::mma(ka, qb[rb][ks], s[rb]);
+        s[kb] = E::mma(ka, qb[ks], s[kb]);
       }
-      v8 pb[RB][2];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float top = kNegInf;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          if constexpr (masked) {
-            const int key = base + 32 * kb + 8 * (v >> 2) + 4 * hh + (v & 3);
-            s[rb][v] = key < sees[rb] ? s[rb][v] * a.scale2 : kNegInf;
-            top = fmaxf(top, s[rb][v]);
-          } else {
-            s[rb][v] *= a.scale2;
-            top = fmaxf(top, s[rb][v]);
-          }
+      for (int v = 0; v < 16; ++v) {
+        if constexpr (masked) {
+          const int key = base + 32 * kb + 8 * (v >> 2) + 4 * hh + (v & 3);
+          s[kb][v] = key < sees ? s[kb][v] : kNegInf;
         }
-        top = fmaxf(top, xor_lane<32>(top));
-        // (nothing yet: any maximum counts as moved)
-        if (__builtin_amdgcn_ballot_w64(top > m[rb] + kMargin)) {
-          const float up = fmaxf(m[rb], top);
-          const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[rb] - up);
-          l[rb] *= r;
-#pragma unroll
-          for (int mb = 0; mb < kMB; ++mb) O[rb][mb] *= r;
-          m[rb] = up;
-        }
-        const float nm = m[rb] == kNegInf ? 0.0f : -m[rb];
-        float p[16];
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          p[v] = __builtin_amdgcn_exp2f(s[rb][v] + nm);
-          l[rb] += p[v];
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          pb[rb][c] = __builtin_bit_cast(v8, make_uint4(E::pack(p[8 * c], p[8 * c + 1]), E::pack(p[8 * c + 2], p[8 * c + 3]),
-                                                        E::pack(p[8 * c + 4], p[8 * c + 5]), E::pack(p[8 * c + 6], p[8 * c + 7])));
+        top = fmaxf(top, s[kb][v]);
       }
-      bool odd = false;
+    }
+    top = fmaxf(top, xor_lane<32>(top)) * a.scale2;
+    // (nothing yet: any maximum counts as moved)
+    if (__builtin_amdgcn_ballot_w64(top > m + kMargin)) {
+      const float up = fmaxf(m, top);
+      const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+      l *= r;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint8_t* vc = vt + (32 * kb + 16 * c) * kRow;
+      for (int mb = 0; mb < kMB; ++mb) O[mb] *= r;
+      m = up;
+    }
+    const float nm = m == kNegInf ? 0.0f : -m;
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb) {
+      float p[16];
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        p[v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], a.scale2, nm));
+        l += p[v];
+      }
+      v8 pb[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        pb[c] = __builtin_bit_cast(v8, make_uint4(E::pack(p[8 * c], p[8 * c + 1]), E::pack(p[8 * c + 2], p[8 * c + 3]),
+                                                  E::pack(p[8 * c + 4], p[8 * c + 5]), E::pack(p[8 * c + 6], p[8 * c + 7])));
+      u32x4_t w[2][kMB];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int mb = 0; mb < kMB; ++mb) {
+          const uint8_t* vc = vt + (32 * kb + 16 * c) * kRow;
           const i16x4_t lo = read_tr16(vc + (tA[0] ^ (mb << 6))), hi = read_tr16(vc + (tA[1] ^ (mb << 6)));
-          u32x4_t w = __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          if constexpr (masked) {
-            // a value that is no finite number must not reach rows that do not see it (0 times it is no 0): it goes in
-            // as 0, and is added below to the rows that do
+          w[c][mb] = __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      bool odd = false;
+      if constexpr (masked) {
+        // a value that is no finite number must not reach rows that do not see it (0 times it is no 0): it goes in as 0,
+        // and is added below to the rows that do
+        u16x2_t most = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool b0 = (w[i] & E::kExp & 0xffffu) == (E::kExp & 0xffffu), b1 = (w[i] & E::kExp & 0xffff0000u) == (E::kExp & 0xffff0000u);
-              odd = odd || b0 || b1;
-              w[i] = (b0 ? 0u : w[i] & 0xffffu) | (b1 ? 0u : w[i] & 0xffff0000u);
-            }
-          }
-          const v8 va = __builtin_bit_cast(v8, w);
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) O[rb][mb] = E::mma(va, pb[rb][c], O[rb][mb]);
+          for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[c][mb][i] & 0x7FFF7FFFu));
+        odd = __builtin_amdgcn_ballot_w64(most[0] >= E::kExp || most[1] >= E::kExp);
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t u = w[c][mb][i];
+                w[c][mb][i] = ((u & 0x7FFFu) >= E::kExp ? 0u : u & 0xFFFFu) | (((u >> 16) & 0x7FFFu) >= E::kExp ? 0u : u & 0xFFFF0000u);
+              }
         }
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int mb = 0; mb < kMB; ++mb) O[mb] = E::mma(__builtin_bit_cast(v8, w[c][mb]), pb[c], O[mb]);
       if constexpr (masked) {
-        if (__builtin_amdgcn_ballot_w64(odd)) {
+        if (odd) {
+          __builtin_amdgcn_wave_barrier();
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            __builtin_amdgcn_wave_barrier();
+          for (int c = 0; c < 2; ++c) {  // element j of lane half h is key 16 c + 4 h + j, or 16 c + 8 + 4 h + j - 4
+            const u32x4_t u = __builtin_bit_cast(u32x4_t, pb[c]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {  // element j of lane half h is key 16 c + 4 h + j, or 16 c + 8 + 4 h + j - 4
-              const u32x4_t u = __builtin_bit_cast(u32x4_t, pb[rb][c]);
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                s_p[wv][16 * c + 8 * (j >> 2) + 4 * hh + (j & 3)][rl] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
-            }
-            __builtin_amdgcn_wave_barrier();
+            for (int j = 0; j < 8; ++j)
+              s_p[wv][16 * c + 8 * (j >> 2) + 4 * hh + (j & 3)][rl] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+          }
+          __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-            for (int key = 0; key < 32; ++key) {
-              const float p = E::value(s_p[wv][key][rl]);
-              const bool in = base + 32 * kb + key < sees[rb];
-              const int kr = 32 * kKB * kh + 32 * kb + key;
+          for (int key = 0; key < 32; ++key) {
+            const float pk = E::value(s_p[wv][key][rl]);
+            const bool in = base + 32 * kb + key < sees;
+            const int kr = 32 * kKB * kh + 32 * kb + key;
 #pragma unroll
-              for (int mb = 0; mb < kMB; ++mb)
+            for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                  const int d = 32 * mb + 8 * (v >> 2) + 4 * hh + (v & 3);
-                  const uint32_t x = *reinterpret_cast<const uint16_t*>(vt + kr * kRow + (((d >> 3) ^ swizzle<D>(kr & 15)) << 4) + 2 * (d & 7));
-                  if (in && (x & (E::kExp & 0xffffu)) == (E::kExp & 0xffffu)) O[rb][mb][v] += p * E::value(x);
-                }
-            }
+              for (int v = 0; v < 16; ++v) {
+                const int d = 32 * mb + 8 * (v >> 2) + 4 * hh + (v & 3);
+                const uint32_t x = *reinterpret_cast<const uint16_t*>(vt + kr * kRow + (((d >> 3) ^ swizzle<D>(kr & 15)) << 4) + 2 * (d & 7));
+                if (in && (x & 0x7FFFu) >= E::kExp) O[mb][v] += pk * E::value(x);
+              }
           }
         }
       }
@@ -364,11 +365,10 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB
     step(it, std::integral_constant<int, 0>{});
     if (it + 1 < n_tiles) step(it + 1, std::integral_constant<int, 1>{});
   }
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) l[rb] += xor_lane<32>(l[rb]);  // both halves' keys
+  l += xor_lane<32>(l);  // both halves' keys
 
   if constexpr (KS == 2) {  // the second key half's states into the first's, through the tile buffers
-    static_assert(RB == 1 && WR * kMB * 16 * 64 * 4 + WR * 2 * 64 * 4 <= 4 * Gm::kTileBytes, "the states fit both buffers");
+    static_assert(WR * kMB * 16 * 64 * 4 + WR * 2 * 64 * 4 <= 4 * Gm::kTileBytes, "the states fit both buffers");
     __syncthreads();
     constexpr int kPer = kMB * 16 * 64, kFit = 2 * Gm::kTileBytes / 4;  // floats
     auto slot = [&](int i) -> float* { return i < kFit ? reinterpret_cast<float*>(L0) + i : reinterpret_cast<float*>(L1) + (i - kFit); };
@@ -378,50 +378,45 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(RB
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) slot(at + (mb * 16 + v) * 64)[lane] = O[0][mb][v];
-      slot(at + kPer)[lane] = m[0];
-      slot(at + kPer + 64)[lane] = l[0];
+        for (int v = 0; v < 16; ++v) slot(at + (mb * 16 + v) * 64)[lane] = O[mb][v];
+      slot(at + kPer)[lane] = m;
+      slot(at + kPer + 64)[lane] = l;
     }
     __syncthreads();
     if (kh == 1) return;
     const float m1 = slot(at + kPer)[lane], l1 = slot(at + kPer + 64)[lane];
-    const float up = fmaxf(m[0], m1);
+    const float up = fmaxf(m, m1);
     // (a state of nothing has a sum of 0; NaN alone leaves a maximum of -inf, and a sum that says so)
-    const float f0 = l[0] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[0] - up), f1 = l1 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m1 - up);
-    l[0] = (l[0] == 0.0f ? 0.0f : l[0] * f0) + (l1 == 0.0f ? 0.0f : l1 * f1);
-    m[0] = up;
+    const float f0 = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - up), f1 = l1 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m1 - up);
+    l = (l == 0.0f ? 0.0f : l * f0) + (l1 == 0.0f ? 0.0f : l1 * f1);
+    m = up;
 #pragma unroll
     for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) O[0][mb][v] = O[0][mb][v] * f0 + slot(at + (mb * 16 + v) * 64)[lane] * f1;
+      for (int v = 0; v < 16; ++v) O[mb][v] = O[mb][v] * f0 + slot(at + (mb * 16 + v) * 64)[lane] * f1;
   }
+  if (row >= n_rows) return;
+  const int64_t orow = static_cast<int64_t>(q0 + qi) * a.H + h;
+  const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+  const float up = fmaxf(m, sk);
+  const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - up);
+  const float sum = (l == 0.0f ? 0.0f : l * f) + (sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - up));
+  const float r = sum == 0.0f ? 0.0f : f / sum;
+  uint16_t* op = a.out + orow * D + 4 * hh;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    if (row[rb] >= n_rows) continue;
-    const int32_t qi = row[rb] / a.G;
-    const int32_t h = head * a.G + (row[rb] - qi * a.G);
-    const int64_t orow = static_cast<int64_t>(q0 + qi) * a.H + h;
-    const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
-    const float up = fmaxf(m[rb], sk);
-    const float f = l[rb] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[rb] - up);
-    const float sum = (l[rb] == 0.0f ? 0.0f : l[rb] * f) + (sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - up));
-    const float r = sum == 0.0f ? 0.0f : f / sum;
-    uint16_t* op = a.out + orow * D + 4 * hh;
+  for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
-    for (int mb = 0; mb < kMB; ++mb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint2*>(op + 32 * mb + 8 * i) = make_uint2(E::pack(O[rb][mb][4 * i] * r, O[rb][mb][4 * i + 1] * r),
-                                                                     E::pack(O[rb][mb][4 * i + 2] * r, O[rb][mb][4 * i + 3] * r));
-    if (a.lse && hh == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
-  }
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint2*>(op + 32 * mb + 8 * i) = make_uint2(E::pack(O[mb][4 * i] * r, O[mb][4 * i + 1] * r),
+                                                                   E::pack(O[mb][4 * i + 2] * r, O[mb][4 * i + 3] * r));
+  if (a.lse && hh == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 using prompt_fn = void (*)(PromptArgs);
-template <int RB, int WR, int KS>
+template <int WR, int KS>
 prompt_fn pick_prompt(int32_t dtype, int32_t d) {
-  if (dtype == AEKV_F16) return d == 64 ? prompt_attention_kernel<AEKV_F16, 64, RB, WR, KS> : prompt_attention_kernel<AEKV_F16, 128, RB, WR, KS>;
-  return d == 64 ? prompt_attention_kernel<AEKV_BF16, 64, RB, WR, KS> : prompt_attention_kernel<AEKV_BF16, 128, RB, WR, KS>;
+  if (dtype == AEKV_F16) return d == 64 ? prompt_attention_kernel<AEKV_F16, 64, WR, KS> : prompt_attention_kernel<AEKV_F16, 128, WR, KS>;
+  return d == 64 ? prompt_attention_kernel<AEKV_BF16, 64, WR, KS> : prompt_attention_kernel<AEKV_BF16, 128, WR, KS>;
 }
 
 }  // namespace
@@ -458,15 +453,14 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
                q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q, cu_seqlens_k, sink,
                static_cast<uint16_t*>(out), lse, static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B),
                static_cast<int32_t>(H), static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
-               softmax_scale * kLog2e};
-  // large launches take 256 rows per workgroup, the others 64
+               fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f};
   const int64_t rows = n_q * (H / heads);
-  const bool large = heads * (rows / 256) >= 512;
-  const int per = large ? 256 : 64;
+  const bool large = heads * (rows / 128) >= 512;
+  const int per = large ? 128 : 64;
   const int64_t tiles = rows / per + B;  // at least every sequence's, whatever their lengths
   if (tiles * heads > kMaxGridThreads / 256)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld H=%lld exceed the grid", who, (long long)B, (long long)n_q, (long long)H);
-  auto fn = large ? pick_prompt<2, 4, 1>(dtype, d) : pick_prompt<1, 2, 2>(dtype, d);
+  auto fn = large ? pick_prompt<4, 1>(dtype, d) : pick_prompt<2, 2>(dtype, d);
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(tiles * heads)), dim3(256), 0, as_stream(stream), a);
   return check_launch(who);
 }

@@ -197,3 +197,37 @@ def test_prompt_refusals(dev):
         prompt_attention(q, k, v, cu, 0.09, out=torch.empty(50, 4, 64, dtype=torch.bfloat16, device=dev))
     with pytest.raises(RuntimeError):
         prompt_attention(q, k, v, cu, 0.09, cu_seqlens_k=torch.zeros(3, dtype=torch.int32, device=dev))
+
+
+@pytest.mark.parametrize("dtype,dim,H,hk,lens", [(torch.bfloat16, 128, 16, 8, [3000, 1, 1203, 64]), (torch.float16, 64, 32, 8, [2500]), (torch.bfloat16, 64, 24, 12, [700] * 5)])
+def test_prompt_many_rows(dev, dtype, dim, H, hk, lens):
+    """Launches of many rows take larger row tiles: sampled rows of every sequence against the plain form in 64 bits."""
+    q, k, v = _inputs(dev, 20, dtype, dim, H, hk, lens, lens, pad=2)
+    cu = _cu(lens)
+    scale = dim ** -0.5
+    out, lse = prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=dev), scale, return_lse=True)
+    assert not out[cu[-1]:].any() and (lse[cu[-1]:] == -math.inf).all()
+    for b, n in enumerate(lens):
+        kk, vv = (x[cu[b]:cu[b + 1]].cpu() for x in (k, v))
+        rows = sorted({0, n - 1, n // 2, *(int(i) for i in torch.randint(0, n, (6,), generator=torch.Generator().manual_seed(b)))})
+        for i in rows:
+            one = q[cu[b] + i:cu[b] + i + 1].cpu()
+            want, bound, wl, lb = R.prompt_attention_ref(one, kk[:i + 1], vv[:i + 1], [0, 1], [0, i + 1], scale)
+            R.within(out[cu[b] + i:cu[b] + i + 1], want, bound, f"row {i} of {b}")
+            R.within(lse[cu[b] + i:cu[b] + i + 1].double().cpu(), wl, lb, f"lse of row {i} of {b}")
+
+
+def test_prompt_many_rows_masked_places(dev):
+    """The larger row tiles keep what a row does not see out of it as the others do."""
+    lens, H, hk, dim = [2300, 2000], 16, 8, 128
+    q, k, v = (x.clone() for x in _inputs(dev, 21, torch.bfloat16, dim, H, hk, lens, lens, pad=5))
+    cu = torch.tensor(_cu(lens), dtype=torch.int32, device=dev)
+    clean = prompt_attention(q, k, v, cu, 0.09)
+    for x in (k, v):
+        x[4300:] = NAN
+        x[1111, 3] = NAN
+        x[2300 + 1990] = math.inf
+    got = prompt_attention(q, k, v, cu, 0.09)
+    assert torch.equal(got[:1111], clean[:1111]) and torch.equal(got[2300:2300 + 1990], clean[2300:2300 + 1990])
+    assert torch.equal(got[1111:2300, :6], clean[1111:2300, :6]) and torch.equal(got[1111:2300, 8:], clean[1111:2300, 8:])
+    assert got[1111:2300, 6:8].isnan().all()
