@@ -4,10 +4,12 @@
 // Reference: the encode is aether_2b/turbo_quant.py:127-166; the reference engine appends coded blocks with torch.cat
 // (aether_2b/serving.py:327-346).
 //
-// D / 8 lanes hold one vector, 8 elements each (one 16-byte load of a 16-bit type); the lanes of a vector store its codes
-// contiguously.
+// Two layouts, bit for bit alike.  Small calls (and fp32): D / 8 lanes hold one vector, 8 elements each, so that a decode
+// step's few vectors spread over many waves; bound by the chain of a wave (load, exchanges, divisions, store).  Large
+// calls: 32 elements to a lane (tq_fast_lane.h), a wave taking VPW consecutive tokens of one head of K or V, so that it
+// reads whole rows and writes its codes contiguously; bound by the reads and writes.
 #include "paged_cache.h"
-#include "tq_device.h"
+#include "tq_fast_lane.h"
 
 namespace aekv {
 namespace {
@@ -75,13 +77,113 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   }
 }
 
-template <int DT>
+constexpr int kTableThreads = 256;
+
+// Sequence and place of token n (packed: sequences from b0 on are searched).
+__device__ __forceinline__ int64_t token_slot(const AppendArgs& a, int64_t n, int64_t* b, int64_t* at) {
+  *b = a.cu ? packed_sequence(a.cu, a.B, n) : n / a.per_seq;
+  if (*b < 0) return -1;
+  *at = a.cu ? n - a.cu[*b] : n - *b * a.per_seq;
+  return a.start[*b] + *at;
+}
+
+template <int DT, int D, int BITS>
+__global__ __launch_bounds__(kTableThreads, 4) void kv_append_rows_kernel(AppendArgs a, float cq) {
+  using F = FastEnc<BITS, D>;
+  constexpr int LPV = F::LPV, VPW = F::VPW, NW = F::LB / 4;
+  const int lane = threadIdx.x & 63;
+  const int v = lane / LPV, g = lane % LPV;
+  __shared__ uint4 dm_tab[LPV][4];  // diag sign masks of a lane part's 16 packed words
+  if (threadIdx.x < 16 * LPV) {
+    const int gg = threadIdx.x >> 4, k = threadIdx.x & 15;
+    reinterpret_cast<uint32_t*>(dm_tab[gg])[k] = (a.diag[32 * gg + 2 * k] < 0.0f ? 0x8000u : 0u) |
+                                                (a.diag[32 * gg + 2 * k + 1] < 0.0f ? 0x80000000u : 0u);
+  }
+  __syncthreads();
+  // the wave's tokens, head, and K or V (neighbouring waves take neighbouring heads: whole token rows are read together)
+  const uint32_t heads = static_cast<uint32_t>(a.pool.heads);
+  const uint32_t grp = blockIdx.x * (kTableThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tile = grp / (2 * heads), kh = grp - tile * 2 * heads;
+  const bool is_v = kh >= heads;
+  const int32_t h = static_cast<int32_t>(is_v ? kh - heads : kh);
+  const int64_t n0 = static_cast<int64_t>(tile) * VPW;
+  if (n0 >= a.n_tokens) return;
+  const uint8_t* x = static_cast<const uint8_t*>(is_v ? a.v : a.k) + (is_v ? h * a.v_head : h * a.k_head) * 2;
+  const int64_t stride = (is_v ? a.v_token : a.k_token) * 2;
+  uint8_t* codes = is_v ? a.pool.v_codes : a.pool.k_codes;
+  float* scale = is_v ? a.pool.v_scale : a.pool.k_scale;
+  const int64_t n = n0 + v < a.n_tokens ? n0 + v : a.n_tokens - 1;  // (a last tile's spare lanes read its last token)
+  uint32_t w[16];
+  {
+    const uint4* p = reinterpret_cast<const uint4*>(x + n * stride + 64 * g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 t = p[i];
+      w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+    }
+  }
+  int64_t b = -1, at = 0;
+  const int64_t slot = token_slot(a, n, &b, &at);
+  const int64_t row = n0 + v < a.n_tokens && b >= 0 ? cache_row(a.pool, b, h, slot) : -1;
+  if (row >= 0 && g == 0 && !is_v && a.weights && slot < a.capacity) {
+    const int64_t t = (b * heads + h) * a.capacity + slot;
+    a.weights[t] = 0.0f;
+    a.tokens[t] = a.token[b] + static_cast<int32_t>(at);
+  }
+  uint32_t dm[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 d = dm_tab[g][i];
+    dm[4 * i] = d.x, dm[4 * i + 1] = d.y, dm[4 * i + 2] = d.z, dm[4 * i + 3] = d.w;
+  }
+  auto exact = [&] {  // the wave's vectors by the other layout, read again
+    constexpr int EPL = 8, LPV8 = D / EPL, NB = BITS == 8 ? EPL : EPL / 2;
+    const int sub = lane % LPV8;
+#pragma unroll 1
+    for (int i = lane / LPV8; i < VPW; i += 64 / LPV8) {
+      const bool in = n0 + i < a.n_tokens;
+      float e[EPL], m;
+      load_elems<DT, EPL>(x + (n0 + i) * stride, sub * EPL, in, e);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) e[j] *= a.diag[sub * EPL + j];
+      const Bytes<NB> c = encode_lane<BITS, D, false>(e, sub, a.wscale, &m);
+      int64_t bb = -1, aa = 0;
+      const int64_t s = in ? token_slot(a, n0 + i, &bb, &aa) : -1;
+      const int64_t r = bb >= 0 ? cache_row(a.pool, bb, h, s) : -1;
+      if (r >= 0) {
+        *reinterpret_cast<Bytes<NB>*>(codes + r * F::RB + sub * NB) = c;
+        if (sub == 0) scale[r] = m / F::Q;
+      }
+    }
+  };
+  auto store = [&](const uint32_t (&o)[NW], float m) {
+    if (row < 0) return;
+    uint4* p = reinterpret_cast<uint4*>(codes + row * F::RB + g * F::LB);
+#pragma unroll
+    for (int i = 0; i < NW / 4; ++i) p[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    if (g == 0) scale[row] = m / F::Q;
+  };
+  fast_encode_lane<DT, BITS, D>(w, dm, g, a.wscale, cq, exact, store);
+}
+
+// Elements of K and V together from which a call takes the second layout (4-bit D = 128 / 8-bit D = 64, first against
+// second: 524288 elements 3.7 / 3.5 and 4.4 / 4.7 us, 1048576 4.0 / 3.9 and 4.8 / 4.7, 2097152 4.9 / 4.8 and 4.8 / 5.0;
+// a prompt batch of 98 M elements, 334 MB, 176 and 81 us, 4.1 TB/s).
+constexpr int64_t kRowsElements = int64_t(1) << 21;
+
 using append_fn = void (*)(AppendArgs);
+using rows_fn = void (*)(AppendArgs, float);
 
 template <int DT>
-append_fn<DT> pick_append(int d, int bits) {
+append_fn pick_append(int d, int bits) {
   if (d == 64) return bits == 8 ? kv_append_kernel<DT, 64, 8> : kv_append_kernel<DT, 64, 4>;
   return bits == 8 ? kv_append_kernel<DT, 128, 8> : kv_append_kernel<DT, 128, 4>;
+}
+
+template <int DT>
+rows_fn pick_rows(int d, int bits) {
+  if (d == 64) return bits == 8 ? kv_append_rows_kernel<DT, 64, 8> : kv_append_rows_kernel<DT, 64, 4>;
+  return bits == 8 ? kv_append_rows_kernel<DT, 128, 8> : kv_append_rows_kernel<DT, 128, 4>;
 }
 
 }  // namespace
@@ -167,9 +269,16 @@ extern "C" int aekv_kv_append(const void* k, const void* v, int32_t dtype, int64
   a.per_seq = n_tokens / B;
   a.capacity = capacity;
   a.wscale = wht_scale(d);
-  const dim3 grid(static_cast<uint32_t>(ceil_div(lanes, 256)));
+  const hipStream_t st = as_stream(stream);
+  if (dtype != AEKV_F32 && n_tokens * 2 * heads * d >= kRowsElements) {
+    const int64_t groups = ceil_div(n_tokens, static_cast<int64_t>(64 / (d / 32))) * 2 * heads;
+    auto fn = dtype == AEKV_F16 ? pick_rows<AEKV_F16>(d, bits) : pick_rows<AEKV_BF16>(d, bits);
+    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(ceil_div(groups, kTableThreads / 64))), dim3(kTableThreads), 0, st, a,
+                       (bits == 8 ? 127.0f : 7.0f) * a.wscale);
+    return check_launch(who);
+  }
   auto fn = dtype == AEKV_F32 ? pick_append<AEKV_F32>(d, bits)
             : dtype == AEKV_F16 ? pick_append<AEKV_F16>(d, bits) : pick_append<AEKV_BF16>(d, bits);
-  hipLaunchKernelGGL(fn, grid, dim3(256), 0, as_stream(stream), a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(ceil_div(lanes, 256))), dim3(256), 0, st, a);
   return check_launch(who);
 }

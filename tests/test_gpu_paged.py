@@ -361,6 +361,55 @@ def test_append_skips_bad_pages_and_counts(dev):
     assert torch.equal(cache.k_codes, before)
 
 
+@pytest.mark.parametrize("bits,dim,dtype", [(4, 64, torch.bfloat16), (4, 128, torch.bfloat16), (8, 64, torch.float16), (8, 128, torch.float16), (4, 128, torch.float32)])
+def test_append_many_rows(dev, bits, dim, dtype):
+    """Large calls take another layout: packed sequences of odd lengths with zeros, infinities, NaN, values near ties of the
+    rounding and the smallest and largest numbers among them, and a uniform batch of strided views."""
+    heads, page = 5, 32
+    lens = [700, 0, 1, 33, 1501]
+    B, N = len(lens), sum(lens) + 9
+    cache, table, _ = _cache(dev, 38, bits, dim, heads, page, [1600] * B)
+    table[3, 0] = -1
+    kv = randn_outliers((N, 2, heads, dim), seed=39).to(dev)
+    kv[5, 0, 2], kv[17, 1, 1, 7], kv[40, 0, 0, 3], kv[700, 1] = 0, math.inf, NAN, 2.0 ** -130
+    kv[900:1000] = torch.randint(-3, 4, (100, 2, heads, dim), device=dev, generator=_gen(dev, 40)).to(kv.dtype)  # many ties
+    kv[1100:1110] *= 2.0 ** 100 if dtype != torch.float16 else 2.0 ** 10
+    kv = kv.to(dtype)
+    k, v = kv[:, 0], kv[:, 1]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    start = [3, 0, 5, 60, 100]
+    want = _expect_append(cache, k, v, table.cpu(), start, cu)
+    tracker = SlotTracker(B, heads, 1600, device=dev)
+    tracker.weights.fill_(2.0)
+    append_tokens(cache, k, v, table, torch.tensor(start, dtype=torch.int32, device=dev), cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev), tracker=tracker,
+                  token=torch.tensor(start, dtype=torch.int32, device=dev))
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        if w.is_floating_point():
+            nan = w.isnan()
+            assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], w[~nan])
+    # the two vectors that hold an infinity or a NaN (tokens 17 and 40 of the first sequence) have no codes to compare
+    for got, w, token, head in ((cache.k_codes, want[0], 40, 0), (cache.v_codes, want[2], 17, 1)):
+        fine = torch.ones(w.shape[:3], dtype=torch.bool, device=dev)
+        fine[int(table[0, (3 + token) // page]), head, (3 + token) % page] = False
+        assert torch.equal(got[fine], w[fine])
+    for b in range(B):
+        for h in range(heads):
+            t, wt = tracker.tokens[b, h].tolist(), tracker.weights[b, h].tolist()
+            # (slot 1600 is past the table: the last token has no place)
+            assert t[start[b]:start[b] + lens[b]] == list(range(start[b], min(start[b] + lens[b], 1600))) or b == 3
+            assert all(x == 2.0 for x in wt[:start[b]]) and all(x == 2.0 for x in wt[start[b] + lens[b]:])
+    T = 260
+    cache, table, _ = _cache(dev, 41, bits, dim, heads, page, [300] * 4)
+    kv = randn_outliers((4, T, 2 * heads, dim), seed=42).to(dev).to(dtype)
+    k, v = kv[:, :, :heads], kv[:, :, heads:]
+    want = _expect_append(cache, k.reshape(4 * T, heads, dim), v.reshape(4 * T, heads, dim), table.cpu(), [0, 7, 60, 31], [T * b for b in range(5)])
+    append_tokens(cache, k, v, table, torch.tensor([0, 7, 60, 31], dtype=torch.int32, device=dev))
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        assert torch.equal(got, w)
+
+
 # ---- eviction --------------------------------------------------------------------------------------------------
 
 def _check_evict(dev, bits, dim, heads, page, lengths, keep, first, recent, weights=None, seed=0, capacity=None):
