@@ -34,6 +34,7 @@ namespace {
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMargin = 8.0f;  // log2 units: a row's maximum moves when it is exceeded by this (weights up to 2^8)
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kStep = 32, kRound = kStep * kWaves;
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
@@ -191,6 +192,103 @@ __device__ __forceinline__ void load_step(const PagedArgs& a, int32_t kh, int32_
   }
 }
 
+// A step of 32 slots on its way into LDS, straight from memory.  K: unit l (16 bytes) of a load is what lane l will read.
+// V: the rows (slots 16 k + 4 g + i) in the order (k, i, g), so that a lane's word of its slots 16 k + 4 g + i lies at
+// 4 k + i rows of 64 lanes' words: every read is one run of the lanes.  Scales: K's 32, then V's.
+template <int D, int BITS>
+struct Stage {
+  using G = PagedGeom<D, BITS>;
+  static constexpr int kHalf = 32 * G::kRowBytes;    // K's bytes, and V's
+  static constexpr int kBytes = 2 * kHalf + 256;
+  static constexpr int kLoads = 2 * (kHalf / 1024) + 1;  // load instructions of a step
+  static constexpr int kStages = G::kRowBytes == 128 ? 2 : 3;
+};
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef const __attribute__((address_space(1))) void global_void_t;
+// 16 (4) bytes per lane from each lane's own address to `to` and on, lane after lane.
+__device__ __forceinline__ void load_lds16(const void* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((global_void_t*)from, (lds_void_t*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(const void* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((global_void_t*)from, (lds_void_t*)to, 4, 0, 0);
+}
+
+// Issues a step's loads; p0 and p1 are its tiles' pages (a tile without one reads the pool's first rows, and is masked).
+template <int D, int BITS>
+__device__ __forceinline__ void issue_step(const PagedArgs& a, int32_t kh, int32_t slot, int32_t p0, int32_t p1, int lane, uint8_t* st) {
+  using S = Stage<D, BITS>;
+  constexpr int RB = PagedGeom<D, BITS>::kRowBytes;
+  const int32_t in_page = (1 << a.pool.page_shift) - 1;
+  const int64_t r0 = p0 < 0 ? 0 : ((static_cast<int64_t>(p0) * a.pool.heads + kh) << a.pool.page_shift) + (slot & in_page);
+  const int64_t r1 = p1 < 0 ? 0 : ((static_cast<int64_t>(p1) * a.pool.heads + kh) << a.pool.page_shift) + ((slot + 16) & in_page);
+  const int n = lane & 15, g = lane >> 4;
+  if constexpr (RB == 32) {  // both tiles in one load: 2 units a row
+    const int64_t row = lane < 32 ? r0 : r1;
+    const int u = lane & 31;
+    load_lds16(a.pool.k_codes + row * RB + 16 * u, st);
+    // LDS row R = u / 2 of the tile is slot 4 (R % 4) + R / 4
+    load_lds16(a.pool.v_codes + row * RB + (4 * ((u >> 1) & 3) + (u >> 3)) * RB + 16 * (u & 1), st + S::kHalf);
+  } else {
+    constexpr int PER = RB / 64;  // loads of a tile
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        load_lds16(a.pool.k_codes + (k ? r1 : r0) * RB + (n * RB + g * (RB / 4) + 16 * q), st + 1024 * (PER * k + q));
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const int u = 64 * q + lane, R = u / (RB / 16);
+        load_lds16(a.pool.v_codes + (k ? r1 : r0) * RB + ((4 * (R & 3) + (R >> 2)) * RB + 16 * (u % (RB / 16))), st + S::kHalf + 1024 * (PER * k + q));
+      }
+  }
+  const int64_t row = ((lane & 16) ? r1 : r0) + n;
+  load_lds4((lane < 32 ? a.pool.k_scale : a.pool.v_scale) + row, st + 2 * S::kHalf);
+}
+
+// Reads a landed step back.
+template <int D, int BITS>
+__device__ __forceinline__ void read_step(const uint8_t* st, int lane, StepData<D, BITS>& s) {
+  using G = PagedGeom<D, BITS>;
+  using S = Stage<D, BITS>;
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if constexpr (G::kKW == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(st + 512 * k + 32 * n + 8 * g);
+      s.k[k][0] = w.x, s.k[k][1] = w.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < G::kKW / 4; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(st + 1024 * (G::kKW / 4 * k + i) + 16 * lane);
+        s.k[k][4 * i] = w.x, s.k[k][4 * i + 1] = w.y, s.k[k][4 * i + 2] = w.z, s.k[k][4 * i + 3] = w.w;
+      }
+    }
+    s.ks[k] = *reinterpret_cast<const f32x4_t*>(st + 2 * S::kHalf + 64 * k + 16 * g);
+    s.vs[k] = *reinterpret_cast<const f32x4_t*>(st + 2 * S::kHalf + 128 + 64 * k + 16 * g);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint8_t* vr = st + S::kHalf + 64 * G::kVB * j + G::kVB * lane;
+    if constexpr (G::kVB == 2) s.v[j][0] = *reinterpret_cast<const uint16_t*>(vr);
+    else if constexpr (G::kVB == 4) s.v[j][0] = *reinterpret_cast<const uint32_t*>(vr);
+    else {
+      const uint2 w = *reinterpret_cast<const uint2*>(vr);
+      s.v[j][0] = w.x, s.v[j][1] = w.y;
+    }
+  }
+}
+
+// Waits until at most N of the wave's memory operations are on their way (its loads land in order).  The empty asm keeps
+// the LDS reads that follow from moving up.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));  // vmcnt alone
+  asm volatile("" ::: "memory");
+}
+
 // Dim e of the eight slots as bf16 with the offset kBias.
 template <int D, int BITS>
 __device__ __forceinline__ bf16x8_t values_bf16(const uint32_t (&v)[8][PagedGeom<D, BITS>::kWords], int e) {
@@ -212,20 +310,25 @@ __device__ __forceinline__ bf16x8_t values_bf16(const uint32_t (&v)[8][PagedGeom
   return __builtin_bit_cast(bf16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
 }
 
+// A row's query as it lies in memory: this lane's D / 4 elements (a row past the last reads the first).
+template <int D>
+__device__ __forceinline__ void load_query(const PagedArgs& a, int64_t b, int32_t kh, int32_t row, bool in, int lane, uint4 (&w)[D / 32]) {
+  const int32_t t = in ? row / a.G : 0, h = kh * a.G + (in ? row - t * a.G : 0);
+  const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (b * a.q_batch + t * a.q_token + h * a.q_head + (lane >> 4) * (D / 4)));
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) w[i] = qp[i];
+}
+
 // A row's query, rotated, in two fp16 parts in the products' order; *factor takes a score to a logit in log2 units.
 template <int DT, int D, int BITS>
-__device__ __forceinline__ void query_parts(const PagedArgs& a, int64_t b, int32_t kh, int32_t row, bool in, int lane,
+__device__ __forceinline__ void query_parts(const PagedArgs& a, const uint4 (&qw)[D / 32], bool in, int lane,
                                             f16x8_t (&hi)[D / 32], f16x8_t (&lo)[D / 32], float* factor) {
   constexpr int N = D / 4;
   const int g = lane >> 4;
   float x[N];
-  const int32_t t = in ? row / a.G : 0, h = kh * a.G + (in ? row - t * a.G : 0);
-  const int64_t at = b * a.q_batch + t * a.q_token + h * a.q_head + g * N;
-  const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at);
 #pragma unroll
   for (int i = 0; i < N / 8; ++i) {
-    const uint4 w = qp[i];
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t u[4] = {qw[i].x, qw[i].y, qw[i].z, qw[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       x[8 * i + 2 * j] = DT == AEKV_BF16 ? bf16_to_f32(u[j] & 0xffffu) : f16_to_f32(u[j] & 0xffffu);
@@ -287,9 +390,14 @@ __device__ __forceinline__ void store_row(void* out, int64_t at, const float (&y
 template <int DT, int D, int BITS, int MT>
 __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs a) {
   using G = PagedGeom<D, BITS>;
-  constexpr int N = D / 4;
-  __shared__ __align__(16) float s_o[kWaves - 1][MT * N][64];
-  __shared__ float s_ml[kWaves - 1][MT][2][64];
+  using S = Stage<D, BITS>;
+  constexpr int N = D / 4, NS = S::kStages;
+  // a ring of stages for each wave; afterwards stage w holds wave w + 1's state for the merge.  Arrays of their own, so
+  // that the compiler sees that loads into one do not write what is read from another.
+  __shared__ __align__(16) uint8_t st0[kWaves * S::kBytes];
+  __shared__ __align__(16) uint8_t st1[kWaves * S::kBytes];
+  __shared__ __align__(16) uint8_t st2[NS == 3 ? kWaves * S::kBytes : 16];
+  static_assert(MT * (N + 2) * 256 <= kWaves * S::kBytes, "a wave's state fits a stage");
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups: pieces innermost, then row blocks, then KV heads, then sequences
@@ -306,61 +414,70 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
   if (split > 0 && p0 >= p1) return;  // (the merge knows how many pieces a sequence has)
 
-  f16x8_t qhi[MT][D / 32], qlo[MT][D / 32];
-  float factor[MT], m[MT], l[MT];
-  int32_t row[MT], sees[MT], sees_all = 0x7fffffff;
-  f32x4_t o[MT][G::kNE], ones_sum[MT];
+  // the queries are requested first, then the first steps; the rotation runs while those are on their way
+  int32_t row[MT];
+  uint4 qw[MT][D / 32];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     row[t] = (rb * MT + t) * 16 + (lane & 15);
+    load_query<D>(a, b, kh, row[t], row[t] < a.rows, lane, qw[t]);
+  }
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
+  int32_t pages = -1;
+  const int32_t first = p0 + kStep * wave;
+  const int n_steps = first < p1 ? (p1 - first + kRound - 1) / kRound : 0;
+  uint32_t bad[NS] = {};  // bit k: tile k of the stage's step has no page
+  auto stage = [&](auto which) -> uint8_t* {
+    return (decltype(which)::value == 0 ? st0 : decltype(which)::value == 1 ? st1 : st2) + wave * S::kBytes;
+  };
+  auto load = [&](int i, auto which) __attribute__((always_inline)) {
+    if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+    const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
+    bad[decltype(which)::value] = (g0 < 0 ? 1u : 0u) | (g1 < 0 ? 2u : 0u);
+    issue_step<D, BITS>(a, kh, first + kRound * i, g0, g1, lane, stage(which));
+  };
+  if (n_steps > 0) load(0, std::integral_constant<int, 0>{});
+  if (NS == 3 && n_steps > 1) load(1, std::integral_constant<int, 1>{});
+
+  f16x8_t qhi[MT][D / 32], qlo[MT][D / 32];
+  float factor[MT], m[MT], l[MT];
+  int32_t sees[MT];
+  f32x4_t o[MT][G::kNE], ones_sum[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
     const bool in = row[t] < a.rows;
-    query_parts<DT, D, BITS>(a, b, kh, row[t], in, lane, qhi[t], qlo[t], &factor[t]);
+    query_parts<DT, D, BITS>(a, qw[t], in, lane, qhi[t], qlo[t], &factor[t]);
     sees[t] = in ? max(n - a.T + 1 + row[t] / a.G, 0) : n;
     m[t] = kNegInf, l[t] = 0.0f;
 #pragma unroll
     for (int e = 0; e < G::kNE; ++e) o[t][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     ones_sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  sees_all = max(n - a.T + 1 + rb * MT * 16 / a.G, 0);  // the fewest that a row of the block sees
+  const int32_t sees_all = max(n - a.T + 1 + rb * MT * 16 / a.G, 0);  // the fewest that a row of the block sees
 
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
-  int32_t pages = -1;
-  StepData<D, BITS> buf[2];
-  const int32_t first = p0 + kStep * wave;
-  const int n_steps = first < p1 ? (p1 - first + kRound - 1) / kRound : 0;
-  uint32_t bad[2] = {0, 0};  // bit k: tile k of the buffered step has no page
-  auto load = [&](int i, auto which) {
-    constexpr int w = decltype(which)::value;
-    if (i >= n_steps) return;
-    if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
-    const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
-    bad[w] = (g0 < 0 ? 1u : 0u) | (g1 < 0 ? 2u : 0u);
-    load_step<D, BITS, true>(a, kh, first + kRound * i, g0, g1, lane, buf[w]);
-  };
-  auto compute = [&](int i, auto which) {
-    constexpr int w = decltype(which)::value;
-    const StepData<D, BITS>& s = buf[w];
-    const int32_t base = first + kRound * i;
+  // a landed step; `whole`: every row sees all of it
+  auto body = [&](const StepData<D, BITS>& s, int32_t base, uint32_t none, auto whole_c) __attribute__((always_inline)) {
+    constexpr bool whole = decltype(whole_c)::value;
     f16x8_t kc[2][D / 32];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) kc[k][c] = codes_f16<BITS>(&s.k[k][c * BITS / 4]);
     bf16x8_t phi[MT], plo[MT];
-    const bool whole = bad[w] == 0 && base + kStep <= sees_all;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       f32x4_t x[2];
       score_step<D, BITS>(kc, s.ks, qhi[t], qlo[t], factor[t], x);
       bool hide[2][4] = {};
-      if (!whole)
+      if constexpr (!whole) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            hide[k][j] = ((bad[w] >> k) & 1u) || base + 16 * k + 4 * g + j >= sees[t];
+            hide[k][j] = ((none >> k) & 1u) || base + 16 * k + 4 * g + j >= sees[t];
             x[k][j] = hide[k][j] ? kNegInf : x[k][j];
           }
+      }
       if (a.logits && row[t] < a.rows) {
         float* lg = a.logits + ((b * a.pool.heads + kh) * a.rows + row[t]) * a.logit_slots + base + 4 * g;
         *reinterpret_cast<f32x4_t*>(lg) = x[0];
@@ -369,14 +486,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
       float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
       top = fmaxf(top, xor_lane<16>(top));
       top = fmaxf(top, xor_lane<32>(top));
-      if (__builtin_amdgcn_ballot_w64(top > m[t])) {
-        const float up = fmaxf(m[t], top);
-        const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[t] - up);
+      // (each row by itself: a row's bits do not depend on the others')
+      const bool moved = top > m[t] + kMargin;
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+        const float r = moved ? __builtin_amdgcn_exp2f(m[t] - top) : 1.0f;
         l[t] *= r;
 #pragma unroll
         for (int e = 0; e < G::kNE; ++e) o[t][e] *= r;
         ones_sum[t] *= r;
-        m[t] = up;
+        m[t] = moved ? top : m[t];
       }
       const float nm = m[t] == kNegInf ? 0.0f : -m[t];
       float c[2][4];
@@ -387,7 +505,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
           const float p = __builtin_amdgcn_exp2f(x[k][j] + nm);
           l[t] += p;
           c[k][j] = p * s.vs[k][j];
-          if (!whole) c[k][j] = hide[k][j] ? 0.0f : c[k][j];  // (whatever a hidden slot's scale is)
+          if constexpr (!whole) c[k][j] = hide[k][j] ? 0.0f : c[k][j];  // (whatever a hidden slot's scale is)
         }
       uint32_t h[4], r[4];
 #pragma unroll
@@ -420,14 +538,29 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
       }
     }
   };
-  load(0, std::integral_constant<int, 0>{});
+  // one step: the loads of the one NS - 1 ahead go out, then this one's are waited for
+  auto compute = [&](int i, auto which) __attribute__((always_inline)) {
+    constexpr int w = decltype(which)::value;
+    if (i + NS - 1 < n_steps) {
+      load(i + NS - 1, std::integral_constant<int, (w + NS - 1) % NS>{});
+      wait_loads<(NS - 1) * S::kLoads>();
+    } else {
+      wait_loads<0>();
+    }
+    StepData<D, BITS> s;
+    read_step<D, BITS>(stage(which), lane, s);
+    const int32_t base = first + kRound * i;
+    if (bad[w] == 0 && base + kStep <= sees_all) body(s, base, 0u, std::true_type{});
+    else body(s, base, bad[w], std::false_type{});
+  };
 #pragma unroll 1
-  for (int i = 0; i < n_steps; i += 2) {
-    load(i + 1, std::integral_constant<int, 1>{});
+  for (int i = 0; i < n_steps; i += NS) {
     compute(i, std::integral_constant<int, 0>{});
-    if (i + 1 < n_steps) {
-      load(i + 2, std::integral_constant<int, 0>{});
-      compute(i + 1, std::integral_constant<int, 1>{});
+    if (i + 1 >= n_steps) break;
+    compute(i + 1, std::integral_constant<int, 1>{});
+    if constexpr (NS == 3) {
+      if (i + 2 >= n_steps) break;
+      compute(i + 2, std::integral_constant<int, 2>{});
     }
   }
 
@@ -442,22 +575,31 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[t][G::kNE * i + e] = o[t][e][i] - G::kBias * ones_sum[t][i];
   }
+  // state of wave w + 1: word i of row tile t at (t (N + 2) + i) 64 + lane, then its maximum and sum
+  auto state = [&](int w) { return reinterpret_cast<float*>(NS == 3 ? (w == 0 ? st0 : w == 1 ? st1 : st2) : (w == 0 ? st0 : w == 1 ? st1 : st0 + kWaves * S::kBytes / 2)); };
+  static_assert(NS == 3 || 2 * MT * (N + 2) * 256 <= kWaves * S::kBytes, "two states fit a stage");
+  __syncthreads();  // every wave has read its last stage
   if (wave > 0) {
+    float* p = state(wave - 1);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) s_o[wave - 1][t * N + i][lane] = y[t][i];
-      s_ml[wave - 1][t][0][lane] = m[t];
-      s_ml[wave - 1][t][1][lane] = l[t];
+      for (int i = 0; i < N; ++i) p[(t * (N + 2) + i) * 64 + lane] = y[t][i];
+      p[(t * (N + 2) + N) * 64 + lane] = m[t];
+      p[(t * (N + 2) + N + 1) * 64 + lane] = l[t];
     }
   }
   __syncthreads();
   if (wave > 0) return;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    float top = m[t];
+    float top = m[t], pm[kWaves - 1], pl[kWaves - 1];
 #pragma unroll
-    for (int w = 0; w < kWaves - 1; ++w) top = fmaxf(top, s_ml[w][t][0][lane]);
+    for (int w = 0; w < kWaves - 1; ++w) {
+      pm[w] = state(w)[(t * (N + 2) + N) * 64 + lane];
+      pl[w] = state(w)[(t * (N + 2) + N + 1) * 64 + lane];
+      top = fmaxf(top, pm[w]);
+    }
     // (a state of nothing has a sum of 0; NaN alone leaves a maximum of -inf, and a sum that says so)
     const float f = l[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
     l[t] = l[t] == 0.0f ? 0.0f : l[t] * f;
@@ -465,11 +607,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
     for (int i = 0; i < N; ++i) y[t][i] *= f;
 #pragma unroll
     for (int w = 0; w < kWaves - 1; ++w) {
-      const float lw = s_ml[w][t][1][lane];
-      const float fw = lw == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][t][0][lane] - top);
-      l[t] += lw == 0.0f ? 0.0f : lw * fw;
+      const float fw = pl[w] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm[w] - top);
+      l[t] += pl[w] == 0.0f ? 0.0f : pl[w] * fw;
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[t][i] = fmaf(s_o[w][t * N + i][lane], fw, y[t][i]);
+      for (int i = 0; i < N; ++i) y[t][i] = fmaf(state(w)[(t * (N + 2) + i) * 64 + lane], fw, y[t][i]);
     }
     m[t] = top;
     if (row[t] >= a.rows) continue;
@@ -620,7 +761,9 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
       const bool in = row < a.rows;
       f16x8_t hi[NC], lo[NC];
       float factor;
-      query_parts<DT, D, BITS>(a, b, kh, row, in, lane, hi, lo, &factor);
+      uint4 qw[NC];
+      load_query<D>(a, b, kh, row, in, lane, qw);
+      query_parts<DT, D, BITS>(a, qw, in, lane, hi, lo, &factor);
 #pragma unroll
       for (int c = 0; c < NC; ++c) s_hi[t][c][lane] = hi[c], s_lo[t][c][lane] = lo[c];
       if (g == 0) {
@@ -706,10 +849,14 @@ paged_fn pick_weights(int d, int bits) {
 }
 
 // Pieces of a sequence: enough workgroups for the chip (2048: two per CU, four times over, which evens out sequences of
-// different lengths), none without a whole round of slots.
+// different lengths), but none of fewer than 512 slots beyond 512 workgroups (a workgroup's rotations and merge cost as
+// much as some 500 slots), and none without a whole round of slots.
 int64_t paged_pieces(int64_t groups, int64_t slots) {
+  const int64_t few = ceil_div(512, groups), some = ceil_div(slots, 512);
   const int64_t want = ceil_div(2048, groups), most = ceil_div(slots, kRound);
-  const int64_t n = want < most ? want : most;
+  int64_t n = few > some ? few : some;
+  n = n < want ? n : want;
+  n = n < most ? n : most;
   return n < 1 ? 1 : n;
 }
 

@@ -260,14 +260,14 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
       }
     }
     top = fmaxf(top, xor_lane<32>(top)) * a.scale2;
-    // (nothing yet: any maximum counts as moved)
-    if (__builtin_amdgcn_ballot_w64(top > m + kMargin)) {
-      const float up = fmaxf(m, top);
-      const float r = up == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+    // (each row by itself: a row's bits do not depend on the others')
+    const bool moved = top > m + kMargin;
+    if (__builtin_amdgcn_ballot_w64(moved)) {
+      const float r = moved ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
       l *= r;
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb) O[mb] *= r;
-      m = up;
+      m = moved ? top : m;
     }
     const float nm = m == kNegInf ? 0.0f : -m;
 #pragma unroll
