@@ -80,18 +80,21 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   int rows = 0, run = 0;
   auto load_round = [&](int base) __attribute__((always_inline)) {
     const int left = min(n - base, kRound);
-    rows = (left + kSelThreads - 1) / kSelThreads;
+    rows = __builtin_amdgcn_readfirstlane((left + kSelThreads - 1) / kSelThreads);
     run = base + wave * rows * 64;
     float wt[kRegRows];
     int32_t tk[kRegRows];
 #pragma unroll
     for (int r = 0; r < kRegRows; ++r) {
-      const int i = run + 64 * r + lane;
-      if (r < rows && i < n) wt[r] = w[i], tk[r] = tok[i];
+      if (r >= rows) break;
+      const int i = min(run + 64 * r + lane, n - 1);
+      wt[r] = w[i], tk[r] = tok[i];
     }
 #pragma unroll
-    for (int r = 0; r < kRegRows; ++r)
-      key[r] = r < rows && run + 64 * r + lane < n ? evict_key(wt[r], tk[r], a.first, recent_from) : 0u;
+    for (int r = 0; r < kRegRows; ++r) {
+      if (r >= rows) break;
+      key[r] = evict_key(wt[r], tk[r], a.first, recent_from);
+    }
   };
   const bool one_round = n <= kRound;
   if (one_round) load_round(0);
@@ -104,9 +107,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     for (int base = 0; base < n; base += kRound) {
       if (!one_round) load_round(base);
 #pragma unroll
-      for (int r = 0; r < kRegRows; ++r)
-        if (r < rows && run + 64 * r + lane < n && (shift == 21 || (key[r] >> (shift + width)) == (prefix >> (shift + width))))
+      for (int r = 0; r < kRegRows; ++r) {
+        if (r >= rows) break;
+        if (run + 64 * r + lane < n && (shift == 21 || (key[r] >> (shift + width)) == (prefix >> (shift + width))))
           atomicAdd(&hist[(key[r] >> shift) & ((1u << width) - 1)], 1u);
+      }
     }
     __syncthreads();
     // bins from the top: thread t holds bins 2047 - 2 t and the one below
@@ -142,7 +147,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     uint64_t mine = 0, total;
 #pragma unroll
     for (int r = 0; r < kRegRows; ++r) {
-      const bool in = r < rows && run + 64 * r + lane < n;
+      if (r >= rows) break;
+      const bool in = run + 64 * r + lane < n;
       mine += __popcll(__builtin_amdgcn_ballot_w64(in && (key[r] >> shift) == (prefix >> shift)));
     }
     uint64_t rank = ties + wave_prefix(mine, s_part, lane, wave, &total);
@@ -151,8 +157,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     uint64_t count = 0;
 #pragma unroll
     for (int r = 0; r < kRegRows; ++r) {
+      if (r >= rows) break;
       const int i = run + 64 * r + lane;
-      const bool in = r < rows && i < n;
+      const bool in = i < n;
       const bool tie = in && (key[r] >> shift) == (prefix >> shift);
       const uint64_t tm = __builtin_amdgcn_ballot_w64(tie);
       const bool kept = in && ((key[r] >> shift) > (prefix >> shift) || (tie && rank + __popcll(tm & below) < static_cast<uint64_t>(need)));
@@ -166,6 +173,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     moved += total;
 #pragma unroll
     for (int r = 0; r < kRegRows; ++r) {
+      if (r >= rows) break;
       const int i = run + 64 * r + lane;
       const bool h = (hole >> r) & 1u, m = (mover >> r) & 1u;
       const uint64_t hm = __builtin_amdgcn_ballot_w64(h), mm = __builtin_amdgcn_ballot_w64(m);

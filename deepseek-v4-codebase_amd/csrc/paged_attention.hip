@@ -712,20 +712,35 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   if (a.lse && lane == 0) a.lse[orow] = sum == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(sum);
 }
 
-// The weights of a sequence's slots from the logits that the attention left and the rows' log sums: a thread per slot.
+// The weights of a sequence's slots from the logits that the attention left and the rows' log sums: four slots to a thread.
+constexpr int kAddSlots = 1024;  // of a workgroup
+
 __global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blocks) {
-  const int32_t j = static_cast<int32_t>(blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int32_t j = static_cast<int32_t>(blockIdx.x % blocks) * kAddSlots + 4 * threadIdx.x;
   const int64_t bk = blockIdx.x / blocks, b = bk / a.pool.heads;
   const int32_t kh = static_cast<int32_t>(bk - b * a.pool.heads);
-  if (j >= newest_sees(a, b)) return;
+  const int32_t n = newest_sees(a, b);
+  if (j >= n) return;
   const float* lg = a.logits + bk * a.rows * a.logit_slots + j;
-  float sum = 0.0f;
+  float* w = a.weights + bk * a.capacity + j;
+  const bool vec = (a.capacity & 3) == 0 && j + 4 <= n;  // (weights is 16-byte aligned: the launcher checks)
+  f32x4_t before = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (vec) before = *reinterpret_cast<const f32x4_t*>(w);
 #pragma unroll 4
   for (int32_t r = 0; r < a.rows; ++r) {
     const int32_t t = r / a.G;
-    sum += __builtin_amdgcn_exp2f(lg[r * a.logit_slots] - a.lse[(b * a.T + t) * a.H + kh * a.G + (r - t * a.G)]);
+    const float lse = a.lse[(b * a.T + t) * a.H + kh * a.G + (r - t * a.G)];
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lg + r * a.logit_slots);  // (the step's 32 slots are all there)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse);
   }
-  if (sum != 0.0f) a.weights[bk * a.capacity + j] += sum;
+  if (vec) {
+    *reinterpret_cast<f32x4_t*>(w) = before + sum;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i < n) w[i] += sum[i];
+  }
 }
 
 // The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
@@ -848,12 +863,13 @@ paged_fn pick_weights(int d, int bits) {
   return bits == 8 ? paged_weights_kernel<DT, 128, 8> : paged_weights_kernel<DT, 128, 4>;
 }
 
-// Pieces of a sequence: enough workgroups for the chip (2048: two per CU, four times over, which evens out sequences of
-// different lengths), but none of fewer than 512 slots beyond 512 workgroups (a workgroup's rotations and merge cost as
+// Pieces of a sequence: enough workgroups for the chip (1536: three per CU, twice over, which evens out sequences of
+// different lengths; one sequence of 262144 slots x 12 heads, 1024 / 1536 / 2048 / 3000 workgroups: 111 / 101 / 109 / 113 us,
+// 64 ragged ones of up to 16384 slots x 4 heads 122 / 119 / 117 / 119), but none of fewer than 512 slots beyond 512 workgroups (a workgroup's rotations and merge cost as
 // much as some 500 slots), and none without a whole round of slots.
 int64_t paged_pieces(int64_t groups, int64_t slots) {
   const int64_t few = ceil_div(512, groups), some = ceil_div(slots, 512);
-  const int64_t want = ceil_div(2048, groups), most = ceil_div(slots, kRound);
+  const int64_t want = ceil_div(1536, groups), most = ceil_div(slots, kRound);
   int64_t n = few > some ? few : some;
   n = n < want ? n : want;
   n = n < most ? n : most;
@@ -905,9 +921,9 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   if (weights && capacity < 0) return fail(AEKV_ERR_SHAPE, "%s: capacity=%lld", who, (long long)capacity);
   if (B == 0 || T == 0) return AEKV_OK;
   if (!q || !lengths || !diag || !out) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
-  if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) || !is_aligned(diag, 16) || (q_batch_stride % 8) ||
+  if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) || !is_aligned(diag, 16) || !is_aligned(weights, 16) || (q_batch_stride % 8) ||
       (q_token_stride % 8) || (q_head_stride % 8))
-    return fail(AEKV_ERR_ALIGN, "%s: q rows, out, diag and workspace must be 16-byte aligned", who);
+    return fail(AEKV_ERR_ALIGN, "%s: q rows, out, diag, weights and workspace must be 16-byte aligned", who);
   const int64_t slots = max_pages * page_size, rows = T * (H / heads);
   const int mt = paged_row_tiles(rows, d);
   const int64_t blocks = ceil_div(rows, 16 * mt);
@@ -955,7 +971,7 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   }
   if (!a.weights) return AEKV_OK;
   if (a.logits) {
-    const int32_t per = static_cast<int32_t>(ceil_div(reach, 256));
+    const int32_t per = static_cast<int32_t>(ceil_div(reach, kAddSlots));
     hipLaunchKernelGGL(paged_add_kernel, dim3(static_cast<uint32_t>(B * heads * per)), dim3(256), 0, st, a, per);
     return check_launch(who);
   }
