@@ -361,10 +361,10 @@ static PyObject* f_kv_evict(PyObject* self, PyObject* const* args, Py_ssize_t na
 }
 
 /* aekv_prompt_attention(q, k, v, dtype, q_token, q_head, k_token, k_head, v_token, v_head, cu_q, cu_k, B, n_q, n_k, H,
- * heads, d, sink, scale, out, lse, clear_rest, stream) */
+ * heads, d, sink, scale, out, lse, clear_rest, ws, ws_bytes, stream) */
 static PyObject* f_prompt_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  if (want_args(nargs, 24, "aekv_prompt_attention")) return NULL;
+  if (want_args(nargs, 26, "aekv_prompt_attention")) return NULL;
   void* q = ptr_arg(A(0));
   void* k = ptr_arg(A(1));
   void* v = ptr_arg(A(2));
@@ -380,10 +380,12 @@ static PyObject* f_prompt_attention(PyObject* self, PyObject* const* args, Py_ss
   void* out = ptr_arg(A(20));
   void* lse = ptr_arg(A(21));
   const int32_t clear = i32_arg(A(22));
-  void* st = ptr_arg(A(23));
-  RETURN_STATUS_UNLOCKED(aekv_prompt_attention(q, k, v, dt, n[0], n[1], n[2], n[3], n[4], n[5], (const int32_t*)cq,
+  void* ws = ptr_arg(A(23));
+  const size_t wsb = (size_t)i64_arg(A(24));
+  void* st = ptr_arg(A(25));
+  RETURN_STATUS(aekv_prompt_attention(q, k, v, dt, n[0], n[1], n[2], n[3], n[4], n[5], (const int32_t*)cq,
                                                (const int32_t*)ck, B, nq, nk, H, hk, d, (const float*)sink, sm, out,
-                                               (float*)lse, clear, st));
+                                               (float*)lse, clear, ws, wsb, st));
 }
 
 static PyMethodDef methods[] = {

@@ -38,7 +38,7 @@ SYMBOLS = (
     "aekv_csa_decode_workspace_size", "aekv_csa_decode_quant", "aekv_sparse_sink_attention_ws",
     "aekv_tiled_prefill_attention_ws", "aekv_sink_attention_workspace_size", "aekv_prefill_counts",
     "aekv_kv_append", "aekv_paged_attention_workspace_size", "aekv_paged_attention", "aekv_kv_evict_workspace_size",
-    "aekv_kv_evict", "aekv_prompt_attention",
+    "aekv_kv_evict", "aekv_prompt_attention", "aekv_prompt_attention_workspace_size",
 )
 
 # size of the static device scratch behind aekv_csa_indexer_topk_quant_noalloc (AEKV_STATIC_SCRATCH_BYTES)
@@ -113,7 +113,8 @@ def lib() -> ctypes.CDLL:
         "aekv_kv_evict_workspace_size": ([I64_] * 4, SZ),
         "aekv_kv_evict": ([I32_, I32_, P, P, P, P, I64_, I64_, I32_, P, I64_, I64_, P, P, P, I64_, P, I64_, I64_, I64_, P, SZ, P],
                           ctypes.c_int),
-        "aekv_prompt_attention": ([P, P, P, I32_] + [I64_] * 6 + [P, P] + [I64_] * 5 + [I32_, P, F, P, P, I32_, P], ctypes.c_int),
+        "aekv_prompt_attention": ([P, P, P, I32_] + [I64_] * 6 + [P, P] + [I64_] * 5 + [I32_, P, F, P, P, I32_, P, SZ, P], ctypes.c_int),
+        "aekv_prompt_attention_workspace_size": ([I64_] * 5 + [I32_], SZ),
         "aekv_sink_attention_workspace_size": ([I32_, I64_, I64_, I64_, I64_, I64_, I64_], SZ),
     }
     for name, (argtypes, restype) in sig.items():
@@ -239,6 +240,11 @@ def paged_ws_bytes(B: int, T: int, H: int, heads: int, d: int, slots: int, track
 @functools.lru_cache(maxsize=1024)
 def evict_ws_bytes(B: int, heads: int, keep: int, slots: int) -> int:
     return lib().aekv_kv_evict_workspace_size(B, heads, keep, slots)
+
+
+@functools.lru_cache(maxsize=1024)
+def prompt_ws_bytes(B: int, n_q: int, n_k: int, H: int, heads: int, d: int) -> int:
+    return lib().aekv_prompt_attention_workspace_size(B, n_q, n_k, H, heads, d)
 
 
 def require_device(name: str, *tensors: Optional[torch.Tensor]) -> None:

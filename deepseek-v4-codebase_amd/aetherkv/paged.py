@@ -104,8 +104,9 @@ class SlotTracker:
     def from_tensor(cls, storage: torch.Tensor) -> "SlotTracker":
         """A tracker over an existing int32 [2, B, kv_heads, capacity] (used in place)."""
         _lib.require_device("storage", storage)
-        if storage.dtype != torch.int32 or storage.dim() != 4 or storage.size(0) != 2 or not storage.is_contiguous():
-            raise RuntimeError(f"storage must be contiguous int32 [2, B, kv_heads, capacity], got {storage.dtype} "
+        if storage.dtype != torch.int32 or storage.dim() != 4 or storage.size(0) != 2 or not storage.is_contiguous() \
+                or storage.data_ptr() % 16:
+            raise RuntimeError(f"storage must be contiguous, 16-byte aligned int32 [2, B, kv_heads, capacity], got {storage.dtype} "
                                f"{tuple(storage.shape)}")
         self = cls.__new__(cls)
         self._set(storage)

@@ -13,9 +13,15 @@ from .decode import _check_out, _iptr, _sink_f32
 from .paged import _counts, _one_device, _rows
 
 
+def prompt_workspace(B: int, n_q: int, n_k: int, H: int, kv_heads: int, dim: int, device) -> torch.Tensor:
+    """Workspace of prompt_attention (B sequences, n_q rows of q, n_k of k; empty where it needs none)."""
+    return torch.empty(_lib.prompt_ws_bytes(int(B), int(n_q), int(n_k), int(H), int(kv_heads), int(dim)), dtype=torch.uint8, device=device)
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, *,
                      cu_seqlens_k: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None,
-                     return_lse: bool = False, out: Optional[torch.Tensor] = None):
+                     return_lse: bool = False, workspace: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None):
     """out_i = sum_j p_ij v_j over the keys j <= i + (keys - queries) of query i's sequence.
 
     q [N, H, D], k and v [M, kv_heads, D], bf16 or fp16, D 64 or 128, H a multiple of kv_heads (query head h reads KV head
@@ -39,7 +45,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise RuntimeError(f"cu_seqlens must be int32 [B + 1], got {tuple(cu_seqlens.shape)}")
     B = cu_seqlens.size(0) - 1
     dev = q.device
-    _one_device(dev, k, v, cu_seqlens, cu_seqlens_k, sink, out)
+    _one_device(dev, k, v, cu_seqlens, cu_seqlens_k, sink, workspace, out)
     cq = _counts("cu_seqlens", cu_seqlens, B + 1)
     if cu_seqlens_k is None:
         if M != N:
@@ -55,11 +61,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     else:
         _check_out("out", out, q.dtype, q.numel(), dev)
     lse = torch.empty((N, H), dtype=torch.float32, device=dev) if return_lse else None
+    need = _lib.prompt_ws_bytes(B, N, M, H, hk, D)
     with _lib.on_device(dev):
+        stream = _lib.raw_stream(dev)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
         rc = _lib.hot("aekv_prompt_attention")(
             qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), _lib.TORCH_TO_AEKV[q.dtype], qr.stride(0), qr.stride(1),
             kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1), cq.data_ptr(), ck.data_ptr(), B, N, M, H, hk, D,
-            _iptr(sk), float(softmax_scale), out.data_ptr(), _iptr(lse), clear, _lib.raw_stream(dev))
+            _iptr(sk), float(softmax_scale), out.data_ptr(), _iptr(lse), clear, _iptr(ws),
+            0 if ws is None else ws.numel(), stream)
     _lib.check(rc, "aekv_prompt_attention")
     out = out if out.dim() == 3 else out.view(q.shape)
     return (out, lse) if return_lse else out

@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blo
 
 // The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
 // row of the KV head's group, 16 at a time (their query parts in LDS), and adds the sums over the rows.
-constexpr int kWeightTiles = 4;  // row tiles whose parts LDS holds at a time
+constexpr int kWeightTiles = 8;  // row tiles whose parts LDS holds at a time
 
 template <int DT, int D, int BITS>
 __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {

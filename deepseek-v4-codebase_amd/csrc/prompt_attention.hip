@@ -29,6 +29,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMargin = 8.0f;        // log2 units
 constexpr int kTile = 64;              // keys of a tile
+constexpr int kPieceTiles = 8;         // least tiles of a piece of the keys
 constexpr int kBufWord3 = 0x00020000;  // buffer resource word 3: raw 32-bit data, range-checked
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -50,6 +51,8 @@ struct PromptArgs {
   const float* sink;    // [H] or null
   uint16_t* out;        // [n_q, H, D]
   float* lse;           // [n_q, H] or null
+  float* part;          // [n_q, H, n_split, D + 4] where the keys are split: max, sum (log2 units), 2 pad, output
+  int32_t n_split, tiles;
   int32_t n_q, n_k, B, H, heads, G;
   int32_t clear;        // rows in no sequence: 0 to leave out as it is, 1 to write zeros
   float scale2;         // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
@@ -91,38 +94,43 @@ __device__ __forceinline__ int swizzle(int r) {
 
 __device__ __forceinline__ i16x4_t read_tr16(const uint8_t* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p)); }
 
-// The sequence and row tile of the workgroup's `t`-th tile (tiles of `rows` rows of G per query, in the sequences' order;
-// a sequence's last rows, which see the most keys, come first).  False past the last tile.
-__device__ __forceinline__ bool find_tile(const PromptArgs& a, int64_t t, int rows, int lane, int32_t* seq, int32_t* first) {
-  int64_t before = 0;
+struct TileAt {
+  int32_t q0, lq, k0, lk;  // the sequence's queries and keys
+  int32_t row;             // the tile's first row
+};
+
+// The workgroup's `t`-th tile (tiles of `rows` rows of G per query, in the sequences' order; a sequence's last rows, which
+// see the most keys, come first).  False past the last tile.  Lanes look at a sequence each, in one memory round.
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, int32_t t, int rows, int lane, TileAt* at) {
+  int32_t before = 0;  // (n_q H, with a tile's rows, fits 31 bits)
   for (int32_t base = 0; base < a.B; base += 64) {
-    const int32_t b = base + lane;
-    int64_t n = 0;
-    if (b < a.B) {
-      const int32_t q0 = min(max(a.cu_q[b], 0), a.n_q), q1 = min(max(a.cu_q[b + 1], q0), a.n_q);
-      n = ((q1 - q0) * a.G + rows - 1) / rows;  // (n_q H, with a tile's rows, fits 31 bits)
-    }
-    int64_t s = n;  // inclusive sum over the lanes
+    const int32_t b = min(base + lane, a.B - 1);
+    const int32_t c0 = a.cu_q[b], c1 = a.cu_q[b + 1], d0 = a.cu_k[b], d1 = a.cu_k[b + 1];
+    const int32_t q0 = min(max(c0, 0), a.n_q), lq = min(max(c1, q0), a.n_q) - q0;
+    const int32_t k0 = min(max(d0, 0), a.n_k), lk = min(max(d1, k0), a.n_k) - k0;
+    int32_t s = base + lane < a.B ? (lq * a.G + rows - 1) / rows : 0;  // inclusive sum over the lanes
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(s, d);
+      const int32_t o = __shfl_up(s, d);
       if (lane >= d) s += o;
     }
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > t);
     if (past) {
-      const int at = __builtin_ctzll(past);
-      const int64_t upto = before + __shfl(s, at);  // the tiles up to the sequence's last
-      *seq = base + at;
-      *first = static_cast<int32_t>(upto - 1 - t) * rows;
+      const int l = __builtin_ctzll(past);
+      at->q0 = __builtin_amdgcn_readlane(q0, l);
+      at->lq = __builtin_amdgcn_readlane(lq, l);
+      at->k0 = __builtin_amdgcn_readlane(k0, l);
+      at->lk = __builtin_amdgcn_readlane(lk, l);
+      at->row = (before + __builtin_amdgcn_readlane(s, l) - 1 - t) * rows;
       return true;
     }
-    before += __shfl(s, 63);
+    before += __builtin_amdgcn_readlane(s, 63);
   }
   return false;
 }
 
 template <int DT, int D, int WR, int KS>
-__global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2))) void prompt_attention_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void prompt_attention_kernel(PromptArgs a) {
   using E = Elem<DT>;
   using Gm = PromptGeom<D>;
   using v8 = typename E::v8;
@@ -142,24 +150,27 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
   const int lane = threadIdx.x & 63, rl = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wv % WR, kh = wv / WR;
+  // workgroups: KV heads innermost, then row tiles, then pieces of the keys
   const int32_t head = static_cast<int32_t>(blockIdx.x % a.heads);
-
-  // rows in no sequence: shared out over the workgroups
-  {
-    const int32_t q0 = min(max(a.cu_q[0], 0), a.n_q), q1 = min(max(a.cu_q[a.B], q0), a.n_q);
-    const int64_t words = static_cast<int64_t>(q0 + a.n_q - q1) * a.H * (D / 2);
+  uint32_t index = blockIdx.x / a.heads;
+  int32_t split = 0;
+  if (a.n_split > 1) {
+    split = static_cast<int32_t>(index / a.tiles);
+    index -= split * a.tiles;
+  }
+  TileAt at;
+  const bool found = find_tile(a, static_cast<int32_t>(index), kRows, lane, &at);
+  if (a.clear || a.lse) {  // rows in no sequence: shared out over the workgroups
+    const int32_t s0 = min(max(a.cu_q[0], 0), a.n_q), s1 = min(max(a.cu_q[a.B], s0), a.n_q);
+    const int64_t words = static_cast<int64_t>(s0 + a.n_q - s1) * a.H * (D / 2);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * (64 * kWaves) + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * (64 * kWaves)) {
-      const int64_t r = i / (D / 2), row = r < static_cast<int64_t>(q0) * a.H ? r : r + static_cast<int64_t>(q1 - q0) * a.H;
+      const int64_t r = i / (D / 2), row = r < static_cast<int64_t>(s0) * a.H ? r : r + static_cast<int64_t>(s1 - s0) * a.H;
       if (a.clear) reinterpret_cast<uint32_t*>(a.out)[row * (D / 2) + i % (D / 2)] = 0;
       if (a.lse && i % (D / 2) == 0) a.lse[row] = kNegInf;
     }
   }
-  int32_t seq;
-  int32_t row0;
-  if (!find_tile(a, blockIdx.x / a.heads, kRows, lane, &seq, &row0)) return;  // (the whole workgroup)
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  const int32_t q0 = min(max(a.cu_q[seq], 0), a.n_q), lq = min(max(a.cu_q[seq + 1], q0), a.n_q) - q0;
-  const int32_t k0 = min(max(a.cu_k[seq], 0), a.n_k), lk = min(max(a.cu_k[seq + 1], k0), a.n_k) - k0;
+  if (!found) return;  // (the whole workgroup)
+  const int32_t q0 = at.q0, lq = at.lq, k0 = at.k0, lk = at.lk, row0 = at.row;
   const int32_t n_rows = lq * a.G;
   auto sees_of = [&](int32_t row) {  // keys that a row sees
     const int64_t s = static_cast<int64_t>(row / a.G) + 1 + lk - lq;
@@ -167,7 +178,12 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
   };
   const int32_t last_row = (row0 + kRows < n_rows ? row0 + kRows : n_rows) - 1;
   const int32_t n_keys = __builtin_amdgcn_readfirstlane(sees_of(last_row));
-  const int n_tiles = (n_keys + kTile - 1) / kTile;
+  const int all_tiles = (n_keys + kTile - 1) / kTile;
+  int first_tile = 0, n_tiles = all_tiles;
+  if (a.n_split > 1) {
+    const int per_piece = max((all_tiles + a.n_split - 1) / a.n_split, kPieceTiles);
+    first_tile = min(split * per_piece, all_tiles), n_tiles = min(first_tile + per_piece, all_tiles);
+  }
 
   // rows past the last are computed as copies of it
   const int32_t w0 = row0 + 32 * wr;  // the wave's first row
@@ -359,9 +375,9 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
     if (end <= wave_least) tile(it, kt, std::false_type{});
     else if (it * kTile < wave_most) tile(it, kt, std::true_type{});
   };
-  if (n_tiles > 0) load_tile(0, std::integral_constant<int, 0>{});
+  if (first_tile < n_tiles) load_tile(first_tile, std::integral_constant<int, 0>{});
 #pragma unroll 1
-  for (int it = 0; it < n_tiles; it += 2) {
+  for (int it = first_tile; it < n_tiles; it += 2) {
     step(it, std::integral_constant<int, 0>{});
     if (it + 1 < n_tiles) step(it + 1, std::integral_constant<int, 1>{});
   }
@@ -397,6 +413,18 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
   }
   if (row >= n_rows) return;
   const int64_t orow = static_cast<int64_t>(q0 + qi) * a.H + h;
+  if (a.n_split > 1) {
+    float* p = a.part + (orow * a.n_split + split) * (D + 4);
+    if (hh == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
+    if (first_tile < n_tiles) {  // (an empty piece's sum of 0 says that it has no output)
+#pragma unroll
+      for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(p + 4 + 32 * mb + 8 * i + 4 * hh) = make_float4(O[mb][4 * i], O[mb][4 * i + 1], O[mb][4 * i + 2], O[mb][4 * i + 3]);
+    }
+    return;
+  }
   const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
   const float up = fmaxf(m, sk);
   const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - up);
@@ -412,6 +440,37 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(2)
   if (a.lse && hh == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
+// Merges the pieces of the rows: D / 4 lanes hold a row, 4 dims each.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
+  using E = Elem<DT>;
+  constexpr int PER = D / 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / PER) + threadIdx.x / PER;
+  if (row >= static_cast<int64_t>(a.n_q) * a.H) return;
+  const int32_t n = static_cast<int32_t>(row / a.H), h = static_cast<int32_t>(row - static_cast<int64_t>(n) * a.H);
+  if (n < a.cu_q[0] || n >= a.cu_q[a.B]) return;  // in no sequence
+  const int j = threadIdx.x % PER;
+  const float* p = a.part + row * a.n_split * (D + 4);
+  const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+  float top = sk;
+#pragma unroll 4
+  for (int s = 0; s < a.n_split; ++s) top = fmaxf(top, p[s * (D + 4)]);
+  float sum = sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - top);
+  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < a.n_split; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(p + s * (D + 4));
+    if (ml.y == 0.0f) continue;  // nothing seen
+    const float4 o = *reinterpret_cast<const float4*>(p + s * (D + 4) + 4 + 4 * j);
+    const float f = __builtin_amdgcn_exp2f(ml.x - top);
+    sum += ml.y * f;
+    x[0] = fmaf(o.x, f, x[0]), x[1] = fmaf(o.y, f, x[1]), x[2] = fmaf(o.z, f, x[2]), x[3] = fmaf(o.w, f, x[3]);
+  }
+  const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(a.out + row * D + 4 * j) = make_uint2(E::pack(x[0] * r, x[1] * r), E::pack(x[2] * r, x[3] * r));
+  if (a.lse && j == 0) a.lse[row] = sum == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
 using prompt_fn = void (*)(PromptArgs);
 template <int WR, int KS>
 prompt_fn pick_prompt(int32_t dtype, int32_t d) {
@@ -419,17 +478,40 @@ prompt_fn pick_prompt(int32_t dtype, int32_t d) {
   return d == 64 ? prompt_attention_kernel<AEKV_BF16, 64, WR, KS> : prompt_attention_kernel<AEKV_BF16, 128, WR, KS>;
 }
 
+// How a launch is cut: rows of a workgroup, and pieces of the keys where the row tiles alone leave CUs without a workgroup
+// (as many as are resident together: three of a CU at head dim 64, two at 128).
+struct PromptPlan {
+  int64_t rows, tiles, split;
+};
+PromptPlan plan_prompt(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d) {
+  PromptPlan p;
+  const int64_t rows = n_q * (H / heads);
+  p.rows = heads * (rows / 128) >= 512 ? 128 : 64;
+  p.tiles = rows / p.rows + B;  // at least every sequence's, whatever their lengths
+  const int64_t room = (d == 64 ? 768 : 512) / (p.tiles * heads), most = ceil_div(n_k, static_cast<int64_t>(kTile * kPieceTiles));
+  p.split = room < most ? room : most;
+  if (p.split < 1) p.split = 1;
+  return p;
+}
+
 }  // namespace
 }  // namespace aekv
 
 using namespace aekv;
+
+extern "C" size_t aekv_prompt_attention_workspace_size(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads,
+                                                       int32_t d) {
+  if (B <= 0 || n_q <= 0 || n_k <= 0 || H <= 0 || heads <= 0 || d <= 0) return 0;
+  const PromptPlan p = plan_prompt(B, n_q, n_k, H, heads, d);
+  return p.split > 1 ? static_cast<size_t>(n_q * H) * static_cast<size_t>(p.split) * (d + 4) * 4 : 0;
+}
 
 extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
                                      int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
                                      int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens_q,
                                      const int32_t* cu_seqlens_k, int64_t B, int64_t n_q, int64_t n_k, int64_t H,
                                      int64_t heads, int32_t d, const float* sink, float softmax_scale, void* out,
-                                     float* lse, int32_t clear_rest, void* stream) {
+                                     float* lse, int32_t clear_rest, void* ws, size_t ws_bytes, void* stream) {
   const char* who = "aekv_prompt_attention";
   if (dtype != AEKV_F16 && dtype != AEKV_BF16) return fail(AEKV_ERR_DTYPE, "%s: q, k and v must be F16 or BF16", who);
   if (d != 64 && d != 128) return fail(AEKV_ERR_UNSUPPORTED, "%s: head dim %d (64 or 128 supported)", who, d);
@@ -449,18 +531,25 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
   if (k_token_stride * 2 * kTile > 0x3fffffff || v_token_stride * 2 * kTile > 0x3fffffff || k_token_stride < 0 || v_token_stride < 0)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: token strides of %lld and %lld elements", who, (long long)k_token_stride,
                 (long long)v_token_stride);
+  const PromptPlan plan = plan_prompt(B, n_q, n_k, H, heads, d);
+  const size_t want = aekv_prompt_attention_workspace_size(B, n_q, n_k, H, heads, d);
+  if (want && (!ws || ws_bytes < want)) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
+  if (!is_aligned(ws, 16)) return fail(AEKV_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  if (plan.tiles * heads * plan.split > kMaxGridThreads / 256 || ceil_div(n_q * H, 256 / (d / 4)) > kMaxGridThreads / 256)
+    return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld H=%lld exceed the grid", who, (long long)B, (long long)n_q, (long long)H);
   PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), q_token_stride,
                q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q, cu_seqlens_k, sink,
-               static_cast<uint16_t*>(out), lse, static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B),
-               static_cast<int32_t>(H), static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
+               static_cast<uint16_t*>(out), lse, static_cast<float*>(ws), static_cast<int32_t>(plan.split), static_cast<int32_t>(plan.tiles),
+               static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B), static_cast<int32_t>(H),
+               static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
                fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f};
-  const int64_t rows = n_q * (H / heads);
-  const bool large = heads * (rows / 128) >= 512;
-  const int per = large ? 128 : 64;
-  const int64_t tiles = rows / per + B;  // at least every sequence's, whatever their lengths
-  if (tiles * heads > kMaxGridThreads / 256)
-    return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld H=%lld exceed the grid", who, (long long)B, (long long)n_q, (long long)H);
-  auto fn = large ? pick_prompt<4, 1>(dtype, d) : pick_prompt<2, 2>(dtype, d);
-  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(tiles * heads)), dim3(256), 0, as_stream(stream), a);
+  const hipStream_t st = as_stream(stream);
+  auto fn = plan.rows == 128 ? pick_prompt<4, 1>(dtype, d) : pick_prompt<2, 2>(dtype, d);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(plan.tiles * heads * plan.split)), dim3(256), 0, st, a);
+  if (const int rc = check_launch(who)) return rc;
+  if (plan.split == 1) return AEKV_OK;
+  auto mg = dtype == AEKV_F16 ? (d == 64 ? prompt_merge_kernel<AEKV_F16, 64> : prompt_merge_kernel<AEKV_F16, 128>)
+                              : (d == 64 ? prompt_merge_kernel<AEKV_BF16, 64> : prompt_merge_kernel<AEKV_BF16, 128>);
+  hipLaunchKernelGGL(mg, dim3(static_cast<uint32_t>(ceil_div(n_q * H, 256 / (d / 4)))), dim3(256), 0, st, a);
   return check_launch(who);
 }

@@ -358,13 +358,15 @@ int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_scale, void* 
  * .. cu_seqlens_q[b + 1] and keys cu_seqlens_k[b] .. (int32 [B + 1], non-decreasing); its i-th query sees keys
  * j <= i + (keys - queries).  out [n_q, H, d] contiguous; lse fp32 [n_q, H] (nullable): log of the row's sum of
  * exponentials, the sink's (fp32 [H] or NULL) among them.  A query that sees nothing gives 0.  Rows in no
- * sequence: out is left as it is (clear_rest 0) or 0 (1), lse is -inf.  d = 64 or 128. */
+ * sequence: out is left as it is (clear_rest 0) or 0 (1), lse is -inf.  d = 64 or 128.  Workspace:
+ * aekv_prompt_attention_workspace_size bytes (0 for most sizes), 16-byte aligned; its contents never matter. */
+size_t aekv_prompt_attention_workspace_size(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d);
 int aekv_prompt_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
                           int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
                           int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens_q,
                           const int32_t* cu_seqlens_k, int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads,
                           int32_t d, const float* sink, float softmax_scale, void* out, float* lse,
-                          int32_t clear_rest, void* stream);
+                          int32_t clear_rest, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -231,3 +231,62 @@ def test_prompt_many_rows_masked_places(dev):
     assert torch.equal(got[:1111], clean[:1111]) and torch.equal(got[2300:2300 + 1990], clean[2300:2300 + 1990])
     assert torch.equal(got[1111:2300, :6], clean[1111:2300, :6]) and torch.equal(got[1111:2300, 8:], clean[1111:2300, 8:])
     assert got[1111:2300, 6:8].isnan().all()
+
+
+@pytest.mark.parametrize("dtype,dim,H,hk,lq,lk", [(torch.bfloat16, 128, 4, 2, [3, 1, 70], [1500, 513, 2100]), (torch.float16, 64, 8, 1, [1], [5003]), (torch.bfloat16, 64, 2, 2, [600], [600]),
+                                                  (torch.float16, 128, 12, 4, [5, 0, 40], [100, 3000, 1030])])
+@pytest.mark.parametrize("sink", [False, True])
+def test_prompt_few_rows_over_many_keys(dev, dtype, dim, H, hk, lq, lk, sink):
+    """Launches of few rows split the keys over workgroups: rows that see one piece, all of them, or none."""
+    from aetherkv.prompt import prompt_workspace
+
+    q, k, v = _inputs(dev, 30, dtype, dim, H, hk, lq, lk, pad=3)
+    cq, ck = (torch.tensor(_cu(x), dtype=torch.int32, device=dev) for x in (lq, lk))
+    assert prompt_workspace(len(lq), q.size(0), k.size(0), H, hk, dim, dev).numel() > 0
+    sk = torch.randn(H, device=dev, generator=_gen(dev, 31)) if sink else None
+    scale = dim ** -0.5
+    ws = prompt_workspace(len(lq), q.size(0), k.size(0), H, hk, dim, dev).fill_(255)
+    out, lse = prompt_attention(q, k, v, cq, scale, cu_seqlens_k=ck, sink=sk, return_lse=True, workspace=ws)
+    want, bound, wl, lb = R.prompt_attention_ref(q.cpu(), k.cpu(), v.cpu(), _cu(lq), _cu(lk), scale, None if sk is None else sk.cpu())
+    R.within(out, want, bound, "out")
+    none = wl == -math.inf
+    got = lse.double().cpu()
+    assert torch.equal(got == -math.inf, none)
+    R.within(got[~none], wl[~none], lb[~none], "lse")
+    again, lse2 = prompt_attention(q, k, v, cq, scale, cu_seqlens_k=ck, sink=sk, return_lse=True)
+    assert torch.equal(again, out) and torch.equal(lse2, lse)
+    given = torch.full_like(out, 5.0)
+    prompt_attention(q, k, v, cq, scale, cu_seqlens_k=ck, sink=sk, out=given)
+    assert (given[-3:] == 5).all() and torch.equal(given[:-3], out[:-3])
+
+
+def test_prompt_split_masked_places_and_captured(dev):
+    lq, lk, H, hk, dim = [50, 20], [1200, 700], 4, 2, 64
+    q, k, v = (x.clone() for x in _inputs(dev, 32, torch.bfloat16, dim, H, hk, lq, lk, pad=2))
+    cq, ck = (torch.tensor(_cu(x), dtype=torch.int32, device=dev) for x in (lq, lk))
+    clean = prompt_attention(q, k, v, cq, 0.125, cu_seqlens_k=ck)
+    for x in (k, v):
+        x[1190], x[1200 + 699], x[1900:] = NAN, math.inf, NAN
+    got = prompt_attention(q, k, v, cq, 0.125, cu_seqlens_k=ck)
+    assert torch.equal(got[:40], clean[:40]) and torch.equal(got[50:69], clean[50:69]) and got[40:50].isnan().all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        prompt_attention(q, k, v, cq, 0.125, cu_seqlens_k=ck)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    outs = []
+    for g in graphs:  # two graphs, each with a workspace of its own
+        with torch.cuda.graph(g):
+            outs.append(prompt_attention(q, k, v, cq, 0.125, cu_seqlens_k=ck))
+    for rep in range(3):
+        q.copy_(torch.randn(q.shape, device=dev, generator=_gen(dev, rep)))
+        k.copy_(torch.randn(k.shape, device=dev, generator=_gen(dev, 10 + rep)))
+        v.copy_(torch.randn(v.shape, device=dev, generator=_gen(dev, 20 + rep)))
+        want = prompt_attention(q, k, v, cq, 0.125, cu_seqlens_k=ck)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)

@@ -48,8 +48,8 @@ def _evict(lib, d=128, bits=4, B=3, lengths=FAKE, weights=FAKE, tokens=FAKE, cap
                              p["max_pages"], B, lengths, weights, tokens, cap, seen, keep, first, recent, ws, wsb, None)
 
 
-def _prompt(lib, q=FAKE, k=FAKE, v=FAKE, dtype=L.BF16, st=(512, 128, 256, 128, 256, 128), cq=FAKE, ck=FAKE, B=2, nq=10, nk=10, H=4, hk=2, d=128, out=FAKE):
-    return lib.aekv_prompt_attention(q, k, v, dtype, *st, cq, ck, B, nq, nk, H, hk, d, None, 0.1, out, None, 0, None)
+def _prompt(lib, q=FAKE, k=FAKE, v=FAKE, dtype=L.BF16, st=(512, 128, 256, 128, 256, 128), cq=FAKE, ck=FAKE, B=2, nq=10, nk=10, H=4, hk=2, d=128, out=FAKE, ws=FAKE, wsb=1 << 30):
+    return lib.aekv_prompt_attention(q, k, v, dtype, *st, cq, ck, B, nq, nk, H, hk, d, None, 0.1, out, None, 0, ws, wsb, None)
 
 
 @pytest.mark.parametrize("call", [_append, _attend, _evict])
@@ -117,6 +117,10 @@ def test_prompt_refusals(lib):
     assert _prompt(lib, st=(512, 128, 252, 128, 256, 128)) == L.ERR_ALIGN
     assert _prompt(lib, B=0) == L.ERR_SHAPE
     assert _prompt(lib, nq=0) == L.OK
+    need = lib.aekv_prompt_attention_workspace_size(2, 10, 100000, 4, 2, 128)
+    assert need > 0 and _prompt(lib, nk=100000, wsb=need - 1) == L.ERR_WORKSPACE
+    assert _prompt(lib, nk=100000, ws=ctypes.c_void_p(0x10008), wsb=need) == L.ERR_ALIGN
+    assert lib.aekv_prompt_attention_workspace_size(2, 10, 10, 4, 2, 128) == 0
 
 
 def test_python_calls_refuse_cpu_tensors_and_wrong_arguments():
