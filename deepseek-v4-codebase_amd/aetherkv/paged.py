@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .decode import _check_out, _f32, _i32, _iptr, _sink_f32
+from .decode import _check_out, _i32, _sink_f32
 from .turbo_quant import PolarQuant
 
 
@@ -47,10 +47,22 @@ class PagedKVCache:
 
     def _set(self, quant, k_codes, k_scale, v_codes, v_scale) -> None:
         self.quant, self.bits = quant, quant.bits
-        self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
+        self._tensors = (k_codes, k_scale, v_codes, v_scale)
+        self._ptrs = tuple(t.data_ptr() for t in self._tensors)  # (the cache owns its tensors: they stay where they are)
         self.pages, self.kv_heads, self.page_size = k_scale.shape
         self.dim = k_codes.size(3) * (1 if quant.bits == 8 else 2)
-        self.device = k_codes.device
+        self.device, self._index = k_codes.device, k_codes.get_device()
+        self._diag: Optional[torch.Tensor] = None
+
+    k_codes = property(lambda self: self._tensors[0])
+    k_scale = property(lambda self: self._tensors[1])
+    v_codes = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
+
+    def _diag_ptr(self) -> int:
+        if self._diag is None:
+            self._diag = self.quant._diag(self.dim, self.device)
+        return self._diag.data_ptr()
 
     @classmethod
     def from_tensors(cls, quant: PolarQuant, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
@@ -113,25 +125,30 @@ class SlotTracker:
         return self
 
 
-def _counts(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
-    """A per-sequence count as contiguous int32 [B]."""
-    if t.dim() != 1 or t.size(0) != B or t.is_floating_point():
-        raise RuntimeError(f"{name} must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
-    return _i32(t)
+# The calls below are made once per layer and token, so their host cost counts: every tensor method costs some 0.1 us, a
+# new view or conversion several times that, so what is already in the kernels' form is passed as it is.
+_INT32 = torch.int32
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+
+
+def _counts(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    """A per-sequence count as contiguous int32 [n]."""
+    if t.shape != (n,) or t.is_floating_point():
+        raise RuntimeError(f"{name} must be int32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    return t if t.dtype is _INT32 and t.is_contiguous() else _i32(t)
 
 
 def _table(page_table: torch.Tensor) -> torch.Tensor:
     if page_table.dim() != 2 or page_table.is_floating_point():
         raise RuntimeError(f"page_table must be int32 [B, max_pages], got {page_table.dtype} {tuple(page_table.shape)}")
-    return _i32(page_table)
+    return page_table if page_table.dtype is _INT32 and page_table.is_contiguous() else _i32(page_table)
 
 
-def _one_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    """The kernels get raw pointers: every tensor of a call must be on the cache's device."""
-    index = device.index if device.index is not None else torch.cuda.current_device()
+def _one_device(index: int, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels get raw pointers: every tensor of a call must be on the device `index`."""
     for t in tensors:
         if t is not None and t.get_device() != index:
-            raise RuntimeError(f"every tensor of the call must be on {device}, got one on {t.device}")
+            raise RuntimeError(f"every tensor of the call must be on the HIP device {index}, got one on {t.device}")
 
 
 def _check_tracker(tracker: SlotTracker, cache: PagedKVCache, B: int) -> None:
@@ -140,22 +157,31 @@ def _check_tracker(tracker: SlotTracker, cache: PagedKVCache, B: int) -> None:
                            f"{cache.kv_heads}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [.., heads, D] with rows the kernels can read in place: contiguous in D, 16-byte aligned; else a copy."""
-    e = 16 // t.element_size()
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
+    """t [.., heads, D] with rows the kernels can read in place (contiguous in D, 16-byte aligned; else a copy), and its
+    strides."""
     st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(s % e for s in st[:-1]):
-        return _lib.aligned(t, 16)
-    return t
+    e = 8 if t.dtype is not torch.float32 else 4
+    if st[-1] == 1 and not t.data_ptr() % 16:
+        for s in st[:-1]:
+            if s % e:
+                break
+        else:
+            return t, st
+    t = _lib.aligned(t, 16)
+    return t, t.stride()
 
 
-def _flat_tokens(t: torch.Tensor) -> torch.Tensor:
-    """[B, T, heads, D] -> [B * T, heads, D], a view where the strides allow it."""
-    B, T, H, D = t.shape
-    if B == 1 or T == 1 or t.stride(0) == T * t.stride(1):
-        n, s = B * T, (t.stride(1) if T > 1 else t.stride(0))
-        return t.as_strided((n, H, D), (s, t.stride(2), t.stride(3)))
-    return t.reshape(B * T, H, D)
+def _token_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """[B, T, heads, D] as B * T tokens: the tensor (or a copy), the stride of a token and of a head."""
+    t, st = _rows(t)
+    B, T = t.size(0), t.size(1)
+    if T == 1:
+        return t, st[0], st[2]
+    if B == 1 or st[0] == T * st[1]:
+        return t, st[1], st[2]
+    t = t.contiguous()
+    return t, t.stride(1), t.stride(2)
 
 
 def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
@@ -168,36 +194,43 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
     views are read in place.  The codes are PolarQuant.encode's, bit for bit.  With a tracker, the slots' weights start at
     0 and their token indices at token[b] (int32 [B]: the sequence's tokens before this call)."""
     B = page_table.size(0)
-    want = 4 if cu_seqlens is None else 3
-    if k.dim() != want or v.dim() != want or k.shape != v.shape or k.shape[-2:] != (cache.kv_heads, cache.dim):
-        shape = "[B, T" if cu_seqlens is None else "[N"
-        raise RuntimeError(f"append_tokens expects k and v {shape}, {cache.kv_heads}, {cache.dim}], got {tuple(k.shape)} "
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != (4 if cu_seqlens is None else 3) or v.shape != shape or shape[-2] != cache.kv_heads or shape[-1] != cache.dim:
+        want = "[B, T" if cu_seqlens is None else "[N"
+        raise RuntimeError(f"append_tokens expects k and v {want}, {cache.kv_heads}, {cache.dim}], got {tuple(shape)} "
                            f"and {tuple(v.shape)}")
-    if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise RuntimeError(f"k and v must be bfloat16, float16 or float32 alike, got {k.dtype} and {v.dtype}")
-    if cu_seqlens is None and k.size(0) != B:
-        raise RuntimeError(f"k holds {k.size(0)} sequences, page_table {B}")
+    code = _TYPES.get(dtype)
+    if code is None or v.dtype is not dtype:
+        raise RuntimeError(f"k and v must be bfloat16, float16 or float32 alike, got {dtype} and {v.dtype}")
     if (tracker is None) != (token is None):
         raise RuntimeError("append_tokens: a tracker and the sequences' token counts come together")
-    _one_device(cache.device, k, v, page_table, start, cu_seqlens, token, None if tracker is None else tracker.storage)
+    _one_device(cache._index, k, v, page_table, start, cu_seqlens, token, None if tracker is None else tracker.storage)
     table, start = _table(page_table), _counts("start", start, B)
-    cu = None if cu_seqlens is None else _counts("cu_seqlens", cu_seqlens, B + 1)
+    if cu_seqlens is None:
+        if shape[0] != B:
+            raise RuntimeError(f"k holds {shape[0]} sequences, page_table {B}")
+        cu, n = None, B * shape[1]
+        k, kt, kh = _token_rows(k)
+        v, vt, vh = _token_rows(v)
+    else:
+        cu, n = _counts("cu_seqlens", cu_seqlens, B + 1), shape[0]
+        k, (kt, kh, _) = _rows(k)
+        v, (vt, vh, _) = _rows(v)
+    weights = tokens = first = None
+    capacity = 0
     if tracker is not None:
         _check_tracker(tracker, cache, B)
         token = _counts("token", token, B)
-    kr, vr = _rows(k if cu is not None else _flat_tokens(k)), _rows(v if cu is not None else _flat_tokens(v))
+        weights, tokens, first, capacity = tracker.weights.data_ptr(), tracker.tokens.data_ptr(), token.data_ptr(), tracker.capacity
+    kc, ks, vc, vs = cache._ptrs
     dev = cache.device
-    diag = cache.quant._diag(cache.dim, dev)
     with _lib.on_device(dev):
         rc = _lib.hot("aekv_kv_append")(
-            kr.data_ptr(), vr.data_ptr(), _lib.TORCH_TO_AEKV[k.dtype], kr.stride(0), kr.stride(1), vr.stride(0),
-            vr.stride(1), kr.size(0), _iptr(cu), B, start.data_ptr(), cache.dim, cache.bits, diag.data_ptr(),
-            cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(), cache.v_scale.data_ptr(),
-            cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1),
-            None if tracker is None else tracker.weights.data_ptr(),
-            None if tracker is None else tracker.tokens.data_ptr(), 0 if tracker is None else tracker.capacity,
-            _iptr(token), _lib.raw_stream(dev))
-    _lib.check(rc, "aekv_kv_append")
+            k.data_ptr(), v.data_ptr(), code, kt, kh, vt, vh, n, None if cu is None else cu.data_ptr(), B,
+            start.data_ptr(), cache.dim, cache.bits, cache._diag_ptr(), kc, ks, vc, vs, cache.pages, cache.kv_heads,
+            cache.page_size, table.data_ptr(), table.size(1), weights, tokens, capacity, first, _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "aekv_kv_append")
 
 
 def paged_attention_workspace(B: int, T: int, H: int, kv_heads: int, dim: int, slots: int, device, *,
@@ -217,40 +250,44 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     reads KV head h // (H // kv_heads).  Token t sees slots j < lengths[b] - T + 1 + t.  sink [H] (or a scalar): a logit
     counted once in the normaliser.  A row that sees nothing gives 0.  With a tracker, weights[b, kv head, j] grows by
     the attention weight of slot j, summed over the group's heads and the T tokens.  Returns [B, T, H, D] like q."""
-    if q.dim() != 4 or q.size(3) != cache.dim:
-        raise RuntimeError(f"q must be [B, T, H, {cache.dim}], got {tuple(q.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError(f"q must be bfloat16 or float16, got {q.dtype}")
-    B, T, H, D = q.shape
-    if H % cache.kv_heads:
-        raise RuntimeError(f"{H} query heads are no multiple of {cache.kv_heads} KV heads")
-    if page_table.size(0) != B:
-        raise RuntimeError(f"q holds {B} sequences, page_table {page_table.size(0)}")
-    _one_device(cache.device, q, page_table, lengths, sink, workspace, out, None if tracker is None else tracker.storage)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4 or shape[3] != cache.dim:
+        raise RuntimeError(f"q must be [B, T, H, {cache.dim}], got {tuple(shape)}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise RuntimeError(f"q must be bfloat16 or float16, got {dtype}")
+    B, T, H, D = shape
+    heads = cache.kv_heads
+    if H % heads:
+        raise RuntimeError(f"{H} query heads are no multiple of {heads} KV heads")
+    _one_device(cache._index, q, page_table, lengths, sink, workspace, out, None if tracker is None else tracker.storage)
     table, lengths = _table(page_table), _counts("lengths", lengths, B)
-    if tracker is not None:
-        _check_tracker(tracker, cache, B)
-    qr = _rows(q)
+    table_rows, max_pages = table.shape
+    if table_rows != B:
+        raise RuntimeError(f"q holds {B} sequences, page_table {table_rows}")
+    q, st = _rows(q)
     sk = None if sink is None else _sink_f32(sink, H)
     dev = cache.device
-    diag = cache.quant._diag(D, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty(shape, dtype=dtype, device=dev)
     else:
-        _check_out("out", out, q.dtype, q.numel(), dev)
-    need = _lib.paged_ws_bytes(B, T, H, cache.kv_heads, D, table.size(1) * cache.page_size, 0 if tracker is None else 1)
+        _check_out("out", out, dtype, q.numel(), dev)
+    weights, capacity, tracked = None, 0, 0
+    if tracker is not None:
+        _check_tracker(tracker, cache, B)
+        weights, capacity, tracked = tracker.weights.data_ptr(), tracker.capacity, 1
+    kc, ks, vc, vs = cache._ptrs
+    need = _lib.paged_ws_bytes(B, T, H, heads, D, max_pages * cache.page_size, tracked) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_paged_attention")(
-            qr.data_ptr(), _lib.TORCH_TO_AEKV[q.dtype], qr.stride(0), qr.stride(1), qr.stride(2), B, T, H, D, cache.bits,
-            diag.data_ptr(), cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(),
-            cache.v_scale.data_ptr(), cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1),
-            lengths.data_ptr(), _iptr(sk), None if tracker is None else tracker.weights.data_ptr(),
-            0 if tracker is None else tracker.capacity, float(softmax_scale), _iptr(ws), 0 if ws is None else ws.numel(),
-            out.data_ptr(), stream)
-    _lib.check(rc, "aekv_paged_attention")
-    return out if out.dim() == 4 else out.view(q.shape)
+            q.data_ptr(), _TYPES[dtype], st[0], st[1], st[2], B, T, H, D, cache.bits, cache._diag_ptr(), kc, ks, vc, vs,
+            cache.pages, heads, cache.page_size, table.data_ptr(), max_pages, lengths.data_ptr(),
+            None if sk is None else sk.data_ptr(), weights, capacity, float(softmax_scale),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), out.data_ptr(), stream)
+    if rc:
+        _lib.check(rc, "aekv_paged_attention")
+    return out if out.dim() == 4 else out.view(shape)
 
 
 def evict_workspace(B: int, kv_heads: int, keep: int, slots: int, device) -> torch.Tensor:
@@ -268,19 +305,21 @@ def evict_by_weight(cache: PagedKVCache, page_table: torch.Tensor, lengths: torc
     every number).  Kept slots below `keep` stay where they are; the evicted ones below `keep`, in order, take the kept
     slots from `keep` on, in order, with their weight and token index: cached keys carry their rotation, so attention
     does not depend on the order of the slots.  `lengths` is only read: clamp it to `keep` once every layer is done."""
-    B = page_table.size(0)
-    _one_device(cache.device, page_table, lengths, seen, workspace, tracker.storage)
+    B, max_pages = page_table.shape
+    _one_device(cache._index, page_table, lengths, seen, workspace, tracker.storage)
     table, lengths, seen = _table(page_table), _counts("lengths", lengths, B), _counts("seen", seen, B)
     _check_tracker(tracker, cache, B)
     keep, first, recent = int(keep), int(first), int(recent)
     dev = cache.device
-    need = _lib.evict_ws_bytes(B, cache.kv_heads, keep, min(table.size(1) * cache.page_size, tracker.capacity))
+    kc, ks, vc, vs = cache._ptrs
+    need = _lib.evict_ws_bytes(B, cache.kv_heads, keep, min(max_pages * cache.page_size, tracker.capacity)) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_kv_evict")(
-            cache.dim, cache.bits, cache.k_codes.data_ptr(), cache.k_scale.data_ptr(), cache.v_codes.data_ptr(),
-            cache.v_scale.data_ptr(), cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), table.size(1), B,
-            lengths.data_ptr(), tracker.weights.data_ptr(), tracker.tokens.data_ptr(), tracker.capacity,
-            seen.data_ptr(), keep, first, recent, _iptr(ws), 0 if ws is None else ws.numel(), stream)
-    _lib.check(rc, "aekv_kv_evict")
+            cache.dim, cache.bits, kc, ks, vc, vs, cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), max_pages,
+            B, lengths.data_ptr(), tracker.weights.data_ptr(), tracker.tokens.data_ptr(), tracker.capacity,
+            seen.data_ptr(), keep, first, recent, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            stream)
+    if rc:
+        _lib.check(rc, "aekv_kv_evict")

@@ -9,8 +9,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .decode import _check_out, _iptr, _sink_f32
-from .paged import _counts, _one_device, _rows
+from .decode import _check_out, _sink_f32
+from .paged import _TYPES, _counts, _one_device, _rows
 
 
 def prompt_workspace(B: int, n_q: int, n_k: int, H: int, kv_heads: int, dim: int, device) -> torch.Tensor:
@@ -31,21 +31,22 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     once in the normaliser.  A query that sees nothing gives 0.  Rows of q in no sequence: a given `out` keeps them, a new
     one holds 0.  Returns out [N, H, D], with return_lse (out, lse fp32 [N, H]): the log of every row's sum of
     exponentials, the sink's among them (-inf for rows in no sequence)."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.size(2) != q.size(2):
-        raise RuntimeError(f"prompt_attention expects q [N, H, D] and k, v [M, kv_heads, D], got {tuple(q.shape)}, "
-                           f"{tuple(k.shape)} and {tuple(v.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise RuntimeError(f"q, k and v must be bfloat16 or float16 alike, got {q.dtype}, {k.dtype} and {v.dtype}")
-    _lib.require_device("q", q, k, v, cu_seqlens, cu_seqlens_k, sink, out)
-    N, H, D = q.shape
-    M, hk, _ = k.shape
+    shape, dtype, ks = q.shape, q.dtype, k.shape
+    if len(shape) != 3 or len(ks) != 3 or v.shape != ks or ks[2] != shape[2]:
+        raise RuntimeError(f"prompt_attention expects q [N, H, D] and k, v [M, kv_heads, D], got {tuple(shape)}, "
+                           f"{tuple(ks)} and {tuple(v.shape)}")
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
+        raise RuntimeError(f"q, k and v must be bfloat16 or float16 alike, got {dtype}, {k.dtype} and {v.dtype}")
+    N, H, D = shape
+    M, hk, _ = ks
     if hk < 1 or H % hk:
         raise RuntimeError(f"{H} query heads are no multiple of {hk} KV heads")
     if cu_seqlens.dim() != 1 or cu_seqlens.size(0) < 2:
         raise RuntimeError(f"cu_seqlens must be int32 [B + 1], got {tuple(cu_seqlens.shape)}")
     B = cu_seqlens.size(0) - 1
+    _lib.require_device("q", q)
     dev = q.device
-    _one_device(dev, k, v, cu_seqlens, cu_seqlens_k, sink, workspace, out)
+    _one_device(q.get_device(), k, v, cu_seqlens, cu_seqlens_k, sink, workspace, out)
     cq = _counts("cu_seqlens", cu_seqlens, B + 1)
     if cu_seqlens_k is None:
         if M != N:
@@ -53,23 +54,26 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         ck = cq
     else:
         ck = _counts("cu_seqlens_k", cu_seqlens_k, B + 1)
-    qr, kr, vr = _rows(q), _rows(k), _rows(v)
+    q, (qt, qh, _) = _rows(q)
+    k, (kt, kh, _) = _rows(k)
+    v, (vt, vh, _) = _rows(v)
     sk = None if sink is None else _sink_f32(sink, H)
     clear = 0
     if out is None:
-        out, clear = torch.empty(q.shape, dtype=q.dtype, device=dev), 1
+        out, clear = torch.empty(shape, dtype=dtype, device=dev), 1
     else:
-        _check_out("out", out, q.dtype, q.numel(), dev)
+        _check_out("out", out, dtype, q.numel(), dev)
     lse = torch.empty((N, H), dtype=torch.float32, device=dev) if return_lse else None
-    need = _lib.prompt_ws_bytes(B, N, M, H, hk, D)
+    need = _lib.prompt_ws_bytes(B, N, M, H, hk, D) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream)
+        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_prompt_attention")(
-            qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), _lib.TORCH_TO_AEKV[q.dtype], qr.stride(0), qr.stride(1),
-            kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1), cq.data_ptr(), ck.data_ptr(), B, N, M, H, hk, D,
-            _iptr(sk), float(softmax_scale), out.data_ptr(), _iptr(lse), clear, _iptr(ws),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _TYPES[dtype], qt, qh, kt, kh, vt, vh, cq.data_ptr(),
+            ck.data_ptr(), B, N, M, H, hk, D, None if sk is None else sk.data_ptr(), float(softmax_scale), out.data_ptr(),
+            None if lse is None else lse.data_ptr(), clear, None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel(), stream)
-    _lib.check(rc, "aekv_prompt_attention")
-    out = out if out.dim() == 3 else out.view(q.shape)
+    if rc:
+        _lib.check(rc, "aekv_prompt_attention")
+    out = out if out.dim() == 3 else out.view(shape)
     return (out, lse) if return_lse else out

@@ -866,8 +866,11 @@ paged_fn pick_weights(int d, int bits) {
 // Pieces of a sequence: enough workgroups for the chip (1536: three per CU, twice over, which evens out sequences of
 // different lengths; one sequence of 262144 slots x 12 heads, 1024 / 1536 / 2048 / 3000 workgroups: 111 / 101 / 109 / 113 us,
 // 64 ragged ones of up to 16384 slots x 4 heads 122 / 119 / 117 / 119), but none of fewer than 512 slots beyond 512 workgroups (a workgroup's rotations and merge cost as
-// much as some 500 slots), and none without a whole round of slots.
+// much as some 500 slots), and none without a whole round of slots.  Tables of up to kOnePiece slots are not split: the
+// merge's launch costs more than their few rounds.
+constexpr int64_t kOnePiece = 512;
 int64_t paged_pieces(int64_t groups, int64_t slots) {
+  if (slots <= kOnePiece) return 1;
   const int64_t few = ceil_div(512, groups), some = ceil_div(slots, 512);
   const int64_t want = ceil_div(1536, groups), most = ceil_div(slots, kRound);
   int64_t n = few > some ? few : some;
