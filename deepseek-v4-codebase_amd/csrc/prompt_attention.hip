@@ -55,6 +55,7 @@ struct PromptArgs {
   int32_t n_split, tiles;
   int32_t n_q, n_k, B, H, heads, G;
   int32_t clear;        // rows in no sequence: 0 to leave out as it is, 1 to write zeros
+  int32_t by_work;      // the tiles' order: 0 the sequences', else by work (half of a power of two above every level)
   float scale2;         // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
   int32_t flip;         // scale is negative the queries' signs are flipped: a row's largest product is its largest logit
 };
@@ -129,6 +130,44 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int32_t t, int ro
   return false;
 }
 
+__device__ __forceinline__ int32_t lane_sum(int32_t v) {
+  auto step = [&](auto hl) { v += __builtin_bit_cast(int32_t, xor_lane<decltype(hl)::value>(__builtin_bit_cast(float, v))); };
+  step(std::integral_constant<int, 1>{}), step(std::integral_constant<int, 2>{}), step(std::integral_constant<int, 4>{});
+  step(std::integral_constant<int, 8>{}), step(std::integral_constant<int, 16>{}), step(std::integral_constant<int, 32>{});
+  return v;
+}
+
+// The same of up to 64 sequences by the tiles' work, the most keys first: a sequence's tiles have the levels `from` ..
+// from + its tiles, a level being the keys that one tile of rows adds, and the t-th of all is found by halving over levels.
+// It shortens the launch's end, where the longest tiles of the last sequence would run alone, and costs the keys' locality:
+// all sequences' keys are in use at once.
+__device__ __forceinline__ bool find_tile_by_work(const PromptArgs& a, int32_t t, int rows, int lane, TileAt* at) {
+  const int32_t b = min(lane, a.B - 1);
+  const int32_t c0 = a.cu_q[b], c1 = a.cu_q[b + 1], d0 = a.cu_k[b], d1 = a.cu_k[b + 1];
+  const int32_t q0 = min(max(c0, 0), a.n_q), lq = min(max(c1, q0), a.n_q) - q0;
+  const int32_t k0 = min(max(d0, 0), a.n_k), lk = min(max(d1, k0), a.n_k) - k0;
+  const int32_t tiles = lane < a.B ? (lq * a.G + rows - 1) / rows : 0;
+  const int64_t ahead = static_cast<int64_t>(max(lk - lq, 0)) * a.G / rows;
+  const int32_t from = static_cast<int32_t>(ahead < (1 << 25) ? ahead : 1 << 25);
+  auto at_least = [&](int32_t level) { return min(max(from + tiles - level, 0), tiles); };  // own tiles of that level or more
+  if (lane_sum(tiles) <= t) return false;
+  int32_t level = 0;  // the highest with more than t tiles at or above it
+#pragma unroll 1
+  for (int32_t bit = a.by_work; bit > 0; bit >>= 1)
+    if (lane_sum(at_least(level + bit)) > t) level += bit;
+  const int32_t above = lane_sum(at_least(level + 1));
+  uint64_t with = __builtin_amdgcn_ballot_w64(at_least(level) > at_least(level + 1));  // sequences with a tile of it
+  for (int32_t i = above; i < t && with; ++i) with &= with - 1;
+  if (!with) return false;  // (offsets that are no prefix sums)
+  const int l = __builtin_ctzll(with);
+  at->q0 = __builtin_amdgcn_readlane(q0, l);
+  at->lq = __builtin_amdgcn_readlane(lq, l);
+  at->k0 = __builtin_amdgcn_readlane(k0, l);
+  at->lk = __builtin_amdgcn_readlane(lk, l);
+  at->row = (level - __builtin_amdgcn_readlane(from, l)) * rows;
+  return true;
+}
+
 template <int DT, int D, int WR, int KS>
 __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void prompt_attention_kernel(PromptArgs a) {
   using E = Elem<DT>;
@@ -159,7 +198,8 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
     index -= split * a.tiles;
   }
   TileAt at;
-  const bool found = find_tile(a, static_cast<int32_t>(index), kRows, lane, &at);
+  const bool found = a.by_work ? find_tile_by_work(a, static_cast<int32_t>(index), kRows, lane, &at)
+                               : find_tile(a, static_cast<int32_t>(index), kRows, lane, &at);
   if (a.clear || a.lse) {  // rows in no sequence: shared out over the workgroups
     const int32_t s0 = min(max(a.cu_q[0], 0), a.n_q), s1 = min(max(a.cu_q[a.B], s0), a.n_q);
     const int64_t words = static_cast<int64_t>(s0 + a.n_q - s1) * a.H * (D / 2);
@@ -411,9 +451,9 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
 #pragma unroll
       for (int v = 0; v < 16; ++v) O[mb][v] = O[mb][v] * f0 + slot(at + (mb * 16 + v) * 64)[lane] * f1;
   }
-  if (row >= n_rows) return;
   const int64_t orow = static_cast<int64_t>(q0 + qi) * a.H + h;
   if (a.n_split > 1) {
+    if (row >= n_rows) return;
     float* p = a.part + (orow * a.n_split + split) * (D + 4);
     if (hh == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
     if (first_tile < n_tiles) {  // (an empty piece's sum of 0 says that it has no output)
@@ -430,14 +470,40 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
   const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - up);
   const float sum = (l == 0.0f ? 0.0f : l * f) + (sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - up));
   const float r = sum == 0.0f ? 0.0f : f / sum;
-  uint16_t* op = a.out + orow * D + 4 * hh;
+  if (a.lse && hh == 0 && row < n_rows) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
+  if constexpr (KS == 1) {
+    // a lane holds 8-byte pieces of its row: the wave's rows go through LDS, their 16-byte chunks swizzled, so that a store
+    // writes whole rows and passes by the caches, which keep the keys (64 prompts of 1024, 12 heads of 4: 354 -> 346 us)
+    constexpr int kLanes = kRow / 16;  // of a row
+    static_assert(kWaves * 32 * kRow <= 2 * Gm::kTileBytes, "the rows fit a buffer");
+    uint8_t* const w = L0 + wv * 32 * kRow;
+    __syncthreads();  // the last tile's readers are done
 #pragma unroll
-  for (int mb = 0; mb < kMB; ++mb)
+    for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint2*>(op + 32 * mb + 8 * i) = make_uint2(E::pack(O[mb][4 * i] * r, O[mb][4 * i + 1] * r),
-                                                                   E::pack(O[mb][4 * i + 2] * r, O[mb][4 * i + 3] * r));
-  if (a.lse && hh == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(w + rl * kRow + (((4 * mb + i) ^ (rl % kLanes)) << 4) + 8 * hh) =
+            make_uint2(E::pack(O[mb][4 * i] * r, O[mb][4 * i + 1] * r), E::pack(O[mb][4 * i + 2] * r, O[mb][4 * i + 3] * r));
+    __builtin_amdgcn_wave_barrier();
+    const int c = lane % kLanes;
+#pragma unroll
+    for (int i = 0; i < 32; i += 64 / kLanes) {
+      const int wr_row = i + lane / kLanes, at_row = w0 + wr_row;
+      if (at_row >= n_rows) continue;
+      const int32_t qn = at_row / a.G, hn = head * a.G + (at_row - qn * a.G);
+      __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(w + wr_row * kRow + ((c ^ (wr_row % kLanes)) << 4)),
+                                  reinterpret_cast<u32x4_t*>(a.out + (static_cast<int64_t>(q0 + qn) * a.H + hn) * D + 8 * c));
+    }
+  } else {
+    if (row >= n_rows) return;
+    uint16_t* op = a.out + orow * D + 4 * hh;
+#pragma unroll
+    for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(op + 32 * mb + 8 * i) = make_uint2(E::pack(O[mb][4 * i] * r, O[mb][4 * i + 1] * r),
+                                                                     E::pack(O[mb][4 * i + 2] * r, O[mb][4 * i + 3] * r));
+  }
 }
 
 // Merges the pieces of the rows: D / 4 lanes hold a row, 4 dims each.
@@ -537,12 +603,20 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
   if (!is_aligned(ws, 16)) return fail(AEKV_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
   if (plan.tiles * heads * plan.split > kMaxGridThreads / 256 || ceil_div(n_q * H, 256 / (d / 4)) > kMaxGridThreads / 256)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld n_q=%lld H=%lld exceed the grid", who, (long long)B, (long long)n_q, (long long)H);
+  // By work where the keys and values that an XCD reads are at most three times its 4 MB L2 (a KV head's workgroups lie on
+  // 8 / heads XCDs, or an XCD has heads / 8): 16 prompts of up to 2048, 12 heads of 4, 9.7 MB: 132 against 142 us; 8 of 2048,
+  // 8.4 MB: 128 against 144; 64 of 1024, 34 MB: 360 against 340; 32 of 2048, 16 heads of 16, 67 MB: 1007 against 712.
+  int32_t by_work = 0;
+  if (B > 1 && B <= 64 && plan.tiles * heads > (d == 64 ? 768 : 512) && n_k * ceil_div(heads, static_cast<int64_t>(8)) * 4 * d <= (12 << 20)) {
+    const int64_t levels = n_k * (H / heads) / plan.rows + plan.tiles;
+    for (by_work = 1; by_work < (1 << 25) && 2 * by_work <= levels;) by_work *= 2;
+  }
   PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), q_token_stride,
                q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q, cu_seqlens_k, sink,
                static_cast<uint16_t*>(out), lse, static_cast<float*>(ws), static_cast<int32_t>(plan.split), static_cast<int32_t>(plan.tiles),
                static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B), static_cast<int32_t>(H),
                static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
-               fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f};
+               by_work, fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f};
   const hipStream_t st = as_stream(stream);
   auto fn = plan.rows == 128 ? pick_prompt<4, 1>(dtype, d) : pick_prompt<2, 2>(dtype, d);
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(plan.tiles * heads * plan.split)), dim3(256), 0, st, a);

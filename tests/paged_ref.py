@@ -114,7 +114,8 @@ def prompt_attention_ref(q, k, v, cu_q, cu_k, scale, sink=None):
                 sk = -math.inf if sink is None else float(sink[h])
                 r = cu_q[b] + i
                 if n == 0:
-                    lse[r, h] = sk
+                    # the sink in units of log2 and back: two products and the rounding of both constants, 4 2^-24 of it
+                    lse[r, h], lb[r, h] = sk, 2.0 ** -22 * abs(sk) if sk > -math.inf else 0.0
                     continue
                 qd = q[r, h].double()
                 logit = kk[:n] @ qd * scale

@@ -290,3 +290,16 @@ def test_prompt_split_masked_places_and_captured(dev):
         graphs[1].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("B", [2, 63, 64, 65])
+@pytest.mark.parametrize("H,hk,most", [(32, 32, 40), (48, 16, 90)])
+def test_prompt_many_tiles_of_many_sequences(dev, B, H, hk, most):
+    """More tiles than run together, of chunks with different numbers of keys before them, fewer keys than queries, and
+    nothing: each row is written once, whatever the order that the tiles are taken in."""
+    rng = torch.Generator().manual_seed(B)
+    lq = [int(x) for x in torch.randint(0, most, (B,), generator=rng)]
+    lk = [max(0, n + (0, 70, -3, 300)[i % 4]) for i, n in enumerate(lq)]
+    if B == 2:
+        lq, lk = [most * 9, most * 3], [most * 9, most * 3 + 700]
+    _check(dev, torch.bfloat16, 64, H, hk, lq, lk, sink=True, seed=B, pad=2)
