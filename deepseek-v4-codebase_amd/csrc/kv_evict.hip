@@ -7,7 +7,8 @@
 // the kept slots from `keep` on, in increasing order.  Sources and destinations are disjoint: the rows move in place, in
 // parallel, and only as many as there are holes.
 //
-// Two launches: one workgroup per (sequence, head) selects and lists the moves, then the whole chip moves the rows.
+// One workgroup per (sequence, head) selects and lists the moves; it makes them itself where they are few, and the whole
+// chip makes them in a second launch where they can be many.
 #include "paged_cache.h"
 
 namespace aekv {
@@ -34,6 +35,58 @@ __device__ __forceinline__ uint32_t evict_key(float w, int32_t token, int32_t fi
   return order_key(w + 0.0f);
 }
 
+// 16 lanes move one slot: its code rows, scales, weight and token.  kMoves slots at a time, so that their dependent loads
+// (the move, the pages, the rows) overlap: those of the `count` listed moves from `first` on, every `step`.
+constexpr int kMoves = 4;
+
+template <int ROW>
+__device__ __forceinline__ void move_slots(const EvictArgs& a, int64_t bh, int64_t b, const int2* moves, int count, int first, int step) {
+  constexpr int NB = ROW / 16;
+  struct alignas(NB) W { uint8_t x[NB]; };
+  const int32_t h = static_cast<int32_t>(bh - b * a.pool.heads);
+  const int sub = threadIdx.x & 15;
+  for (; first < count; first += step) {
+    int2 mv[kMoves];
+    int64_t src[kMoves], dst[kMoves];
+    W kc[kMoves], vc[kMoves];
+    uint32_t extra[kMoves];
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) mv[i] = moves[min(first + i, count - 1)];  // (the last again past the end: not stored)
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      src[i] = cache_row(a.pool, b, h, mv[i].x);
+      dst[i] = cache_row(a.pool, b, h, mv[i].y);
+    }
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int64_t r = src[i] < 0 ? 0 : src[i];  // (a pool has a first row)
+      kc[i] = *reinterpret_cast<const W*>(a.pool.k_codes + r * ROW + sub * NB);
+      vc[i] = *reinterpret_cast<const W*>(a.pool.v_codes + r * ROW + sub * NB);
+      // lanes 0 .. 3: K scale, V scale, weight, token
+      const int64_t slot = bh * a.capacity + mv[i].x;
+      const uint32_t* from = sub == 0   ? reinterpret_cast<const uint32_t*>(a.pool.k_scale) + r
+                             : sub == 1 ? reinterpret_cast<const uint32_t*>(a.pool.v_scale) + r
+                             : sub == 2 ? reinterpret_cast<const uint32_t*>(a.weights) + slot
+                                        : reinterpret_cast<const uint32_t*>(a.tokens) + slot;
+      extra[i] = *from;
+    }
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      if (first + i >= count) break;
+      const bool there = src[i] >= 0 && dst[i] >= 0;
+      if (there) {
+        *reinterpret_cast<W*>(a.pool.k_codes + dst[i] * ROW + sub * NB) = kc[i];
+        *reinterpret_cast<W*>(a.pool.v_codes + dst[i] * ROW + sub * NB) = vc[i];
+      }
+      const int64_t slot = bh * a.capacity + mv[i].y;
+      if (sub == 0 && there) reinterpret_cast<uint32_t*>(a.pool.k_scale)[dst[i]] = extra[i];
+      if (sub == 1 && there) reinterpret_cast<uint32_t*>(a.pool.v_scale)[dst[i]] = extra[i];
+      if (sub == 2) reinterpret_cast<uint32_t*>(a.weights)[slot] = extra[i];
+      if (sub == 3) a.tokens[slot] = static_cast<int32_t>(extra[i]);
+    }
+  }
+}
+
 // One workgroup per (sequence, head).  Its waves own consecutive runs of slots, 64 kRegRows or fewer each, whose keys stay in
 // registers while the threshold is found; longer rows go through in rounds of kRound slots, read again for each pass.
 //
@@ -58,7 +111,13 @@ __device__ __forceinline__ uint64_t wave_prefix(uint64_t mine, uint64_t* part, i
   return before;
 }
 
+// ROW: 0 lists the moves for the launch that makes them; else a row's moves are at most kOwnMoves, and the workgroup makes
+// them itself, from a list in LDS.
+constexpr int kOwnMoves = kSelThreads / 16 * kMoves;
+
+template <int ROW>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+  __shared__ int2 s_moves[ROW ? kOwnMoves : 1];
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t s_sum[kWaves];
   __shared__ uint64_t s_part[kWaves];
@@ -70,7 +129,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   const int32_t n = min(a.lengths[b], cap);
   const int64_t recent_from = static_cast<int64_t>(a.seen[b]) - a.recent;
   if (n <= a.keep) {  // (the whole workgroup)
-    if (tid == 0) a.counts[bh] = 0;
+    if (ROW == 0 && tid == 0) a.counts[bh] = 0;
     return;
   }
   const float* w = a.weights + bh * a.capacity;
@@ -140,7 +199,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   }
   // in slot order: of the keys that share the threshold's bits the first `need` stay; holes and movers by their ranks
   uint64_t ties = 0, moved = 0;  // of the rounds before; holes low, movers high
-  int2* mv = a.moves + bh * a.most;
+  int2* const mv = ROW ? s_moves : a.moves + bh * a.most;
   const uint64_t below = (1ull << lane) - 1;
   for (int base = 0; base < n; base += kRound) {
     if (!one_round) load_round(base);
@@ -182,63 +241,20 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       at += __popcll(hm) + (static_cast<uint64_t>(__popcll(mm)) << 32);
     }
   }
-  if (tid == 0) a.counts[bh] = static_cast<int32_t>(moved & 0xffffffffu);  // (as many movers: keep slots stay)
+  const int count = static_cast<int>(moved & 0xffffffffu);  // (as many movers: keep slots stay)
+  if constexpr (ROW == 0) {
+    if (tid == 0) a.counts[bh] = count;
+  } else {
+    __syncthreads();
+    move_slots<ROW>(a, bh, b, s_moves, count, (tid >> 4) * kMoves, kOwnMoves);
+  }
 }
-
-// 16 lanes move one slot: its code rows, scales, weight and token.  kMoves slots at a time, so that their dependent loads
-// (the move, the pages, the rows) overlap.
-constexpr int kMoves = 4;
 
 template <int ROW>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-  constexpr int NB = ROW / 16;
-  struct alignas(NB) W { uint8_t x[NB]; };
   const int64_t bh = blockIdx.y;
-  const int64_t b = bh / a.pool.heads;
-  const int32_t h = static_cast<int32_t>(bh - b * a.pool.heads);
-  const int count = a.counts[bh];
-  const int sub = threadIdx.x & 15;
-  const int2* moves = a.moves + bh * a.most;
-  for (int first = (blockIdx.x * 16 + (threadIdx.x >> 4)) * kMoves; first < count; first += gridDim.x * 16 * kMoves) {
-    int2 mv[kMoves];
-    int64_t src[kMoves], dst[kMoves];
-    W kc[kMoves], vc[kMoves];
-    uint32_t extra[kMoves];
-#pragma unroll
-    for (int i = 0; i < kMoves; ++i) mv[i] = moves[min(first + i, count - 1)];  // (the last again past the end: not stored)
-#pragma unroll
-    for (int i = 0; i < kMoves; ++i) {
-      src[i] = cache_row(a.pool, b, h, mv[i].x);
-      dst[i] = cache_row(a.pool, b, h, mv[i].y);
-    }
-#pragma unroll
-    for (int i = 0; i < kMoves; ++i) {
-      const int64_t r = src[i] < 0 ? 0 : src[i];  // (a pool has a first row)
-      kc[i] = *reinterpret_cast<const W*>(a.pool.k_codes + r * ROW + sub * NB);
-      vc[i] = *reinterpret_cast<const W*>(a.pool.v_codes + r * ROW + sub * NB);
-      // lanes 0 .. 3: K scale, V scale, weight, token
-      const int64_t slot = bh * a.capacity + mv[i].x;
-      const uint32_t* from = sub == 0   ? reinterpret_cast<const uint32_t*>(a.pool.k_scale) + r
-                             : sub == 1 ? reinterpret_cast<const uint32_t*>(a.pool.v_scale) + r
-                             : sub == 2 ? reinterpret_cast<const uint32_t*>(a.weights) + slot
-                                        : reinterpret_cast<const uint32_t*>(a.tokens) + slot;
-      extra[i] = *from;
-    }
-#pragma unroll
-    for (int i = 0; i < kMoves; ++i) {
-      if (first + i >= count) break;
-      const bool there = src[i] >= 0 && dst[i] >= 0;
-      if (there) {
-        *reinterpret_cast<W*>(a.pool.k_codes + dst[i] * ROW + sub * NB) = kc[i];
-        *reinterpret_cast<W*>(a.pool.v_codes + dst[i] * ROW + sub * NB) = vc[i];
-      }
-      const int64_t slot = bh * a.capacity + mv[i].y;
-      if (sub == 0 && there) reinterpret_cast<uint32_t*>(a.pool.k_scale)[dst[i]] = extra[i];
-      if (sub == 1 && there) reinterpret_cast<uint32_t*>(a.pool.v_scale)[dst[i]] = extra[i];
-      if (sub == 2) reinterpret_cast<uint32_t*>(a.weights)[slot] = extra[i];
-      if (sub == 3) a.tokens[slot] = static_cast<int32_t>(extra[i]);
-    }
-  }
+  move_slots<ROW>(a, bh, bh / a.pool.heads, a.moves + bh * a.most, a.counts[bh],
+                  static_cast<int>(blockIdx.x * 16 + (threadIdx.x >> 4)) * kMoves, static_cast<int>(gridDim.x) * 16 * kMoves);
 }
 
 int64_t evict_most(int64_t keep, int64_t slots) { return keep >= slots ? 0 : (keep < slots - keep ? keep : slots - keep); }
@@ -288,12 +304,14 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   a.recent = static_cast<int32_t>(recent);
   a.most = static_cast<int32_t>(evict_most(keep, slots));
   const hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<uint32_t>(B * heads)), dim3(kSelThreads), 0, st, a);
+  const int row = d * bits / 8;
+  const bool own = a.most > 0 && a.most <= kOwnMoves;
+  auto sel = !own ? evict_select_kernel<0> : row == 32 ? evict_select_kernel<32> : row == 64 ? evict_select_kernel<64> : evict_select_kernel<128>;
+  hipLaunchKernelGGL(sel, dim3(static_cast<uint32_t>(B * heads)), dim3(kSelThreads), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
-  if (a.most == 0) return AEKV_OK;  // keep = 0: nothing stays, nothing moves
+  if (own || a.most == 0) return AEKV_OK;  // (keep = 0: nothing stays, nothing moves)
   const int64_t per = ceil_div(a.most, 16 * kMoves);
   const dim3 grid(static_cast<uint32_t>(per < 64 ? per : 64), static_cast<uint32_t>(B * heads));
-  const int row = d * bits / 8;
   auto fn = row == 32 ? evict_move_kernel<32> : row == 64 ? evict_move_kernel<64> : evict_move_kernel<128>;
   hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, a);
   return check_launch(who);
