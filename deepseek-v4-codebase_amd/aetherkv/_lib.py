@@ -172,9 +172,6 @@ def raw_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
 class _Nothing:
     def __enter__(self):
         return None

@@ -108,9 +108,12 @@ class SlotTracker:
         self._set(torch.zeros((2, int(batch), int(kv_heads), int(capacity)), dtype=torch.int32, device=dev))
 
     def _set(self, storage: torch.Tensor) -> None:
-        self.storage = storage
-        self.weights, self.tokens = storage[0].view(torch.float32), storage[1]
+        self._storage, self._weights, self._tokens = storage, storage[0].view(torch.float32), storage[1]
         self.batch, self.kv_heads, self.capacity = storage.shape[1:]
+
+    storage = property(lambda self: self._storage)
+    weights = property(lambda self: self._weights)
+    tokens = property(lambda self: self._tokens)
 
     @classmethod
     def from_tensor(cls, storage: torch.Tensor) -> "SlotTracker":
@@ -149,6 +152,12 @@ def _one_device(index: int, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise RuntimeError(f"every tensor of the call must be on the HIP device {index}, got one on {t.device}")
+
+
+def _given(workspace: torch.Tensor) -> torch.Tensor:
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise RuntimeError(f"workspace must be contiguous uint8, got {workspace.dtype} {tuple(workspace.shape)}")
+    return workspace
 
 
 def _check_tracker(tracker: SlotTracker, cache: PagedKVCache, B: int) -> None:
@@ -204,7 +213,7 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
         raise RuntimeError(f"k and v must be bfloat16, float16 or float32 alike, got {dtype} and {v.dtype}")
     if (tracker is None) != (token is None):
         raise RuntimeError("append_tokens: a tracker and the sequences' token counts come together")
-    _one_device(cache._index, k, v, page_table, start, cu_seqlens, token, None if tracker is None else tracker.storage)
+    _one_device(cache._index, k, v, page_table, start, cu_seqlens, token, None if tracker is None else tracker._storage)
     table, start = _table(page_table), _counts("start", start, B)
     if cu_seqlens is None:
         if shape[0] != B:
@@ -221,7 +230,7 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
     if tracker is not None:
         _check_tracker(tracker, cache, B)
         token = _counts("token", token, B)
-        weights, tokens, first, capacity = tracker.weights.data_ptr(), tracker.tokens.data_ptr(), token.data_ptr(), tracker.capacity
+        weights, tokens, first, capacity = tracker._weights.data_ptr(), tracker._tokens.data_ptr(), token.data_ptr(), tracker.capacity
     kc, ks, vc, vs = cache._ptrs
     dev = cache.device
     with _lib.on_device(dev):
@@ -259,7 +268,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     heads = cache.kv_heads
     if H % heads:
         raise RuntimeError(f"{H} query heads are no multiple of {heads} KV heads")
-    _one_device(cache._index, q, page_table, lengths, sink, workspace, out, None if tracker is None else tracker.storage)
+    _one_device(cache._index, q, page_table, lengths, sink, workspace, out, None if tracker is None else tracker._storage)
     table, lengths = _table(page_table), _counts("lengths", lengths, B)
     table_rows, max_pages = table.shape
     if table_rows != B:
@@ -274,12 +283,12 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     weights, capacity, tracked = None, 0, 0
     if tracker is not None:
         _check_tracker(tracker, cache, B)
-        weights, capacity, tracked = tracker.weights.data_ptr(), tracker.capacity, 1
+        weights, capacity, tracked = tracker._weights.data_ptr(), tracker.capacity, 1
     kc, ks, vc, vs = cache._ptrs
     need = _lib.paged_ws_bytes(B, T, H, heads, D, max_pages * cache.page_size, tracked) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
+        ws = _given(workspace) if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_paged_attention")(
             q.data_ptr(), _TYPES[dtype], st[0], st[1], st[2], B, T, H, D, cache.bits, cache._diag_ptr(), kc, ks, vc, vs,
             cache.pages, heads, cache.page_size, table.data_ptr(), max_pages, lengths.data_ptr(),
@@ -306,7 +315,7 @@ def evict_by_weight(cache: PagedKVCache, page_table: torch.Tensor, lengths: torc
     slots from `keep` on, in order, with their weight and token index: cached keys carry their rotation, so attention
     does not depend on the order of the slots.  `lengths` is only read: clamp it to `keep` once every layer is done."""
     B, max_pages = page_table.shape
-    _one_device(cache._index, page_table, lengths, seen, workspace, tracker.storage)
+    _one_device(cache._index, page_table, lengths, seen, workspace, tracker._storage)
     table, lengths, seen = _table(page_table), _counts("lengths", lengths, B), _counts("seen", seen, B)
     _check_tracker(tracker, cache, B)
     keep, first, recent = int(keep), int(first), int(recent)
@@ -315,10 +324,10 @@ def evict_by_weight(cache: PagedKVCache, page_table: torch.Tensor, lengths: torc
     need = _lib.evict_ws_bytes(B, cache.kv_heads, keep, min(max_pages * cache.page_size, tracker.capacity)) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
+        ws = _given(workspace) if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_kv_evict")(
             cache.dim, cache.bits, kc, ks, vc, vs, cache.pages, cache.kv_heads, cache.page_size, table.data_ptr(), max_pages,
-            B, lengths.data_ptr(), tracker.weights.data_ptr(), tracker.tokens.data_ptr(), tracker.capacity,
+            B, lengths.data_ptr(), tracker._weights.data_ptr(), tracker._tokens.data_ptr(), tracker.capacity,
             seen.data_ptr(), keep, first, recent, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
             stream)
     if rc:

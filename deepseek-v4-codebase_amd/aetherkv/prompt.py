@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .decode import _check_out, _sink_f32
-from .paged import _TYPES, _counts, _one_device, _rows
+from .paged import _TYPES, _counts, _given, _one_device, _rows
 
 
 def prompt_workspace(B: int, n_q: int, n_k: int, H: int, kv_heads: int, dim: int, device) -> torch.Tensor:
@@ -67,7 +67,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     need = _lib.prompt_ws_bytes(B, N, M, H, hk, D) if workspace is None else 0
     with _lib.on_device(dev):
         stream = _lib.raw_stream(dev)
-        ws = workspace if workspace is not None else _lib.workspace(need, dev, stream) if need else None
+        ws = _given(workspace) if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_prompt_attention")(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _TYPES[dtype], qt, qh, kt, kh, vt, vh, cq.data_ptr(),
             ck.data_ptr(), B, N, M, H, hk, D, None if sk is None else sk.data_ptr(), float(softmax_scale), out.data_ptr(),

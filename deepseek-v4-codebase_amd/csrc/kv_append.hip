@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 
 constexpr int kTableThreads = 256;
 
-// Sequence and place of token n (packed: sequences from b0 on are searched).
+// Token n's sequence, its place among that sequence's new tokens, and its slot.
 __device__ __forceinline__ int64_t token_slot(const AppendArgs& a, int64_t n, int64_t* b, int64_t* at) {
   *b = a.cu ? packed_sequence(a.cu, a.B, n) : n / a.per_seq;
   if (*b < 0) return -1;

@@ -153,8 +153,9 @@ __device__ __forceinline__ int32_t load_pages(const PagedArgs& a, int64_t b, int
   return page >= 0 && page < a.pool.pages ? page : -1;
 }
 
-template <int D, int BITS, bool WITH_V>
-__device__ __forceinline__ void load_step(const PagedArgs& a, int32_t kh, int32_t slot, int32_t p0, int32_t p1, int lane,
+// A step's K codes and scales.
+template <int D, int BITS>
+__device__ __forceinline__ void load_keys(const PagedArgs& a, int32_t kh, int32_t slot, int32_t p0, int32_t p1, int lane,
                                           StepData<D, BITS>& s) {
   using G = PagedGeom<D, BITS>;
   const int n = lane & 15, g = lane >> 4;
@@ -176,19 +177,6 @@ __device__ __forceinline__ void load_step(const PagedArgs& a, int32_t kh, int32_
       }
     }
     s.ks[k] = *reinterpret_cast<const f32x4_t*>(a.pool.k_scale + row + 4 * g);
-    if constexpr (WITH_V) {
-      s.vs[k] = *reinterpret_cast<const f32x4_t*>(a.pool.v_scale + row + 4 * g);
-      const uint8_t* vr = a.pool.v_codes + row * G::kRowBytes + (4 * g * G::kRowBytes + n * G::kVB);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (G::kVB == 2) s.v[4 * k + i][0] = *reinterpret_cast<const uint16_t*>(vr + i * G::kRowBytes);
-        else if constexpr (G::kVB == 4) s.v[4 * k + i][0] = *reinterpret_cast<const uint32_t*>(vr + i * G::kRowBytes);
-        else {
-          const uint2 w = *reinterpret_cast<const uint2*>(vr + i * G::kRowBytes);
-          s.v[4 * k + i][0] = w.x, s.v[4 * k + i][1] = w.y;
-        }
-      }
-    }
   }
 }
 
@@ -794,7 +782,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
     auto load = [&](int i) __attribute__((always_inline)) {
       if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
       g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
-      load_step<D, BITS, false>(a, kh, first + kRound * i, g0, g1, lane, next);
+      load_keys<D, BITS>(a, kh, first + kRound * i, g0, g1, lane, next);
     };
     if (n_steps > 0) load(0);
 #pragma unroll 1
@@ -864,10 +852,12 @@ paged_fn pick_weights(int d, int bits) {
 }
 
 // Pieces of a sequence: enough workgroups for the chip (1536: three per CU, twice over, which evens out sequences of
-// different lengths; one sequence of 262144 slots x 12 heads, 1024 / 1536 / 2048 / 3000 workgroups: 111 / 101 / 109 / 113 us,
-// 64 ragged ones of up to 16384 slots x 4 heads 122 / 119 / 117 / 119), but none of fewer than 512 slots beyond 512 workgroups (a workgroup's rotations and merge cost as
-// much as some 500 slots), and none without a whole round of slots.  Tables of up to kOnePiece slots are not split: the
-// merge's launch costs more than their few rounds.
+// different lengths; one sequence of 262144 slots x 12 heads, 1024 / 1536 / 2048 / 3000 workgroups: 111 / 101 / 109 / 113
+// us, 64 ragged ones of up to 16384 slots x 4 heads 122 / 119 / 117 / 119), but none of fewer than 512 slots beyond 512
+// workgroups (a workgroup's rotations and merge cost as much as some 500 slots), and none without a whole round of slots.
+// Tables of up to kOnePiece slots are not split: for many sequences the merge's launch costs more than their few rounds
+// (64 of 256 / 512 / 768 slots x 4 heads, split 12.3 / 13.8 / 15.5 us, whole 9.7 / 11.6 / 13.9), for one it costs as much of
+// the host's time as it saves of the card's (512 slots, replayed from a graph 9.5 and 11.3 us, called 13.8 and 10.1).
 constexpr int64_t kOnePiece = 512;
 int64_t paged_pieces(int64_t groups, int64_t slots) {
   if (slots <= kOnePiece) return 1;

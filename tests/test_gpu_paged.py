@@ -606,3 +606,36 @@ def test_step_captured_and_replayed(dev):
         assert torch.equal(tracker.storage, t.storage) and torch.equal(lengths, ln)
         for x, y in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), (c.k_codes, c.k_scale, c.v_codes, c.v_scale)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 64), (4, 128), (8, 64), (8, 128)])
+def test_evict_many_moves(dev, bits, dim):
+    """More moves than the selecting workgroup makes by itself (256), and as many."""
+    _check_evict(dev, bits, dim, 2, 16, [700, 560, 301, 300], 300, 4, 10, seed=bits + dim)
+    _check_evict(dev, bits, dim, 1, 16, [512, 300], 256, 4, 10, seed=bits + dim)
+
+
+@pytest.mark.parametrize("keep", [200, 19900])
+def test_evict_few_moves_of_long_rows(dev, keep):
+    _check_evict(dev, 4, 64, 2, 256, [20000, 17000], keep, 4, 64, seed=keep)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 64), (4, 128), (8, 64), (8, 128)])
+def test_attention_more_rows_than_the_weights_pass_holds(dev, bits, dim):
+    _check_attention(dev, bits, dim, torch.bfloat16, 16, 1, 3, 70, [90, 33, 150], True, True, seed=bits + dim)
+
+
+def test_workspaces_that_are_no_bytes_are_refused(dev):
+    from aetherkv.prompt import prompt_attention
+
+    cache = PagedKVCache(PolarQuant(4), 4, 2, 64, page_size=16, device=dev)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+    n = torch.full((1,), 3, dtype=torch.int32, device=dev)
+    q = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16, device=dev)
+    for ws in (torch.empty(1 << 16, dtype=torch.float32, device=dev), torch.empty(1 << 17, dtype=torch.uint8, device=dev)[::2]):
+        with pytest.raises(RuntimeError, match="workspace"):
+            paged_attention(q, cache, table, n, 0.1, workspace=ws)
+        with pytest.raises(RuntimeError, match="workspace"):
+            evict_by_weight(cache, table, n, SlotTracker(1, 2, 64, device=dev), n, 1, workspace=ws)
+        with pytest.raises(RuntimeError, match="workspace"):
+            prompt_attention(q[0], q[0], q[0], torch.tensor([0, 1], dtype=torch.int32, device=dev), 0.1, workspace=ws)

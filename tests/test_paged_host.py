@@ -178,3 +178,13 @@ def test_where_slots_lie(tmp_path):
     assert row(0, 0, -1) == -1 and row(0, 0, 64) == -1 and row(0, 0, 1 << 40) == -1
     big = torch.tensor([[0x7ffffffe]], dtype=torch.int32)
     assert row(0, 11, 4095, pages=0x7fffffff, heads=12, shift=12, t=big) == (0x7ffffffe * 12 + 11) * 4096 + 4095
+
+
+def test_attention_workspace_holds_logits_for_few_rows_and_up_to_2_gib(lib):
+    size = lambda B, T, slots, tracked: lib.aekv_paged_attention_workspace_size(B, T, 8, 2, 128, slots, tracked)  # noqa: E731
+    lse = lambda B, T: 4 * B * T * 8  # noqa: E731
+    # 64 sequences x 2 heads x 4 rows x 2^20 slots are 2 GiB, with 32 more slots beyond it
+    assert size(64, 1, (1 << 20) - 32, 1) - size(64, 1, (1 << 20) - 32, 0) == lse(64, 1) + 64 * 2 * 4 * ((1 << 20) - 32) * 4
+    assert size(64, 1, 1 << 20, 1) - size(64, 1, 1 << 20, 0) == lse(64, 1)
+    assert size(1, 4, 1024, 1) - size(1, 4, 1024, 0) == lse(1, 4) + 2 * 16 * 1024 * 4
+    assert size(1, 5, 1024, 1) - size(1, 5, 1024, 0) == lse(1, 5)  # 20 rows: scored again
