@@ -549,15 +549,22 @@ prompt_fn pick_prompt(int32_t dtype, int32_t d) {
 
 // How a launch is cut: rows of a workgroup, and pieces of the keys where the row tiles alone leave CUs without a workgroup
 // (as many as are resident together: three of a CU at head dim 64, two at 128).
+//
+// 128 rows to a workgroup read a tile of keys once for twice the rows; 64 give twice the workgroups.  128 where
+// they fill the chip by themselves, or in at least two pieces of enough work to pay for the pieces' merge: 12 heads of 4,
+// dim 128, 64 / 128 rows: 1024 queries over 8192 keys (the least) 81 / 69 us, over 32768 287 / 225, 512 over 8192 46 / 48;
+// 16 heads of 16, 2048 over 8192 (one piece of 128) 149 / 160.
 struct PromptPlan {
   int64_t rows, tiles, split;
 };
+constexpr int64_t kWideWork = int64_t(3) << 25;  // rows x keys of a sequence
 PromptPlan plan_prompt(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d) {
   PromptPlan p;
-  const int64_t rows = n_q * (H / heads);
-  p.rows = heads * (rows / 128) >= 512 ? 128 : 64;
+  const int64_t rows = n_q * (H / heads), resident = d == 64 ? 768 : 512;
+  const bool wide = heads * (rows / 128) >= 512 || (n_q * H * (n_k / B) >= kWideWork && 2 * heads * (rows / 128 + B) <= resident);
+  p.rows = wide ? 128 : 64;
   p.tiles = rows / p.rows + B;  // at least every sequence's, whatever their lengths
-  const int64_t room = (d == 64 ? 768 : 512) / (p.tiles * heads), most = ceil_div(n_k, static_cast<int64_t>(kTile * kPieceTiles));
+  const int64_t room = resident / (p.tiles * heads), most = ceil_div(n_k, static_cast<int64_t>(kTile * kPieceTiles));
   p.split = room < most ? room : most;
   if (p.split < 1) p.split = 1;
   return p;

@@ -303,3 +303,19 @@ def test_prompt_many_tiles_of_many_sequences(dev, B, H, hk, most):
     if B == 2:
         lq, lk = [most * 9, most * 3], [most * 9, most * 3 + 700]
     _check(dev, torch.bfloat16, 64, H, hk, lq, lk, sink=True, seed=B, pad=2)
+
+
+@pytest.mark.parametrize("dtype,dim,H,hk,lq,lk", [(torch.bfloat16, 128, 12, 4, [130, 1, 66], [66000, 66000, 40000]), (torch.float16, 64, 16, 2, [200], [33000])])
+def test_prompt_wide_pieces(dev, dtype, dim, H, hk, lq, lk):
+    """128 rows to a workgroup with the keys in pieces: enough work, few row tiles.  Checked on some rows."""
+    q, k, v = _inputs(dev, 7, dtype, dim, H, hk, lq, lk)
+    cq, ck = _cu(lq), _cu(lk)
+    out = prompt_attention(q, k, v, torch.tensor(cq, dtype=torch.int32, device=dev), dim ** -0.5,
+                           cu_seqlens_k=torch.tensor(ck, dtype=torch.int32, device=dev))
+    for b, n in enumerate(lq):
+        for i in sorted({0, n // 2, n - 1}):
+            see = max(0, i + 1 + lk[b] - n)  # one query over the keys that it sees
+            r = cq[b] + i
+            one = slice(ck[b], ck[b] + see)
+            want, bound, _, _ = R.prompt_attention_ref(q[r:r + 1].cpu(), k[one].cpu(), v[one].cpu(), [0, 1], [0, see], dim ** -0.5)
+            R.within(out[r:r + 1], want, bound, f"sequence {b}, query {i}")
