@@ -5,9 +5,10 @@
 // (aether_2b/serving.py:327-346).
 //
 // Two layouts, bit for bit alike.  Small calls (and fp32): D / 8 lanes hold one vector, 8 elements each, so that a decode
-// step's few vectors spread over many waves; bound by the chain of a wave (load, exchanges, divisions, store).  Large
-// calls: 32 elements to a lane (tq_fast_lane.h), a wave taking VPW consecutive tokens of one head of K or V, so that it
-// reads whole rows and writes its codes contiguously; bound by the reads and writes.
+// step's few vectors spread over many waves; bound by the chain of a wave (load, exchanges, divisions, store): 64 tokens x
+// 4 heads 3.9 us.  Large calls: 32 elements to a lane (tq_fast_lane.h), a wave taking VPW consecutive tokens of one head of
+// K or V, so that it reads whole rows and writes its codes contiguously; bound by the reads and writes: 8 prompts of up to
+// 8192 tokens x 12 heads, 334 MB, 80 us, 4.2 TB/s of a copy's 5.0.
 #include "paged_cache.h"
 #include "tq_fast_lane.h"
 

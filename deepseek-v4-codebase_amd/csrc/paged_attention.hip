@@ -9,7 +9,19 @@
 //
 // Work split.  The T tokens x G heads of a KV head's group are rows; a workgroup takes 16 MT of them and one piece of the
 // sequence, its four waves alternate over steps of 32 slots, and their states are merged through LDS.  Where a launch has
-// too few workgroups the sequence is split over n_split pieces, merged by a second kernel.
+// too few workgroups the sequence is split over n_split pieces, merged by a second kernel.  One pass: running maximum and
+// sum, the output rescaled only where a row's maximum moved by more than kMargin.
+//
+// Loads.  A wave's steps go straight into LDS, each wave in a ring of its own of three stages (two where a row has 128
+// bytes, so that three workgroups stay on a CU), the next two requested before a step is waited for: with the loads in
+// registers a CU held one step of each wave (one sequence of 262144 slots, 12 heads: 120 us, staged 109).  The queries and
+// the first steps are requested before the rotation runs.
+//
+// Measured (dim 128, 4 bits).  One sequence of 262144 slots, 12 heads of 12: 428 MB in 87 to 91 us, 4.7 to 4.9 TB/s, what a
+// large copy reaches (5.0), with the merge 96 us.  64 ragged sequences of up to 16384 slots, 12 heads of 4, tracked: 86 to 91
+// us, the merge 5 and the weights' sum 10.  A form with 40 of a step's 222 vector instructions less took as long (104.8 and
+// 106.0 us for the three): the reads bound it.  16 tokens x 8 heads of 8 sequences of up to 5001 slots, dim 64, 8 bits: 20
+// us, the rotations, four steps behind one another in each wave, and the merge of the waves.
 //
 // Matrix layout (v_mfma_f32_16x16x32: A lane l holds A[l % 16][8 (l / 16) + j], B lane l holds B[8 (l / 16) + j][l % 16],
 // D lane l register i holds D[4 (l / 16) + i][l % 16]), g = l / 16:
@@ -635,7 +647,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   }
 }
 
-// Merges the pieces of one row and rotates it back: the workgroup's waves take every fourth piece each.
+// Merges the pieces of one row and rotates it back: the workgroup's waves take every fourth piece each.  Bound by the chain
+// of its loads: 12 rows of 128 pieces 8 us with four pieces requested at a time, 6.5 with eight (sixteen, whose registers
+// halve the waves on a CU, made 2048 rows of 5 pieces 0.8 us slower).
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   constexpr int PER = D / 64;
@@ -651,20 +665,41 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   float m = kNegInf, l = 0.0f, x[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) x[i] = 0.0f;
-#pragma unroll 4
-  for (int s = wave; s < pieces; s += kWaves) {
-    const float* ps = p + static_cast<int64_t>(s) * (D + 4);
-    const float pm = ps[0], pl = ps[1];
-    float v[PER];
+  // CH pieces at a time, all their loads issued together (a piece past the last reads the last, as an empty one)
+  auto merge = [&](auto ch) __attribute__((always_inline)) {
+    constexpr int CH = decltype(ch)::value;
+    for (int s0 = wave; s0 < pieces; s0 += kWaves * CH) {
+      float pm[CH], pl[CH], v[CH][PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = ps[4 + PER * lane + i];
-    const float top = fmaxf(m, pm);
-    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top), fp = pl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm - top);
-    l = (l == 0.0f ? 0.0f : l * f) + (pl == 0.0f ? 0.0f : pl * fp);
+      for (int c = 0; c < CH; ++c) {
+        const int s = s0 + kWaves * c;
+        const float* ps = p + static_cast<int64_t>(min(s, pieces - 1)) * (D + 4);
+        pm[c] = ps[0], pl[c] = ps[1];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = x[i] * f + v[i] * fp;
-    m = top;
-  }
+        for (int i = 0; i < PER; ++i) v[c][i] = ps[4 + PER * lane + i];
+      }
+      float top = m;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (s0 + kWaves * c >= pieces) pm[c] = kNegInf, pl[c] = 0.0f;
+        top = fmaxf(top, pm[c]);
+      }
+      const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      l = l == 0.0f ? 0.0f : l * f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] *= f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const float fp = pl[c] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm[c] - top);
+        l += pl[c] == 0.0f ? 0.0f : pl[c] * fp;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] += v[c][i] * fp;
+      }
+      m = top;
+    }
+  };
+  if (pieces <= 2 * kWaves) merge(std::integral_constant<int, 2>{});
+  else merge(std::integral_constant<int, 8>{});
 #pragma unroll
   for (int i = 0; i < PER; ++i) s_o[wave][PER * lane + i] = x[i];
   if (lane == 0) s_ml[wave][0] = m, s_ml[wave][1] = l;
@@ -701,6 +736,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
 }
 
 // The weights of a sequence's slots from the logits that the attention left and the rows' log sums: four slots to a thread.
+// Reads 4 bytes per row and slot, reads and writes the weights: 64 sequences x 4 heads x 3 rows of up to 16384 slots, 10 us.
 constexpr int kAddSlots = 1024;  // of a workgroup
 
 __global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blocks) {
@@ -732,7 +768,9 @@ __global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blo
 }
 
 // The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
-// row of the KV head's group, 16 at a time (their query parts in LDS), and adds the sums over the rows.
+// row of the KV head's group, 16 at a time (their query parts in LDS), and adds the sums over the rows.  Bound by the
+// rotations that come before the first step and then the vector work of the scores: 128 rows, 8 sequences x 2 heads of up
+// to 5001 slots, dim 64, 8 bits: 14 us.
 constexpr int kWeightTiles = 8;  // row tiles whose parts LDS holds at a time
 
 template <int DT, int D, int BITS>
