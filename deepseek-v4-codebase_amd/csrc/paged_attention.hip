@@ -18,9 +18,8 @@
 // the first steps are requested before the rotation runs.
 //
 // Measured (dim 128, 4 bits).  One sequence of 262144 slots, 12 heads of 12: 428 MB in 87 to 91 us, 4.7 to 4.9 TB/s, what a
-// large copy reaches (5.0), with the merge 96 us.  64 ragged sequences of up to 16384 slots, 12 heads of 4, tracked: 86 to 91
-// us, the merge 5 and the weights' sum 10.  A form with 40 of a step's 222 vector instructions less took as long (104.8 and
-// 106.0 us for the three): the reads bound it.  16 tokens x 8 heads of 8 sequences of up to 5001 slots, dim 64, 8 bits: 20
+// large copy reaches (5.0), with the merge 96 us.  64 ragged sequences of up to 16384 slots, 12 heads of 4, tracked: 78
+// us, the merge 5 and the weights' sum 10 (a form with 40 of a step's 222 vector instructions less took as long).  16 tokens x 8 heads of 8 sequences of up to 5001 slots, dim 64, 8 bits: 20
 // us, the rotations, four steps behind one another in each wave, and the merge of the waves.
 //
 // Matrix layout (v_mfma_f32_16x16x32: A lane l holds A[l % 16][8 (l / 16) + j], B lane l holds B[8 (l / 16) + j][l % 16],
@@ -69,11 +68,49 @@ struct PagedArgs {
   int32_t reach;                     // slots of a sequence that can be seen: the table's, or the tracker's capacity
   int64_t capacity, logit_slots;
   int32_t T, H, G, rows, row_blocks, n_split;
+  int32_t B, ranked;                 // workgroups by their sequences' lengths: 1 up to 64 of them, 2 up to kRanked; 0: by index
   float scale2, wscale;              // softmax scale * log2(e), fp32(D^-1/2)
 };
 
 // Slots of sequence b that its last token sees.
 __device__ __forceinline__ int32_t newest_sees(const PagedArgs& a, int64_t b) { return max(min(a.lengths[b], a.reach), 0); }
+// The sequence that comes r-th when the longest come first, by eighths of a power of two, equal ones by their index; *n: its
+// slots.  The r-th largest key bit by bit, then its holder; a lane holds a sequence of each CH.
+template <int CH>
+__device__ __forceinline__ int32_t ranked_sequence(const PagedArgs& a, int32_t r, int lane, int32_t* n) {
+  int32_t len[CH], key[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int32_t b = 64 * c + lane;
+    len[c] = newest_sees(a, min(b, a.B - 1));
+    // 1 + 8 times the exponent and 3 bits of the length + 1, below 256 (31 exponents); 0 past the last sequence
+    key[c] = b < a.B ? 1 + static_cast<int32_t>((__builtin_bit_cast(uint32_t, static_cast<float>(len[c] + 1)) >> 20) - (127u << 3)) : 0;
+  }
+  auto count = [&](int32_t least) __attribute__((always_inline)) {
+    int m = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) m += __popcll(__builtin_amdgcn_ballot_w64(key[c] >= least));
+    return m;
+  };
+  int32_t v = 0;
+#pragma unroll
+  for (int bit = 128; bit > 0; bit >>= 1)
+    if (count(v | bit) > r) v |= bit;
+  int k = r - count(v + 1);
+  int32_t b = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const uint64_t eq = __builtin_amdgcn_ballot_w64(key[c] == v);
+    const uint64_t it = __builtin_amdgcn_ballot_w64(key[c] == v && __popcll(eq & ((1ull << lane) - 1)) == k);
+    if (it) {
+      const int at = __builtin_ctzll(it);
+      b = 64 * c + at, *n = __builtin_amdgcn_readlane(len[c], at);
+    }
+    k -= __popcll(eq);
+  }
+  return b;
+}
+
 // The piece length of a sequence of n slots: whole rounds of the workgroup's waves.
 __device__ __forceinline__ int32_t piece_slots(int32_t n, int32_t n_split) {
   const int32_t per = (n + n_split - 1) / n_split;
@@ -407,9 +444,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   const int32_t rb = static_cast<int32_t>(wg % a.row_blocks);
   wg /= a.row_blocks;
   const int32_t kh = static_cast<int32_t>(wg % a.pool.heads);
-  const int64_t b = wg / a.pool.heads;
-
-  const int32_t n = newest_sees(a, b);
+  int64_t b = wg / a.pool.heads;
+  int32_t n;
+  if (a.ranked == 1) b = ranked_sequence<1>(a, static_cast<int32_t>(b), lane, &n);
+  else if (a.ranked == 2) b = ranked_sequence<8>(a, static_cast<int32_t>(b), lane, &n);
+  else n = newest_sees(a, b);
   const int32_t piece = piece_slots(n, a.n_split);
   const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
   if (split > 0 && p0 >= p1) return;  // (the merge knows how many pieces a sequence has)
@@ -907,6 +946,12 @@ int64_t paged_pieces(int64_t groups, int64_t slots) {
   return n < 1 ? 1 : n;
 }
 
+// A batch whose workgroups do not all run together starts its longest sequences first, so that no long one is left for the
+// end, where pieces can be long enough for that to count: finding the order costs a workgroup some 1 us.  By index / longest
+// first, 12 heads of 4, dim 128, 4 bits: 64 ragged sequences of up to 16384 slots 98.3 / 85.9 us, one of 16384 among 63 of
+// 1024 47.3 / 35.8, in pieces of 682 slots (16 of up to 16384) 34.3 / 36.7.
+constexpr int64_t kRanked = 512, kRankedSlots = 2048;
+
 // Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.
 int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 : 1; }
 
@@ -988,6 +1033,8 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   a.rows = static_cast<int32_t>(rows);
   a.row_blocks = static_cast<int32_t>(blocks);
   a.n_split = static_cast<int32_t>(paged_pieces(B * heads * blocks, slots));
+  a.B = static_cast<int32_t>(B);
+  a.ranked = B > 1 && B <= kRanked && reach / a.n_split >= kRankedSlots && B * heads * blocks * a.n_split > 768 ? (B <= 64 ? 1 : 2) : 0;
   a.scale2 = softmax_scale * kLog2e;
   a.wscale = wht_scale(d);
   const hipStream_t st = as_stream(stream);

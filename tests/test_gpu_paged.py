@@ -639,3 +639,12 @@ def test_workspaces_that_are_no_bytes_are_refused(dev):
             evict_by_weight(cache, table, n, SlotTracker(1, 2, 64, device=dev), n, 1, workspace=ws)
         with pytest.raises(RuntimeError, match="workspace"):
             prompt_attention(q[0], q[0], q[0], torch.tensor([0, 1], dtype=torch.int32, device=dev), 0.1, workspace=ws)
+
+
+@pytest.mark.parametrize("B,heads", [(50, 16), (66, 12)])
+def test_attention_of_a_ragged_batch_longest_first(dev, B, heads):
+    """Batches of more workgroups than run together start their longest sequences first (up to 64 sequences and beyond in
+    two forms): lengths of one bucket, equal ones, none, the longest last."""
+    lens = [(0, 3, 17, 18, 1, 40, 17, 33)[i % 8] for i in range(B)]
+    lens[1], lens[-2], lens[-1] = 300, 290, 4096
+    _check_attention(dev, 4, 64, torch.bfloat16, 16, heads, 1, 1, lens, False, True, seed=B)
