@@ -562,6 +562,10 @@ prompt_fn pick_prompt(int32_t dtype, int32_t d) {
 // they fill the chip by themselves, or in at least two pieces of enough work to pay for the pieces' merge: 12 heads of 4,
 // dim 128, 64 / 128 rows: 1024 queries over 8192 keys (the least) 81 / 69 us, over 32768 287 / 225, 512 over 8192 46 / 48;
 // 16 heads of 16, 2048 over 8192 (one piece of 128) 149 / 160.
+//
+// Pieces have to save a row the time of some kPieceTiles tiles, which is what their merge costs: 16 heads of 2, dim 64, whole / in
+// pieces: 1024 queries over their own keys 14.0 / 18.6 us, 1500 18.7 / 23.6, 64 queries over 2048 keys 22.3 / 13.3, 16 over
+// 1024 13.6 / 12.5.
 struct PromptPlan {
   int64_t rows, tiles, split;
 };
@@ -572,9 +576,10 @@ PromptPlan plan_prompt(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t h
   const bool wide = heads * (rows / 128) >= 512 || (n_q * H * (n_k / B) >= kWideWork && 2 * heads * (rows / 128 + B) <= resident);
   p.rows = wide ? 128 : 64;
   p.tiles = rows / p.rows + B;  // at least every sequence's, whatever their lengths
-  const int64_t room = resident / (p.tiles * heads), most = ceil_div(n_k, static_cast<int64_t>(kTile * kPieceTiles));
+  const int64_t sees = (n_q < n_k ? n_k - n_q / 2 : n_k / 2) / B, piece = kTile * kPieceTiles;  // keys of a row, on average
+  const int64_t room = resident / (p.tiles * heads), most = ceil_div(sees, piece);
   p.split = room < most ? room : most;
-  if (p.split < 1) p.split = 1;
+  if (p.split < 1 || 8 * sees * (p.split - 1) < 7 * piece * p.split) p.split = 1;
   return p;
 }
 

@@ -234,7 +234,7 @@ def test_prompt_many_rows_masked_places(dev):
 
 
 @pytest.mark.parametrize("dtype,dim,H,hk,lq,lk", [(torch.bfloat16, 128, 4, 2, [3, 1, 70], [1500, 513, 2100]), (torch.float16, 64, 8, 1, [1], [5003]), (torch.bfloat16, 64, 2, 2, [600], [600]),
-                                                  (torch.float16, 128, 12, 4, [5, 0, 40], [100, 3000, 1030])])
+                                                  (torch.float16, 128, 12, 4, [5, 0, 40], [100, 3000, 1030]), (torch.bfloat16, 64, 2, 2, [2000], [2000])])
 @pytest.mark.parametrize("sink", [False, True])
 def test_prompt_few_rows_over_many_keys(dev, dtype, dim, H, hk, lq, lk, sink):
     """Launches of few rows split the keys over workgroups: rows that see one piece, all of them, or none."""
@@ -242,7 +242,8 @@ def test_prompt_few_rows_over_many_keys(dev, dtype, dim, H, hk, lq, lk, sink):
 
     q, k, v = _inputs(dev, 30, dtype, dim, H, hk, lq, lk, pad=3)
     cq, ck = (torch.tensor(_cu(x), dtype=torch.int32, device=dev) for x in (lq, lk))
-    assert prompt_workspace(len(lq), q.size(0), k.size(0), H, hk, dim, dev).numel() > 0
+    # (600 queries over their own keys see too few for pieces to pay; 2000 do not)
+    assert (prompt_workspace(len(lq), q.size(0), k.size(0), H, hk, dim, dev).numel() > 0) == (lk != [600])
     sk = torch.randn(H, device=dev, generator=_gen(dev, 31)) if sink else None
     scale = dim ** -0.5
     ws = prompt_workspace(len(lq), q.size(0), k.size(0), H, hk, dim, dev).fill_(255)
