@@ -15,6 +15,10 @@ New fused decode path over quantised KV:
                              and the grouped output projection
   aetherkv.prefill           chunked prefill through the quantised reader: every target of a chunk
                              scored and attended in one launch each (csa_prefill, hca_prefill)
+Per-head caches, beside the reference's shared compressed blocks:
+  aetherkv.prompt            prompt_attention: causal attention of packed sequences, grouped heads
+  aetherkv.paged             PagedKVCache in TurboQuant codes: append_tokens, paged_attention, and
+                             evict_by_weight by the weights that a SlotTracker accumulates
 All compute runs in libaetherkv.so (hand-written HIP for gfx950, C ABI in include/aetherkv.h).
 """
 from .loader import cuda_build_environment, cuda_extension_unavailable_reason, load_aether_cuda_kernels
