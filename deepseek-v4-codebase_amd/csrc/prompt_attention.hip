@@ -109,33 +109,33 @@ struct TileAt {
 };
 
 // The workgroup's `t`-th tile (tiles of `rows` rows of G per query, in the sequences' order; a sequence's last rows, which
-// see the most keys, come first).  False past the last tile.  Lanes look at a sequence each, in one memory round.
+// see the most keys, come first).  Sequence b, whose rows start at r, has the places from floor(r / rows) + b on: at least
+// as many as tiles, and rows / tiles + B in all.  64 sequences are looked at in a memory round, so that up to 64 are searched
+// in one round, up to 4096 in two.  False where the place has no tile.
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int32_t t, int rows, int lane, TileAt* at) {
-  int32_t before = 0;  // (n_q H, with a tile's rows, fits 31 bits)
-  for (int32_t base = 0; base < a.B; base += 64) {
-    const int32_t b = min(base + lane, a.B - 1);
+  int32_t lo = 0, hi = a.B;
+  for (;;) {
+    const int32_t step = (hi - lo + 63) / 64, b = lo + min(step * lane, hi - 1 - lo);
     const int32_t c0 = a.cu_q[b], c1 = a.cu_q[b + 1], d0 = a.cu_k[b], d1 = a.cu_k[b + 1];
-    const int32_t q0 = min(max(c0, 0), a.n_q), lq = min(max(c1, q0), a.n_q) - q0;
-    const int32_t k0 = min(max(d0, 0), a.n_k), lk = min(max(d1, k0), a.n_k) - k0;
-    int32_t s = base + lane < a.B ? (lq * a.G + rows - 1) / rows : 0;  // inclusive sum over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int32_t o = __shfl_up(s, d);
-      if (lane >= d) s += o;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > t);
-    if (past) {
-      const int l = __builtin_ctzll(past);
+    const int32_t q0 = min(max(c0, 0), a.n_q);  // (n_q H, with a tile's rows, fits 31 bits)
+    const int32_t place = q0 * a.G / rows;
+    const uint64_t from = __builtin_amdgcn_ballot_w64(t - place >= b && step * lane < hi - lo);
+    if (!from) return false;  // before the first sequence
+    const int l = 63 - __builtin_clzll(from);
+    if (step == 1) {
+      const int32_t lq = min(max(c1, q0), a.n_q) - q0;
+      const int32_t k0 = min(max(d0, 0), a.n_k), lk = min(max(d1, k0), a.n_k) - k0;
+      const int32_t tiles = (lq * a.G + rows - 1) / rows, left = tiles - 1 - (t - place - b);
       at->q0 = __builtin_amdgcn_readlane(q0, l);
       at->lq = __builtin_amdgcn_readlane(lq, l);
       at->k0 = __builtin_amdgcn_readlane(k0, l);
       at->lk = __builtin_amdgcn_readlane(lk, l);
-      at->row = (before + __builtin_amdgcn_readlane(s, l) - 1 - t) * rows;
-      return true;
+      at->row = __builtin_amdgcn_readlane(left, l) * rows;
+      return at->row >= 0;
     }
-    before += __builtin_amdgcn_readlane(s, 63);
+    lo += l * step;
+    hi = min(lo + step, hi);
   }
-  return false;
 }
 
 __device__ __forceinline__ int32_t lane_sum(int32_t v) {

@@ -320,3 +320,18 @@ def test_prompt_wide_pieces(dev, dtype, dim, H, hk, lq, lk):
             one = slice(ck[b], ck[b] + see)
             want, bound, _, _ = R.prompt_attention_ref(q[r:r + 1].cpu(), k[one].cpu(), v[one].cpu(), [0, 1], [0, see], dim ** -0.5)
             R.within(out[r:r + 1], want, bound, f"sequence {b}, query {i}")
+
+
+@pytest.mark.parametrize("B", [129, 4096, 4100])
+def test_prompt_very_many_sequences(dev, B):
+    """Sequences are searched 64 at a time: one round to 64, two to 4096, three beyond; with rows before the first one."""
+    lq = [(1, 0, 2, 0, 3, 1)[i % 6] for i in range(B)]
+    lq[B // 2] = 150
+    q, k, v = _inputs(dev, 3, torch.bfloat16, 64, 2, 1, [5] + lq, [5] + lq, pad=4)
+    cu = [c for c in _cu([5] + lq)[1:]]
+    out, lse = prompt_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device=dev), 0.125, return_lse=True)
+    want, bound, wl, lb = R.prompt_attention_ref(q.cpu(), k.cpu(), v.cpu(), cu, cu, 0.125)
+    R.within(out, want, bound, "out")
+    none = wl == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, none)
+    R.within(lse.double().cpu()[~none], wl[~none], lb[~none], "lse")
