@@ -14,8 +14,6 @@
 namespace aekv {
 namespace {
 
-constexpr int kSelThreads = 1024;
-
 struct EvictArgs {
   PagePool pool;
   const int32_t* lengths;  // [B]
@@ -95,11 +93,12 @@ __device__ __forceinline__ void move_slots(const EvictArgs& a, int64_t bh, int64
 // share the bits above, searched from its largest bin by all waves.  A level whose bin is kept whole ends it.
 // The order: ballots rank a wave's ties, holes and movers by slot; one word per wave carries the counts between waves.
 //
-// Bound by its barriers and the chain of its loads: 1088 slots with up to 64 moves made here 13.6 us (16 sequences x 4 heads;
-// the launch of their own that they had before 18.0 against 15.8 us for the call), 16384 slots 27 us (96 rows).
-constexpr int kWaves = kSelThreads / 64, kRegRows = 16, kRound = kSelThreads * kRegRows, kBins = 2048;
+// Bound by its barriers and the chain of its loads: 1088 slots with up to 64 moves made here 10 us (16 sequences x 4 heads;
+// with the moves in a launch of their own 2 us more), 16384 slots 27 us (96 rows).
+constexpr int kRegRows = 16, kBins = 2048;
 
 // The waves' counts before this one's, and their total, for two counters (the first below 2^32, packed with the second).
+template <int kWaves>
 __device__ __forceinline__ uint64_t wave_prefix(uint64_t mine, uint64_t* part, int lane, int wave, uint64_t* total) {
   __syncthreads();  // the readers of the call before are done
   if (lane == 0) part[wave] = mine;
@@ -117,10 +116,11 @@ __device__ __forceinline__ uint64_t wave_prefix(uint64_t mine, uint64_t* part, i
 
 // ROW: 0 lists the moves for the launch that makes them; else a row's moves are at most kOwnMoves, and the workgroup makes
 // them itself, from a list in LDS.
-constexpr int kOwnMoves = kSelThreads / 16 * kMoves;
+constexpr int kOwnMoves = 256;
 
-template <int ROW>
+template <int ROW, int kSelThreads>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+  constexpr int kWaves = kSelThreads / 64, kRound = kSelThreads * kRegRows, kPer = kBins / kSelThreads;
   __shared__ int2 s_moves[ROW ? kOwnMoves : 1];
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t s_sum[kWaves];
@@ -177,9 +177,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       }
     }
     __syncthreads();
-    // bins from the top: thread t holds bins 2047 - 2 t and the one below
-    const uint32_t h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
-    uint32_t s = h0 + h1;
+    // bins from the top: thread t holds the kPer from 2047 - kPer t down
+    uint32_t h[kPer], own = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) own += h[i] = hist[kBins - 1 - kPer * tid - i];
+    uint32_t s = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t o = __shfl_up(s, d);
@@ -190,10 +192,13 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     uint32_t above = 0;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) above += v < wave ? s_sum[v] : 0;
-    above += s - h0 - h1;  // keys in higher bins than this thread's
+    above += s - own;  // keys in higher bins than this thread's
     const uint32_t want = static_cast<uint32_t>(need);
-    if (above < want && above + h0 >= want) s_found[0] = kBins - 1 - 2 * tid, s_found[1] = want - above, s_found[2] = h0;
-    else if (above + h0 < want && above + h0 + h1 >= want) s_found[0] = kBins - 2 - 2 * tid, s_found[1] = want - above - h0, s_found[2] = h1;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (above < want && above + h[i] >= want) s_found[0] = kBins - 1 - kPer * tid - i, s_found[1] = want - above, s_found[2] = h[i];
+      above += h[i];
+    }
     if (need == 0 && tid == 0) s_found[0] = kBins - 1, s_found[1] = 0, s_found[2] = -1;
     __syncthreads();
     prefix |= static_cast<uint32_t>(s_found[0]) << shift;
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       const bool in = run + 64 * r + lane < n;
       mine += __popcll(__builtin_amdgcn_ballot_w64(in && (key[r] >> shift) == (prefix >> shift)));
     }
-    uint64_t rank = ties + wave_prefix(mine, s_part, lane, wave, &total);
+    uint64_t rank = ties + wave_prefix<kWaves>(mine, s_part, lane, wave, &total);
     ties += total;
     uint32_t hole = 0, mover = 0;  // bit r: the slot of row r
     uint64_t count = 0;
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       mover |= (m ? 1u : 0u) << r;
       count += __popcll(__builtin_amdgcn_ballot_w64(h)) + (static_cast<uint64_t>(__popcll(__builtin_amdgcn_ballot_w64(m))) << 32);
     }
-    uint64_t at = moved + wave_prefix(count, s_part, lane, wave, &total);
+    uint64_t at = moved + wave_prefix<kWaves>(count, s_part, lane, wave, &total);
     moved += total;
 #pragma unroll
     for (int r = 0; r < kRegRows; ++r) {
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     if (tid == 0) a.counts[bh] = count;
   } else {
     __syncthreads();
-    move_slots<ROW>(a, bh, b, s_moves, count, (tid >> 4) * kMoves, kOwnMoves);
+    move_slots<ROW>(a, bh, b, s_moves, count, (tid >> 4) * kMoves, kSelThreads / 16 * kMoves);
   }
 }
 
@@ -260,6 +265,18 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
   move_slots<ROW>(a, bh, bh / a.pool.heads, a.moves + bh * a.most, a.counts[bh],
                   static_cast<int>(blockIdx.x * 16 + (threadIdx.x >> 4)) * kMoves, static_cast<int>(gridDim.x) * 16 * kMoves);
 }
+
+using evict_fn = void (*)(EvictArgs);
+template <int THREADS>
+evict_fn pick_select(int row) {
+  return row == 0 ? evict_select_kernel<0, THREADS> : row == 32 ? evict_select_kernel<32, THREADS>
+       : row == 64 ? evict_select_kernel<64, THREADS> : evict_select_kernel<128, THREADS>;
+}
+// Slots of a row up to which eight waves select, whose keys they hold in registers; beyond, sixteen.  More waves shorten the
+// passes and make each barrier longer; sixteen fill half a CU.  8 / 16 waves (256 threads: 4), with a copy of the weights
+// before each call, 3 to 5 us: 16 sequences x 4 heads of 1088 slots to 1024 12.3 / 16.6 us (12.5), 256 x 8 42 / 87 (35), 16 x 4
+// of 4000 to 3900 16.1 / 18.4 (4096: 23.3), 64 x 8 of 8000 to 7900 40 / 51, 8 x 12 of 16384 to 4096 70.6 / 60.1.
+constexpr int64_t kSmallRow = 8192;
 
 int64_t evict_most(int64_t keep, int64_t slots) { return keep >= slots ? 0 : (keep < slots - keep ? keep : slots - keep); }
 
@@ -310,8 +327,8 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   const hipStream_t st = as_stream(stream);
   const int row = d * bits / 8;
   const bool own = a.most > 0 && a.most <= kOwnMoves;
-  auto sel = !own ? evict_select_kernel<0> : row == 32 ? evict_select_kernel<32> : row == 64 ? evict_select_kernel<64> : evict_select_kernel<128>;
-  hipLaunchKernelGGL(sel, dim3(static_cast<uint32_t>(B * heads)), dim3(kSelThreads), 0, st, a);
+  auto sel = slots <= kSmallRow ? pick_select<512>(own ? row : 0) : pick_select<1024>(own ? row : 0);
+  hipLaunchKernelGGL(sel, dim3(static_cast<uint32_t>(B * heads)), dim3(slots <= kSmallRow ? 512 : 1024), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
   if (own || a.most == 0) return AEKV_OK;  // (keep = 0: nothing stays, nothing moves)
   const int64_t per = ceil_div(a.most, 16 * kMoves);

@@ -648,3 +648,9 @@ def test_attention_of_a_ragged_batch_longest_first(dev, B, heads):
     lens = [(0, 3, 17, 18, 1, 40, 17, 33)[i % 8] for i in range(B)]
     lens[1], lens[-2], lens[-1] = 300, 290, 4096
     _check_attention(dev, 4, 64, torch.bfloat16, 16, heads, 1, 1, lens, False, True, seed=B)
+
+
+@pytest.mark.parametrize("length", [8191, 8192, 8193])
+def test_evict_around_the_rows_of_more_waves(dev, length):
+    _check_evict(dev, 8, 128, 1, 16, [length, length - 100, 90], length - 200, 4, 64, seed=length)
+    _check_evict(dev, 4, 64, 1, 16, [length, length // 2], length // 3, 4, 64, seed=length)
