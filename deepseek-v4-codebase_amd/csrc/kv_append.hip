@@ -7,8 +7,9 @@
 // Two layouts, bit for bit alike.  Small calls (and fp32): D / 8 lanes hold one vector, 8 elements each, so that a decode
 // step's few vectors spread over many waves; bound by the chain of a wave (load, exchanges, divisions, store): 64 tokens x
 // 4 heads 3.9 us.  Large calls: 32 elements to a lane (tq_fast_lane.h), a wave taking VPW consecutive tokens of one head of
-// K or V, so that it reads whole rows and writes its codes contiguously; bound by the reads and writes: 8 prompts of up to
-// 8192 tokens x 12 heads, 334 MB, 80 us, 4.2 TB/s of a copy's 5.0.
+// K or V, so that it reads whole rows and writes its codes contiguously; bound by its vector instructions (some 500 a wave,
+// the codec's own 435 among them) with the reads and writes close behind: 8 prompts of up to
+// 8192 tokens x 12 heads, 334 MB, 75 us, 4.4 TB/s of a copy's 5.0 (81 with a search in 64 bits in every lane).
 #include "paged_cache.h"
 #include "tq_fast_lane.h"
 
@@ -88,6 +89,34 @@ __device__ __forceinline__ int64_t token_slot(const AppendArgs& a, int64_t n, in
   return a.start[*b] + *at;
 }
 
+// The same for a wave's tokens n0 + v (n0 uniform, fewer than `span` of them): n0's sequence is found once, with scalar
+// loads, and lanes step on from it only where the span leaves it.
+__device__ __forceinline__ int64_t token_slot_near(const AppendArgs& a, uint32_t n0, uint32_t v, uint32_t span, int32_t* b, int32_t* at) {
+  const int32_t n = static_cast<int32_t>(n0 + v), B = static_cast<int32_t>(a.B);
+  if (a.cu) {
+    int32_t lo = -1, hi = B + 1;  // cu[lo] <= n0 < cu[hi], as if cu[-1] were lowest and cu[B + 1] highest
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (a.cu[mid] <= static_cast<int32_t>(n0)) lo = mid;
+      else hi = mid;
+    }
+    int32_t own = lo;
+    if (lo < B && a.cu[lo + 1] < static_cast<int64_t>(n0) + span)
+      while (own < B && a.cu[own + 1] <= n) ++own;
+    if (own < 0 || own >= B) {
+      *b = -1, *at = 0;
+      return -1;
+    }
+    *b = own, *at = n - a.cu[own];
+  } else {
+    const uint32_t per = static_cast<uint32_t>(a.per_seq), first = n0 / per;
+    uint32_t own = first, place = n0 - first * per + v;
+    while (place >= per) place -= per, ++own;
+    *b = static_cast<int32_t>(own), *at = static_cast<int32_t>(place);
+  }
+  return static_cast<int64_t>(a.start[*b]) + *at;
+}
+
 template <int DT, int D, int BITS>
 __global__ __launch_bounds__(kTableThreads, 4) void kv_append_rows_kernel(AppendArgs a, float cq) {
   using F = FastEnc<BITS, D>;
@@ -113,23 +142,23 @@ __global__ __launch_bounds__(kTableThreads, 4) void kv_append_rows_kernel(Append
   const int64_t stride = (is_v ? a.v_token : a.k_token) * 2;
   uint8_t* codes = is_v ? a.pool.v_codes : a.pool.k_codes;
   float* scale = is_v ? a.pool.v_scale : a.pool.k_scale;
-  const int64_t n = n0 + v < a.n_tokens ? n0 + v : a.n_tokens - 1;  // (a last tile's spare lanes read its last token)
+  const uint32_t last = static_cast<uint32_t>(a.n_tokens - 1 - n0), vn = min(static_cast<uint32_t>(v), last);  // (spare lanes of the last tile read its last token)
   uint32_t w[16];
   {
-    const uint4* p = reinterpret_cast<const uint4*>(x + n * stride + 64 * g);
+    const uint4* p = reinterpret_cast<const uint4*>(x + n0 * stride + vn * stride + 64 * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 t = p[i];
       w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
     }
   }
-  int64_t b = -1, at = 0;
-  const int64_t slot = token_slot(a, n, &b, &at);
-  const int64_t row = n0 + v < a.n_tokens && b >= 0 ? cache_row(a.pool, b, h, slot) : -1;
+  int32_t b = -1, at = 0;
+  const int64_t slot = token_slot_near(a, static_cast<uint32_t>(n0), vn, VPW, &b, &at);
+  const int64_t row = static_cast<uint32_t>(v) <= last && b >= 0 ? cache_row(a.pool, b, h, slot) : -1;
   if (row >= 0 && g == 0 && !is_v && a.weights && slot < a.capacity) {
-    const int64_t t = (b * heads + h) * a.capacity + slot;
+    const int64_t t = (static_cast<int64_t>(b) * heads + h) * a.capacity + slot;
     a.weights[t] = 0.0f;
-    a.tokens[t] = a.token[b] + static_cast<int32_t>(at);
+    a.tokens[t] = a.token[b] + at;
   }
   uint32_t dm[16];
 #pragma unroll
@@ -169,7 +198,7 @@ __global__ __launch_bounds__(kTableThreads, 4) void kv_append_rows_kernel(Append
 
 // Elements of K and V together from which a call takes the second layout (4-bit D = 128 / 8-bit D = 64, first against
 // second: 524288 elements 3.7 / 3.5 and 4.4 / 4.7 us, 1048576 4.0 / 3.9 and 4.8 / 4.7, 2097152 4.9 / 4.8 and 4.8 / 5.0;
-// a prompt batch of 98 M elements, 334 MB, 176 and 81 us, 4.1 TB/s).
+// a prompt batch of 98 M elements, 334 MB, 176 and 75 us).
 constexpr int64_t kRowsElements = int64_t(1) << 21;
 
 using append_fn = void (*)(AppendArgs);

@@ -654,3 +654,39 @@ def test_attention_of_a_ragged_batch_longest_first(dev, B, heads):
 def test_evict_around_the_rows_of_more_waves(dev, length):
     _check_evict(dev, 8, 128, 1, 16, [length, length - 100, 90], length - 200, 4, 64, seed=length)
     _check_evict(dev, 4, 64, 1, 16, [length, length // 2], length // 3, 4, 64, seed=length)
+
+
+@pytest.mark.parametrize("shape", ["three each", "one each", "short packed", "packed from the second row on"])
+def test_append_large_calls_of_many_sequences(dev, shape):
+    """A wave's tokens of a large call belong to many sequences: equal ones, and packed ones with empty ones between."""
+    heads, dim, page = 4, 128, 16
+    if shape.endswith("each"):
+        B, T = (1400, 3) if shape[0] == "t" else (2100, 1)
+        lens, off = [T] * B, 0
+    else:
+        lens, off = [(0, 1, 0, 5, 2, 0, 0, 40, 3)[i % 9] for i in range(450)], (1 if "second" in shape else 0)
+        B, T = len(lens), 0
+    cache, table, _ = _cache(dev, 60, 4, dim, heads, page, [max(lens) + 16] * B)
+    N = off + sum(lens) + (3 if not T else 0)
+    k, v = (torch.randn(N, heads, dim, device=dev, generator=_gen(dev, 61 + i)).to(torch.bfloat16) for i in range(2))
+    cu = [off]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    start = [b % 16 for b in range(B)]
+    assert N * 2 * heads * dim >= 1 << 21
+    tracker = SlotTracker(B, heads, table.size(1) * page, device=dev)
+    tracker.weights.fill_(9.0)
+    token = torch.arange(B, dtype=torch.int32, device=dev) * 100
+    want = _expect_append(cache, k, v, table.cpu(), start, cu)
+    args = dict(tracker=tracker, token=token)
+    if T:
+        k, v = k.view(B, T, heads, dim), v.view(B, T, heads, dim)
+    else:
+        args["cu_seqlens"] = torch.tensor(cu, dtype=torch.int32, device=dev)
+    append_tokens(cache, k, v, table, torch.tensor(start, dtype=torch.int32, device=dev), **args)
+    for got, w in zip((cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale), want):
+        assert torch.equal(got, w)
+    i = torch.arange(tracker.capacity, device=dev)[None] - torch.tensor(start, device=dev)[:, None]
+    new = ((i >= 0) & (i < torch.tensor(lens, device=dev)[:, None]))[:, None].expand_as(tracker.weights)
+    assert torch.equal(tracker.weights, torch.where(new, 0.0, 9.0))
+    assert torch.equal(tracker.tokens[new], (token[:, None] + i)[:, None].expand_as(new)[new].int())
