@@ -690,11 +690,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
 // of its loads: 12 rows of 128 pieces 8 us with four pieces requested at a time, 6.5 with eight (sixteen, whose registers
 // halve the waves on a CU, made 2048 rows of 5 pieces 0.8 us slower).
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
+__device__ __forceinline__ void merge_row(const PagedArgs& a, int64_t orow) {
   constexpr int PER = D / 64;
   __shared__ float s_o[kWaves][D], s_ml[kWaves][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t orow = blockIdx.x;
   const int64_t b = orow / (static_cast<int64_t>(a.T) * a.H);
   const int32_t h = static_cast<int32_t>(orow % a.H);
   const int32_t n = newest_sees(a, b);
@@ -774,15 +773,50 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
   if (a.lse && lane == 0) a.lse[orow] = sum == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(sum);
 }
 
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedArgs a) {
+  merge_row<DT, D>(a, blockIdx.x);
+}
+
 // The weights of a sequence's slots from the logits that the attention left and the rows' log sums: four slots to a thread.
 // Reads 4 bytes per row and slot, reads and writes the weights: 64 sequences x 4 heads x 3 rows of up to 16384 slots, 10 us.
-constexpr int kAddSlots = 1024;  // of a workgroup
+// MERGED: the log sums come from the pieces' maxima and sums (16 lanes to a row), so that the pieces' merge need not come first.
+constexpr int kAddSlots = 1024;   // of a workgroup
+constexpr int kLogitRows = 16;    // most rows of a KV head whose logits are kept
 
-__global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blocks) {
-  const int32_t j = static_cast<int32_t>(blockIdx.x % blocks) * kAddSlots + 4 * threadIdx.x;
-  const int64_t bk = blockIdx.x / blocks, b = bk / a.pool.heads;
+template <bool MERGED, int D>
+__device__ __forceinline__ void add_weights(const PagedArgs& a, uint32_t block, int32_t blocks) {
+  __shared__ float s_lse[kLogitRows];
+  const int32_t j0 = static_cast<int32_t>(block % blocks) * kAddSlots, j = j0 + 4 * static_cast<int32_t>(threadIdx.x);
+  const int64_t bk = block / blocks, b = bk / a.pool.heads;
   const int32_t kh = static_cast<int32_t>(bk - b * a.pool.heads);
   const int32_t n = newest_sees(a, b);
+  if (j0 >= n) return;  // (the whole workgroup)
+  const int32_t r = static_cast<int32_t>(threadIdx.x) >> 4, own = min(r, a.rows - 1), t = own / a.G, h = kh * a.G + (own - t * a.G);
+  const int64_t orow = (b * a.T + t) * a.H + h;
+  float lse;
+  if constexpr (MERGED) {
+    const int32_t piece = piece_slots(n, a.n_split), pieces = (n + piece - 1) / piece;
+    const float* p = a.part + orow * a.n_split * (D + 4);
+    float m = kNegInf, l = 0.0f;
+    for (int s = threadIdx.x & 15; s < pieces; s += 16) {
+      const float2 ml = *reinterpret_cast<const float2*>(p + static_cast<int64_t>(s) * (D + 4));
+      const float top = fmaxf(m, ml.x);
+      l = (l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(m - top)) + (ml.y == 0.0f ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - top));
+      m = top;
+    }
+    const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
+    float top = fmaxf(m, sk);
+    top = fmaxf(top, xor_lane<1>(top)), top = fmaxf(top, xor_lane<2>(top)), top = fmaxf(top, xor_lane<4>(top)), top = fmaxf(top, xor_lane<8>(top));
+    l = l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(m - top);
+    l += xor_lane<1>(l), l += xor_lane<2>(l), l += xor_lane<4>(l), l += xor_lane<8>(l);
+    l += sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - top);
+    lse = l == 0.0f ? -kNegInf : top + __builtin_amdgcn_logf(l);
+  } else {
+    lse = a.lse[orow];
+  }
+  if ((threadIdx.x & 15) == 0) s_lse[r] = lse;
+  __syncthreads();
   if (j >= n) return;
   const float* lg = a.logits + bk * a.rows * a.logit_slots + j;
   float* w = a.weights + bk * a.capacity + j;
@@ -790,20 +824,28 @@ __global__ __launch_bounds__(256) void paged_add_kernel(PagedArgs a, int32_t blo
   f32x4_t before = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
   if (vec) before = *reinterpret_cast<const f32x4_t*>(w);
 #pragma unroll 4
-  for (int32_t r = 0; r < a.rows; ++r) {
-    const int32_t t = r / a.G;
-    const float lse = a.lse[(b * a.T + t) * a.H + kh * a.G + (r - t * a.G)];
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lg + r * a.logit_slots);  // (the step's 32 slots are all there)
+  for (int32_t i = 0; i < a.rows; ++i) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lg + i * a.logit_slots);  // (the step's 32 slots are all there)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(x[i] - lse);
+    for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(x[e] - s_lse[i]);
   }
   if (vec) {
     *reinterpret_cast<f32x4_t*>(w) = before + sum;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (j + i < n) w[i] += sum[i];
+    for (int e = 0; e < 4; ++e)
+      if (j + e < n) w[e] += sum[e];
   }
+}
+
+__global__ __launch_bounds__(kThreads) void paged_add_kernel(PagedArgs a, int32_t blocks) { add_weights<false, 64>(a, blockIdx.x, blocks); }
+
+// Both ends of a tracked call in pieces, in one launch: `rows` workgroups merge a row each, the others add (the 64 sequences
+// above 96.4 -> 94.9 us).
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_add_kernel(PagedArgs a, uint32_t rows, int32_t blocks) {
+  if (blockIdx.x < rows) merge_row<DT, D>(a, blockIdx.x);
+  else add_weights<true, D>(a, blockIdx.x - rows, blocks);
 }
 
 // The weights of a piece of a sequence's slots, from the rows' log sums: each wave scores steps of 32 slots against every
@@ -958,7 +1000,7 @@ int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 :
 // Tracked calls of few rows keep their logits and sum them afterwards; of many rows the scores are computed again, which
 // reads a slot's K codes instead of 8 bytes a row.
 size_t paged_logit_bytes(int64_t B, int64_t heads, int64_t rows, int64_t slots) {
-  if (rows > 16) return 0;
+  if (rows > kLogitRows) return 0;
   const double bytes = 4.0 * static_cast<double>(B) * heads * rows * static_cast<double>(slots + 32);
   return bytes > 2147483648.0 ? 0 : static_cast<size_t>(B * heads * rows) * align_up(static_cast<size_t>(slots), 32) * 4;
 }
@@ -1041,6 +1083,13 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   auto fn = dtype == AEKV_F16 ? pick_paged<AEKV_F16>(d, bits, mt) : pick_paged<AEKV_BF16>(d, bits, mt);
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(B * heads * blocks * a.n_split)), dim3(kThreads), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
+  const int32_t per = a.logits ? static_cast<int32_t>(ceil_div(reach, kAddSlots)) : 0;
+  if (a.n_split > 1 && a.logits) {
+    auto mg = dtype == AEKV_F16 ? (d == 64 ? paged_merge_add_kernel<AEKV_F16, 64> : paged_merge_add_kernel<AEKV_F16, 128>)
+                                : (d == 64 ? paged_merge_add_kernel<AEKV_BF16, 64> : paged_merge_add_kernel<AEKV_BF16, 128>);
+    hipLaunchKernelGGL(mg, dim3(static_cast<uint32_t>(B * T * H + B * heads * per)), dim3(kThreads), 0, st, a, static_cast<uint32_t>(B * T * H), per);
+    return check_launch(who);
+  }
   if (a.n_split > 1) {
     auto mg = dtype == AEKV_F16 ? (d == 64 ? paged_merge_kernel<AEKV_F16, 64> : paged_merge_kernel<AEKV_F16, 128>)
                                 : (d == 64 ? paged_merge_kernel<AEKV_BF16, 64> : paged_merge_kernel<AEKV_BF16, 128>);
@@ -1049,8 +1098,7 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   }
   if (!a.weights) return AEKV_OK;
   if (a.logits) {
-    const int32_t per = static_cast<int32_t>(ceil_div(reach, kAddSlots));
-    hipLaunchKernelGGL(paged_add_kernel, dim3(static_cast<uint32_t>(B * heads * per)), dim3(256), 0, st, a, per);
+    hipLaunchKernelGGL(paged_add_kernel, dim3(static_cast<uint32_t>(B * heads * per)), dim3(kThreads), 0, st, a, per);
     return check_launch(who);
   }
   a.n_split = static_cast<int32_t>(paged_pieces(B * heads, slots));
