@@ -42,8 +42,10 @@ class PagedKVCache:
         rows = (int(pages), int(kv_heads), int(page_size))
         dtype = torch.int8 if quant.bits == 8 else torch.uint8
         row = dim * quant.bits // 8
-        self._set(quant, *(torch.zeros(rows + (row,), dtype=dtype, device=dev) if i % 2 == 0 else
-                           torch.zeros(rows, dtype=torch.float32, device=dev) for i in range(4)))
+        tensors = [torch.zeros(rows + (row,), dtype=dtype, device=dev) if i % 2 == 0 else
+                   torch.zeros(rows, dtype=torch.float32, device=dev) for i in range(4)]
+        _lib.require_device("PagedKVCache", *tensors)  # (the calls compare their tensors' device with the cache's)
+        self._set(quant, *tensors)
 
     def _set(self, quant, k_codes, k_scale, v_codes, v_scale) -> None:
         self.quant, self.bits = quant, quant.bits
@@ -105,7 +107,9 @@ class SlotTracker:
         if batch < 1 or kv_heads < 1 or capacity < 1:
             raise ValueError(f"SlotTracker needs batch, kv_heads, capacity >= 1, got {batch}, {kv_heads}, {capacity}")
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        self._set(torch.zeros((2, int(batch), int(kv_heads), int(capacity)), dtype=torch.int32, device=dev))
+        storage = torch.zeros((2, int(batch), int(kv_heads), int(capacity)), dtype=torch.int32, device=dev)
+        _lib.require_device("SlotTracker", storage)
+        self._set(storage)
 
     def _set(self, storage: torch.Tensor) -> None:
         self._storage, self._weights, self._tokens = storage, storage[0].view(torch.float32), storage[1]

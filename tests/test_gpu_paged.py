@@ -690,3 +690,54 @@ def test_append_large_calls_of_many_sequences(dev, shape):
     new = ((i >= 0) & (i < torch.tensor(lens, device=dev)[:, None]))[:, None].expand_as(tracker.weights)
     assert torch.equal(tracker.weights, torch.where(new, 0.0, 9.0))
     assert torch.equal(tracker.tokens[new], (token[:, None] + i)[:, None].expand_as(new)[new].int())
+
+
+def test_attention_shared_and_repeated_pages(dev):
+    """Pages that sequences share, and a page that a sequence has twice; a query expanded over the heads."""
+    cache = _fill(dev, 80, 4, 128, 2, 16, 9)
+    table = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5], [6, 6, 6, 7]], dtype=torch.int32, device=dev)
+    n = torch.tensor([64, 50, 60], dtype=torch.int32, device=dev)
+    q = torch.randn(3, 1, 1, 128, device=dev, generator=_gen(dev, 81)).to(torch.bfloat16).expand(3, 1, 6, 128)
+    tracker = SlotTracker(3, 2, 64, device=dev)
+    got = paged_attention(q, cache, table, n, 0.1, tracker=tracker)
+    want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, table), q.cpu(), n.tolist(), 0.1, None, 64)
+    R.within(got, want, bound, "out")
+    R.within(tracker.weights, w, wb + 2.0 ** -23 * w, "weights")
+
+
+@pytest.mark.parametrize("T", [1, 9])
+def test_long_tracked_attention_in_two_graphs_and_streams(dev, T):
+    """Two captured calls in pieces, with logits (T = 1) and with the scores again (T = 9), replayed on two streams at once
+    and among eager calls: each graph has a workspace of its own."""
+    heads, H, dim, page, lens = 2, 6, 64, 64, [3000, 700, 0]
+    cache, table, n = _cache(dev, 82, 8, dim, heads, page, lens)
+    q = torch.randn(2, 3, T, H, dim, device=dev, generator=_gen(dev, 83)).to(torch.float16)
+    trackers = [SlotTracker(3, heads, table.size(1) * page, device=dev) for _ in range(3)]
+    call = lambda i, t: paged_attention(q[i], cache, table, n, 0.125, tracker=trackers[t])  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0, 2)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            outs.append(call(i, i))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(3):
+        q.copy_(torch.randn(q.shape, device=dev, generator=_gen(dev, 90 + rep)))
+        want, weights = [], []
+        for i in range(2):
+            trackers[2].storage.zero_()
+            want.append(call(i, 2).clone())
+            weights.append(trackers[2].weights.clone())
+            trackers[i].storage.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        call(0, 2)
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i]) and torch.equal(trackers[i].weights, weights[i]), f"graph {i}, replay {rep}"

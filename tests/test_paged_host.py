@@ -188,3 +188,14 @@ def test_attention_workspace_holds_logits_for_few_rows_and_up_to_2_gib(lib):
     assert size(64, 1, 1 << 20, 1) - size(64, 1, 1 << 20, 0) == lse(64, 1)
     assert size(1, 4, 1024, 1) - size(1, 4, 1024, 0) == lse(1, 4) + 2 * 16 * 1024 * 4
     assert size(1, 5, 1024, 1) - size(1, 5, 1024, 0) == lse(1, 5)  # 20 rows: scored again
+
+
+def test_caches_and_trackers_are_on_a_device():
+    """A cache in host memory would hand the kernels host pointers: it cannot be made."""
+    from aetherkv import PolarQuant
+    from aetherkv.paged import PagedKVCache, SlotTracker
+
+    with pytest.raises(RuntimeError, match="device"):
+        PagedKVCache(PolarQuant(4), 4, 2, 128, page_size=16, device="cpu")
+    with pytest.raises(RuntimeError, match="device"):
+        SlotTracker(1, 2, 64, device="cpu")
