@@ -516,8 +516,9 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
   }
 }
 
-// Merges the pieces of the rows: D / 4 lanes hold a row, 4 dims each.  Bound by reading them: 5 us for 11744 rows of 2
-// pieces, dim 64, 6 MB.
+// Merges the pieces of the rows: D / 4 lanes hold a row, 4 dims each.  Bound by the chain of its loads, so that they go out
+// together: 64 queries over 8192 keys, 16 heads of 2, dim 64, 16 pieces: the call 17.2 us, one piece after another 23.4; 11744
+// rows of 2 pieces, 6 MB, 4 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
   using E = Elem<DT>;
@@ -525,24 +526,46 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / PER) + threadIdx.x / PER;
   if (row >= static_cast<int64_t>(a.n_q) * a.H) return;
   const int32_t n = static_cast<int32_t>(row / a.H), h = static_cast<int32_t>(row - static_cast<int64_t>(n) * a.H);
-  if (n < a.cu_q[0] || n >= a.cu_q[a.B]) return;  // in no sequence
   const int j = threadIdx.x % PER;
   const float* p = a.part + row * a.n_split * (D + 4);
+  const int32_t c0 = a.cu_q[0], c1 = a.cu_q[a.B];
   const float sk = a.sink ? a.sink[h] * kLog2e : kNegInf;
-  float top = sk;
-#pragma unroll 4
-  for (int s = 0; s < a.n_split; ++s) top = fmaxf(top, p[s * (D + 4)]);
-  float sum = sk == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sk - top);
+  float top = sk, sum = sk == kNegInf ? 0.0f : 1.0f;
   float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = 0; s < a.n_split; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p + s * (D + 4));
-    if (ml.y == 0.0f) continue;  // nothing seen
-    const float4 o = *reinterpret_cast<const float4*>(p + s * (D + 4) + 4 + 4 * j);
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    sum += ml.y * f;
-    x[0] = fmaf(o.x, f, x[0]), x[1] = fmaf(o.y, f, x[1]), x[2] = fmaf(o.z, f, x[2]), x[3] = fmaf(o.w, f, x[3]);
-  }
+  // CH pieces at a time, all their loads issued together (a piece past the last reads the last, and counts as empty)
+  auto merge = [&](auto ch) __attribute__((always_inline)) {
+    constexpr int CH = decltype(ch)::value;
+    for (int s0 = 0; s0 < a.n_split; s0 += CH) {
+      float2 ml[CH];
+      float4 o[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const float* ps = p + min(s0 + c, a.n_split - 1) * (D + 4);
+        ml[c] = *reinterpret_cast<const float2*>(ps);
+        o[c] = *reinterpret_cast<const float4*>(ps + 4 + 4 * j);
+      }
+      float up = top;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (s0 + c >= a.n_split || ml[c].y == 0.0f) ml[c] = make_float2(kNegInf, 0.0f), o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // (nothing seen)
+        up = fmaxf(up, ml[c].x);
+      }
+      const float r = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+      sum = sum == 0.0f ? 0.0f : sum * r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= r;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const float f = ml[c].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[c].x - up);
+        sum += ml[c].y == 0.0f ? 0.0f : ml[c].y * f;
+        x[0] = fmaf(o[c].x, f, x[0]), x[1] = fmaf(o[c].y, f, x[1]), x[2] = fmaf(o[c].z, f, x[2]), x[3] = fmaf(o[c].w, f, x[3]);
+      }
+      top = up;
+    }
+  };
+  if (a.n_split <= 2) merge(std::integral_constant<int, 2>{});
+  else merge(std::integral_constant<int, 4>{});
+  if (n < c0 || n >= c1) return;  // in no sequence
   const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
   *reinterpret_cast<uint2*>(a.out + row * D + 4 * j) = make_uint2(E::pack(x[0] * r, x[1] * r), E::pack(x[2] * r, x[3] * r));
   if (a.lse && j == 0) a.lse[row] = sum == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
@@ -564,8 +587,8 @@ prompt_fn pick_prompt(int32_t dtype, int32_t d) {
 // 16 heads of 16, 2048 over 8192 (one piece of 128) 149 / 160.
 //
 // Pieces have to save a row the time of some kPieceTiles tiles, which is what their merge costs: 16 heads of 2, dim 64, whole / in
-// pieces: 1024 queries over their own keys 14.0 / 18.6 us, 1500 18.7 / 23.6, 64 queries over 2048 keys 22.3 / 13.3, 16 over
-// 1024 13.6 / 12.5.
+// pieces: 1024 queries over their own keys 14.0 / 18.6 us, 1500 18.7 / 23.6, 64 queries over 2048 keys 22.3 / 11.6, 16 over
+// 1024 13.6 / 10.9.
 struct PromptPlan {
   int64_t rows, tiles, split;
 };
