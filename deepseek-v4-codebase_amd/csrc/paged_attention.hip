@@ -195,10 +195,11 @@ struct StepData {
 };
 
 // The wave's page ids: lane 2 i + k holds that of tile k (16 slots) of its i-th step from `first`; -1 where a tile has none.
-__device__ __forceinline__ int32_t load_pages(const PagedArgs& a, int64_t b, int32_t first, int32_t end, int lane) {
+// (What the table says past the sequence's end does not matter: those slots are hidden.)
+__device__ __forceinline__ int32_t load_pages(const PagedArgs& a, int64_t b, int32_t first, int lane) {
   const int64_t slot = static_cast<int64_t>(first) + kRound * (lane >> 1) + 16 * (lane & 1);
   int32_t page = -1;
-  if (slot < end) page = a.pool.table[b * a.pool.max_pages + (slot >> a.pool.page_shift)];
+  if (slot < a.reach) page = a.pool.table[b * a.pool.max_pages + (slot >> a.pool.page_shift)];
   return page >= 0 && page < a.pool.pages ? page : -1;
 }
 
@@ -445,10 +446,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   wg /= a.row_blocks;
   const int32_t kh = static_cast<int32_t>(wg % a.pool.heads);
   int64_t b = wg / a.pool.heads;
-  int32_t n;
+  int32_t n, pages = -1;
   if (a.ranked == 1) b = ranked_sequence<1>(a, static_cast<int32_t>(b), lane, &n);
   else if (a.ranked == 2) b = ranked_sequence<8>(a, static_cast<int32_t>(b), lane, &n);
-  else n = newest_sees(a, b);
+  if (a.n_split == 1) pages = load_pages(a, b, kStep * wave, lane);  // (of a whole sequence: not after its length)
+  if (!a.ranked) n = newest_sees(a, b);
   const int32_t piece = piece_slots(n, a.n_split);
   const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
   if (split > 0 && p0 >= p1) return;  // (the merge knows how many pieces a sequence has)
@@ -462,7 +464,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
     load_query<D>(a, b, kh, row[t], row[t] < a.rows, lane, qw[t]);
   }
   const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
-  int32_t pages = -1;
   const int32_t first = p0 + kStep * wave;
   const int n_steps = first < p1 ? (p1 - first + kRound - 1) / kRound : 0;
   uint32_t bad[NS] = {};  // bit k: tile k of the stage's step has no page
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
     return (decltype(which)::value == 0 ? st0 : decltype(which)::value == 1 ? st1 : st2) + wave * S::kBytes;
   };
   auto load = [&](int i, auto which) __attribute__((always_inline)) {
-    if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+    if ((i & 31) == 0 && (i > 0 || a.n_split > 1)) pages = load_pages(a, b, first + kRound * i, lane);
     const int32_t g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
     bad[decltype(which)::value] = (g0 < 0 ? 1u : 0u) | (g1 < 0 ? 2u : 0u);
     issue_step<D, BITS>(a, kh, first + kRound * i, g0, g1, lane, stage(which));
@@ -703,15 +704,15 @@ __device__ __forceinline__ void merge_row(const PagedArgs& a, int64_t orow) {
   float m = kNegInf, l = 0.0f, x[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) x[i] = 0.0f;
-  // CH pieces at a time, all their loads issued together (a piece past the last reads the last, as an empty one)
+  // CH pieces at a time, all their loads issued together (a piece past the last counts as empty)
   auto merge = [&](auto ch) __attribute__((always_inline)) {
     constexpr int CH = decltype(ch)::value;
-    for (int s0 = wave; s0 < pieces; s0 += kWaves * CH) {
+    for (int s0 = wave; s0 < (CH < 8 ? wave + 1 : pieces); s0 += kWaves * CH) {  // (2, 4: one pass, whose loads do not wait for the length)
       float pm[CH], pl[CH], v[CH][PER];
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int s = s0 + kWaves * c;
-        const float* ps = p + static_cast<int64_t>(min(s, pieces - 1)) * (D + 4);
+        const float* ps = p + static_cast<int64_t>(min(s, a.n_split - 1)) * (D + 4);
         pm[c] = ps[0], pl[c] = ps[1];
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[c][i] = ps[4 + PER * lane + i];
@@ -719,7 +720,11 @@ __device__ __forceinline__ void merge_row(const PagedArgs& a, int64_t orow) {
       float top = m;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        if (s0 + kWaves * c >= pieces) pm[c] = kNegInf, pl[c] = 0.0f;
+        if (s0 + kWaves * c >= pieces) {  // (what lies there is anything)
+          pm[c] = kNegInf, pl[c] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v[c][i] = 0.0f;
+        }
         top = fmaxf(top, pm[c]);
       }
       const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
@@ -736,7 +741,8 @@ __device__ __forceinline__ void merge_row(const PagedArgs& a, int64_t orow) {
       m = top;
     }
   };
-  if (pieces <= 2 * kWaves) merge(std::integral_constant<int, 2>{});
+  if (a.n_split <= 2 * kWaves) merge(std::integral_constant<int, 2>{});
+  else if (a.n_split <= 4 * kWaves) merge(std::integral_constant<int, 4>{});
   else merge(std::integral_constant<int, 8>{});
 #pragma unroll
   for (int i = 0; i < PER; ++i) s_o[wave][PER * lane + i] = x[i];
@@ -899,7 +905,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
     int32_t pages = -1, g0 = -1, g1 = -1;
     StepData<D, BITS> s, next;
     auto load = [&](int i) __attribute__((always_inline)) {
-      if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, p1, lane);
+      if ((i & 31) == 0) pages = load_pages(a, b, first + kRound * i, lane);
       g0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)), g1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1);
       load_keys<D, BITS>(a, kh, first + kRound * i, g0, g1, lane, next);
     };
