@@ -62,7 +62,8 @@ struct PromptArgs {
   int32_t n_split, tiles;
   int32_t n_q, n_k, B, H, heads, G;
   int32_t clear;        // rows in no sequence: 0 to leave out as it is, 1 to write zeros
-  int32_t by_work;      // the tiles' order: 0 the sequences', else by work (half of a power of two above every level)
+  int32_t by_work;      // the tiles' order: 0 the sequences', -1 that without gaps, else by work (half of a power of two above
+                        // every level)
   uint32_t fold;        // tiles of the launch's second round of workgroups, which are taken from its end; 0: none
   float scale2;         // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
   int32_t flip;         // scale is negative the queries' signs are flipped: a row's largest product is its largest logit
@@ -138,6 +139,31 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int32_t t, int ro
   }
 }
 
+// The same of up to 64 sequences with every place before the last tile's taken: where the workgroups about fill the chip,
+// places without a tile among them leave some parts of it with more than fits, and a second round.
+__device__ __forceinline__ bool find_tile_dense(const PromptArgs& a, int32_t t, int rows, int lane, TileAt* at) {
+  const int32_t b = min(lane, a.B - 1);
+  const int32_t c0 = a.cu_q[b], c1 = a.cu_q[b + 1], d0 = a.cu_k[b], d1 = a.cu_k[b + 1];
+  const int32_t q0 = min(max(c0, 0), a.n_q), lq = min(max(c1, q0), a.n_q) - q0;
+  const int32_t k0 = min(max(d0, 0), a.n_k), lk = min(max(d1, k0), a.n_k) - k0;
+  const int32_t tiles = lane < a.B ? (lq * a.G + rows - 1) / rows : 0;
+  int32_t s = tiles;  // inclusive sum over the lanes
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(s, d);
+    if (lane >= d) s += o;
+  }
+  const uint64_t mine = __builtin_amdgcn_ballot_w64(s > t && s - tiles <= t);
+  if (!mine) return false;
+  const int l = __builtin_ctzll(mine);
+  at->q0 = __builtin_amdgcn_readlane(q0, l);
+  at->lq = __builtin_amdgcn_readlane(lq, l);
+  at->k0 = __builtin_amdgcn_readlane(k0, l);
+  at->lk = __builtin_amdgcn_readlane(lk, l);
+  at->row = (__builtin_amdgcn_readlane(s, l) - 1 - t) * rows;
+  return true;
+}
+
 __device__ __forceinline__ int32_t lane_sum(int32_t v) {
   auto step = [&](auto hl) { v += __builtin_bit_cast(int32_t, xor_lane<decltype(hl)::value>(__builtin_bit_cast(float, v))); };
   step(std::integral_constant<int, 1>{}), step(std::integral_constant<int, 2>{}), step(std::integral_constant<int, 4>{});
@@ -208,8 +234,9 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
     index = 3 * a.fold - 1 - index;
   }
   TileAt at;
-  const bool found = a.by_work ? find_tile_by_work(a, static_cast<int32_t>(index), kRows, lane, &at)
-                               : find_tile(a, static_cast<int32_t>(index), kRows, lane, &at);
+  const bool found = a.by_work > 0   ? find_tile_by_work(a, static_cast<int32_t>(index), kRows, lane, &at)
+                     : a.by_work < 0 ? find_tile_dense(a, static_cast<int32_t>(index), kRows, lane, &at)
+                                     : find_tile(a, static_cast<int32_t>(index), kRows, lane, &at);
   if (a.clear || a.lse) {  // rows in no sequence: shared out over the workgroups
     const int32_t s0 = min(max(a.cu_q[0], 0), a.n_q), s1 = min(max(a.cu_q[a.B], s0), a.n_q);
     const int64_t words = static_cast<int64_t>(s0 + a.n_q - s1) * a.H * (D / 2);
@@ -581,10 +608,14 @@ prompt_fn pick_prompt(int32_t dtype, int32_t d) {
 // How a launch is cut: rows of a workgroup, and pieces of the keys where the row tiles alone leave CUs without a workgroup
 // (as many as are resident together: three of a CU at head dim 64, two at 128).
 //
-// 128 rows to a workgroup read a tile of keys once for twice the rows; 64 give twice the workgroups.  128 where
-// they fill the chip by themselves, or in at least two pieces of enough work to pay for the pieces' merge: 12 heads of 4,
-// dim 128, 64 / 128 rows: 1024 queries over 8192 keys (the least) 81 / 69 us, over 32768 287 / 225, 512 over 8192 46 / 48;
-// 16 heads of 16, 2048 over 8192 (one piece of 128) 149 / 160.
+// 128 rows to a workgroup read a tile of keys once for twice the rows; 64 give twice the workgroups.  128 where they fill the
+// chip; of several sequences with tiles of like work also where they about fill it and (as if all were as long) run together;
+// and in at least two pieces of enough work to pay for the pieces' merge.  64 / 128 rows, dim 128:
+// 8 x 512 queries over 4096 keys, 16 heads of 2, 512 tiles 194 / 142 us; 10 x 512 over their own, 12 heads of 4, 480 27.7 /
+// 20.6; 5 x 512 over 4096, 16 of 2, 320 131 / 122; below: 7 x 384 over 1024, 12 of 4, 252 27.3 / 27.6; above: 15 x 320 over
+// 2112, 12 of 12, 540 98 / 110; tiles of different work: 2 x 2048 over their own, 12 of 4, 384 46 / 51, one of 4096 71 / 74.
+// In pieces, 12 heads of 4: 1024 queries over 8192 keys (the least) 81 / 69, over 32768 287 / 225, 512 over 8192 46 / 48; 16
+// heads of 16, 2048 over 8192 (one piece of 128) 149 / 160.
 //
 // Pieces have to save a row the time of some kPieceTiles tiles, which is what their merge costs: 16 heads of 2, dim 64, whole / in
 // pieces: 1024 queries over their own keys 14.0 / 18.6 us, 1500 18.7 / 23.6, 64 queries over 2048 keys 22.3 / 11.6, 16 over
@@ -596,7 +627,10 @@ constexpr int64_t kWideWork = int64_t(3) << 25;  // rows x keys of a sequence
 PromptPlan plan_prompt(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d) {
   PromptPlan p;
   const int64_t rows = n_q * (H / heads), resident = d == 64 ? 768 : 512;
-  const bool wide = heads * (rows / 128) >= 512 || (n_q * H * (n_k / B) >= kWideWork && 2 * heads * (rows / 128 + B) <= resident);
+  const int64_t groups = heads * (rows / 128);
+  const bool alike = B > 1 && (2 * n_q <= n_k || n_q / B <= 1024);  // tiles of like work
+  const int64_t each = rows / B, tiles = heads * B * ceil_div(each - each / 64, static_cast<int64_t>(128));  // (a buffer's end may be unused)
+  const bool wide = groups >= 512 || (alike && groups >= (d == 64 ? 400 : 300) && tiles <= resident) || (n_q * H * (n_k / B) >= kWideWork && 2 * heads * (rows / 128 + B) <= resident);
   p.rows = wide ? 128 : 64;
   p.tiles = rows / p.rows + B;  // at least every sequence's, whatever their lengths
   const int64_t sees = (n_q < n_k ? n_k - n_q / 2 : n_k / 2) / B, piece = kTile * kPieceTiles;  // keys of a row, on average
@@ -656,6 +690,8 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
   if (B > 1 && B <= 64 && plan.tiles * heads > (d == 64 ? 768 : 512) && n_k * ceil_div(heads, static_cast<int64_t>(8)) * 4 * d <= (12 << 20)) {
     const int64_t levels = n_k * (H / heads) / plan.rows + plan.tiles;
     for (by_work = 1; by_work < (1 << 25) && 2 * by_work <= levels;) by_work *= 2;
+  } else if (B > 1 && B <= 64 && plan.tiles * heads * plan.split > 256) {
+    by_work = -1;
   }
   // Tiles come with the most keys first; the second workgroup of each CU is taken from the short end of its round, so that the
   // pairs have like work (one prompt of 11000, 12 heads of 4: 400 -> 381 us; 8192, 16 heads of 16: 300 -> 288; else 0 to 3 %).

@@ -335,3 +335,27 @@ def test_prompt_very_many_sequences(dev, B):
     none = wl == -math.inf
     assert torch.equal(lse.cpu() == -math.inf, none)
     R.within(lse.double().cpu()[~none], wl[~none], lb[~none], "lse")
+
+
+@pytest.mark.parametrize("dtype,dim,H,hk,lq,lk", [(torch.bfloat16, 128, 16, 2, [512] * 8, [600] * 8), (torch.float16, 64, 32, 16, [200, 0, 333, 90, 512, 1, 400, 256] * 2, [300, 10, 400, 90, 700, 1500, 512, 300] * 2)])
+def test_prompt_tiles_that_about_fill_the_chip(dev, dtype, dim, H, hk, lq, lk):
+    """Several sequences whose 128-row tiles run together: every tile has its place, in the sequences' order without gaps.
+    Checked on some rows, and every row against the call on its sequence alone, up to the kernels' own roundings."""
+    q, k, v = _inputs(dev, 9, dtype, dim, H, hk, lq, lk, pad=3)
+    cq, ck = _cu(lq), _cu(lk)
+    out = prompt_attention(q, k, v, torch.tensor(cq, dtype=torch.int32, device=dev), dim ** -0.5,
+                           cu_seqlens_k=torch.tensor(ck, dtype=torch.int32, device=dev))
+    assert not out[cq[-1]:].any()
+    for b, n in enumerate(lq):
+        if n == 0:
+            continue
+        one = prompt_attention(q[cq[b]:cq[b + 1]], k[ck[b]:ck[b + 1]], v[ck[b]:ck[b + 1]], torch.tensor([0, n], dtype=torch.int32, device=dev), dim ** -0.5,
+                               cu_seqlens_k=torch.tensor([0, lk[b]], dtype=torch.int32, device=dev))
+        # (both are within the same bound of the exact value; values are below 6, weights sum to 1)
+        tol = 4 * torch.finfo(dtype).eps
+        assert ((out[cq[b]:cq[b + 1]].float() - one.float()).abs() <= tol * (1 + one.float().abs()) * 6).all(), f"sequence {b}"
+        for i in sorted({0, n - 1}):
+            see, r = max(0, i + 1 + lk[b] - n), cq[b] + i
+            keys = slice(ck[b], ck[b] + see)
+            want, bound, _, _ = R.prompt_attention_ref(q[r:r + 1].cpu(), k[keys].cpu(), v[keys].cpu(), [0, 1], [0, see], dim ** -0.5)
+            R.within(out[r:r + 1], want, bound, f"sequence {b}, query {i}")
