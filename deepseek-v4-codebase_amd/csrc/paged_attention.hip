@@ -13,14 +13,15 @@
 // sum, the output rescaled only where a row's maximum moved by more than kMargin.
 //
 // Loads.  A wave's steps go straight into LDS, each wave in a ring of its own of three stages (two where a row has 128
-// bytes, so that three workgroups stay on a CU), the next two requested before a step is waited for: with the loads in
+// bytes, so that two workgroups stay on a CU), the next ones requested before a step is waited for: with the loads in
 // registers a CU held one step of each wave (one sequence of 262144 slots, 12 heads: 120 us, staged 109).  The queries and
 // the first steps are requested before the rotation runs.
 //
 // Measured (dim 128, 4 bits).  One sequence of 262144 slots, 12 heads of 12: 428 MB in 87 to 91 us, 4.7 to 4.9 TB/s, what a
-// large copy reaches (5.0), with the merge 96 us.  64 ragged sequences of up to 16384 slots, 12 heads of 4, tracked: 78
-// us, the merge 5 and the weights' sum 10 (a form with 40 of a step's 222 vector instructions less took as long).  16 tokens x 8 heads of 8 sequences of up to 5001 slots, dim 64, 8 bits: 20
-// us, the rotations, four steps behind one another in each wave, and the merge of the waves.
+// large copy reaches (5.0), with the merge 96 us.  64 ragged sequences of up to 16384 slots, 12 heads of 4, tracked: 75 us,
+// the merge and the weights' sum 13 (a form with 40 of a step's 222 vector instructions less took as long).  16 tokens x 8
+// heads of 8 sequences of up to 5001 slots, dim 64, 8 bits: 20 us, the rotations, four steps behind one another in each
+// wave, and the merge of the waves.
 //
 // Matrix layout (v_mfma_f32_16x16x32: A lane l holds A[l % 16][8 (l / 16) + j], B lane l holds B[8 (l / 16) + j][l % 16],
 // D lane l register i holds D[4 (l / 16) + i][l % 16]), g = l / 16:

@@ -13,10 +13,10 @@
 // over many keys take the keys in pieces, merged by a second kernel.
 //
 // Bound by the matrix instructions and the exponentials between them, which two waves of a SIMD (three at dim 64) overlap:
-// 16384 tokens, 12 heads of 4, dim 128: 787 to 824 us, 1000 to 1050 TFLOP/s, where a large bf16 product reaches 1228.  Two
+// 16384 tokens, 12 heads of 4, dim 128: 787 to 845 us by box, 980 to 1050 TFLOP/s, where a large bf16 product reaches 1228.  Two
 // row groups to a wave read a key for twice the rows but leave one wave to a SIMD, and went through accumulation registers:
 // 1494 us.  Short sequences are bound by what comes around the loop (offsets, queries, first tile, output: some 10 us of a
-// workgroup that its neighbour on the CU covers in part): 16 of up to 2048, 120 to 125 us, 730 TFLOP/s.
+// workgroup that its neighbour on the CU covers in part): 16 of up to 2048, 120 to 126 us, 710 to 740 TFLOP/s.
 //
 // Matrix layout (v_mfma_f32_32x32x16: A lane l holds A[l % 32][8 (l / 32) + j], B lane l holds B[8 (l / 32) + j][l % 32],
 // D lane l register v holds D[8 (v / 4) + 4 (l / 32) + v % 4][l % 32]), h = l / 32:
