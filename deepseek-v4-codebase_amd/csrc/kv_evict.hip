@@ -209,6 +209,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   // in slot order: of the keys that share the threshold's bits the first `need` stay; holes and movers by their ranks
   uint64_t ties = 0, moved = 0;  // of the rounds before; holes low, movers high
   int2* const mv = ROW ? s_moves : a.moves + bh * a.most;
+  const uint32_t room = ROW ? kOwnMoves : static_cast<uint32_t>(a.most);
   const uint64_t below = (1ull << lane) - 1;
   for (int base = 0; base < n; base += kRound) {
     if (!one_round) load_round(base);
@@ -245,12 +246,15 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       const int i = run + 64 * r + lane;
       const bool h = (hole >> r) & 1u, m = (mover >> r) & 1u;
       const uint64_t hm = __builtin_amdgcn_ballot_w64(h), mm = __builtin_amdgcn_ballot_w64(m);
-      if (h) mv[(at & 0xffffffffu) + __popcll(hm & below)].y = i;
-      if (m) mv[(at >> 32) + __popcll(mm & below)].x = i;
+      const uint32_t to = static_cast<uint32_t>(at) + __popcll(hm & below), from = static_cast<uint32_t>(at >> 32) + __popcll(mm & below);
+      if (h && to < room) mv[to].y = i;
+      if (m && from < room) mv[from].x = i;
       at += __popcll(hm) + (static_cast<uint64_t>(__popcll(mm)) << 32);
     }
   }
-  const int count = static_cast<int>(moved & 0xffffffffu);  // (as many movers: keep slots stay)
+  // as many holes as movers, `room` at most: keep slots stay.  (Weights that another stream changes meanwhile, which a long
+  // row reads again for every pass, break that; no move may then go anywhere else.)
+  const int count = static_cast<int>(min(min(static_cast<uint32_t>(moved), static_cast<uint32_t>(moved >> 32)), room));
   if constexpr (ROW == 0) {
     if (tid == 0) a.counts[bh] = count;
   } else {
