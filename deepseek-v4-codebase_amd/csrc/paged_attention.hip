@@ -1,7 +1,7 @@
 // Attention of a sequence's newest tokens over its paged per-head cache in TurboQuant codes.
 //
 // Token t (of T, the last T slots of each sequence) of query head h sees slots j < lengths[b] - T + 1 + t of KV head
-// h / (H / heads):  l_j = scale q . K_j,  p_j = exp(l_j) / (sum exp(l) + exp(sink_h)),  out = sum_j p_j V_j.
+// h / (H / heads), as far as the table, or the tracker, reaches:  l_j = scale q . K_j,  p_j = exp(l_j) / (sum exp(l) + exp(sink_h)),  out = sum_j p_j V_j.
 // With the codec's orthogonal rotation R = c Had diag (K_j = s_j R^T codes_j) both products stay in the rotated domain:
 //   q . K_j = s_j (R q) . codes_j        sum_j p_j V_j = R^T sum_j p_j s_j codes_j
 // so a query is rotated once, an output is rotated back once, and a cached row costs its codes and one scale: the kernel
@@ -75,6 +75,11 @@ struct PagedArgs {
 
 // Slots of sequence b that its last token sees.
 __device__ __forceinline__ int32_t newest_sees(const PagedArgs& a, int64_t b) { return max(min(a.lengths[b], a.reach), 0); }
+// Of its n such slots those that token `tok` of the T newest sees.  The causal bound counts back from the given length, which
+// may lie past what can be reached; that is cut off afterwards.
+__device__ __forceinline__ int32_t token_sees(const PagedArgs& a, int32_t length, int32_t n, int32_t tok) {
+  return min(max(length - (a.T - 1 - tok), 0), n);  // (length >= 0: nothing overflows)
+}
 // The sequence that comes r-th when the longest come first, by eighths of a power of two, equal ones by their index; *n: its
 // slots.  The r-th largest key bit by bit, then its holder; a lane holds a sequence of each CH.
 template <int CH>
@@ -452,6 +457,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   else if (a.ranked == 2) b = ranked_sequence<8>(a, static_cast<int32_t>(b), lane, &n);
   if (a.n_split == 1) pages = load_pages(a, b, kStep * wave, lane);  // (of a whole sequence: not after its length)
   if (!a.ranked) n = newest_sees(a, b);
+  const int32_t length = max(a.lengths[b], 0);
   const int32_t piece = piece_slots(n, a.n_split);
   const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
   if (split > 0 && p0 >= p1) return;  // (the merge knows how many pieces a sequence has)
@@ -488,13 +494,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedArgs 
   for (int t = 0; t < MT; ++t) {
     const bool in = row[t] < a.rows;
     query_parts<DT, D, BITS>(a, qw[t], in, lane, qhi[t], qlo[t], &factor[t]);
-    sees[t] = in ? max(n - a.T + 1 + row[t] / a.G, 0) : n;
+    sees[t] = in ? token_sees(a, length, n, row[t] / a.G) : n;
     m[t] = kNegInf, l[t] = 0.0f;
 #pragma unroll
     for (int e = 0; e < G::kNE; ++e) o[t][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     ones_sum[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  const int32_t sees_all = max(n - a.T + 1 + rb * MT * 16 / a.G, 0);  // the fewest that a row of the block sees
+  const int32_t sees_all = token_sees(a, length, n, rb * MT * 16 / a.G);  // the fewest that a row of the block sees
 
   // a landed step; `whole`: every row sees all of it
   auto body = [&](const StepData<D, BITS>& s, int32_t base, uint32_t none, auto whole_c) __attribute__((always_inline)) {
@@ -874,7 +880,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
   wg /= a.n_split;
   const int32_t kh = static_cast<int32_t>(wg % a.pool.heads);
   const int64_t b = wg / a.pool.heads;
-  const int32_t n = newest_sees(a, b);
+  const int32_t n = newest_sees(a, b), length = max(a.lengths[b], 0);
   const int32_t piece = piece_slots(n, a.n_split);
   const int32_t p0 = split * static_cast<int64_t>(piece) < n ? split * piece : n, p1 = min(static_cast<int64_t>(p0) + piece, static_cast<int64_t>(n));
   if (p0 >= p1) return;  // (the whole workgroup)
@@ -899,7 +905,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedArgs a) {
         const int32_t tok = in ? row / a.G : 0, h = in ? kh * a.G + (row - tok * a.G) : 0;
         s_f[t][lane] = factor;
         s_lse[t][lane] = a.lse[(b * a.T + tok) * a.H + h];
-        s_sees[t][lane] = in ? max(n - a.T + 1 + tok, 0) : 0;
+        s_sees[t][lane] = in ? token_sees(a, length, n, tok) : 0;
       }
     }
     __syncthreads();

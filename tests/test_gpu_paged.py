@@ -741,3 +741,40 @@ def test_long_tracked_attention_in_two_graphs_and_streams(dev, T):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i], want[i]) and torch.equal(trackers[i].weights, weights[i]), f"graph {i}, replay {rep}"
+
+
+# ---- bounds of sequences and trackers ----------------------------------------------------------------------------
+
+def _ref_by_token(cache, table, q, lengths, scale, sink, capacity):
+    """The plain form one token at a time: token t of T is the newest one of a sequence of lengths - T + 1 + t slots, of which
+    those past the table, or the tracker, are cut off."""
+    B, T, H, _ = q.shape
+    parts = [R.paged_attention_ref(R.HostCache(cache, table), q[:, t:t + 1].cpu(), [n - T + 1 + t for n in lengths], scale,
+                                   None if sink is None else sink.cpu(), capacity) for t in range(T)]
+    out, bound, w, wb = zip(*parts)
+    # (the tokens' weights add up in fp32: T additions)
+    return torch.cat(out, 1), torch.cat(bound, 1), sum(w), sum(wb) + 2.0 ** -23 * T * sum(w)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 64), (8, 128)])
+@pytest.mark.parametrize("T,group", [(4, 2), (9, 2), (3, 7)])
+@pytest.mark.parametrize("lengths,slots,capacity", [([90, 72, 71, 70, 40], 96, 70), ([5000, 97, 99, 96, 3], 96, None), ([5000, 98, 96, 2, 0], 96, 96),
+                                                    ([2 ** 31 - 1, 1283, 1290, -(2 ** 31)], 1280, None), ([1282, 1279, 1300], 1280, 1276)])
+def test_attention_causal_bound_of_lengths_past_the_end(dev, bits, dim, T, group, lengths, slots, capacity):
+    """The causal bound counts back from the given length; what lies past the table or the tracker is cut off afterwards, so
+    that earlier tokens of a sequence that is longer than both see all that is there."""
+    heads, page, B = 2, 16, len(lengths)
+    cache, table, _ = _cache(dev, 100 + T, bits, dim, heads, page, [slots] * B)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    q = torch.randn(B, T, heads * group, dim, device=dev, generator=_gen(dev, 101)).to(torch.bfloat16)
+    sink = torch.randn(heads * group, device=dev, generator=_gen(dev, 102))
+    tracker = None
+    if capacity is not None:
+        tracker = SlotTracker(B, heads, capacity, device=dev)
+        tracker.weights.uniform_(0, 3, generator=_gen(dev, 103))
+        before = tracker.weights.double().cpu()
+    got = paged_attention(q, cache, table, n, dim ** -0.5, sink=sink, tracker=tracker)
+    want, bound, w, wb = _ref_by_token(cache, table, q, lengths, dim ** -0.5, sink, capacity)
+    R.within(got, want, bound, "out")
+    if tracker is not None:
+        R.within(tracker.weights, before + w, wb + 2.0 ** -23 * (before + w), "weights")
