@@ -359,3 +359,51 @@ def test_prompt_tiles_that_about_fill_the_chip(dev, dtype, dim, H, hk, lq, lk):
             keys = slice(ck[b], ck[b] + see)
             want, bound, _, _ = R.prompt_attention_ref(q[r:r + 1].cpu(), k[keys].cpu(), v[keys].cpu(), [0, 1], [0, see], dim ** -0.5)
             R.within(out[r:r + 1], want, bound, f"sequence {b}, query {i}")
+
+
+def _all_rows(q, k, v, lq, lk, scale, lift=0.0):
+    """Every row's output in 64 bits, on the device, and its bound: u |out| + (u + 2 delta + (n + 16) 2^-24) sum p |v|, u of
+    the type (the output's rounding, and each weight's), delta a logit's error, and `lift` times sum |v|, for weights below
+    the type's normal numbers."""
+    H, hk, D, u = q.size(1), k.size(1), q.size(2), R.U[q.dtype]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    bound = torch.full_like(out, R.TINY[q.dtype])
+    cq, ck = _cu(lq), _cu(lk)
+    for b in range(len(lq)):
+        hidden = torch.arange(lk[b], device=q.device) > torch.arange(lq[b], device=q.device)[:, None] + lk[b] - lq[b]
+        none = hidden.all(-1)
+        for h in range(H):
+            qq, kk, vv = q[cq[b]:cq[b + 1], h].double(), k[ck[b]:ck[b + 1], h // (H // hk)].double(), v[ck[b]:ck[b + 1], h // (H // hk)].double()
+            if none.all():
+                continue
+            x = (qq @ kk.t() * scale).masked_fill_(hidden, -math.inf)
+            p = torch.softmax(x, -1).masked_fill_(none[:, None], 0.0)
+            o = p @ vv
+            size = abs(scale) * (qq.abs() @ kk.abs().t()) * (D + 8) * 2.0 ** -24 + x.abs() * 2.0 ** -21
+            delta = size.masked_fill_(hidden, 0.0).amax(-1, keepdim=True)
+            n = (~hidden).sum(-1, keepdim=True)
+            out[cq[b]:cq[b + 1], h] = o
+            bound[cq[b]:cq[b + 1], h] += u * o.abs() + (u + 2 * delta + (n + 16) * 2.0 ** -24) * (p @ vv.abs()) + lift * ((~hidden).double() @ vv.abs())
+    return out, bound
+
+
+@pytest.mark.parametrize("dim,H,hk,lq,lk", [(64, 2, 1, [40], [16384]), (64, 48, 48, [1024], [16384]), (128, 8, 4, [3000, 64], [17000, 16384]), (64, 2, 2, [17000], [17000]),
+                                            (128, 2, 1, [3, 5, 8], [20000, 33000, 16384])])
+def test_prompt_small_weights_under_one_dominant_key(dev, dim, H, hk, lq, lk):
+    """A first key that takes nearly all of the weight and holds no value: the output is made of the small weights alone, which
+    have to keep their bits although they are far below the largest."""
+    dtype, gap = torch.float16, 17.0
+    q, k, v = (x.clone() for x in _inputs(dev, 40, dtype, dim, H, hk, lq, lk))
+    q *= 0.3
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    v += 1.0
+    for c in _cu(lk)[:-1]:
+        k[c], v[c] = 0.0, 0.0
+        k[c, :, 0] = gap * dim ** 0.5 / 8.0
+    cu = lambda x: torch.tensor(_cu(x), dtype=torch.int32, device=dev)  # noqa: E731
+    out = prompt_attention(q, k, v, cu(lq), dim ** -0.5, cu_seqlens_k=cu(lk))
+    # a weight is held as 2^7 and up times exp2(its distance to the reference), the largest at 2^7 at least: one that is no
+    # normal fp16 number is off by half of 2^-24, 2^-32 of the sum of weights
+    want, bound = _all_rows(q, k, v, lq, lk, dim ** -0.5, lift=2.0 ** -32)
+    R.within(out, want.cpu(), bound.cpu(), "out")
