@@ -38,6 +38,7 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMargin = 8.0f;        // log2 units
+constexpr float kFar = 0x1p22f;        // log2 units: below, a logit is rounded by a quarter at most
 constexpr int kTile = 64;              // keys of a tile
 constexpr int kPieceTiles = 8;         // least tiles of a piece of the keys
 constexpr int kBufWord3 = 0x00020000;  // buffer resource word 3: raw 32-bit data, range-checked
@@ -367,13 +368,23 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
       for (int mb = 0; mb < kMB; ++mb) O[mb] *= r;
       m = moved ? to : m;
     }
-    const float nm = m == kNegInf ? 0.0f : -m;
+    float nm = m == kNegInf ? 0.0f : -m, by = a.scale2;
+    // beyond kFar the reference, which is a rounded logit, may lie further from the exact product than the exponentials reach:
+    // there a row's logits are all rounded as the reference was
+    const bool far = fabsf(m) > kFar && m > kNegInf;
+    if (__builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kb][v] = far ? s[kb][v] * a.scale2 + nm : s[kb][v];
+      by = far ? 1.0f : by, nm = far ? 0.0f : nm;
+    }
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb) {
       float p[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        p[v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], a.scale2, nm));
+        p[v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], by, nm));
         l += p[v];
       }
       v8 pb[2];

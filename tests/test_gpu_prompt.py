@@ -407,3 +407,44 @@ def test_prompt_small_weights_under_one_dominant_key(dev, dim, H, hk, lq, lk):
     # normal fp16 number is off by half of 2^-24, 2^-32 of the sum of weights
     want, bound = _all_rows(q, k, v, lq, lk, dim ** -0.5, lift=2.0 ** -32)
     R.within(out, want.cpu(), bound.cpu(), "out")
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 300.0), (torch.float16, 20000.0), (torch.bfloat16, 2.0 ** 14), (torch.bfloat16, 2.0 ** 40)])
+@pytest.mark.parametrize("dim,H,hk,lq,lk", [(64, 4, 2, [150], [150]), (128, 2, 2, [20], [1500]), (128, 32, 16, [2100], [2100])])
+def test_prompt_logits_far_from_zero(dev, dtype, size, dim, H, hk, lq, lk):
+    """Logits so large that neighbouring fp32 numbers lie further apart than the exponentials reach: equal keys share the weight
+    and a larger one takes it all, as where every logit is rounded to fp32 before the largest is subtracted."""
+    q, k, v = (x.clone() for x in _inputs(dev, 41, dtype, dim, H, hk, lq, lk))
+    q.fill_(size)
+    k.fill_(size)
+    first = lk[0] - lq[0] + 10  # the key that counts: the first ten queries do not see it
+    k[first] = size * 1.25
+    cu = lambda x: torch.tensor(_cu(x), dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = prompt_attention(q, k, v, cu(lq), dim ** -0.5, cu_seqlens_k=cu(lk), return_lse=True)
+    vv = v.double().repeat_interleave(H // hk, 1)
+    n = torch.arange(lk[0] - lq[0] + 1, first + 1, device=dev)[:, None, None]
+    want = vv[first].expand(lq[0], H, dim).clone()
+    want[:10] = vv.cumsum(0)[n[:, 0, 0] - 1] / n
+    weight = want.abs()
+    weight[:10] = vv.abs().cumsum(0)[n[:, 0, 0] - 1] / n
+    # equal weights are rounded alike: the output's rounding, and the sums'
+    u = R.U[dtype]
+    R.within(out, want.cpu(), (u * want.abs() + (2 * u + (lk[0] + 16) * 2.0 ** -24) * weight + R.TINY[dtype]).cpu(), "out")
+    top = torch.where(torch.arange(lq[0]) < 10, float(q[0, 0, 0]), float(k[first, 0, 0])).double() * size * dim ** 0.5
+    count = torch.where(torch.arange(lq[0]) < 10, torch.arange(lq[0]) + lk[0] - lq[0] + 1, 1).double().log()
+    # the product's sum, the scale in log2 units, and back: (dim + 8) roundings of the size of the logit
+    R.within(lse.double().cpu(), (top + count)[:, None].expand(lq[0], H), ((dim + 8) * 2.0 ** -24 * top + 2.0 ** -20 * (1 + count))[:, None].expand(lq[0], H), "lse")
+
+
+@pytest.mark.parametrize("lens", [[100], [4000]])
+def test_prompt_far_row_leaves_its_neighbours_bits(dev, lens):
+    q, k, v = (x.clone() for x in _inputs(dev, 44, torch.bfloat16, 128, 16, 8, lens, lens))
+    cu = torch.tensor(_cu(lens), dtype=torch.int32, device=dev)
+    clean = prompt_attention(q, k, v, cu, 0.09)
+    q[70, 3] *= 2.0 ** 40
+    got = prompt_attention(q, k, v, cu, 0.09)
+    # the far row: the value of its largest logit
+    top = (q[70, 3].double() @ k[:71, 1].double().t()).argmax()
+    assert torch.equal(got[70, 3], v[top, 1])
+    got[70, 3] = clean[70, 3]
+    assert torch.equal(got, clean)
