@@ -840,7 +840,7 @@ __device__ __forceinline__ void add_weights(const PagedArgs& a, uint32_t block, 
   for (int32_t i = 0; i < a.rows; ++i) {
     const f32x4_t x = *reinterpret_cast<const f32x4_t*>(lg + i * a.logit_slots);  // (the step's 32 slots are all there)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(x[e] - s_lse[i]);
+    for (int e = 0; e < 4; ++e) sum[e] += x[e] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(x[e] - s_lse[i]);  // (hidden: nothing, whatever the row's sum is)
   }
   if (vec) {
     *reinterpret_cast<f32x4_t*>(w) = before + sum;

@@ -778,3 +778,24 @@ def test_attention_causal_bound_of_lengths_past_the_end(dev, bits, dim, T, group
     R.within(got, want, bound, "out")
     if tracker is not None:
         R.within(tracker.weights, before + w, wb + 2.0 ** -23 * (before + w), "weights")
+
+
+@pytest.mark.parametrize("T,group", [(2, 2), (3, 5), (9, 2), (12, 3)])
+@pytest.mark.parametrize("length", [60, 1290])
+def test_attention_nan_row_leaves_the_weights_of_slots_it_does_not_see(dev, T, group, length):
+    """A query that holds NaN adds NaN to the slots that it sees, and nothing to a missing page's or to later tokens' slots."""
+    heads, dim, page = 2, 64, 16
+    cache, table, n = _cache(dev, 110, 4, dim, heads, page, [length, length])
+    table[0, 1] = -1
+    q = torch.randn(2, T, heads * group, dim, device=dev, generator=_gen(dev, 111)).to(torch.bfloat16)
+    clean, got = (SlotTracker(2, heads, table.size(1) * page, device=dev) for _ in range(2))
+    for t in (clean, got):
+        t.weights.uniform_(0, 3, generator=_gen(dev, 112))
+    paged_attention(q, cache, table, n, 0.125, tracker=clean)
+    q[0, 0, 1] = NAN  # the first token, KV head 0: it does not see the last T - 1 slots
+    paged_attention(q, cache, table, n, 0.125, tracker=got)
+    sees = torch.zeros(2, heads, clean.capacity, dtype=torch.bool, device=dev)
+    sees[0, 0, :length - T + 1] = True
+    sees[0, 0, page:2 * page] = False
+    assert got.weights[sees].isnan().all()
+    assert torch.equal(got.weights[~sees], clean.weights[~sees])
