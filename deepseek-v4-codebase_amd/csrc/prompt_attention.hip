@@ -70,7 +70,9 @@ struct PromptArgs {
                         // every level)
   uint32_t fold;        // tiles of the launch's second round of workgroups, which are taken from its end; 0: none
   float scale2;         // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
-  int32_t flip;         // scale is negative the queries' signs are flipped: a row's largest product is its largest logit
+  int32_t flip;         // scale is negative the queries' signs are flipped: a row's largest product is its largest logit.  Where
+  uint32_t nan;         // it is NaN, 1 stands for it and the queries become NaN (0x7fff is one in both types; else 0): only
+                        // what a row sees meets them
 };
 
 template <int DT>
@@ -278,6 +280,7 @@ __global__ __launch_bounds__(64 * WR * KS) __attribute__((amdgpu_waves_per_eu(D 
   for (int ks = 0; ks < kKSteps; ++ks) {
     uint4 w = *reinterpret_cast<const uint4*>(qp + 16 * ks);
     if (a.flip) w.x ^= 0x80008000u, w.y ^= 0x80008000u, w.z ^= 0x80008000u, w.w ^= 0x80008000u;
+    if (a.nan) w.x |= a.nan, w.y |= a.nan, w.z |= a.nan, w.w |= a.nan;
     qb[ks] = __builtin_bit_cast(v8, w);
   }
   const int32_t wave_least = __builtin_amdgcn_readfirstlane(sees_of(w0 < n_rows ? w0 : n_rows - 1));
@@ -712,12 +715,13 @@ extern "C" int aekv_prompt_attention(const void* q, const void* k, const void* v
   // Tiles come with the most keys first; the second workgroup of each CU is taken from the short end of its round, so that the
   // pairs have like work (one prompt of 11000, 12 heads of 4: 400 -> 381 us; 8192, 16 heads of 16: 300 -> 288; else 0 to 3 %).
   const uint32_t fold = static_cast<uint32_t>(plan.tiles * heads >= 512 ? 256 / heads : 0);
+  const bool none = softmax_scale != softmax_scale;
   PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), q_token_stride,
                q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q, cu_seqlens_k, sink,
                static_cast<uint16_t*>(out), lse, static_cast<float*>(ws), static_cast<int32_t>(plan.split), static_cast<int32_t>(plan.tiles),
                static_cast<int32_t>(n_q), static_cast<int32_t>(n_k), static_cast<int32_t>(B), static_cast<int32_t>(H),
                static_cast<int32_t>(heads), static_cast<int32_t>(H / heads), clear_rest,
-               by_work, fold, fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f};
+               by_work, fold, none ? 1.0f : fmaxf(fabsf(softmax_scale) * kLog2e, 0x1p-126f), softmax_scale < 0.0f, none ? 0x7fff7fffu : 0u};
   const hipStream_t st = as_stream(stream);
   auto fn = plan.rows == 128 ? pick_prompt<4, 1>(dtype, d) : pick_prompt<2, 2>(dtype, d);
   hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(plan.tiles * heads * plan.split)), dim3(256), 0, st, a);

@@ -448,3 +448,15 @@ def test_prompt_far_row_leaves_its_neighbours_bits(dev, lens):
     assert torch.equal(got[70, 3], v[top, 1])
     got[70, 3] = clean[70, 3]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,H,hk,lq,lk", [(64, 4, 2, [40, 7, 90], [20, 0, 200]), (128, 2, 1, [30], [2000]), (128, 32, 16, [2100], [2000])])
+def test_prompt_scale_that_is_no_number(dev, dtype, dim, H, hk, lq, lk):
+    """A NaN scale gives NaN to every row that sees a key, as any other NaN would, and 0 to one that sees nothing."""
+    q, k, v = _inputs(dev, 42, dtype, dim, H, hk, lq, lk)
+    cu = lambda x: torch.tensor(_cu(x), dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = prompt_attention(q, k, v, cu(lq), NAN, cu_seqlens_k=cu(lk), return_lse=True)
+    none = torch.cat([torch.arange(a) + b - a < 0 for a, b in zip(lq, lk)]).to(dev)
+    assert out[~none].isnan().all() and lse[~none].isnan().all()
+    assert not out[none].any() and (lse[none] == -math.inf).all()
