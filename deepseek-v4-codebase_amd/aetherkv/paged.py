@@ -249,6 +249,8 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
 def paged_attention_workspace(B: int, T: int, H: int, kv_heads: int, dim: int, slots: int, device, *,
                               tracked: bool = False) -> torch.Tensor:
     """Workspace of paged_attention; slots = page_table.size(1) * page_size."""
+    if H < 1 or kv_heads < 1 or H % kv_heads:
+        raise RuntimeError(f"{H} query heads are no multiple of {kv_heads} KV heads")
     n = _lib.paged_ws_bytes(int(B), int(T), int(H), int(kv_heads), int(dim), int(slots), int(tracked))
     return torch.empty(n, dtype=torch.uint8, device=device)
 

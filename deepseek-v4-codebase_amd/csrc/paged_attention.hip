@@ -1007,6 +1007,13 @@ int64_t paged_pieces(int64_t groups, int64_t slots) {
 // 1024 47.3 / 35.8, in pieces of 682 slots (16 of up to 16384) 34.3 / 36.7.
 constexpr int64_t kRanked = 512, kRankedSlots = 2048;
 
+// Whether a call of these sizes (a multiple of the KV heads' query heads) fits a launch.
+bool paged_fits(int64_t B, int64_t T, int64_t H, int64_t heads, int64_t blocks) {
+  return B <= 0x7fffffff && H <= 65535 && T <= 0x7fffff && T * (H / heads) <= 0x3fffffff &&
+         static_cast<double>(B) * static_cast<double>(heads * blocks) <= kMaxGridThreads / kThreads / 4 &&
+         static_cast<double>(B) * static_cast<double>(T * H) <= kMaxGridThreads / kThreads;
+}
+
 // Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.
 int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 : 1; }
 
@@ -1025,8 +1032,9 @@ using namespace aekv;
 
 extern "C" size_t aekv_paged_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t heads, int32_t d,
                                                       int64_t slots, int32_t tracked) {
-  if (B <= 0 || T <= 0 || H <= 0 || heads <= 0 || d <= 0 || slots <= 0) return 0;
+  if (B <= 0 || T <= 0 || H <= 0 || heads <= 0 || d <= 0 || slots <= 0 || H % heads || T > 0x7fffff || H > 65535) return 0;
   const int64_t rows = T * (H / heads), blocks = ceil_div(rows, 16 * paged_row_tiles(rows, d));
+  if (!paged_fits(B, T, H, heads, blocks)) return 0;  // (the call refuses it)
   const int64_t n = paged_pieces(B * heads * blocks, slots);
   return (tracked ? align_up(static_cast<size_t>(B * T * H) * 4, 16) + paged_logit_bytes(B, heads, rows, slots) : 0) +
          (n > 1 ? static_cast<size_t>(B * T * H) * static_cast<size_t>(n) * (d + 4) * 4 : 0);
@@ -1055,10 +1063,10 @@ extern "C" int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batc
   if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(ws, 16) || !is_aligned(diag, 16) || !is_aligned(weights, 16) || (q_batch_stride % 8) ||
       (q_token_stride % 8) || (q_head_stride % 8))
     return fail(AEKV_ERR_ALIGN, "%s: q rows, out, diag, weights and workspace must be 16-byte aligned", who);
-  const int64_t slots = max_pages * page_size, rows = T * (H / heads);
+  const int64_t slots = max_pages * page_size, rows = H <= 65535 && T <= 0x7fffff ? T * (H / heads) : 1;
   const int mt = paged_row_tiles(rows, d);
   const int64_t blocks = ceil_div(rows, 16 * mt);
-  if (H > 65535 || T > 0x7fffff || rows > 0x3fffffff || B * heads * blocks > kMaxGridThreads / kThreads / 4 || B * T * H > kMaxGridThreads / kThreads)
+  if (!paged_fits(B, T, H, heads, blocks))
     return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld T=%lld H=%lld exceed the grid", who, (long long)B, (long long)T, (long long)H);
   const size_t want = aekv_paged_attention_workspace_size(B, T, H, heads, d, slots, weights != nullptr);
   if (want && (!ws || ws_bytes < want)) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);

@@ -666,7 +666,8 @@ using namespace aekv;
 
 extern "C" size_t aekv_prompt_attention_workspace_size(int64_t B, int64_t n_q, int64_t n_k, int64_t H, int64_t heads,
                                                        int32_t d) {
-  if (B <= 0 || n_q <= 0 || n_k <= 0 || H <= 0 || heads <= 0 || d <= 0) return 0;
+  if (B <= 0 || n_q <= 0 || n_k <= 0 || H <= 0 || heads <= 0 || d <= 0 || H % heads) return 0;
+  if (n_q > 0x7fffffff || n_k > 0x7fffffff || B > 0x7ffffffe || H > 65535 || n_q * H > 0x7fff0000) return 0;  // (the call refuses it)
   const PromptPlan p = plan_prompt(B, n_q, n_k, H, heads, d);
   return p.split > 1 ? static_cast<size_t>(n_q * H) * static_cast<size_t>(p.split) * (d + 4) * 4 : 0;
 }

@@ -3,8 +3,10 @@ and where slots lie (bad pages among them), checked on the CPU."""
 from __future__ import annotations
 
 import ctypes
+import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -199,3 +201,26 @@ def test_caches_and_trackers_are_on_a_device():
         PagedKVCache(PolarQuant(4), 4, 2, 128, page_size=16, device="cpu")
     with pytest.raises(RuntimeError, match="device"):
         SlotTracker(1, 2, 64, device="cpu")
+
+
+def test_workspace_sizes_of_refused_arguments():
+    """Sizes are asked for before the call that refuses: whatever the arguments, an answer comes back (in a process of its own,
+    as a division by zero would end it), and the Python calls raise."""
+    from aetherkv.paged import paged_attention_workspace
+
+    code = ("import itertools, random\nimport aetherkv._lib as L\nlib = L.lib()\n"
+            "assert lib.aekv_paged_attention_workspace_size(1, 1, 2, 4, 128, 4096, 0) == 0\n"
+            "assert lib.aekv_paged_attention_workspace_size(1, 1, 6, 4, 128, 4096, 1) == 0\n"
+            "v = (-1, 0, 1, 2, 3, 7, 64, 65536, 2 ** 31, 2 ** 40)\nr = random.Random(0)\n"
+            "for _ in range(20000):\n"
+            "    a = [r.choice(v) for _ in range(6)]\n"
+            "    d = r.choice((-1, 0, 64, 96, 128))\n"
+            "    lib.aekv_paged_attention_workspace_size(*a[:4], d, a[4], r.randint(0, 1))\n"
+            "    lib.aekv_kv_evict_workspace_size(*a[:4])\n"
+            "    lib.aekv_prompt_attention_workspace_size(*a[:5], d)\n"
+            "print('done')\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": str(PKG_DIR)})
+    assert done.returncode == 0 and done.stdout.endswith("done\n"), (done.returncode, done.stderr[-500:])
+    for H, heads in ((2, 4), (6, 4), (0, 2), (4, 0)):
+        with pytest.raises(RuntimeError, match="multiple"):
+            paged_attention_workspace(1, 1, H, heads, 128, 4096, "cpu")
