@@ -92,10 +92,21 @@ class PagedKVCache:
         return self
 
     def decode(self, page_table: torch.Tensor, length: int, out_dtype: torch.dtype = torch.bfloat16):
-        """(K, V) [kv_heads, length, dim] of one sequence's first slots, decoded (page_table [max_pages])."""
-        slots = torch.arange(int(length), device=self.device)
-        page, row = page_table.long()[slots // self.page_size], slots % self.page_size
-        return tuple(self.quant.decode(c[page, :, row], s[page, :, row].unsqueeze(-1), out_dtype).transpose(0, 1)
+        """(K, V) [kv_heads, length, dim] of one sequence's first slots, decoded (page_table [max_pages]); 0 for the slots of
+        a page outside the pool."""
+        _one_device(self._index, page_table)
+        if page_table.dim() != 1 or page_table.is_floating_point():
+            raise RuntimeError(f"page_table must be int32 [max_pages], got {page_table.dtype} {tuple(page_table.shape)}")
+        length, slots = int(length), page_table.size(0) * self.page_size
+        if not 0 <= length <= slots:
+            raise RuntimeError(f"decode of {length} slots: page_table has {slots} slots")
+        if not self.pages:
+            return tuple(torch.zeros((self.kv_heads, length, self.dim), dtype=out_dtype, device=self.device) for _ in range(2))
+        slot = torch.arange(length, device=self.device)
+        page, row = page_table.long()[slot // self.page_size], slot % self.page_size
+        none = (page < 0) | (page >= self.pages)
+        page = page.masked_fill(none, 0)
+        return tuple(self.quant.decode(c[page, :, row], s[page, :, row].masked_fill(none[:, None], 0.0).unsqueeze(-1), out_dtype).transpose(0, 1)
                      for c, s in ((self.k_codes, self.k_scale), (self.v_codes, self.v_scale)))
 
 

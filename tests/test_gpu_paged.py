@@ -799,3 +799,24 @@ def test_attention_nan_row_leaves_the_weights_of_slots_it_does_not_see(dev, T, g
     sees[0, 0, page:2 * page] = False
     assert got.weights[sees].isnan().all()
     assert torch.equal(got.weights[~sees], clean.weights[~sees])
+
+
+def test_decode_of_missing_pages_and_past_the_table(dev):
+    """PagedKVCache.decode gives 0 for the slots of a page that a table does not have, and refuses what lies past the table."""
+    cache, table, _ = _cache(dev, 120, 4, 64, 2, 16, [60])
+    want = cache.decode(table[0], 60, torch.float32)
+    row = table[0].clone()
+    row[1] = -1
+    row[3] = cache.pages
+    for got, w in zip(cache.decode(row, 60, torch.float32), want):
+        assert not got[:, 16:32].any() and torch.equal(got[:, :16], w[:, :16]) and torch.equal(got[:, 32:48], w[:, 32:48])
+        assert not got[:, 48:].any()
+    assert all(x.shape == (2, 64, 64) for x in cache.decode(table[0], 64))
+    assert all(x.shape == (2, 0, 64) for x in cache.decode(table[0], 0))
+    for length in (65, 1000, -1):
+        with pytest.raises(RuntimeError, match="slots"):
+            cache.decode(table[0], length)
+    with pytest.raises(RuntimeError, match="page_table"):
+        cache.decode(table, 60)
+    empty = PagedKVCache.from_tensors(cache.quant, cache.k_codes[:0], cache.k_scale[:0], cache.v_codes[:0], cache.v_scale[:0])
+    assert all(x.shape == (2, 20, 64) and not x.any() for x in empty.decode(table[0], 20))
