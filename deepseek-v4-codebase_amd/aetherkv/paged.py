@@ -46,6 +46,7 @@ class PagedKVCache:
                    torch.zeros(rows, dtype=torch.float32, device=dev) for i in range(4)]
         _lib.require_device("PagedKVCache", *tensors)  # (the calls compare their tensors' device with the cache's)
         self._set(quant, *tensors)
+        self._diag = quant._diag(self.dim, self.device)  # (here: a first call may be captured, which a copy from the host may not)
 
     def _set(self, quant, k_codes, k_scale, v_codes, v_scale) -> None:
         self.quant, self.bits = quant, quant.bits
@@ -54,17 +55,11 @@ class PagedKVCache:
         self.pages, self.kv_heads, self.page_size = k_scale.shape
         self.dim = k_codes.size(3) * (1 if quant.bits == 8 else 2)
         self.device, self._index = k_codes.device, k_codes.get_device()
-        self._diag: Optional[torch.Tensor] = None
 
     k_codes = property(lambda self: self._tensors[0])
     k_scale = property(lambda self: self._tensors[1])
     v_codes = property(lambda self: self._tensors[2])
     v_scale = property(lambda self: self._tensors[3])
-
-    def _diag_ptr(self) -> int:
-        if self._diag is None:
-            self._diag = self.quant._diag(self.dim, self.device)
-        return self._diag.data_ptr()
 
     @classmethod
     def from_tensors(cls, quant: PolarQuant, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
@@ -89,6 +84,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: head dim must be 64 or 128, got {self.dim}")
         if self.page_size < 16 or self.page_size > 4096 or self.page_size & (self.page_size - 1):
             raise ValueError(f"PagedKVCache: page_size must be a power of two from 16 to 4096, got {self.page_size}")
+        self._diag = quant._diag(self.dim, self.device)
         return self
 
     def decode(self, page_table: torch.Tensor, length: int, out_dtype: torch.dtype = torch.bfloat16):
@@ -251,7 +247,7 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
     with _lib.on_device(dev):
         rc = _lib.hot("aekv_kv_append")(
             k.data_ptr(), v.data_ptr(), code, kt, kh, vt, vh, n, None if cu is None else cu.data_ptr(), B,
-            start.data_ptr(), cache.dim, cache.bits, cache._diag_ptr(), kc, ks, vc, vs, cache.pages, cache.kv_heads,
+            start.data_ptr(), cache.dim, cache.bits, cache._diag.data_ptr(), kc, ks, vc, vs, cache.pages, cache.kv_heads,
             cache.page_size, table.data_ptr(), table.size(1), weights, tokens, capacity, first, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "aekv_kv_append")
@@ -307,7 +303,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
         stream = _lib.raw_stream(dev)
         ws = _given(workspace) if workspace is not None else _lib.workspace(need, dev, stream) if need else None
         rc = _lib.hot("aekv_paged_attention")(
-            q.data_ptr(), _TYPES[dtype], st[0], st[1], st[2], B, T, H, D, cache.bits, cache._diag_ptr(), kc, ks, vc, vs,
+            q.data_ptr(), _TYPES[dtype], st[0], st[1], st[2], B, T, H, D, cache.bits, cache._diag.data_ptr(), kc, ks, vc, vs,
             cache.pages, heads, cache.page_size, table.data_ptr(), max_pages, lengths.data_ptr(),
             None if sk is None else sk.data_ptr(), weights, capacity, float(softmax_scale),
             None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), out.data_ptr(), stream)

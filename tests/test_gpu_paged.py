@@ -820,3 +820,36 @@ def test_decode_of_missing_pages_and_past_the_table(dev):
         cache.decode(table, 60)
     empty = PagedKVCache.from_tensors(cache.quant, cache.k_codes[:0], cache.k_scale[:0], cache.v_codes[:0], cache.v_scale[:0])
     assert all(x.shape == (2, 20, 64) and not x.any() for x in empty.decode(table[0], 20))
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_first_calls_of_a_cache_captured(dev, given):
+    """A cache whose quantiser has coded nothing yet: its first append and attention may be the captured ones."""
+    heads, dim, page = 2, 64, 16
+    k, v = (torch.randn(2, 1, heads, dim, device=dev, generator=_gen(dev, 130 + i)).to(torch.bfloat16) for i in range(2))
+    q = torch.randn(2, 1, 4, dim, device=dev, generator=_gen(dev, 132)).to(torch.bfloat16)
+    table = torch.arange(4, dtype=torch.int32, device=dev).view(2, 2)
+    zero = torch.zeros(2, dtype=torch.int32, device=dev)
+
+    def make():
+        c = PagedKVCache(PolarQuant(4, seed=7), 4, heads, dim, page_size=page, device=dev)
+        return PagedKVCache.from_tensors(PolarQuant(4, seed=7), c.k_codes, c.k_scale, c.v_codes, c.v_scale) if given else c
+
+    def step(c):
+        append_tokens(c, k, v, table, zero)
+        return paged_attention(q, c, table, zero + 1, 0.125)
+
+    eager, captured = make(), make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step(eager)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(captured)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(captured.k_codes, eager.k_codes) and torch.equal(captured.v_scale, eager.v_scale)
