@@ -108,7 +108,11 @@ class PagedKVCache:
 
 class SlotTracker:
     """Per sequence, KV head and slot of one layer: `weights` fp32, the attention weight accumulated since the slot was
-    filled, and `tokens` int32, the token index that it holds ([B, kv_heads, capacity], views of one int32 tensor)."""
+    filled, and `tokens` int32, the token index that it holds ([B, kv_heads, capacity], views of one int32 tensor).
+
+    Give it the table's slots (max_pages * page_size), or as many as its sequences ever fill: the calls with a tracker end a
+    sequence at its capacity.  What lies behind is not seen by a tracked attention, as its weight could not be counted, and
+    lost to an eviction."""
 
     def __init__(self, batch: int, kv_heads: int, capacity: int, *, device: Optional[torch.device] = None):
         if batch < 1 or kv_heads < 1 or capacity < 1:
@@ -212,7 +216,8 @@ def append_tokens(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_ta
     k, v [B, T, kv_heads, D] (T tokens of every sequence), or packed [N, kv_heads, D] with cu_seqlens int32 [B + 1]
     (sequence b's tokens are cu_seqlens[b] .. cu_seqlens[b + 1]; rows outside are skipped); bf16, fp16 or fp32, strided
     views are read in place.  The codes are PolarQuant.encode's, bit for bit.  With a tracker, the slots' weights start at
-    0 and their token indices at token[b] (int32 [B]: the sequence's tokens before this call)."""
+    0 and their token indices at token[b] (int32 [B]: the sequence's tokens before this call); slots past its capacity get
+    codes alone."""
     B = page_table.size(0)
     shape, dtype = k.shape, k.dtype
     if len(shape) != (4 if cu_seqlens is None else 3) or v.shape != shape or shape[-2] != cache.kv_heads or shape[-1] != cache.dim:
@@ -269,8 +274,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     """Attention of the newest T tokens of every sequence, its last T slots, over its slots [0, lengths[b]).
 
     q [B, T, H, D] bf16 or fp16 (strided views are read in place), H a multiple of the cache's KV heads: query head h
-    reads KV head h // (H // kv_heads).  Token t sees slots j < lengths[b] - T + 1 + t.  sink [H] (or a scalar): a logit
-    counted once in the normaliser.  A row that sees nothing gives 0.  With a tracker, weights[b, kv head, j] grows by
+    reads KV head h // (H // kv_heads).  Token t sees slots j < lengths[b] - T + 1 + t, as far as the table has them, and
+    with a tracker as far as its capacity goes.  sink [H] (or a scalar): a logit counted once in the normaliser.  A row that sees nothing gives 0.  With a tracker, weights[b, kv head, j] grows by
     the attention weight of slot j, summed over the group's heads and the T tokens.  Returns [B, T, H, D] like q."""
     shape, dtype = q.shape, q.dtype
     if len(shape) != 4 or shape[3] != cache.dim:
@@ -326,7 +331,8 @@ def evict_by_weight(cache: PagedKVCache, page_table: torch.Tensor, lengths: torc
     tracker's token indices), then the ones with the largest accumulated weight (equal ones: the lower slot; NaN above
     every number).  Kept slots below `keep` stay where they are; the evicted ones below `keep`, in order, take the kept
     slots from `keep` on, in order, with their weight and token index: cached keys carry their rotation, so attention
-    does not depend on the order of the slots.  `lengths` is only read: clamp it to `keep` once every layer is done."""
+    does not depend on the order of the slots.  A sequence ends at the tracker's capacity: slots behind it are not among
+    those that can stay.  `lengths` is only read: clamp it to `keep` once every layer is done."""
     B, max_pages = page_table.shape
     _one_device(cache._index, page_table, lengths, seen, workspace, tracker._storage)
     table, lengths, seen = _table(page_table), _counts("lengths", lengths, B), _counts("seen", seen, B)

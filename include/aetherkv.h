@@ -307,7 +307,9 @@ int aekv_tiled_prefill_attention_ws(const void* q, const void* kv, const void* s
  * p % page_size of page page_table[b, p / page_size] (int32 [B, max_pages]).  Tables, lengths and starts
  * are device data: a slot outside the table or a page outside the pool is skipped, never accessed.
  * A tracker holds, per sequence, KV head and slot, the accumulated attention weight (fp32) and the token
- * index of the slot (int32), both [B, heads, capacity]. */
+ * index of the slot (int32), both [B, heads, capacity].  With a capacity below the table's slots it ends the
+ * sequences of the calls that are given it there: slots from the capacity on are coded by an append, but a
+ * tracked attention does not see them and an eviction neither counts nor keeps them. */
 
 /* Codes the K and V vectors of n_tokens new tokens (F32/F16/BF16; rows of d contiguous elements, token and
  * head strides in elements, rows 16-byte aligned) into slots start[b], start[b] + 1, ... of their sequences:
@@ -324,7 +326,7 @@ int aekv_kv_append(const void* k, const void* v, int32_t dtype, int64_t k_token_
 
 /* Attention of the newest T tokens of each sequence (its last T slots) over the cache: q [B, T, H, d] bf16 or
  * fp16 (strides in elements), H a multiple of heads, query head h reads KV head h / (H / heads); token t sees
- * slots j < lengths[b] - T + 1 + t; l = softmax_scale q . decode(K_j), p = exp(l) / (sum exp(l) + exp(sink[h]))
+ * slots j < lengths[b] - T + 1 + t, of those that the table has (with weights: below the capacity); l = softmax_scale q . decode(K_j), p = exp(l) / (sum exp(l) + exp(sink[h]))
  * (sink fp32 [H] or NULL), out [B, T, H, d] = sum p decode(V_j), contiguous, in q's type; 0 where nothing is
  * seen.  weights (nullable): weights[b, head, j] += the sum of p_j over the head's query heads and the T
  * tokens.  Workspace: aekv_paged_attention_workspace_size(B, T, H, heads, d, max_pages * page_size,
@@ -340,8 +342,8 @@ int aekv_paged_attention(const void* q, int32_t dtype, int64_t q_batch_stride, i
                          void* stream);
 
 /* Brings every (sequence, head) with n = lengths[b] > keep slots back to `keep`, in place: kept are the highest
- * ranked slots, first those with token index < first or >= seen[b] - recent, then by weight (larger first, NaN
- * above every number), equal ranks by slot.  Kept slots below keep stay; the evicted ones below keep, in
+ * ranked of its slots below min(max_pages * page_size, capacity), first those with token index < first or
+ * >= seen[b] - recent, then by weight (larger first, NaN above every number), equal ranks by slot.  Kept slots below keep stay; the evicted ones below keep, in
  * increasing order, take the kept slots from keep on, in increasing order (codes, scales, weight, token).
  * Slots from keep on are left as they are; lengths are only read (the caller clamps them to keep once every
  * layer is done).  first + recent <= keep.  Workspace: aekv_kv_evict_workspace_size(B, heads, keep,
