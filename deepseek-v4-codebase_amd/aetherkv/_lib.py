@@ -194,7 +194,10 @@ def on_device(device: torch.device):
 # in order, so each reuses the previous call's buffer.  A call that is being captured into a graph
 # always gets a buffer of its own, from the graph's private pool: its replays keep the address, while
 # a cached buffer is replaced when a larger call comes and belongs to the eager calls of its stream.
+# A large one (a tracked call's logits can be 2 GiB) is not kept: it goes back to torch's allocator after
+# the call, for the rest of the program to use or release.
 _ws_cache: dict = {}
+WS_KEEP_BYTES = 64 << 20
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
@@ -202,13 +205,13 @@ def workspace(nbytes: int, device: torch.device, stream: int) -> Optional[torch.
     """A buffer of at least nbytes for a call on `stream`, the current stream of the current device."""
     if nbytes <= 0:
         return None
-    if _capturing():
+    if nbytes > WS_KEEP_BYTES or _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream)
     buf = _ws_cache.get(key)
     if buf is not None and buf.numel() >= nbytes:
         return buf
-    buf = torch.empty(max(nbytes, 2 * buf.numel() if buf is not None else 0), dtype=torch.uint8, device=device)
+    buf = torch.empty(max(nbytes, min(2 * buf.numel(), WS_KEEP_BYTES) if buf is not None else 0), dtype=torch.uint8, device=device)
     _ws_cache[key] = buf
     return buf
 

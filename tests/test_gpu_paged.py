@@ -853,3 +853,25 @@ def test_first_calls_of_a_cache_captured(dev, given):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(captured.k_codes, eager.k_codes) and torch.equal(captured.v_scale, eager.v_scale)
+
+
+def test_attention_large_workspace_is_given_back(dev):
+    """A tracked call over a wide table takes more workspace than is kept between calls: the same results, nothing held."""
+    cache, few, n = _cache(dev, 140, 4, 64, 2, 16, [100, 37, 0, 64])
+    wide = torch.full((4, 1 << 16), -1, dtype=torch.int32, device=dev)
+    wide[:, :few.size(1)] = few
+    q = torch.randn(4, 2, 16, 64, device=dev, generator=_gen(dev, 141)).to(torch.bfloat16)
+    size = paged_attention_workspace(4, 2, 16, 2, 64, wide.numel() // 4 * 16, "meta", tracked=True).numel()
+    assert size > 64 << 20
+    tracker = SlotTracker(4, 2, wide.size(1) * 16, device=dev)
+    paged_attention(q, cache, few, n, 0.125, tracker=SlotTracker(4, 2, few.size(1) * 16, device=dev))
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated(dev)
+    got = paged_attention(q, cache, wide, n, 0.125, tracker=tracker)
+    want, bound, w, wb = R.paged_attention_ref(R.HostCache(cache, few), q.cpu(), n.tolist(), 0.125, capacity=112)
+    R.within(got, want, bound, "out")
+    del got
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated(dev) - held < 1 << 20
+    R.within(tracker.weights[..., :112], w, wb, "weights")
+    assert not tracker.weights[..., 112:].any()

@@ -84,3 +84,17 @@ def test_sizes_follow_a_tensor_count_changed_in_place():
     small = attention_workspace(1, 12, 128, n, 0, "cpu").numel()
     n.fill_(4096)
     assert attention_workspace(1, 12, 128, n, 0, "cpu").numel() > small
+
+
+def test_large_workspaces_are_not_kept(monkeypatch):
+    monkeypatch.setattr(L, "_ws_cache", {})
+    monkeypatch.setattr(L, "_capturing", lambda: False)
+    cpu, keep = torch.device("cpu"), L.WS_KEEP_BYTES
+    small = L.workspace(keep // 4, cpu, 7)
+    big = L.workspace(keep + 1, cpu, 7)
+    assert big.numel() == keep + 1 and big.data_ptr() != small.data_ptr()
+    assert L.workspace(1000, cpu, 7) is small  # the kept one stays
+    assert L.workspace(keep * 3 // 4, cpu, 7).numel() == keep * 3 // 4
+    grown = L.workspace(keep - 16, cpu, 7)  # growing does not pass the limit
+    assert grown.numel() == keep and L.workspace(keep, cpu, 7) is grown
+    assert sum(t.numel() for t in L._ws_cache.values()) == keep
