@@ -264,10 +264,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
 }
 
 template <int ROW>
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-  const int64_t bh = blockIdx.y;
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, uint32_t per) {  // `per` workgroups to a row
+  const uint32_t row = blockIdx.x / per;
+  const int64_t bh = row;
   move_slots<ROW>(a, bh, bh / a.pool.heads, a.moves + bh * a.most, a.counts[bh],
-                  static_cast<int>(blockIdx.x * 16 + (threadIdx.x >> 4)) * kMoves, static_cast<int>(gridDim.x) * 16 * kMoves);
+                  static_cast<int>((blockIdx.x - row * per) * 16 + (threadIdx.x >> 4)) * kMoves, static_cast<int>(per) * 16 * kMoves);
 }
 
 using evict_fn = void (*)(EvictArgs);
@@ -316,7 +317,7 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   if (!is_aligned(ws, 16) || !is_aligned(weights, 4) || !is_aligned(tokens, 4))
     return fail(AEKV_ERR_ALIGN, "%s: misaligned pointer", who);
   if (pages == 0) return AEKV_OK;  // nothing is there
-  if (B * heads > 65535) return fail(AEKV_ERR_UNSUPPORTED, "%s: %lld (sequence, head) rows exceed the grid", who, (long long)(B * heads));
+  if (B * heads > kMaxGridThreads / 1024) return fail(AEKV_ERR_UNSUPPORTED, "%s: %lld (sequence, head) rows exceed the grid", who, (long long)(B * heads));
   a.lengths = lengths;
   a.weights = weights;
   a.tokens = tokens;
@@ -335,9 +336,9 @@ extern "C" int aekv_kv_evict(int32_t d, int32_t bits, void* k_codes, float* k_sc
   hipLaunchKernelGGL(sel, dim3(static_cast<uint32_t>(B * heads)), dim3(slots <= kSmallRow ? 512 : 1024), 0, st, a);
   if (const int rc = check_launch(who)) return rc;
   if (own || a.most == 0) return AEKV_OK;  // (keep = 0: nothing stays, nothing moves)
-  const int64_t per = ceil_div(a.most, 16 * kMoves);
-  const dim3 grid(static_cast<uint32_t>(per < 64 ? per : 64), static_cast<uint32_t>(B * heads));
+  const int64_t all = ceil_div(a.most, 16 * kMoves), per = all < 64 ? all : 64, fit = kMaxGridThreads / 256 / (B * heads);  // (fit >= 4)
+  const uint32_t each = static_cast<uint32_t>(per < fit ? per : fit);
   auto fn = row == 32 ? evict_move_kernel<32> : row == 64 ? evict_move_kernel<64> : evict_move_kernel<128>;
-  hipLaunchKernelGGL(fn, grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(B * heads) * each), dim3(256), 0, st, a, each);
   return check_launch(who);
 }

@@ -875,3 +875,38 @@ def test_attention_large_workspace_is_given_back(dev):
     assert torch.cuda.memory_allocated(dev) - held < 1 << 20
     R.within(tracker.weights[..., :112], w, wb, "weights")
     assert not tracker.weights[..., 112:].any()
+
+
+@pytest.mark.parametrize("keep,slots", [(16, 32), (300, 608)])
+def test_evict_more_rows_than_a_grid_dimension(dev, keep, slots):
+    """70000 (sequence, KV head) rows, with the moves made by the selecting workgroup and by a launch of their own."""
+    B, heads, page = (1000, 70, 16) if slots < 300 else (5000, 14, 16)
+    lens = torch.randint(0, slots + 1, (B,), generator=torch.Generator().manual_seed(1))
+    lens[-1] = slots
+    per = slots // page
+    codes = torch.randint(0, 256, (2, B * per, heads, page, 32), dtype=torch.uint8, device=dev, generator=_gen(dev, 150))
+    scale = torch.rand(2, B * per, heads, page, device=dev, generator=_gen(dev, 151))
+    cache = PagedKVCache.from_tensors(PolarQuant(4), codes[0], scale[0], codes[1], scale[1])
+    table = torch.arange(B * per, dtype=torch.int32, device=dev).view(B, per)
+    tracker = SlotTracker(B, heads, slots, device=dev)
+    # weights that are all different: a permutation of each row's places
+    tracker.weights.copy_(torch.rand(B, heads, slots, device=dev, generator=_gen(dev, 152)).argsort(-1))
+    tracker.tokens.copy_(torch.arange(slots, device=dev).expand(B, heads, slots))
+    n = lens.to(torch.int32).to(dev)
+    weights = tracker.weights.clone()
+    rows = lambda c: c.view(B, per, heads, page, -1).transpose(1, 2).reshape(B, heads, slots, -1)  # noqa: E731
+    before = [rows(x).clone() for x in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)]
+    evict_by_weight(cache, table, n, tracker, n, keep)
+    # stays[slot], and the source of every slot below keep: itself, or for the i-th hole the i-th slot that moves
+    there = torch.arange(slots, device=dev) < n[:, None, None]
+    rank = weights.masked_fill(~there, -1.0).argsort(-1, descending=True)
+    stays = torch.zeros_like(there.expand_as(weights)).scatter_(-1, rank[..., :keep], True) & there
+    place = torch.arange(slots, device=dev).expand_as(weights)
+    hole = ~stays & (place < keep) & (n > keep)[:, None, None]
+    mover = stays & (place >= keep)
+    assert torch.equal(hole.sum(-1), mover.sum(-1))
+    source = place.clone()
+    source[hole] = place[mover]  # (both in row-major order)
+    for got, x in zip((cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale), before):
+        assert torch.equal(rows(got), x.gather(2, source[..., None].expand_as(x)))
+    assert torch.equal(tracker.tokens.long(), source) and torch.equal(tracker.weights, weights.gather(-1, source))
