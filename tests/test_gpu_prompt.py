@@ -460,3 +460,26 @@ def test_prompt_scale_that_is_no_number(dev, dtype, dim, H, hk, lq, lk):
     none = torch.cat([torch.arange(a) + b - a < 0 for a, b in zip(lq, lk)]).to(dev)
     assert out[~none].isnan().all() and lse[~none].isnan().all()
     assert not out[none].any() and (lse[none] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype,dim,H,hk,lq,lk", [
+    # in the sequences' order without gaps: 128 rows to a tile, 64, and 64 with the keys in pieces
+    (torch.bfloat16, 128, 16, 2, [512] * 8, [4096] * 8), (torch.float16, 128, 16, 2, [512] * 5, [4096, 4000, 4096, 3900, 512]),
+    (torch.bfloat16, 128, 12, 4, [700, 0, 77, 513, 64, 1, 300], [700, 0, 77, 513, 64, 1, 300]),
+    (torch.float16, 64, 8, 2, [64, 3, 0, 200] * 2, [3000, 700, 50, 5000] * 2),
+    # by their work
+    (torch.bfloat16, 128, 16, 2, [512] * 8, [600] * 8), (torch.bfloat16, 128, 12, 4, [512] * 10, [512] * 10),
+    (torch.float16, 64, 32, 16, [200, 0, 333, 90, 512, 1, 400, 256] * 2, [300, 10, 400, 90, 700, 1500, 512, 300] * 2),
+    (torch.bfloat16, 128, 12, 4, [700, 33, 2048, 1, 900] * 2, [700, 33, 2048, 1, 900] * 2),
+    # in the sequences' order with gaps: more than 64 of them
+    (torch.bfloat16, 64, 16, 4, [(30, 0, 130, 64, 1)[i % 5] for i in range(90)], [(30, 5, 200, 64, 70)[i % 5] for i in range(90)])])
+def test_prompt_every_row_of_packed_sequences(dev, dtype, dim, H, hk, lq, lk):
+    """Every row of batches whose tiles are taken in each of the orders, within the bound of the kernels' own roundings: a tile
+    left out or given another sequence's keys would show in all its rows."""
+    q, k, v = _inputs(dev, 43, dtype, dim, H, hk, lq, lk, pad=3)
+    cu = lambda x: torch.tensor(_cu(x), dtype=torch.int32, device=dev)  # noqa: E731
+    out = prompt_attention(q, k, v, cu(lq), dim ** -0.5, cu_seqlens_k=cu(lk))
+    assert not out[sum(lq):].any()
+    # (2^-32: weights below fp16's normal numbers; bf16 has fp32's range)
+    want, bound = _all_rows(q, k, v, lq, lk, dim ** -0.5, lift=2.0 ** -32 if dtype == torch.float16 else 0.0)
+    R.within(out, want.cpu(), bound.cpu(), "out")
