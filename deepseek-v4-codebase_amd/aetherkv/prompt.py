@@ -28,7 +28,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     h // (H // kv_heads)); strided views, such as parts of one projection's rows, are read in place.  cu_seqlens int32
     [B + 1]: sequence b's queries are rows cu_seqlens[b] .. cu_seqlens[b + 1]; cu_seqlens_k likewise for the keys (None:
     the same), so that a later chunk of a prompt comes with the keys before it.  sink [H] (or a scalar): a logit counted
-    once in the normaliser.  A query that sees nothing gives 0.  Rows of q in no sequence: a given `out` keeps them, a new
+    once in the normaliser.  Each weight p_ij is rounded once to the type of q, k and v for its product with v; all sums are
+    fp32.  A query that sees nothing gives 0.  Rows of q in no sequence: a given `out` keeps them, a new
     one holds 0.  Returns out [N, H, D], with return_lse (out, lse fp32 [N, H]): the log of every row's sum of
     exponentials, the sink's among them (-inf for rows in no sequence)."""
     shape, dtype, ks = q.shape, q.dtype, k.shape

@@ -1014,7 +1014,9 @@ bool paged_fits(int64_t B, int64_t T, int64_t H, int64_t heads, int64_t blocks) 
          static_cast<double>(B) * static_cast<double>(T * H) <= kMaxGridThreads / kThreads;
 }
 
-// Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.
+// Row tiles of a wave: two share a step's unpacked codes where there are as many rows and registers.  At dim 128 two take all
+// 256 registers and spill (4 bits; at 8 the waves' states do not fit a stage of LDS either), so each 16 rows read the codes
+// again: 32 sequences of 16384 slots, 12 heads of 4, 4 bits, one token (3 rows) 64 us, 5 (15) 72, 16 (48) 160.
 int paged_row_tiles(int64_t rows, int32_t d) { return rows > 16 && d == 64 ? 2 : 1; }
 
 // Tracked calls of few rows keep their logits and sum them afterwards; of many rows the scores are computed again, which
