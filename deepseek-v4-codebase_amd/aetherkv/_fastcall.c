@@ -388,7 +388,127 @@ static PyObject* f_prompt_attention(PyObject* self, PyObject* const* args, Py_ss
                                                (float*)lse, clear, ws, wsb, st));
 }
 
+/* aekv_cross_attention(q, k, v, dtype, q_token, q_head, k_token, k_head, v_token, v_head, cu_q, cu_k, states, B, E, n_q, n_k,
+ * H, heads, d, sink, scale, out, lse, clear_rest, ws, ws_bytes, stream) */
+static PyObject* f_cross_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 28, "aekv_cross_attention")) return NULL;
+  void* q = ptr_arg(A(0));
+  void* k = ptr_arg(A(1));
+  void* v = ptr_arg(A(2));
+  const int32_t dt = i32_arg(A(3));
+  int64_t n[6], s[6];
+  for (int i = 0; i < 6; ++i) n[i] = i64_arg(A(4 + i));
+  void* cq = ptr_arg(A(10));
+  void* ck = ptr_arg(A(11));
+  void* states = ptr_arg(A(12));
+  for (int i = 0; i < 6; ++i) s[i] = i64_arg(A(13 + i));
+  const int32_t d = i32_arg(A(19));
+  void* sink = ptr_arg(A(20));
+  const float sm = f32_arg(A(21));
+  void* out = ptr_arg(A(22));
+  void* lse = ptr_arg(A(23));
+  const int32_t clear = i32_arg(A(24));
+  void* ws = ptr_arg(A(25));
+  const size_t wsb = (size_t)i64_arg(A(26));
+  void* st = ptr_arg(A(27));
+  RETURN_STATUS(aekv_cross_attention(q, k, v, dt, n[0], n[1], n[2], n[3], n[4], n[5], (const int32_t*)cq, (const int32_t*)ck,
+                                     (const int32_t*)states, s[0], s[1], s[2], s[3], s[4], s[5], d, (const float*)sink, sm,
+                                     out, (float*)lse, clear, ws, wsb, st));
+}
+
+/* aekv_rotate_axes(q, k, dtype, n, H, heads, d, q_token, q_head, k_token, k_head, positions, pos_dtype, axes, pos_axis,
+ * pos_token, inv_freq, axis, pairs, first, halves, inverse, q_out, k_out, qo_token, qo_head, ko_token, ko_head, stream) */
+static PyObject* f_rotate_axes(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 29, "aekv_rotate_axes")) return NULL;
+  void* q = ptr_arg(A(0));
+  void* k = ptr_arg(A(1));
+  const int32_t dt = i32_arg(A(2));
+  const int64_t n = i64_arg(A(3));
+  const int32_t H = i32_arg(A(4)), heads = i32_arg(A(5)), d = i32_arg(A(6));
+  int64_t s[4], o[4];
+  for (int i = 0; i < 4; ++i) s[i] = i64_arg(A(7 + i));
+  void* pos = ptr_arg(A(11));
+  const int32_t pdt = i32_arg(A(12)), axes = i32_arg(A(13));
+  const int64_t pa = i64_arg(A(14)), pt = i64_arg(A(15));
+  void* freq = ptr_arg(A(16));
+  void* axis = ptr_arg(A(17));
+  const int32_t pairs = i32_arg(A(18)), first = i32_arg(A(19)), halves = i32_arg(A(20)), inverse = i32_arg(A(21));
+  void* qo = ptr_arg(A(22));
+  void* ko = ptr_arg(A(23));
+  for (int i = 0; i < 4; ++i) o[i] = i64_arg(A(24 + i));
+  void* st = ptr_arg(A(28));
+  RETURN_STATUS_UNLOCKED(aekv_rotate_axes(q, k, dt, n, H, heads, d, s[0], s[1], s[2], s[3], pos, pdt, axes, pa, pt,
+                                          (const float*)freq, (const int32_t*)axis, pairs, first, halves, inverse, qo, ko,
+                                          o[0], o[1], o[2], o[3], st));
+}
+
+/* aekv_pool_reserve(table, B, max_pages, filled, wanted, first, page_size, refs, marks, lacking, pages, segments, n_segments,
+ * ws, ws_bytes, stream) */
+static PyObject* f_pool_reserve(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 16, "aekv_pool_reserve")) return NULL;
+  void* table = ptr_arg(A(0));
+  const int64_t B = i64_arg(A(1)), W = i64_arg(A(2));
+  void* filled = ptr_arg(A(3));
+  void* wanted = ptr_arg(A(4));
+  void* first = ptr_arg(A(5));
+  const int32_t ps = i32_arg(A(6));
+  void* refs = ptr_arg(A(7));
+  void* marks = ptr_arg(A(8));
+  void* lacking = ptr_arg(A(9));
+  const int64_t pages = i64_arg(A(10));
+  void* segs = ptr_arg(A(11));
+  const int64_t n = i64_arg(A(12));
+  void* ws = ptr_arg(A(13));
+  const size_t wsb = (size_t)i64_arg(A(14));
+  void* st = ptr_arg(A(15));
+  RETURN_STATUS(aekv_pool_reserve((int32_t*)table, B, W, (const int32_t*)filled, (const int32_t*)wanted,
+                                  (const int32_t*)first, ps, (int32_t*)refs, (int32_t*)marks, (int32_t*)lacking, pages,
+                                  segs, n, ws, wsb, st));
+}
+
+/* aekv_pool_release(table, B, max_pages, keep, page_size, refs, pages, stream) */
+static PyObject* f_pool_release(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 8, "aekv_pool_release")) return NULL;
+  void* table = ptr_arg(A(0));
+  const int64_t B = i64_arg(A(1)), W = i64_arg(A(2));
+  void* keep = ptr_arg(A(3));
+  const int32_t ps = i32_arg(A(4));
+  void* refs = ptr_arg(A(5));
+  const int64_t pages = i64_arg(A(6));
+  void* st = ptr_arg(A(7));
+  RETURN_STATUS(aekv_pool_release((int32_t*)table, B, W, (const int32_t*)keep, ps, (int32_t*)refs, pages, st));
+}
+
+/* aekv_pool_fork(table, B, max_pages, filled, source, target, n, page_size, refs, pages, ws, ws_bytes, stream) */
+static PyObject* f_pool_fork(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 13, "aekv_pool_fork")) return NULL;
+  void* table = ptr_arg(A(0));
+  const int64_t B = i64_arg(A(1)), W = i64_arg(A(2));
+  void* filled = ptr_arg(A(3));
+  void* source = ptr_arg(A(4));
+  void* target = ptr_arg(A(5));
+  const int64_t n = i64_arg(A(6));
+  const int32_t ps = i32_arg(A(7));
+  void* refs = ptr_arg(A(8));
+  const int64_t pages = i64_arg(A(9));
+  void* ws = ptr_arg(A(10));
+  const size_t wsb = (size_t)i64_arg(A(11));
+  void* st = ptr_arg(A(12));
+  RETURN_STATUS(aekv_pool_fork((int32_t*)table, B, W, (const int32_t*)filled, (const int32_t*)source,
+                               (const int32_t*)target, n, ps, (int32_t*)refs, pages, ws, wsb, st));
+}
+
 static PyMethodDef methods[] = {
+    {"aekv_cross_attention", (PyCFunction)(void (*)(void))f_cross_attention, METH_FASTCALL, NULL},
+    {"aekv_rotate_axes", (PyCFunction)(void (*)(void))f_rotate_axes, METH_FASTCALL, NULL},
+    {"aekv_pool_reserve", (PyCFunction)(void (*)(void))f_pool_reserve, METH_FASTCALL, NULL},
+    {"aekv_pool_release", (PyCFunction)(void (*)(void))f_pool_release, METH_FASTCALL, NULL},
+    {"aekv_pool_fork", (PyCFunction)(void (*)(void))f_pool_fork, METH_FASTCALL, NULL},
     {"aekv_kv_append", (PyCFunction)(void (*)(void))f_kv_append, METH_FASTCALL, NULL},
     {"aekv_paged_attention", (PyCFunction)(void (*)(void))f_paged_attention, METH_FASTCALL, NULL},
     {"aekv_kv_evict", (PyCFunction)(void (*)(void))f_kv_evict, METH_FASTCALL, NULL},

@@ -39,6 +39,8 @@ SYMBOLS = (
     "aekv_tiled_prefill_attention_ws", "aekv_sink_attention_workspace_size", "aekv_prefill_counts",
     "aekv_kv_append", "aekv_paged_attention_workspace_size", "aekv_paged_attention", "aekv_kv_evict_workspace_size",
     "aekv_kv_evict", "aekv_prompt_attention", "aekv_prompt_attention_workspace_size",
+    "aekv_cross_attention", "aekv_cross_attention_workspace_size", "aekv_rotate_axes", "aekv_pool_workspace_size",
+    "aekv_pool_reserve", "aekv_pool_release", "aekv_pool_fork", "aekv_pool_compact", "aekv_pool_renumber",
 )
 
 # size of the static device scratch behind aekv_csa_indexer_topk_quant_noalloc (AEKV_STATIC_SCRATCH_BYTES)
@@ -115,6 +117,16 @@ def lib() -> ctypes.CDLL:
                           ctypes.c_int),
         "aekv_prompt_attention": ([P, P, P, I32_] + [I64_] * 6 + [P, P] + [I64_] * 5 + [I32_, P, F, P, P, I32_, P, SZ, P], ctypes.c_int),
         "aekv_prompt_attention_workspace_size": ([I64_] * 5 + [I32_], SZ),
+        "aekv_cross_attention": ([P, P, P, I32_] + [I64_] * 6 + [P, P, P] + [I64_] * 6 + [I32_, P, F, P, P, I32_, P, SZ, P], ctypes.c_int),
+        "aekv_cross_attention_workspace_size": ([I64_] * 6 + [I32_], SZ),
+        "aekv_rotate_axes": ([P, P, I32_, I64_, I32_, I32_, I32_] + [I64_] * 4 + [P, I32_, I32_, I64_, I64_, P, P, I32_, I32_, I32_, I32_, P, P]
+                             + [I64_] * 4 + [P], ctypes.c_int),
+        "aekv_pool_workspace_size": ([I64_] * 4, SZ),
+        "aekv_pool_reserve": ([P, I64_, I64_, P, P, P, I32_, P, P, P, I64_, P, I64_, P, SZ, P], ctypes.c_int),
+        "aekv_pool_release": ([P, I64_, I64_, P, I32_, P, I64_, P], ctypes.c_int),
+        "aekv_pool_fork": ([P, I64_, I64_, P, P, P, I64_, I32_, P, I64_, P, SZ, P], ctypes.c_int),
+        "aekv_pool_compact": ([P, I64_, P, I64_, P, SZ, P], ctypes.c_int),
+        "aekv_pool_renumber": ([P, I64_, I64_, P, SZ, P], ctypes.c_int),
         "aekv_sink_attention_workspace_size": ([I32_, I64_, I64_, I64_, I64_, I64_, I64_], SZ),
     }
     for name, (argtypes, restype) in sig.items():
@@ -248,6 +260,16 @@ def evict_ws_bytes(B: int, heads: int, keep: int, slots: int) -> int:
 @functools.lru_cache(maxsize=1024)
 def prompt_ws_bytes(B: int, n_q: int, n_k: int, H: int, heads: int, d: int) -> int:
     return lib().aekv_prompt_attention_workspace_size(B, n_q, n_k, H, heads, d)
+
+
+@functools.lru_cache(maxsize=1024)
+def cross_ws_bytes(B: int, E: int, n_q: int, n_k: int, H: int, heads: int, d: int) -> int:
+    return lib().aekv_cross_attention_workspace_size(B, E, n_q, n_k, H, heads, d)
+
+
+@functools.lru_cache(maxsize=1024)
+def pool_ws_bytes(B: int, max_pages: int, forks: int, pages: int) -> int:
+    return lib().aekv_pool_workspace_size(B, max_pages, forks, pages)
 
 
 def require_device(name: str, *tensors: Optional[torch.Tensor]) -> None:

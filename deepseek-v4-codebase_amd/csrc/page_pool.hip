@@ -1,0 +1,398 @@
+// The life of a cache's pages: which are in use (refs[p]: entries of page tables that hold page p), given to sequences,
+// shared by forks, copied before they are written, released, moved together.  One pool serves the caches of all layers, whose
+// tables are one: a page's bytes lie in several tensors.
+//
+//   reserve  every table entry of the slots that are about to be written gets a page of its own: a fresh one where it has none,
+//            and a fresh copy where it shares one with entries that the call does not write (the last of a page's holders, if
+//            the call writes them all, keeps it).  Fresh pages are the lowest unused ones, in the entries' order.
+//   release  entries past the kept slots let go of their pages.
+//   fork     rows take over other rows' pages, all read before any is written.
+//   compact  the k-th unused page below the number of pages in use takes the k-th page in use from there on.
+//
+// Tables and counts are device data: entries outside the pool count as none, rows outside the table are skipped.  What decides is
+// a few thousand whole numbers, which one workgroup reads in some memory rounds: bound by latency.  What moves is a page's bytes
+// in every tensor, by a second launch that reads the number of copies from memory.
+#include "aekv_common.h"
+
+namespace aekv {
+namespace {
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kMaxRows = 8192;    // rows of a table (their offsets lie in LDS)
+constexpr int kSegment = 4096;    // bytes that a wave copies at a time
+constexpr int kHeader = 16;       // ints before the lists in the workspace: copies
+
+struct Segment {
+  uint64_t base;  // of a page's part in one tensor, page 0
+  uint64_t page;  // bytes from a page to the next
+  uint64_t bytes; // at most kSegment, a multiple of 16
+};
+
+struct PoolArgs {
+  int32_t* table;  // [B, W]
+  int32_t B, W, shift;
+  const int32_t* filled;
+  const int32_t* wanted;
+  const int32_t* first;
+  int32_t* refs;     // [pages]
+  int32_t* marks;    // [2, pages]: writers of a shared page, the last of them + 1; 0 between calls
+  int32_t* lacking;  // [1]: pages that could not be given
+  int32_t pages;
+  int32_t* ws;
+};
+
+__device__ __forceinline__ int32_t load_now(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void add(int32_t* p, int32_t v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The sum of v over the threads before this one, and over all (s: kWaves ints, free again after the next barrier).
+__device__ __forceinline__ int32_t scan(int32_t v, int32_t* s, int32_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(x, d);
+    if (lane >= d) x += o;
+  }
+  if (lane == 63) s[wave] = x;
+  __syncthreads();
+  int32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const int32_t n = s[w];
+    if (w < wave) before += n;
+    all += n;
+  }
+  __syncthreads();
+  *total = all;
+  return before + x - v;
+}
+
+// Pages that slots [0, n) lie in, as far as the table has them.
+__device__ __forceinline__ int32_t pages_of(const PoolArgs& a, int32_t n) {
+  const int32_t p = n <= 0 ? 0 : ((n - 1) >> a.shift) + 1;
+  return p < a.W ? p : a.W;
+}
+
+__global__ __launch_bounds__(kThreads) void pool_reserve_kernel(PoolArgs a) {
+  extern __shared__ int32_t offs[];  // [B + 1]: where the rows' entries start
+  __shared__ int32_t s_scan[kWaves];
+  __shared__ int32_t s_copies;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_copies = 0;
+  int32_t entries = 0;
+  for (int32_t b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int32_t b = b0 + tid;
+    int32_t n = 0;
+    if (b < a.B) {
+      const int32_t w = a.wanted[b], f = a.first ? a.first[b] : a.filled[b];
+      const int32_t from = f > 0 ? f >> a.shift : 0;
+      n = max(pages_of(a, w) - from, 0);
+    }
+    int32_t all;
+    const int32_t before = scan(n, s_scan, &all);
+    if (b < a.B) offs[b] = entries + before;
+    entries += all;  // (at most B W, which fits 31 bits)
+  }
+  if (tid == 0) offs[a.B] = entries;
+  __syncthreads();
+  // entry e: its row, and where it lies in the table
+  auto place = [&](int32_t e, int32_t* row, int32_t* i) {
+    int32_t lo = 0, hi = a.B;  // offs[lo] <= e < offs[hi]
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (offs[mid] <= e) lo = mid;
+      else hi = mid;
+    }
+    const int32_t f = a.first ? a.first[lo] : a.filled[lo];
+    *row = lo, *i = (f > 0 ? f >> a.shift : 0) + e - offs[lo];
+  };
+  int32_t* const rank_of = a.ws + kHeader;                             // [entries]: the entry's number among those that take a page, or -1
+  int32_t* const fresh = rank_of + static_cast<int64_t>(a.B) * a.W;    // [entries]
+  int32_t* const copies = fresh + static_cast<int64_t>(a.B) * a.W;     // [entries][2]
+  for (int32_t e = tid; e < entries; e += kThreads) {
+    int32_t row, i;
+    place(e, &row, &i);
+    const int32_t p = a.table[static_cast<int64_t>(row) * a.W + i];
+    if (p >= 0 && p < a.pages && a.refs[p] > 1) {
+      add(a.marks + p, 1);
+      __hip_atomic_fetch_max(a.marks + a.pages + p, e + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  int32_t takes = 0;
+  for (int32_t e0 = 0; e0 < entries; e0 += kThreads) {
+    const int32_t e = e0 + tid;
+    bool take = false;
+    if (e < entries) {
+      int32_t row, i;
+      place(e, &row, &i);
+      const int32_t p = a.table[static_cast<int64_t>(row) * a.W + i];
+      take = p < 0 || p >= a.pages;
+      if (!take) {
+        const int32_t r = a.refs[p];
+        take = r > 1 && !(load_now(a.marks + p) == r && load_now(a.marks + a.pages + p) == e + 1);
+      }
+    }
+    int32_t all;
+    const int32_t before = scan(take, s_scan, &all);
+    if (e < entries) rank_of[e] = take ? takes + before : -1;
+    takes += all;
+  }
+  int32_t found = 0;
+  for (int32_t p0 = 0; p0 < a.pages && found < takes; p0 += kThreads) {
+    const int32_t p = p0 + tid;
+    const bool unused = p < a.pages && a.refs[p] <= 0;
+    int32_t all;
+    const int32_t at = found + scan(unused, s_scan, &all);
+    if (unused && at < takes) fresh[at] = p;
+    found += all;
+  }
+  __syncthreads();
+  for (int32_t e = tid; e < entries; e += kThreads) {
+    int32_t row, i;
+    place(e, &row, &i);
+    int32_t* const entry = a.table + static_cast<int64_t>(row) * a.W + i;
+    const int32_t p = *entry, rank = rank_of[e];
+    const bool had = p >= 0 && p < a.pages;
+    if (had) a.marks[p] = 0, a.marks[a.pages + p] = 0;
+    if (rank < 0) continue;
+    const int32_t to = rank < found ? fresh[rank] : -1;
+    *entry = to;
+    if (had) add(a.refs + p, -1);
+    if (to < 0) continue;
+    a.refs[to] = 1;
+    if (had && (static_cast<int64_t>(i) << a.shift) < a.filled[row]) {
+      const int32_t c = atomicAdd(&s_copies, 1);
+      copies[2 * c] = p, copies[2 * c + 1] = to;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    a.ws[0] = s_copies;
+    if (found < takes) *a.lacking += takes - found;
+  }
+}
+
+__global__ __launch_bounds__(256) void pool_release_kernel(PoolArgs a) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= static_cast<int64_t>(a.B) * a.W) return;
+  const int32_t row = static_cast<int32_t>(at / a.W), i = static_cast<int32_t>(at - static_cast<int64_t>(row) * a.W);
+  if (i < pages_of(a, a.wanted[row])) return;
+  const int32_t p = a.table[at];
+  if (p >= 0 && p < a.pages) add(a.refs + p, -1);
+  if (p != -1) a.table[at] = -1;
+}
+
+// A workgroup has kColumns columns of the table, so that it reads all rows' old entries before it writes any.
+constexpr int kColumns = 16;
+__global__ __launch_bounds__(256) void pool_fork_kernel(PoolArgs a, const int32_t* source, const int32_t* target, int32_t n) {
+  extern __shared__ int32_t owner[];  // [B]: the last fork to a row + 1
+  for (int32_t b = threadIdx.x; b < a.B; b += 256) owner[b] = 0;
+  __syncthreads();
+  for (int32_t j = threadIdx.x; j < n; j += 256) {
+    const int32_t s = source[j], t = target[j];
+    if (s >= 0 && s < a.B && t >= 0 && t < a.B) atomicMax(owner + t, j + 1);
+  }
+  const int32_t i = blockIdx.x * kColumns + threadIdx.x % kColumns;
+  int32_t* const old = a.ws + kHeader;
+  const bool in = i < a.W;
+  for (int32_t j = threadIdx.x / kColumns; in && j < n; j += 256 / kColumns) {
+    const int32_t s = source[j];
+    if (s < 0 || s >= a.B) continue;
+    old[static_cast<int64_t>(j) * a.W + i] = i < pages_of(a, a.filled[s]) ? a.table[static_cast<int64_t>(s) * a.W + i] : -1;
+  }
+  __syncthreads();
+  for (int32_t j = threadIdx.x / kColumns; in && j < n; j += 256 / kColumns) {
+    const int32_t s = source[j], t = target[j];
+    if (s < 0 || s >= a.B || t < 0 || t >= a.B || s == t || owner[t] != j + 1) continue;
+    int32_t* const entry = a.table + static_cast<int64_t>(t) * a.W + i;
+    const int32_t was = *entry, now = old[static_cast<int64_t>(j) * a.W + i];
+    if (was == now) continue;
+    if (was >= 0 && was < a.pages) add(a.refs + was, -1);
+    if (now >= 0 && now < a.pages) add(a.refs + now, 1);
+    *entry = now;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void pool_compact_kernel(PoolArgs a) {
+  __shared__ int32_t s_scan[kWaves];
+  const int tid = threadIdx.x;
+  int32_t* const to = a.ws + kHeader;  // [pages]: where a page from `live` on goes, or -1
+  int32_t* const moves = to + a.pages; // [moves][2]
+  int32_t mine = 0, live;
+  for (int32_t p = tid; p < a.pages; p += kThreads) mine += a.refs[p] > 0;
+  scan(mine, s_scan, &live);
+  int32_t holes = 0, movers = 0;
+  for (int32_t p0 = 0; p0 < a.pages; p0 += kThreads) {
+    const int32_t p = p0 + tid;
+    const bool used = p < a.pages && a.refs[p] > 0;
+    const bool hole = p < live && !used, mover = p >= live && used;
+    int32_t all;
+    const int32_t before = scan((hole ? 1 : 0) + (mover ? 1 << 16 : 0), s_scan, &all);
+    if (hole) moves[2 * (holes + (before & 0xFFFF)) + 1] = p;
+    if (mover) moves[2 * (movers + (before >> 16))] = p;
+    if (p >= live && p < a.pages && !used) to[p] = -1;
+    holes += all & 0xFFFF, movers += all >> 16;
+  }
+  __syncthreads();
+  for (int32_t k = tid; k < holes; k += kThreads) {  // (as many movers)
+    const int32_t p = moves[2 * k], q = moves[2 * k + 1];
+    to[p] = q;
+    a.refs[q] = a.refs[p];
+    a.refs[p] = 0;
+  }
+  if (tid == 0) a.ws[0] = holes, a.ws[1] = live;
+}
+
+__global__ __launch_bounds__(256) void pool_renumber_kernel(int32_t* table, int64_t n, int32_t pages, const int32_t* ws) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= n) return;
+  const int32_t p = table[at];
+  if (p >= ws[1] && p < pages) table[at] = ws[kHeader + p];
+}
+
+// Copies of pages: a wave takes a segment of one copy at a time.
+__global__ __launch_bounds__(256) void pool_copy_kernel(const int32_t* count, const int32_t* copies, const Segment* segs, int32_t n_segs) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t items = static_cast<int64_t>(*count) * n_segs;
+  for (int64_t it = wave; it < items; it += static_cast<int64_t>(gridDim.x) * 4) {
+    const int32_t c = static_cast<int32_t>(it / n_segs), s = static_cast<int32_t>(it - static_cast<int64_t>(c) * n_segs);
+    const Segment g = segs[s];
+    const uint64_t src = g.base + g.page * static_cast<uint32_t>(copies[2 * c]), dst = g.base + g.page * static_cast<uint32_t>(copies[2 * c + 1]);
+    uint4 w[kSegment / 1024];
+#pragma unroll
+    for (int i = 0; i < kSegment / 1024; ++i) {
+      const uint32_t at = 1024 * i + 16 * lane;
+      w[i] = at < g.bytes ? *reinterpret_cast<const uint4*>(src + at) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kSegment / 1024; ++i) {
+      const uint32_t at = 1024 * i + 16 * lane;
+      if (at < g.bytes) *reinterpret_cast<uint4*>(dst + at) = w[i];
+    }
+  }
+}
+
+int check_table(const char* who, const int32_t* table, int64_t B, int64_t W, int64_t pages, const int32_t* refs) {
+  if (B < 0 || W < 0 || pages < 0) return fail(AEKV_ERR_SHAPE, "%s: B=%lld max_pages=%lld pages=%lld", who, (long long)B, (long long)W, (long long)pages);
+  if (B > kMaxRows) return fail(AEKV_ERR_UNSUPPORTED, "%s: a table of %lld rows (%d supported)", who, (long long)B, kMaxRows);
+  if (W > 0x7fffffff || B * W > 0x3fffffff || pages > 0x3fffffff)
+    return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld max_pages=%lld pages=%lld exceed 30 bits", who, (long long)B, (long long)W, (long long)pages);
+  if (B * W > 0 && (!table || !refs)) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  return AEKV_OK;
+}
+int page_shift(int32_t page_size) { return is_pow2(page_size) && page_size >= 16 && page_size <= 4096 ? __builtin_ctz(page_size) : -1; }
+
+int check_segments(const char* who, const void* segs, int64_t n) {
+  if (n < 0 || n > 0x7fffffff) return fail(AEKV_ERR_SHAPE, "%s: %lld segments", who, (long long)n);
+  if (n && (!segs || !is_aligned(segs, 8))) return fail(AEKV_ERR_VALUE, "%s: null or unaligned segments", who);
+  return AEKV_OK;
+}
+
+int launch_copies(const char* who, const int32_t* ws, const int32_t* copies, int64_t most, const void* segs, int64_t n, hipStream_t st) {
+  if (!n || !most) return AEKV_OK;
+  const int64_t blocks = ceil_div(most * n, static_cast<int64_t>(4));
+  hipLaunchKernelGGL(pool_copy_kernel, dim3(static_cast<uint32_t>(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, ws, copies,
+                     static_cast<const Segment*>(segs), static_cast<int32_t>(n));
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace aekv
+
+using namespace aekv;
+
+extern "C" size_t aekv_pool_workspace_size(int64_t B, int64_t max_pages, int64_t n_forks, int64_t pages) {
+  if (B < 0 || max_pages < 0 || n_forks < 0 || pages < 0 || B > kMaxRows || max_pages > 0x7fffffff || B * max_pages > 0x3fffffff || n_forks > 0x3fffffff || pages > 0x3fffffff) return 0;
+  const int64_t reserve = 4 * B * max_pages, fork = n_forks * max_pages, compact = 3 * pages;
+  const int64_t most = reserve > fork ? reserve : fork;
+  return static_cast<size_t>(kHeader + (most > compact ? most : compact)) * 4;
+}
+
+extern "C" int aekv_pool_reserve(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* wanted,
+                                 const int32_t* first, int32_t page_size, int32_t* refs, int32_t* marks, int32_t* lacking,
+                                 int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes,
+                                 void* stream) {
+  const char* who = "aekv_pool_reserve";
+  if (const int rc = check_table(who, table, B, max_pages, pages, refs)) return rc;
+  if (const int rc = check_segments(who, segments, n_segments)) return rc;
+  const int shift = page_shift(page_size);
+  if (shift < 0) return fail(AEKV_ERR_VALUE, "%s: page_size must be a power of two from 16 to 4096, got %d", who, page_size);
+  if (B * max_pages == 0) return AEKV_OK;
+  if (!filled || !wanted || !marks || !lacking) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  const size_t want = aekv_pool_workspace_size(B, max_pages, 0, 0);
+  if (!ws || ws_bytes < want) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
+  if (!is_aligned(ws, 16)) return fail(AEKV_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  PoolArgs a{};
+  a.table = table, a.B = static_cast<int32_t>(B), a.W = static_cast<int32_t>(max_pages), a.shift = shift, a.filled = filled, a.wanted = wanted, a.first = first;
+  a.refs = refs, a.marks = marks, a.lacking = lacking, a.pages = static_cast<int32_t>(pages), a.ws = static_cast<int32_t*>(ws);
+  const hipStream_t st = as_stream(stream);
+  hipLaunchKernelGGL(pool_reserve_kernel, dim3(1), dim3(kThreads), (B + 1) * sizeof(int32_t), st, a);
+  if (const int rc = check_launch(who)) return rc;
+  return launch_copies(who, a.ws, a.ws + kHeader + 2 * B * max_pages, B * max_pages, segments, n_segments, st);
+}
+
+extern "C" int aekv_pool_release(int32_t* table, int64_t B, int64_t max_pages, const int32_t* keep, int32_t page_size,
+                                 int32_t* refs, int64_t pages, void* stream) {
+  const char* who = "aekv_pool_release";
+  if (const int rc = check_table(who, table, B, max_pages, pages, refs)) return rc;
+  const int shift = page_shift(page_size);
+  if (shift < 0) return fail(AEKV_ERR_VALUE, "%s: page_size must be a power of two from 16 to 4096, got %d", who, page_size);
+  if (B * max_pages == 0) return AEKV_OK;
+  if (!keep) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  PoolArgs a{};
+  a.table = table, a.B = static_cast<int32_t>(B), a.W = static_cast<int32_t>(max_pages), a.shift = shift, a.wanted = keep, a.refs = refs, a.pages = static_cast<int32_t>(pages);
+  hipLaunchKernelGGL(pool_release_kernel, dim3(static_cast<uint32_t>(ceil_div(B * max_pages, 256))), dim3(256), 0, as_stream(stream), a);
+  return check_launch(who);
+}
+
+extern "C" int aekv_pool_fork(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* source,
+                              const int32_t* target, int64_t n, int32_t page_size, int32_t* refs, int64_t pages, void* ws,
+                              size_t ws_bytes, void* stream) {
+  const char* who = "aekv_pool_fork";
+  if (const int rc = check_table(who, table, B, max_pages, pages, refs)) return rc;
+  const int shift = page_shift(page_size);
+  if (shift < 0) return fail(AEKV_ERR_VALUE, "%s: page_size must be a power of two from 16 to 4096, got %d", who, page_size);
+  if (n < 0 || n > 0x3fffffff || n * max_pages > 0x3fffffff) return fail(AEKV_ERR_SHAPE, "%s: %lld forks of %lld pages", who, (long long)n, (long long)max_pages);
+  if (B * max_pages == 0 || n == 0) return AEKV_OK;
+  if (!filled || !source || !target) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  const size_t want = aekv_pool_workspace_size(0, max_pages, n, 0);
+  if (!ws || ws_bytes < want) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
+  if (!is_aligned(ws, 16)) return fail(AEKV_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  PoolArgs a{};
+  a.table = table, a.B = static_cast<int32_t>(B), a.W = static_cast<int32_t>(max_pages), a.shift = shift, a.filled = filled, a.refs = refs;
+  a.pages = static_cast<int32_t>(pages), a.ws = static_cast<int32_t*>(ws);
+  hipLaunchKernelGGL(pool_fork_kernel, dim3(static_cast<uint32_t>(ceil_div(max_pages, kColumns))), dim3(256), B * sizeof(int32_t), as_stream(stream), a, source, target,
+                     static_cast<int32_t>(n));
+  return check_launch(who);
+}
+
+extern "C" int aekv_pool_compact(int32_t* refs, int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes,
+                                 void* stream) {
+  const char* who = "aekv_pool_compact";
+  if (pages < 0 || pages > 0x3fffffff) return fail(AEKV_ERR_SHAPE, "%s: %lld pages", who, (long long)pages);
+  if (const int rc = check_segments(who, segments, n_segments)) return rc;
+  const size_t want = aekv_pool_workspace_size(0, 0, 0, pages);
+  if (!ws || ws_bytes < want) return fail(AEKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, want, ws_bytes);
+  if (!is_aligned(ws, 16)) return fail(AEKV_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  if (pages && !refs) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  PoolArgs a{};
+  a.refs = refs, a.pages = static_cast<int32_t>(pages), a.ws = static_cast<int32_t*>(ws);
+  const hipStream_t st = as_stream(stream);
+  hipLaunchKernelGGL(pool_compact_kernel, dim3(1), dim3(kThreads), 0, st, a);
+  if (const int rc = check_launch(who)) return rc;
+  return launch_copies(who, a.ws, a.ws + kHeader + pages, ceil_div(pages, static_cast<int64_t>(2)), segments, n_segments, st);
+}
+
+extern "C" int aekv_pool_renumber(int32_t* table, int64_t n, int64_t pages, const void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "aekv_pool_renumber";
+  if (n < 0 || pages < 0 || pages > 0x3fffffff || n > 0x3fffffff) return fail(AEKV_ERR_SHAPE, "%s: %lld entries of %lld pages", who, (long long)n, (long long)pages);
+  if (n == 0) return AEKV_OK;
+  if (!table) return fail(AEKV_ERR_VALUE, "%s: null pointer", who);
+  if (!ws || ws_bytes < aekv_pool_workspace_size(0, 0, 0, pages)) return fail(AEKV_ERR_WORKSPACE, "%s: the workspace of aekv_pool_compact is needed", who);
+  hipLaunchKernelGGL(pool_renumber_kernel, dim3(static_cast<uint32_t>(ceil_div(n, 256))), dim3(256), 0, as_stream(stream), table, n, static_cast<int32_t>(pages),
+                     static_cast<const int32_t*>(ws));
+  return check_launch(who);
+}

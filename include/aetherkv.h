@@ -370,6 +370,61 @@ int aekv_prompt_attention(const void* q, const void* k, const void* v, int32_t d
                           int32_t d, const float* sink, float softmax_scale, void* out, float* lse,
                           int32_t clear_rest, void* ws, size_t ws_bytes, void* stream);
 
+/* Attention over all states of an encoder: q [n_q, H, d], k and v [n_k, heads, d] bf16 or fp16 (strides in elements, rows
+ * 16-byte aligned), d = 64 or 128.  Sequence b holds queries cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (int32 [B + 1],
+ * non-decreasing; NULL: query b, and n_q = B) and sees the keys cu_seqlens_k[e] .. cu_seqlens_k[e + 1] (int32 [E + 1]) of
+ * e = states[b] (int32 [B]; NULL: b, and E = B); one outside 0 .. E - 1 has none.  out, lse, sink, clear_rest as in
+ * aekv_prompt_attention.  Workspace: aekv_cross_attention_workspace_size bytes, 16-byte aligned; its contents never matter. */
+size_t aekv_cross_attention_workspace_size(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d);
+int aekv_cross_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
+                         int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                         int64_t v_head_stride, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         const int32_t* states, int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, int64_t heads,
+                         int32_t d, const float* sink, float softmax_scale, void* out, float* lse, int32_t clear_rest,
+                         void* ws, size_t ws_bytes, void* stream);
+
+/* Rotary positions on several axes: q [n, H, d] and k [n, heads, d] (either may have 0 heads) in F32, F16 or BF16, strides in
+ * elements, d even, up to 1024, rows aligned to two elements.  Pair i < pairs of token n turns by
+ * positions[axis[i] * pos_axis_stride + n * pos_token_stride] * inv_freq[i] (negative with inverse); it is dims first + 2 i and
+ * first + 2 i + 1 (halves 0, first even) or first + i and first + pairs + i (halves 1, pairs even as well).  positions I32 or
+ * I64; axis int32 [pairs], each below `axes`.  Angles in fp64, the rest in fp32, rounded once.  Other dims are copied; q_out
+ * and k_out may be q and k. */
+int aekv_rotate_axes(const void* q, const void* k, int32_t dtype, int64_t n, int32_t H, int32_t heads, int32_t d,
+                     int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                     const void* positions, int32_t pos_dtype, int32_t axes, int64_t pos_axis_stride,
+                     int64_t pos_token_stride, const float* inv_freq, const int32_t* axis, int32_t pairs, int32_t first,
+                     int32_t halves, int32_t inverse, void* q_out, void* k_out, int64_t qo_token_stride,
+                     int64_t qo_head_stride, int64_t ko_token_stride, int64_t ko_head_stride, void* stream);
+
+/* ---- the life of a pool's pages --------------------------------------------------------------------
+ * refs int32 [pages]: entries of page tables that hold a page; unused at 0.  Tables int32 [B, max_pages] (at most 8192 rows,
+ * 2^30 entries) are changed in place; an entry outside 0 .. pages - 1 holds none.  segments: n_segments times three uint64, the
+ * address of a part of page 0 in some tensor, the bytes from a page to the next, the part's bytes (a multiple of 16, at most
+ * 4096): together all that is copied with a page.  The calls of one pool run one after another.  Workspaces: 16-byte aligned,
+ * aekv_pool_workspace_size(B, max_pages, forks, pages) bytes, with 0 for what a call does not have (reserve: B, max_pages; fork:
+ * max_pages, forks; compact: pages); the contents never matter, but renumber reads what compact left. */
+size_t aekv_pool_workspace_size(int64_t B, int64_t max_pages, int64_t n_forks, int64_t pages);
+/* Slots first[b] .. wanted[b] - 1 (first NULL: filled) are about to be written: every entry of their pages that holds none
+ * gets the lowest unused page, in the entries' order, and one whose page has other holders as well (refs > 1) too, with a copy
+ * of the page where it has slots below filled[b]; if a page's holders are all among the call's entries, the last keeps it.
+ * Without an unused page an entry becomes -1, and *lacking grows by 1.  marks: int32 [2, pages], zeros before and after. */
+int aekv_pool_reserve(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* wanted,
+                      const int32_t* first, int32_t page_size, int32_t* refs, int32_t* marks, int32_t* lacking,
+                      int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes, void* stream);
+/* Entries past the pages of the first keep[b] slots let go of their pages and become -1. */
+int aekv_pool_release(int32_t* table, int64_t B, int64_t max_pages, const int32_t* keep, int32_t page_size, int32_t* refs,
+                      int64_t pages, void* stream);
+/* Row target[j] takes over the pages of the first filled[source[j]] slots of row source[j] (int32 [n]) and lets go of its own;
+ * all rows are read first; the last of several j to one row counts; a row to itself stays; rows outside are skipped. */
+int aekv_pool_fork(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* source,
+                   const int32_t* target, int64_t n, int32_t page_size, int32_t* refs, int64_t pages, void* ws,
+                   size_t ws_bytes, void* stream);
+/* With n pages in use, the k-th unused one below n takes the k-th one in use from n on (bytes and refs); then
+ * aekv_pool_renumber, with the same workspace, for every table (n entries) that holds the pool's pages. */
+int aekv_pool_compact(int32_t* refs, int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes,
+                      void* stream);
+int aekv_pool_renumber(int32_t* table, int64_t n, int64_t pages, const void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,241 @@
+"""Attention over an encoder's states on the GPU against the plain 64-bit form (caches_ref.py)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import caches_ref as C
+import paged_ref as R
+from aetherkv.cross import cross_attention, cross_workspace
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _cu(lens):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+def _t(x, dev):
+    return None if x is None else torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def _check(dev, dtype, dim, H, hk, lq, lk, states=None, sink=False, pad=0, seed=0, gain=1.0, scale=None, offsets=True):
+    nq, nk = sum(lq) + pad, sum(lk) + pad
+    q = (torch.randn(nq, H, dim, device=dev, generator=_gen(dev, seed)) * gain).to(dtype)
+    kv = torch.randn(nk, 2, hk, dim, device=dev, generator=_gen(dev, seed + 1)).to(dtype)
+    k, v = kv[:, 0], kv[:, 1]
+    cq, ck = _cu(lq), _cu(lk)
+    sk = torch.randn(H, device=dev, generator=_gen(dev, seed + 2)) if sink else None
+    scale = dim ** -0.5 if scale is None else scale
+    out, lse = cross_attention(q, k, v, _t(ck, dev), scale, cu_seqlens=_t(cq, dev) if offsets else None, states=_t(states, dev), sink=sk, return_lse=True)
+    want, bound, wl, lb = C.cross_attention_ref(q.cpu(), k.cpu(), v.cpu(), cq, ck, states, scale, None if sk is None else sk.cpu())
+    R.within(out, want, bound, "out")
+    got = lse.double().cpu()
+    none = wl == -math.inf
+    assert torch.equal(got == -math.inf, none)
+    R.within(got[~none], wl[~none], lb[~none], "lse")
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 700])
+def test_one_query_lengths(dev, dtype, dim, n):
+    _check(dev, dtype, dim, 6, 2, [1], [n], seed=n, offsets=n % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(40, 1), (64, 63), (65, 64), (127, 65), (128, 129), (200, 300), (33, 1000), (1000, 40)])
+def test_many_queries(dev, dtype, dim, lq, lk):
+    _check(dev, dtype, dim, 4, 2, [lq], [lk], seed=lq + lk, sink=lq % 2 == 1)
+
+
+@pytest.mark.parametrize("H,hk", [(1, 1), (3, 3), (12, 4), (12, 1), (16, 2), (10, 2), (32, 1), (33, 1), (48, 1), (64, 1), (40, 2)])
+@pytest.mark.parametrize("lq", [[1, 1, 1], [3, 1, 2], [20, 30, 5]])
+def test_head_layouts(dev, H, hk, lq):
+    _check(dev, torch.bfloat16, 128, H, hk, lq, [70, 333, 129], sink=True, seed=H)
+
+
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("lq,lk", [([0], [5]), ([0, 5, 0, 0, 30, 1], [7, 0, 3, 0, 260, 1]), ([1] * 70, [(37 * i) % 300 for i in range(70)]), ([3, 1, 200], [500, 0, 65])])
+def test_packed(dev, lq, lk, pad):
+    out, lse = _check(dev, torch.bfloat16, 64, 4, 2, lq, lk, pad=pad, seed=len(lq)) if sum(lq) + pad else (None, None)
+    if pad:
+        assert not out[-pad:].any() and (lse[-pad:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("offsets", [False, True])
+@pytest.mark.parametrize("states", [[0] * 9, [0, 0, 0, 1, 1, 2, 2, 2, 2], [2, 0, 1, 1, 0, 2, 2, 0, 0], [1, -1, -1, 3, 0, 7, 2, 2, 2 ** 31 - 1]])
+def test_shared_states(dev, states, offsets):
+    _check(dev, torch.float16, 64, 8, 8, [1] * 9, [300, 41, 0], states=states, seed=1, offsets=offsets, sink=True)
+    _check(dev, torch.bfloat16, 128, 6, 2, [5, 0, 7, 1, 1, 30, 2, 0, 9], [300, 41, 0], states=states, seed=2)
+    _check(dev, torch.bfloat16, 64, 6, 2, [50, 0, 70, 1, 1, 130, 20, 0, 9], [300, 41, 0], states=states, seed=3)
+
+
+@pytest.mark.parametrize("B,lq", [(64, 1), (65, 1), (200, 1), (256, 1), (257, 1), (600, 1), (300, 3)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_many_sequences(dev, B, lq, shared):
+    E = 5 if shared else B
+    states = [b * E // B for b in range(B)] if shared else None
+    _check(dev, torch.bfloat16, 64, 2, 1, [lq] * B, [(53 * i) % 180 for i in range(E)], states=states, seed=B, offsets=lq > 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lq", [1, 2, 100])
+@pytest.mark.parametrize("gain,scale", [(1.0, 0.0), (1.0, -0.3), (30.0, None), (1.0, 1e-30), (300.0, 1.0), (100.0, 1000.0)])
+def test_scales(dev, dtype, lq, gain, scale):
+    _check(dev, dtype, 64, 4, 2, [lq], [333], seed=3, gain=gain, scale=scale)
+
+
+def test_the_next_sequences_states_and_the_rows_behind_do_not_reach(dev):
+    """Keys and values outside a sequence's states are NaN and infinities: nothing of them is read."""
+    for lq in (1, 3, 90):
+        q = torch.randn(2 * lq, 4, 128, device=dev, generator=_gen(dev, 0)).bfloat16()
+        k = torch.randn(400, 2, 128, device=dev, generator=_gen(dev, 1)).bfloat16()
+        v = torch.randn(400, 2, 128, device=dev, generator=_gen(dev, 2)).bfloat16()
+        clean = cross_attention(q, k, v, _t([30, 67, 200], dev), 0.1, cu_seqlens=_t([0, lq, 2 * lq], dev))
+        k[:30], k[200:], v[:30], v[200:] = NAN, math.inf, math.inf, NAN
+        assert torch.equal(clean, cross_attention(q, k, v, _t([30, 67, 200], dev), 0.1, cu_seqlens=_t([0, lq, 2 * lq], dev)))
+        # what a sequence sees, it answers for, and the other does not
+        k[40, 0] = NAN
+        out = cross_attention(q, k, v, _t([30, 67, 200], dev), 0.1, cu_seqlens=_t([0, lq, 2 * lq], dev))
+        assert out[:lq, :2].isnan().all() and torch.equal(out[:, 2:], clean[:, 2:]) and torch.equal(out[lq:], clean[lq:])
+
+
+@pytest.mark.parametrize("lq", [1, 80])
+def test_sinks_infinities_and_nan_scale(dev, lq):
+    q = torch.randn(lq, 4, 64, device=dev, generator=_gen(dev, 0)).half()
+    k, v = (torch.randn(150, 2, 64, device=dev, generator=_gen(dev, i)).half() for i in (1, 2))
+    cu, cq = _t([0, 150], dev), _t([0, lq], dev)
+    plain, lse = cross_attention(q, k, v, cu, 0.125, cu_seqlens=cq, return_lse=True)
+    low, lse2 = cross_attention(q, k, v, cu, 0.125, cu_seqlens=cq, sink=torch.full((4,), -math.inf, device=dev), return_lse=True)
+    assert torch.equal(plain, low) and torch.equal(lse, lse2)
+    lowest, _ = cross_attention(q, k, v, cu, 0.125, cu_seqlens=cq, sink=torch.full((4,), torch.finfo(torch.float32).min, device=dev), return_lse=True)
+    assert torch.equal(plain, lowest)
+    assert cross_attention(q, k, v, cu, NAN, cu_seqlens=cq).isnan().all()
+    assert not cross_attention(q, k, v, _t([0, 0], dev), NAN, cu_seqlens=cq).any()  # nothing seen
+    k[7, 0] = -math.inf  # logits of -inf and inf by the queries' signs, or NaN
+    out = cross_attention(q, k, v, cu, 0.125, cu_seqlens=cq)
+    assert out[:, :2].isnan().all() and torch.equal(out[:, 2:], plain[:, 2:])
+
+
+@pytest.mark.parametrize("H,hk,dim,lq", [(4, 2, 64, 1), (4, 2, 64, 70), (6, 3, 128, 1), (6, 1, 128, 40)])
+def test_views_are_read_in_place(dev, H, hk, dim, lq):
+    for pick in (lambda t: t, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1), lambda t: torch.stack([t, t], 1)[:, 1], lambda t: t[:, :, :].clone().as_strided(t.shape, t.contiguous().stride())):
+        q = pick(torch.randn(lq, H, dim, device=dev, generator=_gen(dev, 0)).bfloat16())
+        k, v = (pick(torch.randn(97, hk, dim, device=dev, generator=_gen(dev, i)).bfloat16()) for i in (1, 2))
+        want, bound, _, _ = C.cross_attention_ref(q.cpu(), k.cpu(), v.cpu(), [0, lq], [0, 97], None, 0.1)
+        R.within(cross_attention(q, k, v, _t([0, 97], dev), 0.1, cu_seqlens=_t([0, lq], dev)), want, bound, "out")
+    base = torch.randn(97 * hk * dim + 4, device=dev, generator=_gen(dev, 5)).bfloat16()
+    odd = base[4:].view(97, hk, dim)  # rows off 16 bytes are copied
+    q = torch.randn(lq, H, dim, device=dev, generator=_gen(dev, 0)).bfloat16()
+    assert torch.equal(cross_attention(q, odd, odd, _t([0, 97], dev), 0.1, cu_seqlens=_t([0, lq], dev)),
+                       cross_attention(q, odd.clone(), odd.clone(), _t([0, 97], dev), 0.1, cu_seqlens=_t([0, lq], dev)))
+
+
+def test_out_keeps_rows_in_no_sequence_and_workspaces_are_taken(dev):
+    for lq in (1, 60):
+        q = torch.randn(2 * lq + 4, 4, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+        k, v = (torch.randn(500, 2, 64, device=dev, generator=_gen(dev, i)).bfloat16() for i in (1, 2))
+        cq, ck = _t([3, 3 + lq, 3 + 2 * lq], dev), _t([0, 200, 500], dev)
+        want = cross_attention(q, k, v, ck, 0.1, cu_seqlens=cq)
+        assert not want[:3].any() and not want[-1:].any()
+        out = torch.full_like(q, 7.0)
+        ws = cross_workspace(2, 2, q.size(0), 500, 4, 2, 64, dev).fill_(255)
+        assert cross_attention(q, k, v, ck, 0.1, cu_seqlens=cq, out=out, workspace=ws) is out
+        assert (out[:3] == 7).all() and (out[-1:] == 7).all() and torch.equal(out[3:-1], want[3:-1])
+
+
+def test_offsets_that_are_no_prefix_sums_stay_in_bounds(dev):
+    """Bad offsets give some result, within the tensors."""
+    for N, M, cq, ck in ((64, 300, [0, 64, -5, 64, 0, 1 << 30, 64], [50, 10, 1 << 30, -7, 300, 0, 300]), (6, 300, [5, 0, 6, 0, 6, 3, 6], [300] * 7)):
+        for H in (4, 2):
+            q = torch.randn(N, H, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+            k, v = (torch.randn(M, 2, 64, device=dev, generator=_gen(dev, i)).bfloat16() for i in (1, 2))
+            out = cross_attention(q, k, v, _t(ck, dev), 0.1, cu_seqlens=_t(cq, dev))
+            torch.cuda.synchronize()
+            assert out.shape == q.shape
+
+
+def test_long_states_split_and_merged(dev):
+    for lq, H, hk, n in ((1, 4, 1, 9001), (2, 2, 2, 5000), (50, 4, 4, 9001)):
+        _check(dev, torch.bfloat16, 64, H, hk, [lq], [n], sink=True, seed=n)
+    _check(dev, torch.float16, 128, 3, 1, [1, 1, 1], [6000, 3, 900], seed=9, offsets=False)
+
+
+def test_results_do_not_depend_on_the_others(dev):
+    """The same sequence alone and in a batch: within twice the bound (the parts of a line may lie differently); twice the same
+    call: bit for bit."""
+    q = torch.randn(40, 6, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+    k, v = (torch.randn(40 * 111, 3, 64, device=dev, generator=_gen(dev, i)).bfloat16() for i in (1, 2))
+    ck = _t([111 * i for i in range(41)], dev)
+    a, b = cross_attention(q, k, v, ck, 0.1), cross_attention(q, k, v, ck, 0.1)
+    assert torch.equal(a, b)
+    want, bound, _, _ = C.cross_attention_ref(q.cpu(), k.cpu(), v.cpu(), list(range(41)), [111 * i for i in range(41)], None, 0.1)
+    R.within(a, want, bound, "out")
+
+
+@pytest.mark.parametrize("lq", [1, 70])
+def test_graphs_and_streams(dev, lq):
+    """Two graphs captured on one stream, replayed on two with new lengths: each has a workspace of its own."""
+    data, graphs, outs = [], [], []
+    side = torch.cuda.Stream()
+    for i in range(2):
+        q = torch.randn(3 * lq, 4, 64, device=dev, generator=_gen(dev, i)).bfloat16()
+        k, v = (torch.randn(3000, 2, 64, device=dev, generator=_gen(dev, 10 * i + j)).bfloat16() for j in (1, 2))
+        data.append((q, k, v, _t([0, 1000, 1700, 3000], dev), _t([0, lq, 2 * lq, 3 * lq], dev)))
+    call = lambda d: cross_attention(*d[:3], d[3], 0.1, cu_seqlens=d[4])  # noqa: E731
+    with torch.cuda.stream(side):
+        for d in data:
+            call(d)
+        side.synchronize()
+        for d in data:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(call(d))
+            graphs.append(g)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for ends in ([0, 1000, 1700, 3000], [0, 0, 2999, 3000], [5, 300, 300, 900]):
+        for d in data:
+            d[3].copy_(_t(ends, dev))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for d, out in zip(data, outs):
+            assert torch.equal(out, call(d))
+
+
+def test_empty_calls(dev):
+    q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=dev)
+    k = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)
+    assert cross_attention(q, k, k, _t([0], dev), 0.1).shape == (0, 4, 64)
+    q = torch.randn(3, 4, 64, device=dev).bfloat16()
+    out, lse = cross_attention(q, k, k, _t([0], dev), 0.1, states=_t([0, 1, -1], dev), return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+    out = cross_attention(q, k, k, _t([0, 0], dev), 0.1, cu_seqlens=_t([0, 3], dev), sink=torch.zeros(4, device=dev))
+    assert not out.any()
+
+
+def test_refusals(dev):
+    q, k, cu = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev), torch.zeros(5, 2, 64, dtype=torch.bfloat16, device=dev), _t([0, 2, 5], dev)
+    for args, kw in (((q, k, k, cu), {}), ((q, k, k, cu), dict(states=_t([0, 1], dev))), ((q, k, k, cu), dict(states=torch.zeros(3, device=dev))), ((q, k, k, cu.cpu()), {}),
+                     ((q, k, k[:4], cu), {}), ((q.float(), k.float(), k.float(), cu), {}), ((q, k, k, cu), dict(cu_seqlens=_t([0, 1, 2, 3], dev))),
+                     ((q, k, k, cu), dict(cu_seqlens=_t([0, 1, 3], dev), out=q[:2].clone())), ((q, k, k, cu), dict(cu_seqlens=_t([0, 1, 3], dev), sink=torch.zeros(3, device=dev))),
+                     ((q, k, k, cu), dict(cu_seqlens=_t([0, 1, 3], dev), workspace=torch.empty(16, dtype=torch.uint8, device=dev)))):
+        with pytest.raises(RuntimeError):
+            cross_attention(*args, 0.1, **kw)
