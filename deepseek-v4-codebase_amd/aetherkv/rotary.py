@@ -62,11 +62,12 @@ class AxisRotary:
     axis = property(lambda self: self._axis)
 
 
-def _token_stride(t: torch.Tensor) -> Optional[Tuple[int, int]]:
+def _token_stride(shape, st) -> Optional[Tuple[int, int]]:
     """(token, head) strides of [.., heads, D], its leading dims as one, or None where they are not one stride apart."""
-    shape, st = t.shape, t.stride()
-    if shape[-1] > 1 and st[-1] != 1:
+    if st[-1] != 1 and shape[-1] > 1:
         return None
+    if len(shape) == 3:
+        return st[0], st[1]
     token, tokens = 0, 1
     for i in range(len(shape) - 3, -1, -1):
         if shape[i] == 1:
@@ -76,16 +77,26 @@ def _token_stride(t: torch.Tensor) -> Optional[Tuple[int, int]]:
         elif st[i] != token * tokens:
             return None
         tokens *= shape[i]
-    return token, st[-2] if shape[-2] > 1 else 0
+    return token, st[-2]
 
 
-def _flat(t: torch.Tensor, unit: int) -> Tuple[torch.Tensor, int, int]:
-    """t [.., heads, D], or a copy that the kernel can read, with its strides."""
-    st = _token_stride(t)
-    if st is None or st[0] % 2 or st[1] % 2 or t.data_ptr() % unit:
+def _readable(t: torch.Tensor, shape, unit: int):
+    """t [.., heads, D], or a copy that the kernel can read; its address and (token, head) strides."""
+    st, at = _token_stride(shape, t.stride()), t.data_ptr()
+    if st is None or at % unit or (st[0] % 2 and shape[0] > 1) or (st[1] % 2 and shape[-2] > 1):
         t = _lib.aligned(t, 16)
-        st = (t.size(-2) * t.size(-1), t.size(-1))
-    return t, st[0], st[1]
+        st, at = (shape[-2] * shape[-1], shape[-1]), t.data_ptr()
+    return t, at, st[0] & -2, st[1] & -2  # (a stride that no second row needs may be odd)
+
+
+def _writable(name: str, out: torch.Tensor, shape, dtype, unit: int):
+    if out.shape != shape or out.dtype is not dtype:
+        raise RuntimeError(f"{name} must be {dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    st, at = _token_stride(shape, out.stride()), out.data_ptr()
+    many, heads = math.prod(shape[:-2]) > 1, shape[-2] > 1
+    if st is None or at % unit or (many and (st[0] % 2 or not st[0])) or (heads and (st[1] % 2 or not st[1])):
+        raise RuntimeError(f"{name}: rows must be contiguous, aligned to two elements and one stride per token apart, got strides {out.stride()}")
+    return at, st[0] & -2, st[1] & -2
 
 
 def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: AxisRotary, *, inverse: bool = False,
@@ -96,49 +107,56 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     rows, are read in place.  positions int32 or int64 [axes, ..], with at least the rotary's axes, over the same tokens
     (expanded views too); negative ones turn back.  inverse turns by the negative angles.  out_q, out_k: written instead of new
     tensors; they may be q and k themselves, or other views with one stride per token."""
-    shape, dtype = q.shape, q.dtype
-    if len(shape) < 3 or shape[-1] != rotary.dim:
-        raise RuntimeError(f"q must be [.., H, {rotary.dim}], got {tuple(shape)}")
+    # (made once per layer and token: what a tensor method costs counts here, as in aetherkv.paged)
+    shape, dtype, dim = q.shape, q.dtype, rotary.dim
+    lead = shape[:-2]
+    if len(shape) < 3 or shape[-1] != dim:
+        raise RuntimeError(f"q must be [.., H, {dim}], got {tuple(shape)}")
     code = _TYPES.get(dtype)
     if code is None or (k is not None and k.dtype is not dtype):
         raise RuntimeError(f"q and k must be bfloat16, float16 or float32 alike, got {dtype} and {None if k is None else k.dtype}")
-    if k is not None and (k.shape[:-2] != shape[:-2] or len(k.shape) != len(shape) or k.shape[-1] != rotary.dim):
-        raise RuntimeError(f"k must be [.., kv_heads, {rotary.dim}] over q's tokens {tuple(shape[:-2])}, got {tuple(k.shape)}")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if positions.shape[1:] != shape[:-2] or positions.dim() < 2 or positions.size(0) < rotary.axes:
-        raise RuntimeError(f"positions must be [axes, {', '.join(map(str, shape[:-2]))}] with {rotary.axes} axes or more, got "
-                           f"{tuple(positions.shape)}")
-    _one_device(rotary._index, q, k, positions, out_q, out_k)
-    if k is None and out_k is not None:
+    ptype, pshape = positions.dtype, positions.shape
+    if ptype is not torch.int32 and ptype is not torch.int64:
+        raise RuntimeError(f"positions must be int32 or int64, got {ptype}")
+    if pshape[1:] != lead or len(pshape) < 2 or pshape[0] < rotary.axes:
+        raise RuntimeError(f"positions must be [axes, {', '.join(map(str, lead))}] with {rotary.axes} axes or more, got {tuple(pshape)}")
+    index, dev = rotary._index, rotary.device
+    _one_device(index, q, k, positions, out_q, out_k)
+    kt = kh = hk = kot = koh = 0
+    kp = kop = None
+    if k is not None:
+        kshape = k.shape
+        if kshape[:-2] != lead or len(kshape) != len(shape) or kshape[-1] != dim:
+            raise RuntimeError(f"k must be [.., kv_heads, {dim}] over q's tokens {tuple(lead)}, got {tuple(kshape)}")
+        hk = kshape[-2]
+    elif out_k is not None:
         raise RuntimeError("out_k without k")
-    n = math.prod(shape[:-2])
-    if positions.dim() > 2:
-        positions = positions.reshape(positions.size(0), n)
+    n = lead[0] if len(lead) == 1 else math.prod(lead)
     unit = 4 if dtype is not torch.float32 else 8
-    tensors = []
-    for name, x, out in (("out_q", q, out_q), ("out_k", k, out_k)):
-        if x is None:
-            tensors.append((None, 0, 0, None, None, 0, 0, 0))
-            continue
-        if out is None:
-            out = torch.empty(x.shape, dtype=dtype, device=x.device)
-        elif out.shape != x.shape or out.dtype is not dtype:
-            raise RuntimeError(f"{name} must be {dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
-        to = _token_stride(out)
-        if n and (to is None or to[0] % 2 or to[1] % 2 or out.data_ptr() % unit or (n > 1 and not to[0]) or (x.size(-2) > 1 and not to[1])):
-            raise RuntimeError(f"{name}: rows must be contiguous, aligned to two elements and one stride per token apart, got strides {out.stride()}")
-        flat, t, h = _flat(x, unit)
-        tensors.append((flat.data_ptr(), t, h, out, out.data_ptr(), *(to or (0, 0)), x.size(-2)))
-    (qp, qt, qh, oq, oqp, oqt, oqh, H), (kp, kt, kh, ok, okp, okt, okh, hk) = tensors
+    H = shape[-2]
+    if out_q is None:
+        out_q = torch.empty(shape, dtype=dtype, device=dev)
+        qop, qot, qoh = out_q.data_ptr(), H * dim, dim
+    else:
+        qop, qot, qoh = _writable("out_q", out_q, shape, dtype, unit)
+    if k is not None:
+        if out_k is None:
+            out_k = torch.empty(kshape, dtype=dtype, device=dev)
+            kop, kot, koh = out_k.data_ptr(), hk * dim, dim
+        else:
+            kop, kot, koh = _writable("out_k", out_k, kshape, dtype, unit)
     if n == 0 or H + hk == 0:
-        return oq, ok
-    st = positions.stride()
-    dev = rotary.device
+        return out_q, out_k
+    q, qp, qt, qh = _readable(q, shape, unit)
+    if k is not None:
+        k, kp, kt, kh = _readable(k, kshape, unit)
+    if len(pshape) > 2:
+        positions = positions.reshape(pshape[0], n)
+    pa, pt = positions.stride()
     with _lib.on_device(dev):
         rc = _lib.hot("aekv_rotate_axes")(
-            qp, kp, code, n, H, hk, rotary.dim, qt, qh, kt, kh, positions.data_ptr(), _lib.I32 if positions.dtype is torch.int32 else _lib.I64,
-            positions.size(0), st[0], st[1], *rotary._args, int(bool(inverse)), oqp, okp, oqt, oqh, okt, okh, _lib.raw_stream(dev))
+            qp, kp, code, n, H, hk, dim, qt, qh, kt, kh, positions.data_ptr(), _lib.I32 if ptype is torch.int32 else _lib.I64,
+            pshape[0], pa, pt, *rotary._args, 1 if inverse else 0, qop, kop, qot, qoh, kot, koh, _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, "aekv_rotate_axes")
-    return oq, ok
+    return out_q, out_k

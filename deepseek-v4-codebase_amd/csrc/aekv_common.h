@@ -130,6 +130,13 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+// Two fp32 -> packed f16x2 with round-to-nearest-even (v_cvt_pk_f16_f32).
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  f32x2_t v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+
 // Lane exchange with partner lane ^ HL inside a wave64, on the VALU (no LDS pipe):
 //   1, 2  DPP quad_perm [1,0,3,2] / [2,3,0,1];
 //   4     DPP row_half_mirror (i ^ 7) then quad_perm [3,2,1,0] (i ^ 3);

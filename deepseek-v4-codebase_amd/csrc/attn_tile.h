@@ -45,7 +45,7 @@ struct Elem<AEKV_F16> {
   static constexpr float kLift = 7.0f;  // (kMargin more and 2^15 is below the largest)
   __device__ static f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   __device__ static f32x4_t mma16(v8 a, v8 b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-  __device__ static uint32_t pack(float lo, float hi) { return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16); }
+  __device__ static uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
   __device__ static float value(uint32_t u) { return f16_to_f32(u); }
 };
 

@@ -78,7 +78,7 @@ struct Vec {
 #pragma unroll
     for (int i = 0; i < kBytes / 4; ++i) {
       if constexpr (DT == AEKV_F32) b.u[i] = __builtin_bit_cast(uint32_t, f[i]);
-      else if constexpr (DT == AEKV_F16) b.u[i] = f32_to_f16_bits(f[2 * i]) | (f32_to_f16_bits(f[2 * i + 1]) << 16);
+      else if constexpr (DT == AEKV_F16) b.u[i] = pack_f16x2(f[2 * i], f[2 * i + 1]);
       else b.u[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
     }
     *this = __builtin_bit_cast(Vec, b);
