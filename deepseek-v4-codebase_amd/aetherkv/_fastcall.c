@@ -503,7 +503,24 @@ static PyObject* f_pool_fork(PyObject* self, PyObject* const* args, Py_ssize_t n
                                (const int32_t*)target, n, ps, (int32_t*)refs, pages, ws, wsb, st));
 }
 
+/* aekv_pool_compact(table, n, refs, pages, segments, n_segments, ws, ws_bytes, stream) */
+static PyObject* f_pool_compact(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (want_args(nargs, 9, "aekv_pool_compact")) return NULL;
+  void* table = ptr_arg(A(0));
+  const int64_t n = i64_arg(A(1));
+  void* refs = ptr_arg(A(2));
+  const int64_t pages = i64_arg(A(3));
+  void* segs = ptr_arg(A(4));
+  const int64_t n_segs = i64_arg(A(5));
+  void* ws = ptr_arg(A(6));
+  const size_t wsb = (size_t)i64_arg(A(7));
+  void* st = ptr_arg(A(8));
+  RETURN_STATUS(aekv_pool_compact((int32_t*)table, n, (int32_t*)refs, pages, segs, n_segs, ws, wsb, st));
+}
+
 static PyMethodDef methods[] = {
+    {"aekv_pool_compact", (PyCFunction)(void (*)(void))f_pool_compact, METH_FASTCALL, NULL},
     {"aekv_cross_attention", (PyCFunction)(void (*)(void))f_cross_attention, METH_FASTCALL, NULL},
     {"aekv_rotate_axes", (PyCFunction)(void (*)(void))f_rotate_axes, METH_FASTCALL, NULL},
     {"aekv_pool_reserve", (PyCFunction)(void (*)(void))f_pool_reserve, METH_FASTCALL, NULL},

@@ -125,7 +125,7 @@ def lib() -> ctypes.CDLL:
         "aekv_pool_reserve": ([P, I64_, I64_, P, P, P, I32_, P, P, P, I64_, P, I64_, P, SZ, P], ctypes.c_int),
         "aekv_pool_release": ([P, I64_, I64_, P, I32_, P, I64_, P], ctypes.c_int),
         "aekv_pool_fork": ([P, I64_, I64_, P, P, P, I64_, I32_, P, I64_, P, SZ, P], ctypes.c_int),
-        "aekv_pool_compact": ([P, I64_, P, I64_, P, SZ, P], ctypes.c_int),
+        "aekv_pool_compact": ([P, I64_, P, I64_, P, I64_, P, SZ, P], ctypes.c_int),
         "aekv_pool_renumber": ([P, I64_, I64_, P, SZ, P], ctypes.c_int),
         "aekv_sink_attention_workspace_size": ([I32_, I64_, I64_, I64_, I64_, I64_, I64_], SZ),
     }

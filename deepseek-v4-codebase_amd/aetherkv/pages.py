@@ -148,13 +148,15 @@ class PagePool:
         for t in page_tables:
             self._table(t)
         _one_device(self._index, *page_tables, workspace)
-        # two calls use the workspace: a kept one could serve another call between them
-        ws = _given(workspace) if workspace is not None else self.workspace(0, 0)
+        first, *others = page_tables
         dev = self.device
         with _lib.on_device(dev):
             stream = _lib.raw_stream(dev)
+            # (several calls use the workspace where there are other tables: a kept one could serve another call between them)
+            ws = _given(workspace) if workspace is not None else self.workspace(0, 0) if others else _lib.workspace(_lib.pool_ws_bytes(0, 0, 0, self.pages), dev, stream)
             at, size = ws.data_ptr(), ws.numel()
-            L = _lib.lib()
-            _lib.check(L.aekv_pool_compact(self._refs.data_ptr(), self.pages, *self._args, at, size, stream), "aekv_pool_compact")
-            for t in page_tables:
-                _lib.check(L.aekv_pool_renumber(t.data_ptr(), t.numel(), self.pages, at, size, stream), "aekv_pool_renumber")
+            rc = _lib.hot("aekv_pool_compact")(first.data_ptr(), first.numel(), self._refs.data_ptr(), self.pages, *self._args, at, size, stream)
+            if rc:
+                _lib.check(rc, "aekv_pool_compact")
+            for t in others:
+                _lib.check(_lib.lib().aekv_pool_renumber(t.data_ptr(), t.numel(), self.pages, at, size, stream), "aekv_pool_renumber")

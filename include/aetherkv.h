@@ -397,7 +397,7 @@ int aekv_rotate_axes(const void* q, const void* k, int32_t dtype, int64_t n, int
                      int64_t qo_head_stride, int64_t ko_token_stride, int64_t ko_head_stride, void* stream);
 
 /* ---- the life of a pool's pages --------------------------------------------------------------------
- * refs int32 [pages]: entries of page tables that hold a page; unused at 0.  Tables int32 [B, max_pages] (at most 8192 rows,
+ * refs int32 [pages]: entries of page tables that hold a page; unused at 0.  Tables int32 [B, max_pages] (at most 4096 rows,
  * 2^30 entries) are changed in place; an entry outside 0 .. pages - 1 holds none.  segments: n_segments times three uint64, the
  * address of a part of page 0 in some tensor, the bytes from a page to the next, the part's bytes (a multiple of 16, at most
  * 4096): together all that is copied with a page.  The calls of one pool run one after another.  Workspaces: 16-byte aligned,
@@ -419,9 +419,9 @@ int aekv_pool_release(int32_t* table, int64_t B, int64_t max_pages, const int32_
 int aekv_pool_fork(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* source,
                    const int32_t* target, int64_t n, int32_t page_size, int32_t* refs, int64_t pages, void* ws,
                    size_t ws_bytes, void* stream);
-/* With n pages in use, the k-th unused one below n takes the k-th one in use from n on (bytes and refs); then
- * aekv_pool_renumber, with the same workspace, for every table (n entries) that holds the pool's pages. */
-int aekv_pool_compact(int32_t* refs, int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes,
+/* With u pages in use, the k-th unused one below u takes the k-th one in use from u on (bytes and refs), and the table (n
+ * entries) follows; then aekv_pool_renumber, with the same workspace, for every other table that holds the pool's pages. */
+int aekv_pool_compact(int32_t* table, int64_t n, int32_t* refs, int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes,
                       void* stream);
 int aekv_pool_renumber(int32_t* table, int64_t n, int64_t pages, const void* ws, size_t ws_bytes, void* stream);
 

@@ -45,8 +45,8 @@ def _fork(lib, table=FAKE, B=3, W=4, filled=FAKE, source=FAKE, target=FAKE, n=2,
     return lib.aekv_pool_fork(table, B, W, filled, source, target, n, size, refs, pages, ws, wsb, None)
 
 
-def _compact(lib, refs=FAKE, pages=8, segs=FAKE, n=4, ws=FAKE, wsb=1 << 30):
-    return lib.aekv_pool_compact(refs, pages, segs, n, ws, wsb, None)
+def _compact(lib, table=FAKE, entries=12, refs=FAKE, pages=8, segs=FAKE, n=4, ws=FAKE, wsb=1 << 30):
+    return lib.aekv_pool_compact(table, entries, refs, pages, segs, n, ws, wsb, None)
 
 
 def test_cross_refusals(lib):
@@ -84,7 +84,7 @@ def test_pool_refusals(lib):
         for size in (0, 8, 24, 8192, -16):
             assert call(lib, size=size) == L.ERR_VALUE
         assert call(lib, B=-1) == L.ERR_SHAPE and call(lib, W=-1) == L.ERR_SHAPE and call(lib, pages=-1) == L.ERR_SHAPE
-        assert call(lib, B=8193) == L.ERR_UNSUPPORTED and call(lib, W=1 << 29) == L.ERR_UNSUPPORTED and call(lib, pages=1 << 30) == L.ERR_UNSUPPORTED
+        assert call(lib, B=4097) == L.ERR_UNSUPPORTED and call(lib, W=1 << 29) == L.ERR_UNSUPPORTED and call(lib, pages=1 << 30) == L.ERR_UNSUPPORTED
         assert call(lib, table=None) == L.ERR_VALUE and call(lib, refs=None) == L.ERR_VALUE
         assert call(lib, B=0, table=None) == L.OK and call(lib, W=0, table=None) == L.OK
     for name in ("filled", "wanted", "marks", "lacking"):
@@ -92,7 +92,7 @@ def test_pool_refusals(lib):
     assert _reserve(lib, segs=None) == L.ERR_VALUE and _reserve(lib, segs=ODD) == L.ERR_VALUE and _reserve(lib, n=-1) == L.ERR_SHAPE
     assert _release(lib, keep=None) == L.ERR_VALUE
     assert _fork(lib, source=None) == L.ERR_VALUE and _fork(lib, n=-1) == L.ERR_SHAPE and _fork(lib, n=0, source=None) == L.OK and _fork(lib, n=1 << 30) == L.ERR_SHAPE
-    assert _compact(lib, pages=-1) == L.ERR_SHAPE and _compact(lib, refs=None) == L.ERR_VALUE and _compact(lib, segs=None) == L.ERR_VALUE
+    assert _compact(lib, pages=-1) == L.ERR_SHAPE and _compact(lib, entries=-1) == L.ERR_SHAPE and _compact(lib, table=None) == L.ERR_VALUE and _compact(lib, refs=None) == L.ERR_VALUE and _compact(lib, segs=None) == L.ERR_VALUE
     size = lib.aekv_pool_workspace_size
     for call, need in ((_reserve, size(3, 4, 0, 0)), (_fork, size(0, 4, 2, 0)), (_compact, size(0, 0, 0, 8))):
         assert need > 0 and call(lib, wsb=need - 1) == L.ERR_WORKSPACE and call(lib, ws=None) == L.ERR_WORKSPACE and call(lib, ws=ctypes.c_void_p(0x10008)) == L.ERR_ALIGN
