@@ -706,9 +706,9 @@ CrossPlan plan_cross(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, 
   const int64_t rows = n_q * (H / heads), runs = E > 0 && E < B ? E : B, each = ceil_div(rows, runs);
   const int64_t resident = d == 64 ? 768 : 512;
   if (each <= 32) {
-    p.rows = each <= 16 ? 16 : 32, p.groups = d == 64 ? 1024 : 512, p.least = 1;
+    p.rows = each <= 16 ? 16 : 32, p.groups = 256, p.least = 1;
   } else {
-    p.rows = 128, p.groups = resident, p.least = 8;
+    p.rows = 128, p.groups = resident, p.least = 3;
   }
   const int64_t keys = p.rows <= 32 ? kFewKeys : kManyKeys, start = p.rows <= 32 ? kFewStart : kManyStart;
   const double most = (static_cast<double>(rows / p.rows) + B) * heads * (n_k / keys + 1 + start) / p.least + 1.0;  // parts of the longest line

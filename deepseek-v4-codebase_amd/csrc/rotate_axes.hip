@@ -10,6 +10,10 @@
 // A workgroup takes some tokens with all their heads, so that the heads share a token's cos and sin through LDS; its first
 // loads are under way while those are made.  A thread holds whole pairs: V neighbouring dims (adjacent), or V dims and their
 // partners (halves), so out may be x itself.
+//
+// Bound by reading and writing the rows: 32768 tokens of 12 + 4 heads of 128 in bf16, 268 MB in 50 us, 5.3 TB/s, where a copy of 256
+// MiB reaches 5.5; 5003 tokens of 16 + 16 heads of 64 in fp32, 82 MB in 18 us.  64 tokens take 3.8 us, a launch.  Rows of a
+// workgroup and units under way between half and twice these change no case by more than 5 %.
 #include "aekv_common.h"
 
 namespace aekv {
@@ -98,7 +102,7 @@ __device__ __forceinline__ float2 turn(double p, float f) {
 template <int DT, int V, bool HALVES>
 __global__ __launch_bounds__(kThreads) void rotate_axes_kernel(RotateArgs a) {
   constexpr int kElem = DT == AEKV_F32 ? 4 : 2;
-  constexpr int kBatch = V * kElem >= 32 ? 2 : 4;  // units a thread has under way
+  constexpr int kBatch = V * kElem * (HALVES ? 2 : 1) >= 32 ? 2 : 4;  // units a thread has under way
   __shared__ float2 table[kTable];
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * a.block;
   const int tokens = static_cast<int>(a.n - n0 < a.block ? a.n - n0 : a.block);
