@@ -35,6 +35,8 @@ class PagePool:
         if not caches:
             raise ValueError("PagePool needs a cache")
         head = caches[0]
+        if head.pages < 1:
+            raise ValueError("PagePool needs caches with pages")
         for c in caches[1:]:
             if c.pages != head.pages or c.page_size != head.page_size or c._index != head._index:
                 raise RuntimeError(f"the caches of a pool need the same pages, page size and device, got {c.pages} x {c.page_size} on {c.device} beside "

@@ -80,21 +80,20 @@ def _token_stride(shape, st) -> Optional[Tuple[int, int]]:
     return token, st[-2]
 
 
-def _readable(t: torch.Tensor, shape, unit: int):
-    """t [.., heads, D], or a copy that the kernel can read; its address and (token, head) strides."""
+def _readable(t: torch.Tensor, shape, n: int, unit: int):
+    """t [.., heads, D] of n tokens, or a copy that the kernel can read; its address and (token, head) strides."""
     st, at = _token_stride(shape, t.stride()), t.data_ptr()
-    if st is None or at % unit or (st[0] % 2 and shape[0] > 1) or (st[1] % 2 and shape[-2] > 1):
+    if st is None or at % unit or (st[0] % 2 and n > 1) or (st[1] % 2 and shape[-2] > 1):
         t = _lib.aligned(t, 16)
         st, at = (shape[-2] * shape[-1], shape[-1]), t.data_ptr()
     return t, at, st[0] & -2, st[1] & -2  # (a stride that no second row needs may be odd)
 
 
-def _writable(name: str, out: torch.Tensor, shape, dtype, unit: int):
+def _writable(name: str, out: torch.Tensor, shape, n: int, dtype, unit: int):
     if out.shape != shape or out.dtype is not dtype:
         raise RuntimeError(f"{name} must be {dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     st, at = _token_stride(shape, out.stride()), out.data_ptr()
-    many, heads = math.prod(shape[:-2]) > 1, shape[-2] > 1
-    if st is None or at % unit or (many and (st[0] % 2 or not st[0])) or (heads and (st[1] % 2 or not st[1])):
+    if st is None or at % unit or (n > 1 and (st[0] % 2 or not st[0])) or (shape[-2] > 1 and (st[1] % 2 or not st[1])):
         raise RuntimeError(f"{name}: rows must be contiguous, aligned to two elements and one stride per token apart, got strides {out.stride()}")
     return at, st[0] & -2, st[1] & -2
 
@@ -138,18 +137,18 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
         out_q = torch.empty(shape, dtype=dtype, device=dev)
         qop, qot, qoh = out_q.data_ptr(), H * dim, dim
     else:
-        qop, qot, qoh = _writable("out_q", out_q, shape, dtype, unit)
+        qop, qot, qoh = _writable("out_q", out_q, shape, n, dtype, unit)
     if k is not None:
         if out_k is None:
             out_k = torch.empty(kshape, dtype=dtype, device=dev)
             kop, kot, koh = out_k.data_ptr(), hk * dim, dim
         else:
-            kop, kot, koh = _writable("out_k", out_k, kshape, dtype, unit)
+            kop, kot, koh = _writable("out_k", out_k, kshape, n, dtype, unit)
     if n == 0 or H + hk == 0:
         return out_q, out_k
-    q, qp, qt, qh = _readable(q, shape, unit)
+    q, qp, qt, qh = _readable(q, shape, n, unit)
     if k is not None:
-        k, kp, kt, kh = _readable(k, kshape, unit)
+        k, kp, kt, kh = _readable(k, kshape, n, unit)
     if len(pshape) > 2:
         positions = positions.reshape(pshape[0], n)
     pa, pt = positions.stride()

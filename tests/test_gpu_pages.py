@@ -168,7 +168,7 @@ def test_long_lives(dev, seed):
             b.compact()
 
 
-@pytest.mark.parametrize("pages,rows,width", [(5000, 1500, 3), (3000, 2, 1400), (40000, 64, 500), (1023, 33, 31), (1024, 32, 32), (1025, 1025, 1)])
+@pytest.mark.parametrize("pages,rows,width", [(5000, 1500, 3), (3000, 2, 1400), (40000, 64, 500), (1023, 33, 31), (1024, 32, 32), (1025, 1025, 1), (9000, 128, 32), (9000, 241, 17)])
 def test_large_tables(dev, pages, rows, width):
     b = Both(dev, pages, 16, rows, width, layers=1, heads=1)
     rng = random.Random(pages)
@@ -180,6 +180,19 @@ def test_large_tables(dev, pages, rows, width):
     b.reserve(n, n, first=[0] * rows)
     b.release([x if i % 3 else 0 for i, x in enumerate(n)])
     b.compact()
+
+
+def test_every_entry_shares_its_page(dev):
+    """All entries of a call share pages, up to and past the number that the kernel keeps: 64 rows over one prompt, in calls that
+    write some of them or all."""
+    for width in (1, 63, 64, 65):
+        b = Both(dev, 64 * width + 70, 16, 64, width, layers=1, heads=1)
+        n = [width * 16 - 3] + [0] * 63
+        b.reserve([0] * 64, n)
+        b.fork(n, [0] * 63, list(range(1, 64)))
+        n = [n[0]] * 64
+        b.reserve(n, [x + 2 if i % 3 else 0 for i, x in enumerate(n)])  # every third row writes nothing
+        b.reserve(n, n, first=[0] * 64)
 
 
 def test_many_tables_hold_one_pool(dev):
@@ -319,6 +332,9 @@ def test_refusals(dev):
     a, b = (PagedKVCache(PolarQuant(4), n, 2, 64, page_size=16, device=dev) for n in (8, 9))
     with pytest.raises(RuntimeError, match="same pages"):
         PagePool([a, b])
+    none = PagedKVCache.from_tensors(PolarQuant(4), *(torch.empty((0, 2, 16, 32) if i % 2 == 0 else (0, 2, 16), dtype=torch.uint8 if i % 2 == 0 else torch.float32, device=dev) for i in range(4)))
+    with pytest.raises(ValueError, match="pages"):
+        PagePool([none])
     with pytest.raises(RuntimeError, match="refs"):
         PagePool([a], refs=torch.zeros(9, dtype=torch.int32, device=dev))
     with pytest.raises(RuntimeError, match="refs"):

@@ -97,6 +97,20 @@ def test_in_place_views_and_strides(dev):
         assert (out[:, 1::2] == 7).all()
 
 
+def test_odd_strides_and_leading_dims_of_one(dev):
+    """Rows an odd number of elements apart are copied, whichever leading dim they follow; a stride that no second row needs is not
+    looked at."""
+    axis = _axis(16, 2)
+    for dtype in DTYPES:
+        rotary = AxisRotary(rope_inv_freq(32, 10000.0, dev), axis, 32)
+        base = torch.randn(4000, device=dev, generator=_gen(dev, 0)).to(dtype)
+        pos = torch.randint(0, 3000, (2, 12), device=dev, generator=_gen(dev, 1))
+        for shape, st, p in (((1, 5, 3, 32), (0, 97, 32, 1), pos[:, None, :5]), ((5, 1, 3, 32), (97, 7, 32, 1), pos[:, :5, None]), ((1, 1, 3, 32), (3, 5, 32, 1), pos[:, :1, None]),
+                             ((5, 1, 32), (96, 1, 1), pos[:, :5]), ((5, 3, 32), (99, 33, 1), pos[:, :5]), ((2, 6, 3, 32), (582, 97, 32, 1), pos.view(2, 2, 6)), ((2, 6, 3, 32), (584, 96, 32, 1), pos.view(2, 2, 6)),
+                             ((1, 1, 2, 3, 32), (0, 0, 96, 32, 1), pos[:, None, None, :2])):
+            _check(base[2:].as_strided(shape, st, 2), None, p, rotary, axis)
+
+
 def test_inverse_is_the_gradient(dev):
     """Turning back is the transpose: <rotate(x), y> = <x, inverse(y)>, and differences agree with it."""
     axis = _axis(16, 2)
