@@ -269,9 +269,9 @@ __global__ __launch_bounds__(kThreads) void pool_reserve_kernel(PoolArgs a) {
     if (b < a.B) {
       const int32_t w = a.wanted[b];
       filled = a.filled[b];
-      const int32_t f = a.first ? a.first[b] : filled;
-      from = f > 0 ? f >> a.shift : 0;
-      n = max(pages_of(a, w) - from, 0);
+      const int32_t f = max(a.first ? a.first[b] : filled, 0);
+      from = f >> a.shift;
+      n = w > f ? max(pages_of(a, w) - from, 0) : 0;  // (no slots: no pages, within a page too)
     }
     int32_t all;
     const int32_t before = scan.any(n, &all);

@@ -82,7 +82,7 @@ class PoolRef:
 
     def reserve(self, table, filled, wanted, first=None):
         first = filled if first is None else first
-        entries = [(b, i) for b in range(len(table)) for i in range(max(first[b], 0) // self.size, self.pages(wanted[b], len(table[b])))]
+        entries = [(b, i) for b in range(len(table)) if wanted[b] > max(first[b], 0) for i in range(max(first[b], 0) // self.size, self.pages(wanted[b], len(table[b])))]
         holders = {}
         for b, i in entries:
             if self.has(table[b][i]) and self.refs[table[b][i]] > 1:

@@ -220,6 +220,56 @@ def test_graphs_and_streams(dev, lq):
             assert torch.equal(out, call(d))
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 128)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_many_rows_in_many_sequences(dev, dtype, dim, shared):
+    """Long and short answers of more sequences than one launch takes."""
+    B = 300
+    lq = [(29 * i) % 90 if i % 7 else 0 for i in range(B)]
+    states = [b // 9 if b % 50 else -1 for b in range(B)] if shared else None
+    _check(dev, dtype, dim, 2, 1, lq, [(67 * i) % 230 for i in range(34 if shared else B)], states=states, seed=4, sink=True, pad=2)
+
+
+def test_a_captured_call_of_several_launches(dev):
+    """More sequences than one launch takes, one workspace for all launches of a call, replayed with other states and lengths."""
+    B = 300
+    for per in (1, 25):
+        q = torch.randn(per * B, 4, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+        k, v = (torch.randn(900, 2, 64, device=dev, generator=_gen(dev, i)).bfloat16() for i in (1, 2))
+        ck, st, cq = _t([0, 500, 500, 900], dev), _t([b % 3 for b in range(B)], dev), _t([per * b for b in range(B + 1)], dev)
+        call = lambda: cross_attention(q, k, v, ck, 0.1, cu_seqlens=cq, states=st, return_lse=True)  # noqa: E731
+        call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = call()
+        for ends, pick in (([0, 500, 500, 900], lambda b: b % 3), ([0, 10, 900, 900], lambda b: b // 100), ([0, 0, 0, 1], lambda b: 2), ([0, 300, 600, 900], lambda b: b % 4 - 1)):
+            ck.copy_(_t(ends, dev))
+            st.copy_(_t([pick(b) for b in range(B)], dev))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs, call()):
+                assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits_and_shared_strides(dev):
+    """Rows of keys and values 16 MB apart (their offsets pass 2^32 elements); heads that are one and the same."""
+    stride, M = 8388600, 600
+    base = torch.empty(M * stride, dtype=torch.bfloat16, device=dev)
+    kv = base.view(M, stride)[:, :256].view(M, 2, 2, 64)
+    kv.copy_(torch.randn(M, 2, 2, 64, device=dev, generator=_gen(dev, 1)))
+    for lq in (1, 60):
+        q = torch.randn(lq, 4, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+        cu, cq = _t([0, M], dev), _t([0, lq], dev)
+        near = kv.contiguous()
+        assert torch.equal(cross_attention(q, kv[:, 0], kv[:, 1], cu, 0.1, cu_seqlens=cq), cross_attention(q, near[:, 0], near[:, 1], cu, 0.1, cu_seqlens=cq))
+        k, v = (near[:, i, :1].expand(M, 2, 64) for i in range(2))
+        assert torch.equal(cross_attention(q, k, v, cu, 0.1, cu_seqlens=cq), cross_attention(q, k.contiguous(), v.contiguous(), cu, 0.1, cu_seqlens=cq))
+    wide = base.as_strided((3, 2, 64), (8388608, 64, 1))
+    with pytest.raises(RuntimeError, match="stride"):
+        cross_attention(q, wide, wide, _t([0, 3], dev), 0.1, cu_seqlens=cq)
+
+
 def test_empty_calls(dev):
     q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=dev)
     k = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)

@@ -115,6 +115,18 @@ def test_the_same_row_twice_and_rows_outside(dev):
     b.fork(n, [], [])
 
 
+def test_rows_that_write_nothing(dev):
+    """A row without slots to write takes no page, and keeps what it shares, where the pool is out of pages too."""
+    b = Both(dev, 4, 16, 3, 3)
+    b.reserve([0] * 3, [40, 0, 0])
+    b.fork([40, 0, 0], [0, 0], [1, 2])
+    b.reserve([40] * 3, [40, 41, 40])  # one copy: the others write nothing
+    assert b.rows == [[0, 1, 2], [0, 1, 3], [0, 1, 2]] and b.pool.lacking.item() == 0
+    b.reserve([40, 41, 40], [40, 41, 39], first=[40, 47, 100])
+    b.reserve([0, 0, 0], [0, 0, 0])
+    assert b.rows == [[0, 1, 2], [0, 1, 3], [0, 1, 2]]
+
+
 def test_more_than_the_pool_has(dev):
     b = Both(dev, 5, 16, 3, 4)
     b.reserve([0, 0, 0], [40, 40, 40])
@@ -248,6 +260,108 @@ def test_captured_and_replayed(dev):
         b.check()
         if step == 1:
             b.compact()
+
+
+def test_caches_of_several_forms_and_sizes(dev):
+    """One pool over caches of other widths, heads and dims: every tensor's pages move alike."""
+    caches = [PagedKVCache(PolarQuant(bits), 24, heads, dim, page_size=32, device=dev) for bits, heads, dim in ((4, 1, 64), (8, 3, 128), (8, 1, 64), (4, 5, 128))]
+    gen = torch.Generator(device=dev).manual_seed(0)
+    for c in caches:
+        for t in c._tensors:
+            t.copy_(torch.randint(1, 100, t.shape, device=dev, generator=gen))
+    before = [t.clone() for c in caches for t in c._tensors]
+    pool, table, n = PagePool(caches), torch.full((2, 4), -1, dtype=torch.int32, device=dev), _t([100, 0], dev)
+    pool.reserve(table, _t([0, 0], dev), n)
+    pool.fork(table, n, _t([0], dev), _t([1], dev))
+    pool.reserve(table, _t([100, 100], dev), _t([100, 101], dev), first=_t([100, 0], dev))  # copies of all four pages
+    assert table.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7]]
+    for t, was in zip((t for c in caches for t in c._tensors), before):
+        assert torch.equal(t[4:8], was[:4]) and torch.equal(t[:4], was[:4]) and torch.equal(t[8:], was[8:])
+    pool.release(table, _t([0, 100], dev))
+    pool.compact(table)
+    assert table.tolist() == [[-1] * 4, [0, 1, 2, 3]]
+
+
+def test_pages_past_32_bits(dev):
+    """Tensors of 4.7 GB: copies from and to their last pages."""
+    pages = 9000
+    cache = PagedKVCache(PolarQuant(8), pages, 8, 128, page_size=512, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(0)
+    some = [8999, 8998, 5]
+    for t in cache._tensors:
+        t[some] = torch.randint(-100, 100, t[some].shape, device=dev, generator=gen).to(t.dtype)
+    before = [t[some].clone() for t in cache._tensors]
+    refs = torch.ones(pages, dtype=torch.int32, device=dev)
+    refs[[3, 4, 8997]] = 0
+    pool = PagePool([cache], refs=refs)
+    table = _t([some, [-1] * 3], dev)
+    n = _t([3 * 512, 0], dev)
+    pool.fork(table, n, _t([0], dev), _t([1], dev))
+    assert pool.refs[some].tolist() == [2, 2, 2]
+    pool.reserve(table, _t([3 * 512] * 2, dev), _t([0, 3 * 512], dev), first=_t([0, 0], dev))
+    assert table.tolist() == [some, [3, 4, 8997]]
+    for t, was in zip(cache._tensors, before):
+        assert torch.equal(t[some], was) and torch.equal(t[[3, 4, 8997]], was)
+    pool.release(table, _t([0, 3 * 512], dev))
+    refs.zero_()
+    refs[[3, 4, 8997]] = 1
+    pool.compact(table)
+    assert table.tolist() == [[-1] * 3, [0, 1, 2]] and refs[:3].tolist() == [1, 1, 1] and not refs[3:].any()
+    for t, was in zip(cache._tensors, before):
+        assert torch.equal(t[table[1].long()], was)
+
+
+def test_two_pools_on_two_streams(dev):
+    """Each stream has its own pool and workspace; calls of both lie between each other's."""
+    both, streams = [Both(dev, 400, 16, 32, 10, layers=1, heads=1) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    n = [[0] * 32 for _ in range(2)]
+    rng = random.Random(5)
+    for _ in range(5):
+        more = [[min(160, x + rng.randint(0, 20)) for x in row] for row in n]
+        source = [[rng.randrange(32) for _ in range(6)] for _ in range(2)]
+        args = [[_t(x, dev) for x in (n[i], more[i], source[i], list(range(6)))] for i in range(2)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                both[i].pool.reserve(both[i].table, args[i][0], args[i][1])
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                both[i].pool.fork(both[i].table, args[i][1], args[i][2], args[i][3])
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                both[i].pool.compact(both[i].table)
+        torch.cuda.synchronize()
+        for i, b in enumerate(both):
+            b.model.reserve(b.rows, n[i], more[i], None)
+            b.model.fork(b.rows, more[i], source[i], list(range(6)))
+            b.model.compact(b.rows)
+            b.check()
+            n[i] = [more[i][source[i][j]] if j < 6 else x for j, x in enumerate(more[i])]
+
+
+def test_a_captured_compaction_of_several_tables(dev):
+    b = Both(dev, 40, 16, 4, 4)
+    kept, rows = torch.full((2, 3), -1, dtype=torch.int32, device=dev), [[-1] * 3 for _ in range(2)]
+    want, side = _t([0, 0], dev), torch.cuda.Stream()
+    b.pool.compact(b.table, kept)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        b.pool.compact(b.table, kept)
+    torch.cuda.synchronize()
+    b.check()
+    for n, m, keep in (([60, 30, 10, 64], [48, 20], [0, 30, 0, 64]), ([64] * 4, [48, 48], [64, 0, 20, 3]), ([0] * 4, [0, 0], [0] * 4)):
+        b.reserve([0] * 4, n)
+        b.pool.reserve(kept, want, _t(m, dev))
+        b.model.reserve(rows, [0, 0], m)
+        b.release(keep)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        b.model.compact(b.rows, rows)
+        assert kept.tolist() == rows
+        b.check()
 
 
 def test_serving_loop(dev):

@@ -161,6 +161,18 @@ def test_graph_and_stream(dev):
         assert torch.equal(out, rotate_axes(q, None, pos, rotary)[0])
 
 
+def test_offsets_past_32_bits(dev):
+    """2^31 elements and more: the last tokens turn as they do by themselves."""
+    n, H, D = 1_100_000, 16, 128
+    x = torch.zeros(n, H, D, dtype=torch.bfloat16, device=dev)
+    x[-300:] = torch.randn(300, H, D, device=dev, generator=_gen(dev, 0))
+    pos = torch.arange(n, dtype=torch.int32, device=dev)[None]
+    rotary = AxisRotary(rope_inv_freq(D, 10000.0, dev), [0] * 64, D)
+    want, _ = rotate_axes(x[-300:].clone(), None, pos[:, -300:].clone(), rotary)
+    out, _ = rotate_axes(x, None, pos, rotary, out_q=x)
+    assert out is x and torch.equal(x[-300:], want) and not x[:-300].any()
+
+
 def test_empty(dev):
     rotary = AxisRotary(rope_inv_freq(128, 10000.0, dev), [0] * 64, 128)
     q, k = torch.empty(0, 4, 128, device=dev), torch.empty(0, 2, 128, device=dev)
