@@ -15,8 +15,8 @@
 namespace aekv {
 namespace {
 
-constexpr int kFewKeys = 128;  // keys that a workgroup takes at a time: with few rows
-constexpr int kManyKeys = 64;  // with many rows
+constexpr int kFewShift = 7;   // log2 of a unit's keys: with few rows, all heads that a workgroup takes at a time together
+constexpr int kManyShift = 6;  // with many rows
 constexpr int kFewStart = 1;   // units that a tile costs beside its own
 constexpr int kManyStart = 2;
 constexpr int kTable = 256;    // sequences of a launch
@@ -43,6 +43,7 @@ struct CrossArgs {
   int32_t clear;          // rows in no sequence: 0 to leave out as it is, 1 to write zeros
   int32_t b0, nb;         // the launch's sequences
   int32_t least;          // units of a workgroup's part at least
+  int32_t share;          // log2 of the KV heads that a workgroup takes at a time
   float scale2;           // |softmax scale| * log2(e), not 0 (times a masked product of -inf it stays -inf); where the
   int32_t flip;           // scale is negative the queries' signs are flipped: a row's largest product is its largest logit.  Where
   uint32_t nan;           // it is NaN, 1 stands for it and the queries become NaN (0x7fff is one in both types; else 0)
@@ -91,10 +92,12 @@ __device__ __forceinline__ void clear_rest(const CrossArgs& a, int32_t s0, int32
   }
 }
 
-// A row's queries as a matrix operand's register: signs and NaN as the scale asks for.
-__device__ __forceinline__ uint4 load_query(const CrossArgs& a, const uint16_t* p) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  return make_uint4((w.x ^ a.flip) | a.nan, (w.y ^ a.flip) | a.nan, (w.z ^ a.flip) | a.nan, (w.w ^ a.flip) | a.nan);
+// Queries as matrix operands, with signs and NaN as the scale asks for (rarely: else nothing waits here for them).
+template <int N>
+__device__ __forceinline__ void take_queries(const CrossArgs& a, uint4 (&q)[N]) {
+  if (!(a.flip | a.nan)) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = make_uint4((q[i].x ^ a.flip) | a.nan, (q[i].y ^ a.flip) | a.nan, (q[i].z ^ a.flip) | a.nan, (q[i].w ^ a.flip) | a.nan);
 }
 
 // Four dims (4 c ..) of one finished row, whose sum is relative to m.
@@ -110,8 +113,8 @@ __device__ __forceinline__ void finish(const CrossArgs& a, int64_t orow, int32_t
   if (a.lse && c == 0) a.lse[orow] = sum == 0.0f ? kNegInf : (up + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// The line.  All tiles' units (kKeys keys of a KV head, for a tile of kRows rows) lie in one line: run by run, its KV heads, their
-// tiles, their units.  Every workgroup takes an equal part, so that the chip is loaded evenly whatever the lengths; a tile that lies
+// The line.  All tiles' units (2^kShift keys of a KV head or of a few, for a tile of kRows rows) lie in one line: run by run, its KV
+// heads, their tiles, their units.  Every workgroup takes an equal part, so that the chip is loaded evenly whatever the lengths; a tile that lies
 // in several parts is merged by a second kernel.  A tile's units come behind kStart places without any, for what it costs
 // to begin and end one; a border among those is one before the tile.
 //
@@ -123,18 +126,24 @@ struct LineTable {
   int32_t q0[kTable], lq[kTable], k0[kTable], lk[kTable];
   int64_t sum[4];
 };
+// Units of lk keys: one at least, which ends the tile of rows that see none.
+template <int kShift>
+__device__ __forceinline__ int32_t units_of(const CrossArgs& a, int32_t lk) {
+  const int shift = kShift == kFewShift ? kShift - a.share : kShift;
+  return max((lk + (1 << shift) - 1) >> shift, 1);
+}
 struct LinePart {
   int64_t start, stop, chunk;
   int32_t index;
 };
-template <int D, int kRows, int kKeys, int kStart>
+template <int D, int kRows, int kShift, int kStart>
 __device__ __forceinline__ LinePart line_part(const CrossArgs& a, LineTable& s, int wv, int lane) {
   const int32_t s0 = query_start(a, 0), s1 = max(query_start(a, a.B), s0);
   Run r{};
   int64_t x = 0;
   const int32_t n = min(a.nb - 64 * wv, 64);
   if (n > 0 && find_run(a, a.b0 + 64 * wv, n, lane, &r))
-    x = static_cast<int64_t>((r.lq * a.G + kRows - 1) / kRows) * a.heads * (kStart + max((r.lk + kKeys - 1) / kKeys, 1));
+    x = static_cast<int64_t>((r.lq * a.G + kRows - 1) / kRows) * (a.heads >> a.share) * (kStart + units_of<kShift>(a, r.lk));
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int64_t o = __shfl_up(x, d);
@@ -164,10 +173,10 @@ __device__ __forceinline__ LinePart line_part(const CrossArgs& a, LineTable& s, 
 
 // The tile at place `pos` of the line.
 struct Place {
-  int32_t q0, n_rows, k0, lk, units, head, row0, u0, u1;  // its rows, KV head and units; the part's units of it, if u0 < u1
+  int32_t q0, n_rows, k0, lk, units, head, row0, u0, u1;  // its rows, (first) KV head and units; the part's units of it, if u0 < u1
   int64_t next;                                           // where the part goes on
 };
-template <int kRows, int kKeys, int kStart>
+template <int kRows, int kShift, int kStart>
 __device__ __forceinline__ Place line_place(const CrossArgs& a, const LineTable& s, const LinePart& p, int64_t pos) {
   int32_t lo = kTable;  // the first run that ends behind pos
 #pragma unroll
@@ -179,18 +188,21 @@ __device__ __forceinline__ Place line_place(const CrossArgs& a, const LineTable&
   const int64_t local = pos - uniform(lo ? s.end[lo - 1] : 0);
   at.q0 = __builtin_amdgcn_readfirstlane(s.q0[lo]), at.n_rows = __builtin_amdgcn_readfirstlane(s.lq[lo]) * a.G;
   at.k0 = __builtin_amdgcn_readfirstlane(s.k0[lo]), at.lk = __builtin_amdgcn_readfirstlane(s.lk[lo]);
-  at.units = max((at.lk + kKeys - 1) / kKeys, 1);
+  at.units = units_of<kShift>(a, at.lk);
   const uint32_t places = static_cast<uint32_t>(at.units) + kStart;
   const uint32_t th = static_cast<uint32_t>(local >> 31 ? static_cast<uint64_t>(local) / places : static_cast<uint32_t>(local) / places);  // (tiles x heads fit 32 bits)
   const int64_t from = pos - (local - static_cast<int64_t>(th) * places), end = from + places;  // the tile's
   at.next = end < p.stop ? end : p.stop;
   at.u0 = max(static_cast<int32_t>(pos - from) - kStart, 0), at.u1 = max(static_cast<int32_t>(at.next - from) - kStart, 0);
   const uint32_t tiles = static_cast<uint32_t>(at.n_rows + kRows - 1) / kRows;
-  at.head = static_cast<int32_t>(th / tiles), at.row0 = static_cast<int32_t>(th % tiles * kRows);
+  at.head = static_cast<int32_t>(th / tiles) << a.share, at.row0 = static_cast<int32_t>(th % tiles * kRows);
   if (pos == p.start && threadIdx.x == 0)
     a.desc[p.index] = LineTile{at.u0 > 0 ? from : -1, p.chunk, at.units, at.q0, at.n_rows, at.row0, at.head, 0};
   return at;
 }
+
+// The head that row `at` belongs to, where up to four heads have `rows` each.
+__device__ __forceinline__ int head_of_row(int at, int rows) { return (at >= rows) + (at >= 2 * rows) + (at >= 3 * rows); }
 
 // Merges the tiles that lie in several parts: workgroup i has the tile across the border to part i + 1, if that is the tile's first.
 // Bound by the chain of its loads, so that several parts' go out together and a workgroup has one row to D / 4 threads.
@@ -198,15 +210,15 @@ template <int DT, int D, int kRows, int kStart>
 __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
   const LineTile d = a.desc[blockIdx.x + 1];
   if (d.start < 0 || (d.start + kStart) / d.chunk != blockIdx.x) return;
-  const int32_t q0 = d.q0, n_rows = d.n_rows, row0 = d.row0, head = d.head;
+  const int32_t q0 = d.q0, n_rows = d.n_rows, row0 = d.row0;
   const int32_t last = static_cast<int32_t>((d.start + kStart + d.units - 1) / d.chunk);  // part of the tile's last unit
   const int first_slot = blockIdx.x * d.chunk >= d.start ? 0 : 1;
-  const int c = threadIdx.x % (D / 4), r = blockIdx.y * (256 / (D / 4)) + threadIdx.x / (D / 4);
-  const int32_t row = row0 + r;
-  if (r < kRows && row < n_rows) {
+  const int c = threadIdx.x % (D / 4), at = blockIdx.y * (256 / (D / 4)) + threadIdx.x / (D / 4), rows = min(kRows, n_rows - row0);
+  if (at < rows << a.share) {
+    const int sub = head_of_row(at, rows), r = at - sub * rows, own = d.head + sub;
     float m = kNegInf, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int CH = 4;
+    constexpr int CH = 8;
     for (int32_t w0 = blockIdx.x; w0 <= last; w0 += CH) {
       float2 ml[CH];
       float4 x[CH];
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
       for (int i = 0; i < CH; ++i) {
         const int32_t w = min(w0 + i, last);
         const int slot = w == static_cast<int32_t>(blockIdx.x) ? first_slot : 0;
-        const float* p = a.part + ((2 * static_cast<int64_t>(w) + slot) * kRows + r) * (D + 4);
+        const float* p = a.part + (((2 * static_cast<int64_t>(w) + slot) << a.share) * kRows + sub * kRows + r) * (D + 4);
         ml[i] = *reinterpret_cast<const float2*>(p);
         x[i] = *reinterpret_cast<const float4*>(p + 4 + 4 * c);
       }
@@ -235,34 +247,39 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
       }
       m = up;
     }
-    const int32_t qi = row / a.G, h = head * a.G + (row - qi * a.G);
+    const int32_t row = row0 + r, qi = row / a.G, h = own * a.G + (row - qi * a.G);
     finish<DT, D>(a, static_cast<int64_t>(q0 + qi) * a.H + h, h, c, m, l, o);
   }
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
 //
-// Tiles of 16 NT rows, bound by reading the keys and values.  A wave takes 32 keys of a unit by itself: keys go straight to
-// registers, values to its own part of LDS, both one unit ahead, and no wave waits for another before the tile's end.
+// Tiles of 16 NT rows to each of the workgroup's heads, bound by reading the keys and values: 64 sequences of up to 4096 states, 12
+// heads of 4, dim 128, 305 MB in 50 us, 6.1 TB/s where 256 MB of them can be in the last-level cache, 4.8 TB/s with the merge where
+// nothing is.  A wave takes 32 keys of a unit and head by itself: keys go straight to registers, values to its own part of LDS, both
+// one unit ahead, across tiles too, and no wave waits for another before the tile's end.  Heads that are neighbours in memory are read
+// by one workgroup at the same time: by workgroups of their own the same bytes take 11 % longer.
 //
 // Matrix layout (v_mfma_f32_16x16x32: A lane l holds A[l % 16][8 (l / 16) + j], B lane l holds B[8 (l / 16) + j][l % 16], D lane
 // l register v holds D[4 (l / 16) + v][l % 16]), g = l / 16:
 //   S^T = K Q^T: m = key, n = row; two blocks of 16 keys.
 //   O^T += V^T P^T: m = dim, n = row; lane group g holds keys 4 g + j and 16 + 4 g + j, its own scores.
 template <int DT, int D, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void cross_few_kernel(CrossArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void cross_few_kernel(CrossArgs a) {
   using E = Elem<DT>;
   using v8 = typename E::v8;
   constexpr int kRow = 2 * D, kKS = D / 32, kMB = D / 16, kRT = 16 * NT;
   constexpr int kPer = 1024 / kRow, kLoads = 32 / kPer;  // rows of a staging load, loads of 32 rows
   __shared__ __align__(16) uint8_t V0[4][32 * kRow];
   __shared__ __align__(16) uint8_t V1[4][32 * kRow];
+  __shared__ __align__(16) uint8_t s_more[NT == 1 ? 1 : 4][NT == 1 ? 16 : 32 * kRow];  // the second 16 rows' states
   __shared__ LineTable s_line;
   __shared__ float2 s_ml[4][kRT];
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const LinePart line = line_part<D, kRT, kFewKeys, kFewStart>(a, s_line, wv, lane);
+  const LinePart line = line_part<D, kRT, kFewShift, kFewStart>(a, s_line, wv, lane);
   if (line.start >= line.stop) return;
+  const int shift = kFewShift - a.share, sub = wv & ((1 << a.share) - 1), block = wv >> a.share;  // the wave's head and keys of a unit
 
   // staging: load i of 32 rows writes 1024 bytes, lane l at + 16 l, so lane l loads the chunk that the swizzle puts there
   const int key_in = 16 * lane / kRow, placed = (16 * lane % kRow) / 16;
@@ -278,42 +295,68 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
     tA[e] = key * kRow + ((x ^ swizzle<D>(key & 15)) << 4) + ((n16 & 1) << 3);
   }
 
-  int slot = 0;  // of the next partial tile
-  for (int64_t pos = line.start, next; pos < line.stop; pos = next) {
-    const Place at_line = line_place<kRT, kFewKeys, kFewStart>(a, s_line, line, pos);
-    const int32_t q0 = at_line.q0, n_rows = at_line.n_rows, k0 = at_line.k0, lk = at_line.lk, head = at_line.head, row0 = at_line.row0;
-    const int32_t u0 = at_line.u0, u1 = at_line.u1;
-    next = at_line.next;
-    if (u0 >= u1) continue;
-
-    v8 qb[NT][kKS];
+  struct Tile {
+    Place at;
+    const uint8_t *k, *v;
+  };
+  auto find = [&](int64_t pos, Tile* t) __attribute__((always_inline)) {  // the part's first tile with units from pos on
+    for (; pos < line.stop; pos = t->at.next) {
+      t->at = line_place<kRT, kFewShift, kFewStart>(a, s_line, line, pos);
+      if (t->at.u0 >= t->at.u1) continue;
+      t->k = reinterpret_cast<const uint8_t*>(a.k + t->at.k0 * a.k_token + (t->at.head + sub) * a.k_head);
+      t->v = reinterpret_cast<const uint8_t*>(a.v + t->at.k0 * a.v_token + (t->at.head + sub) * a.v_head);
+      return true;
+    }
+    return false;
+  };
+  uint4 qb[NT][kKS];
+  auto load_queries = [&](const Place& p) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int32_t row = min(row0 + 16 * t + n16, n_rows - 1), qi = row / a.G, h = head * a.G + (row - qi * a.G);
-      const uint16_t* qp = a.q + static_cast<int64_t>(q0 + qi) * a.q_token + h * a.q_head + 8 * g;
+      const int32_t row = min(p.row0 + 16 * t + n16, p.n_rows - 1), qi = row / a.G, h = (p.head + sub) * a.G + (row - qi * a.G);
+      const uint16_t* qp = a.q + static_cast<int64_t>(p.q0 + qi) * a.q_token + h * a.q_head + 8 * g;
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) qb[t][ks] = __builtin_bit_cast(v8, load_query(a, qp + 32 * ks));
+      for (int ks = 0; ks < kKS; ++ks) qb[t][ks] = *reinterpret_cast<const uint4*>(qp + 32 * ks);
     }
-    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + k0 * a.k_token + head * a.k_head);
-    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + k0 * a.v_token + head * a.v_head);
-    u32x4_t kr[2][2][kKS];
-    // the wave's 32 keys of unit u, read through buffer resources whose range ends at the last key: rows past it are zero, as
-    // is all of the unit past the part's last (every step has as many loads under way)
-    auto load = [&](int32_t u, auto buf_c) __attribute__((always_inline)) {
-      constexpr int buf = decltype(buf_c)::value;
-      const int32_t at = u * kFewKeys + 32 * wv, left = u < u1 ? lk - at : 0;
-      const int32_t m = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : left < 32 ? left : 32);  // (the clamp is a vector instruction)
-      const int64_t base = m > 0 ? at : 0;
-      const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kbase + base * k_stride), 0, m > 0 ? (m - 1) * k_stride + kRow : 0, kBufWord3);
-      const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vbase + base * v_stride), 0, m > 0 ? (m - 1) * v_stride + kRow : 0, kBufWord3);
+  };
+  u32x4_t kr[2][2][kKS];
+  // the wave's 32 keys of unit u, read through buffer resources whose range ends at the last key: rows past it are zero, as
+  // is all of the unit past the part's last (every step has as many loads under way)
+  auto load = [&](const uint8_t* k, const uint8_t* v, int32_t lk, int32_t u, int32_t u1, auto buf_c) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_c)::value;
+    const int32_t at = (u << shift) + 32 * block, left = u < u1 ? lk - at : 0;
+    const int32_t m = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : left < 32 ? left : 32);  // (the clamp is a vector instruction)
+    const int64_t base = m > 0 ? at : 0;
+    const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(k + base * k_stride), 0, m > 0 ? (m - 1) * k_stride + kRow : 0, kBufWord3);
+    const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(v + base * v_stride), 0, m > 0 ? (m - 1) * v_stride + kRow : 0, kBufWord3);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int ks = 0; ks < kKS; ++ks) kr[buf][t][ks] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(krs, koff + 64 * ks, 16 * t * k_stride, 0));
-      uint8_t* const dst = buf ? V1[wv] : V0[wv];
+      for (int ks = 0; ks < kKS; ++ks) kr[buf][t][ks] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(krs, koff + 64 * ks, 16 * t * k_stride, 0));
+    uint8_t* const dst = buf ? V1[wv] : V0[wv];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(dst + 1024 * i), 16, voff[i & 3], kPer * i * v_stride, 0, 0);
-    };
+    for (int i = 0; i < kLoads; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(dst + 1024 * i), 16, voff[i & 3], kPer * i * v_stride, 0, 0);
+  };
+
+  // all waves, with their LDS accesses done (and their loads under way)
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // A tile begins with its first unit under way in the first buffer, and its queries: the tile before asks for them
+  int slot = 0;  // of the next partial tile
+  Tile cur;
+  if (!find(line.start, &cur)) return;
+  load_queries(cur.at);
+  load(cur.k, cur.v, cur.at.lk, cur.at.u0, cur.at.u1, std::integral_constant<int, 0>{});
+  for (bool more = true; more;) {
+    Tile next = cur;
+    more = find(cur.at.next, &next);
+    if (!more) next.at.u0 = next.at.u1;  // (nothing to load)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) take_queries(a, qb[t]);
+    const int32_t q0 = cur.at.q0, n_rows = cur.at.n_rows, lk = cur.at.lk, row0 = cur.at.row0, u0 = cur.at.u0, u1 = cur.at.u1;
     float m[NT], l[NT];
     f32x4_t O[NT][kMB];
 #pragma unroll
@@ -325,10 +368,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
     auto step = [&](int32_t u, auto buf_c) __attribute__((always_inline)) {
       constexpr int buf = decltype(buf_c)::value;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's values have been read
-      load(u + 1, std::integral_constant<int, buf ^ 1>{});
+      const bool over = buf && u + 1 >= u1;
+      load(over ? next.k : cur.k, over ? next.v : cur.v, over ? next.at.lk : lk, over ? next.at.u0 : u + 1, over ? next.at.u1 : u1, std::integral_constant<int, buf ^ 1>{});
       if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // (8 loads of keys, 8 of values under way)
       else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      const int32_t at = u * kFewKeys + 32 * wv;
+      const int32_t at = (u << shift) + 32 * block;
       if (at >= lk || u >= u1) return;
       const uint8_t* vt = buf ? V1[wv] : V0[wv];
       v8 pb[NT];
@@ -340,7 +384,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
         for (int kb = 0; kb < 2; ++kb) {
           s[kb] = f32x4_t{};
 #pragma unroll
-          for (int ks = 0; ks < kKS; ++ks) s[kb] = E::mma16(__builtin_bit_cast(v8, kr[buf][kb][ks]), qb[t][ks], s[kb]);
+          for (int ks = 0; ks < kKS; ++ks) s[kb] = E::mma16(__builtin_bit_cast(v8, kr[buf][kb][ks]), __builtin_bit_cast(v8, qb[t][ks]), s[kb]);
         }
         if (at + 32 > lk) {
 #pragma unroll
@@ -389,8 +433,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
         for (int t = 0; t < NT; ++t) O[t][mb] = E::mma16(w, pb[t], O[t][mb]);
       }
     };
-    load(u0, std::integral_constant<int, 0>{});
-    asm volatile("" ::: "memory");
     int32_t u = u0;
     do {
       step(u, std::integral_constant<int, 0>{});
@@ -398,49 +440,58 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
       u += 2;
     } while (u < u1);
 
-    // the waves' states through their own buffers: row n16's four dims at 16 mb + 4 g, chunks swizzled by the row
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    load_queries(next.at);
+    // the waves' states through their own second buffers: row n16's four dims at 16 mb + 4 g, chunks swizzled by the row
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       l[t] += xor_lane<16>(l[t]);
       l[t] += xor_lane<32>(l[t]);
       if (g == 0) s_ml[wv][16 * t + n16] = make_float2(m[t], l[t]);
-      float* const w = reinterpret_cast<float*>(t ? V1[wv] : V0[wv]) + n16 * D;
+      float* const w = reinterpret_cast<float*>(t ? s_more[NT == 1 ? 0 : wv] : V1[wv]) + n16 * D;
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb) *reinterpret_cast<f32x4_t*>(w + 4 * ((4 * mb + g) ^ n16)) = O[t][mb];
     }
-    __syncthreads();
-    const bool whole = u1 - u0 == at_line.units;
-    float* const part = a.part + (2 * static_cast<int64_t>(line.index) + slot) * kRT * (D + 4);
-    for (int r = tid / (D / 4); r < kRT; r += 256 / (D / 4)) {
-      const int c = tid % (D / 4), row = row0 + r;
-      if (row >= n_rows) break;
-      float2 ml[4];
+    meet();
+    const bool whole = u1 - u0 == cur.at.units;
+    float* const part = a.part + ((2 * static_cast<int64_t>(line.index) + slot) << a.share) * kRT * (D + 4);
+    const int rows = min(kRT, n_rows - row0);
+    for (int at = tid / (D / 4); at < rows << a.share; at += 256 / (D / 4)) {
+      const int c = tid % (D / 4), of = head_of_row(at, rows), r = at - of * rows, row = row0 + r;
+      float2 ml[4];  // of the head's waves
       float up = kNegInf;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) ml[w] = s_ml[w][r], up = fmaxf(up, ml[w].x);
+      for (int i = 0; i < 4; ++i) {
+        ml[i] = make_float2(kNegInf, 0.0f);
+        if (of + (i << a.share) < 4) ml[i] = s_ml[of + (i << a.share)][r];
+        up = fmaxf(up, ml[i].x);
+      }
       float sum = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int i = 0; i < 4; ++i) {
         // (a state of nothing has a sum of 0; NaN alone leaves a maximum of -inf, and a sum that says so)
-        const float f = ml[w].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[w].x - up);
-        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(r < 16 ? V0[w] : V1[w]) + (r & 15) * D + 4 * (c ^ (r & 15)));
-        sum += ml[w].y == 0.0f ? 0.0f : ml[w].y * f;
-        if (ml[w].y != 0.0f) o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+        if (ml[i].y == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - up);
+        const int w = of + (i << a.share);
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(NT == 1 || r < 16 ? V1[w] : s_more[NT == 1 ? 0 : w]) + (r & 15) * D + 4 * (c ^ (r & 15)));
+        sum += ml[i].y * f;
+        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
       }
       if (whole) {
-        const int32_t qi = row / a.G, h = head * a.G + (row - qi * a.G);
+        const int32_t qi = row / a.G, h = (cur.at.head + of) * a.G + (row - qi * a.G);
         finish<DT, D>(a, static_cast<int64_t>(q0 + qi) * a.H + h, h, c, up, sum, o);
       } else {
-        float* p = part + r * (D + 4);
+        float* p = part + (of * kRT + r) * (D + 4);
         if (c == 0) *reinterpret_cast<float2*>(p) = make_float2(up, sum);
         *reinterpret_cast<float4*>(p + 4 + 4 * c) = o;
       }
     }
-    __syncthreads();
+    meet();
     slot = 1;
+    cur = next;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads past the last tile write zeros to LDS)
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
@@ -460,7 +511,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void cross_many_kernel(CrossArgs a) {
   using E = Elem<DT>;
   using v8 = typename E::v8;
-  constexpr int kRows = 128, kRow = 2 * D, kBytes = kManyKeys * kRow;
+  constexpr int kRows = 128, kManyKeys = 1 << kManyShift, kRow = 2 * D, kBytes = kManyKeys * kRow;
   constexpr int kMB = D / 32, kKS = D / 16;  // (kKS: products of a block's keys, and of its values)
   constexpr int kAhead = 2;                  // products ahead that their operands are read
   __shared__ __align__(16) uint8_t K0[kBytes], K1[kBytes], V0[kBytes], V1[kBytes];
@@ -468,7 +519,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
 
   const int lane = threadIdx.x & 63, rl = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const LinePart line = line_part<D, kRows, kManyKeys, kManyStart>(a, s_line, wv, lane);
+  const LinePart line = line_part<D, kRows, kManyShift, kManyStart>(a, s_line, wv, lane);
   if (line.start >= line.stop) return;
 
   // staging: load c of wave wv writes bytes [4096 c + 1024 wv, + 1024) of a unit, lane l at + 16 l, so lane l loads the chunk that
@@ -500,7 +551,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
 
   int slot = 0;  // of the next partial tile
   for (int64_t pos = line.start, next; pos < line.stop; pos = next) {
-    const Place at = line_place<kRows, kManyKeys, kManyStart>(a, s_line, line, pos);
+    const Place at = line_place<kRows, kManyShift, kManyStart>(a, s_line, line, pos);
     const int32_t q0 = at.q0, n_rows = at.n_rows, head = at.head, u0 = at.u0, u1 = at.u1;
     next = at.next;
     if (u0 >= u1) continue;
@@ -524,13 +575,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
     load(knext, kleft, k_stride, koff, K0);
 
     // rows past the last are computed as copies of it
-    v8 qb[kKS];
+    uint4 qb[kKS];
     const int32_t row = at.row0 + 32 * wv + rl;
     {
       const int32_t own = row < n_rows ? row : n_rows - 1, qi = own / a.G, h = head * a.G + (own - qi * a.G);
       const uint16_t* qp = a.q + static_cast<int64_t>(q0 + qi) * a.q_token + h * a.q_head + 8 * hh;
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) qb[ks] = __builtin_bit_cast(v8, load_query(a, qp + 16 * ks));
+      for (int ks = 0; ks < kKS; ++ks) qb[ks] = *reinterpret_cast<const uint4*>(qp + 16 * ks);
+      take_queries(a, qb);
     }
 
     // m: the reference that weights are relative to (a maximum less kLift); nm: -m, or 0 where nothing was seen; l: the weights' sum
@@ -609,7 +661,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (keys) {
           if (i + kAhead < kKS) kf[i + kAhead] = key(kt, i + kAhead);
-          sn = E::mma(kf[i], qb[i], sn);
+          sn = E::mma(kf[i], __builtin_bit_cast(v8, qb[i]), sn);
         }
         if constexpr (values) {
           if (i + kAhead < kKS) vf[i + kAhead] = value(vt, i + kAhead);
@@ -643,7 +695,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
     offsets();
     S = f32x16_t{};
 #pragma unroll
-    for (int ks = 0; ks < kKS; ++ks) S = E::mma(key(K0, ks), qb[ks], S);
+    for (int ks = 0; ks < kKS; ++ks) S = E::mma(key(K0, ks), __builtin_bit_cast(v8, qb[ks]), S);
     block(yes, K0 + kSecond, no, V0, u0 * kManyKeys);
     auto step = [&](int32_t s, auto odd) __attribute__((always_inline)) {  // unit s's keys, unit s - 1's values
       constexpr bool p = decltype(odd)::value;
@@ -708,8 +760,8 @@ cross_fn pick_cross(int32_t dtype, int32_t d, int64_t rows, bool merge) {
 }
 
 struct CrossPlan {
-  int64_t rows, groups;  // of a tile; workgroups of a launch
-  int32_t least;         // units of a part at least
+  int64_t rows, groups;  // of a tile and head; workgroups of a launch
+  int32_t least, share;  // units of a part at least; log2 of a tile's heads
 };
 CrossPlan plan_cross(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d) {
   CrossPlan p{};
@@ -717,11 +769,15 @@ CrossPlan plan_cross(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, 
   const int64_t resident = d == 64 ? 768 : 512;
   if (each <= 32) {
     p.rows = each <= 16 ? 16 : 32, p.groups = 256, p.least = 1;
+    // Heads that lie next to each other in a token are read together as long as that leaves tiles for a quarter of the workgroups.  64
+    // sequences of up to 4096 states, 12 heads of 4, dim 128: 67.8 us with one head at a time, 64.9 with two, 63.1 with four (50 of them
+    // the kernel's, 55 with one); dim 64: 39.2, 37.0, 36.6.  With fewer tiles, whose parts are merged: 8 sequences 17.1, 18.8, 23.0
+    while (p.share < 2 && heads % (2 << p.share) == 0 && runs * (heads >> (p.share + 1)) >= 64) ++p.share;
   } else {
     p.rows = 128, p.groups = resident, p.least = 3;
   }
-  const int64_t keys = p.rows <= 32 ? kFewKeys : kManyKeys, start = p.rows <= 32 ? kFewStart : kManyStart;
-  const double most = (static_cast<double>(rows / p.rows) + B) * heads * (n_k / keys + 1 + start) / p.least + 1.0;  // parts of the longest line
+  const int64_t keys = p.rows <= 32 ? (1 << kFewShift) >> p.share : 1 << kManyShift, start = p.rows <= 32 ? kFewStart : kManyStart;
+  const double most = (static_cast<double>(rows / p.rows) + B) * (heads >> p.share) * (n_k / keys + 1 + start) / p.least + 1.0;  // parts of the longest line
   if (p.groups > most) p.groups = static_cast<int64_t>(most);
   return p;
 }
@@ -739,7 +795,7 @@ extern "C" size_t aekv_cross_attention_workspace_size(int64_t B, int64_t E, int6
   if (B <= 0 || E < 0 || n_q <= 0 || n_k < 0 || H <= 0 || heads <= 0 || (d != 64 && d != 128) || H % heads) return 0;
   if (!cross_fits(B, E, n_q, n_k, H)) return 0;  // (the call refuses it)
   const CrossPlan p = plan_cross(B, E, n_q, n_k, H, heads, d);
-  return static_cast<size_t>(p.groups) * sizeof(LineTile) + static_cast<size_t>(p.groups) * 2 * p.rows * (d + 4) * 4;
+  return static_cast<size_t>(p.groups) * sizeof(LineTile) + static_cast<size_t>(p.groups) * 2 * (p.rows << p.share) * (d + 4) * 4;
 }
 
 extern "C" int aekv_cross_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
@@ -783,14 +839,14 @@ extern "C" int aekv_cross_attention(const void* q, const void* k, const void* v,
   const hipStream_t st = as_stream(stream);
   a.desc = static_cast<LineTile*>(ws);
   a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + plan.groups * sizeof(LineTile));
-  a.least = plan.least;
+  a.least = plan.least, a.share = plan.share;
   const uint32_t groups = static_cast<uint32_t>(plan.groups);
   for (int64_t b0 = 0; b0 < B; b0 += kTable) {
     a.b0 = static_cast<int32_t>(b0), a.nb = static_cast<int32_t>(B - b0 < kTable ? B - b0 : kTable);
     hipLaunchKernelGGL(pick_cross(dtype, d, plan.rows, false), dim3(groups), dim3(256), 0, st, a);
     if (const int rc = check_launch(who)) return rc;
     if (groups == 1) continue;
-    hipLaunchKernelGGL(pick_cross(dtype, d, plan.rows, true), dim3(groups - 1, static_cast<uint32_t>(ceil_div(plan.rows * d / 4, 256))), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(pick_cross(dtype, d, plan.rows, true), dim3(groups - 1, static_cast<uint32_t>(ceil_div((plan.rows << plan.share) * d / 4, 256))), dim3(256), 0, st, a);
     if (const int rc = check_launch(who)) return rc;
   }
   return AEKV_OK;
