@@ -2,20 +2,21 @@
 released, and moved together.
 
 A PagePool serves the caches of all layers, which share one page table: it counts for every page the table entries that hold
-it, and keeps three promises for append_tokens and evict_by_weight, which write to the pages of the slots they fill:
+it, and keeps what append_tokens and evict_by_weight need, which write to the pages of the slots they fill:
 
   reserve   the slots that are about to be written lie in pages of their sequence's own
   fork      rows take over other rows' pages without copying them (answers to one prompt, beams, cached prefixes)
   release   the pages behind a sequence's kept slots are free again
   compact   the pages in use are the pool's first ones, so that what lies behind them can be given up
 
-Tables and counts are device tensors and nothing synchronises, so every call can be captured in a graph.  A table entry of -1
+Tables and counts are device tensors and nothing synchronises, so these calls can be captured in a graph.  A table entry of -1
 (any outside the pool) holds no page.  The calls change the table and the pool's counts: those of one pool run one after another
 (on one stream, or with events between).  Rows of a table need not be sequences of the batch: a prefix that is kept for later is
 a row, and attention takes the rows before it, page_table[:B].
 """
 from __future__ import annotations
 
+from array import array
 from typing import Optional, Sequence
 
 import torch
@@ -42,20 +43,22 @@ class PagePool:
                 raise RuntimeError(f"the caches of a pool need the same pages, page size and device, got {c.pages} x {c.page_size} on {c.device} beside "
                                    f"{head.pages} x {head.page_size} on {head.device}")
         self.caches, self.pages, self.page_size, self.device, self._index = caches, head.pages, head.page_size, head.device, head._index
-        if refs is None:
-            refs = torch.zeros(self.pages, dtype=torch.int32, device=self.device)
-        elif refs.dtype != torch.int32 or refs.shape != (self.pages,) or not refs.is_contiguous() or refs.get_device() != self._index:
-            raise RuntimeError(f"refs must be contiguous int32 [{self.pages}] on {self.device}, got {refs.dtype} {tuple(refs.shape)} on {refs.device}")
-        self._refs = refs
-        self._marks = torch.zeros(2, self.pages, dtype=torch.int32, device=self.device)
-        self._lacking = torch.zeros(1, dtype=torch.int32, device=self.device)
-        rows = []
+        # (zeros in one allocation: counts where none are given, the kernels' marks, what reserve lacked)
+        n, own = self.pages, refs is None
+        zeros = torch.zeros((3 if own else 2) * n + 1, dtype=torch.int32, device=self.device)
+        if own:
+            refs = zeros[2 * n + 1:]
+        elif refs.dtype != torch.int32 or refs.shape != (n,) or not refs.is_contiguous() or refs.get_device() != self._index:
+            raise RuntimeError(f"refs must be contiguous int32 [{n}] on {self.device}, got {refs.dtype} {tuple(refs.shape)} on {refs.device}")
+        self._refs, self._marks, self._lacking = refs, zeros[:2 * n].view(2, n), zeros[2 * n:2 * n + 1]
+        rows = array("q")  # where a page's bytes lie: address of page 0, step, bytes
         for c in caches:
             for t in c._tensors:
-                page = t.stride(0) * t.element_size()
-                rows += [(t.data_ptr() + at, page, min(_SEGMENT, page - at)) for at in range(0, page, _SEGMENT)]
-        self._segments = torch.tensor(rows, dtype=torch.int64, device=self.device)  # where a page's bytes lie: address of page 0, step, bytes
-        self._args = (self._segments.data_ptr(), len(rows))
+                page, at = t.stride(0) * t.element_size(), t.data_ptr()
+                for off in range(0, page, _SEGMENT):
+                    rows.extend((at + off, page, min(_SEGMENT, page - off)))
+        self._segments = (torch.frombuffer(rows, dtype=torch.int64) if rows else torch.empty(0, dtype=torch.int64)).to(self.device)
+        self._args = (self._segments.data_ptr(), len(rows) // 3)
 
     refs = property(lambda self: self._refs)
 
@@ -66,7 +69,10 @@ class PagePool:
         return self._lacking
 
     def unused(self) -> torch.Tensor:
-        """The number of pages that no table entry holds (a tensor: nothing waits)."""
+        """The number of pages that no table entry holds (a tensor: nothing waits).  Not within a captured graph: a torch reduction
+        may clear its scratch there by a memset node, which does not hold over replays."""
+        if _lib._capturing():
+            raise RuntimeError("unused() is no call for a captured graph: take it between replays")
         return (self._refs <= 0).sum()
 
     def _table(self, page_table: torch.Tensor):

@@ -247,6 +247,8 @@ def test_captured_and_replayed(dev):
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=side):
         calls()
+        with pytest.raises(RuntimeError, match="captured"):
+            b.pool.unused()
     torch.cuda.synchronize()
     b.check()
     for step, (f, w, k, s) in enumerate([([20, 20, 20, 20], [33, 21, 20, 60], [20] * 4, [3, 0]), ([33, 21, 20, 60], [34] * 4, [33, 0, 20, 60], [1, 1]), ([34, 21, 30, 34], [40, 40, 128, 35], [34, 20, 10, 34], [2, 3])]):
