@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
     const int sub = head_of_row(at, rows), r = at - sub * rows, own = d.head + sub;
     float m = kNegInf, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int CH = 8;
+    constexpr int CH = kRows <= 32 ? 8 : 4;
     for (int32_t w0 = blockIdx.x; w0 <= last; w0 += CH) {
       float2 ml[CH];
       float4 x[CH];
