@@ -19,6 +19,10 @@ Per-head caches, beside the reference's shared compressed blocks:
   aetherkv.prompt            prompt_attention: causal attention of packed sequences, grouped heads
   aetherkv.paged             PagedKVCache in TurboQuant codes: append_tokens, paged_attention, and
                              evict_by_weight by the weights that a SlotTracker accumulates
+  aetherkv.pages             PagePool: the caches' pages given, shared by forks, copied before they are
+                             written, released and compacted
+  aetherkv.rotary            rotate_axes: rotary positions on several axes, of q and k at once
+  aetherkv.cross             cross_attention: queries over an encoder's states, packed, grouped heads
 All compute runs in libaetherkv.so (hand-written HIP for gfx950, C ABI in include/aetherkv.h).
 """
 from .loader import cuda_build_environment, cuda_extension_unavailable_reason, load_aether_cuda_kernels

@@ -13,7 +13,7 @@ layers and only read here: after a step the caller adds the new tokens to `lengt
 clamps them to `keep`.  Slot p of sequence b is row p % page_size of page table[b, p // page_size].  The tables and counts
 are device data that no host check can see, so a slot outside the table or a page outside the pool is skipped, never
 accessed.  Pages may be shared between sequences as long as nothing writes to them: append_tokens and evict_by_weight
-write to the pages of the slots they fill.
+write to the pages of the slots they fill (aetherkv.pages.PagePool gives pages, shares them and copies them in time).
 """
 from __future__ import annotations
 
