@@ -701,6 +701,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
       constexpr bool p = decltype(odd)::value;
       const uint8_t *kt = p ? K1 : K0, *vt = p ? V0 : V1;
       meet();
+      // first in every second unit: else the older of a CU's workgroups always are, the last one ends alone (53.4 for 52.7 us behind 16
+      // prompts, 844 for 832 for a long one)
+      __builtin_amdgcn_s_setprio(p ? 1 : 0);
       load(knext, kleft, k_stride, koff, p ? K0 : K1);
       load(vnext, vleft, v_stride, voff, p ? V1 : V0);
       block(yes, kt, yes, vt, s * kManyKeys - 32);
