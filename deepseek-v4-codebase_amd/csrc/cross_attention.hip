@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kFewShift = 7;   // log2 of a unit's keys: with few rows, all heads that a workgroup takes at a time together
 constexpr int kManyShift = 6;  // with many rows
-constexpr int kFewStart = 1;   // units that a tile costs beside its own
+constexpr int kFewStart = 1;   // units that a tile costs beside its own (measured 0 to 3 and 1 to 4: both sides are 1 to 3 % slower)
 constexpr int kManyStart = 2;
 constexpr int kTable = 256;    // sequences of a launch
 
@@ -496,7 +496,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
 //
-// Tiles of 128 rows, 32 to a wave; units of 64 keys in two blocks.  Bound by the matrix instructions and the exponentials, which one
+// Tiles of 128 rows, 32 to a wave; units of 64 keys in two blocks.  8192 queries over 16384 states, 12 heads of 4, dim 128: 790 to 850
+// us by card, 970 to 1050 TFLOP/s, at 1.8 GHz, as power allows (663 us on zeros); 256 rows to a tile took 924 for 894 then.  Bound by
+// the matrix instructions and the exponentials, which one
 // wave's instructions interleave: while the keys of a block are multiplied with the queries, the weights of the block before are made
 // and those of the block before that are multiplied with their values, three parts that do not wait for each other.  Keys and values go
 // straight to LDS, two buffers each: keys one unit ahead, values at the step that multiplies their keys.
@@ -754,7 +756,9 @@ using cross_fn = void (*)(CrossArgs);
 template <int DT, int D>
 cross_fn pick_rows(int64_t rows, bool merge) {
   if (rows == 16) return merge ? cross_merge_kernel<DT, D, 16, kFewStart> : cross_few_kernel<DT, D, 1>;
-  if (rows == 32) return merge ? cross_merge_kernel<DT, D, 32, kFewStart> : cross_few_kernel<DT, D, 2>;
+  if constexpr (D == 64) {
+    if (rows == 32) return merge ? cross_merge_kernel<DT, D, 32, kFewStart> : cross_few_kernel<DT, D, 2>;
+  }
   return merge ? cross_merge_kernel<DT, D, 128, kManyStart> : cross_many_kernel<DT, D>;
 }
 cross_fn pick_cross(int32_t dtype, int32_t d, int64_t rows, bool merge) {
@@ -769,17 +773,22 @@ struct CrossPlan {
 CrossPlan plan_cross(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d) {
   CrossPlan p{};
   const int64_t rows = n_q * (H / heads), runs = E > 0 && E < B ? E : B, each = ceil_div(rows, runs);
-  const int64_t resident = d == 64 ? 768 : 512;
-  if (each <= 32) {
+  const int64_t resident = d == 64 ? 768 : 512;  // of the many rows' workgroups, by their registers
+  // Few rows by the average run.  Over 64 x up to 4096 states, few / many: dim 128, 12 rows 68.8 / 72.4 us, 18 rows 75.2 / 74.7 (two
+  // blocks of 16; with tiles of 16 93), 30 rows 81.3 / 75.7; dim 64, 24 rows 23.7 / 25.0, 32 rows 24.9 / 26.1, 48 rows 35.6 / 29.0
+  const bool few = each <= (d == 64 ? 32 : 16);
+  if (few) {
+    // (a workgroup per CU: 60 us for 64 sequences of up to 4096 states, 20.6 for one of 16384; with two 60 and 24, with four 64 and 36)
     p.rows = each <= 16 ? 16 : 32, p.groups = 256, p.least = 1;
     // Heads that lie next to each other in a token are read together as long as that leaves tiles for a quarter of the workgroups.  64
     // sequences of up to 4096 states, 12 heads of 4, dim 128: 67.8 us with one head at a time, 64.9 with two, 63.1 with four (50 of them
     // the kernel's, 55 with one); dim 64: 39.2, 37.0, 36.6.  With fewer tiles, whose parts are merged: 8 sequences 17.1, 18.8, 23.0
     while (p.share < 2 && heads % (2 << p.share) == 0 && runs * (heads >> (p.share + 1)) >= 64) ++p.share;
   } else {
+    // (a part begins, ends and is merged at some cost: 16 queries over 16 x 500 states 16.2 us with 3 units at least, 22.5 with 8)
     p.rows = 128, p.groups = resident, p.least = 3;
   }
-  const int64_t keys = p.rows <= 32 ? (1 << kFewShift) >> p.share : 1 << kManyShift, start = p.rows <= 32 ? kFewStart : kManyStart;
+  const int64_t keys = few ? (1 << kFewShift) >> p.share : 1 << kManyShift, start = few ? kFewStart : kManyStart;
   const double most = (static_cast<double>(rows / p.rows) + B) * (heads >> p.share) * (n_k / keys + 1 + start) / p.least + 1.0;  // parts of the longest line
   if (p.groups > most) p.groups = static_cast<int64_t>(most);
   return p;

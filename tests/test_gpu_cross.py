@@ -230,6 +230,19 @@ def test_many_rows_in_many_sequences(dev, dtype, dim, shared):
     _check(dev, dtype, dim, 2, 1, lq, [(67 * i) % 230 for i in range(34 if shared else B)], states=states, seed=4, sink=True, pad=2)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("H,hk", [(8, 8), (12, 4), (12, 6), (9, 3), (32, 2)])
+@pytest.mark.parametrize("kind", ["steps", "ragged", "runs"])
+def test_heads_read_together(dev, dtype, dim, H, hk, kind):
+    """Enough sequences for one workgroup to take two or four KV heads at a time: single queries, a few long answers among short ones
+    (several tiles to a head), runs over the same states; states that end within every part of a unit."""
+    B = 70
+    lq = [1] * B if kind != "ragged" else [(0, 1, 2, 1)[b % 4] + (40 if b in (5, 44) else 0) for b in range(B)]
+    states = [b // 2 for b in range(B)] if kind == "runs" else None
+    lk = [(0, 1, 31, 32, 33, 63, 65, 96, 127, 128, 129, 255, 300, 700)[b % 14] for b in range(B)]
+    _check(dev, dtype, dim, H, hk, lq, lk, states=states, seed=H, sink=hk % 2 == 0, offsets=kind == "ragged")
+
+
 def test_a_captured_call_of_several_launches(dev):
     """More sequences than one launch takes, one workspace for all launches of a call, replayed with other states and lengths."""
     B = 300
