@@ -21,9 +21,9 @@ constexpr int kFewStart = 1;   // units that a tile costs beside its own (measur
 constexpr int kManyStart = 2;
 constexpr int kTable = 256;    // sequences of a launch
 
-struct LineTile {  // the tile that a part starts within
-  int64_t start, chunk;  // its first place, -1: none; places of a part
-  int32_t units, q0, n_rows, row0, head, pad;
+struct alignas(16) LineTile {  // the tile that a part starts within (whole 16 bytes: the partial rows lie behind any number of them)
+  int64_t start, chunk;        // its first place, -1: none; places of a part
+  int32_t units, q0, n_rows, row0, head;
 };
 
 struct CrossArgs {
@@ -197,7 +197,7 @@ __device__ __forceinline__ Place line_place(const CrossArgs& a, const LineTable&
   const uint32_t tiles = static_cast<uint32_t>(at.n_rows + kRows - 1) / kRows;
   at.head = static_cast<int32_t>(th / tiles) << a.share, at.row0 = static_cast<int32_t>(th % tiles * kRows);
   if (pos == p.start && threadIdx.x == 0)
-    a.desc[p.index] = LineTile{at.u0 > 0 ? from : -1, p.chunk, at.units, at.q0, at.n_rows, at.row0, at.head, 0};
+    a.desc[p.index] = LineTile{at.u0 > 0 ? from : -1, p.chunk, at.units, at.q0, at.n_rows, at.row0, at.head};
   return at;
 }
 

@@ -67,6 +67,17 @@ def test_cross_refusals(lib):
         assert _cross(lib, nq=nq, nk=nk, ws=ctypes.c_void_p(0x10008)) == L.ERR_ALIGN
 
 
+def test_cross_partial_rows_are_aligned(lib):
+    """The workspace holds a descriptor per workgroup and behind them partial rows of 16-byte vectors, each (d + 4) fp32: the size
+    is whole 16 bytes for every number of workgroups only if the rows begin on 16 bytes."""
+    for d in (64, 128):
+        for B, E in ((1, 1), (2, 3), (7, 7), (64, 8), (300, 300)):
+            for nq in (B, 3 * B, 200 * B):
+                for H, hk in ((1, 1), (12, 4), (16, 16), (10, 2)):
+                    for nk in (0, 1, 128, 300, 700, 1500, 9001):
+                        assert lib.aekv_cross_attention_workspace_size(B, E, nq, nk, H, hk, d) % 16 == 0, (B, E, nq, nk, H, hk, d)
+
+
 def test_rotate_refusals(lib):
     assert _rotate(lib, dtype=L.I32) == L.ERR_DTYPE and _rotate(lib, pdt=L.F32) == L.ERR_DTYPE
     assert _rotate(lib, n=-1) == L.ERR_SHAPE and _rotate(lib, H=0, hk=0) == L.ERR_SHAPE and _rotate(lib, H=-1) == L.ERR_SHAPE and _rotate(lib, axes=0) == L.ERR_SHAPE
