@@ -119,7 +119,8 @@ struct Entry {
 };
 
 // The call's shared pages, where its entries are kept: a table by page, open to the next slot.
-struct Shared {
+// (Aligned as it is cleared, four slots to a store.)
+struct alignas(16) Shared {
   int32_t page[kSlots], count[kSlots], last[kSlots];  // -1: free; the page's entries in the call, and the last of them
 };
 
@@ -252,6 +253,7 @@ __global__ __launch_bounds__(kThreads) void pool_reserve_kernel(PoolArgs a) {
   __shared__ Shared sh;
   __shared__ int32_t s_scan[2 * kWaves];
   __shared__ int32_t s_copies;
+  static_assert(alignof(Shared) >= sizeof(int4) && kSlots % 4 == 0, "its arrays are cleared by int4");
   static_assert(kSlots == 1 << 13 && (kSlots / 4) % kThreads == 0, "the hash's bits; whole rounds of four slots");
   Scan scan{s_scan, 0};
   const int tid = threadIdx.x;
