@@ -168,6 +168,41 @@ def test_offsets_that_are_no_prefix_sums_stay_in_bounds(dev):
             assert out.shape == q.shape
 
 
+@pytest.mark.parametrize("per", [1, 30])
+def test_bad_offsets_write_nothing_beside_the_output(dev, per):
+    """Offsets that are no prefix sums, states out of range: what lies before and behind `out` and the workspace, whose last byte the
+    call may use, is as it was."""
+    for cq, ck in (([0, 2, -5, 2, 0, 1 << 30, 2], [50, 10, 1 << 30, -7, 300, 0, 300]), ([5, 0, 6, 0, 6, 3, 6], [300] * 7), ([0, 1, 2, 3, 4, 5, 6], [0, 50, 100, 150, 200, 250, 300])):
+        B, H, N, M = 6, 4, 6 * per, 300
+        q = torch.randn(N, H, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+        k, v = (torch.randn(M, 2, 64, device=dev, generator=_gen(dev, i)).bfloat16() for i in (1, 2))
+        rows = torch.full((N + 512, H, 64), 7.0, dtype=torch.bfloat16, device=dev)
+        out = rows[256:256 + N]
+        size = cross_workspace(B, 6, N, M, H, 2, 64, dev).numel()
+        room = torch.full((size + (2 << 20),), 0xA5, dtype=torch.uint8, device=dev)
+        cross_attention(q, k, v, _t(ck, dev), 0.1, cu_seqlens=_t([per * c if 0 < c < 100 else c for c in cq], dev), out=out, states=_t([0, 3, -1, 6, 2 ** 31 - 1, 5], dev),
+                        workspace=room[1 << 20:(1 << 20) + size])
+        assert (rows[:256] == 7).all() and (rows[256 + N:] == 7).all()
+        assert (room[:1 << 20] == 0xA5).all() and (room[(1 << 20) + size:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lq", [1, 40])
+def test_a_sequence_alone_and_among_others(dev, dtype, lq):
+    """A sequence by itself against the same one in a batch: each is within the bound, so they are within twice the bound."""
+    B, lk = 12, [(61 * i) % 400 + 1 for i in range(12)]
+    cq, ck = _cu([lq] * B), _cu(lk)
+    q = torch.randn(B * lq, 6, 64, device=dev, generator=_gen(dev, 0)).to(dtype)
+    k, v = (torch.randn(sum(lk), 3, 64, device=dev, generator=_gen(dev, i)).to(dtype) for i in (1, 2))
+    out, lse = cross_attention(q, k, v, _t(ck, dev), 0.125, cu_seqlens=_t(cq, dev), return_lse=True)
+    _, bound, _, lb = C.cross_attention_ref(q.cpu(), k.cpu(), v.cpu(), cq, ck, None, 0.125)
+    for b in range(B):
+        rows, keys = slice(cq[b], cq[b + 1]), slice(ck[b], ck[b + 1])
+        one, l1 = cross_attention(q[rows], k[keys], v[keys], _t([0, lk[b]], dev), 0.125, cu_seqlens=_t([0, lq], dev), return_lse=True)
+        R.within(one, out[rows].double().cpu(), 2 * bound[rows], "alone")
+        R.within(l1, lse[rows].double().cpu(), 2 * lb[rows], "alone, lse")
+
+
 def test_long_states_split_and_merged(dev):
     for lq, H, hk, n in ((1, 4, 1, 9001), (2, 2, 2, 5000), (50, 4, 4, 9001)):
         _check(dev, torch.bfloat16, 64, H, hk, [lq], [n], sink=True, seed=n)
