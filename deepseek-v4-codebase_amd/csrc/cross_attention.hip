@@ -8,8 +8,10 @@
 // Rows.  The G heads of a KV head's group share its keys, and so do neighbouring sequences that read the same states (the answers
 // to one input): a run's rows are (query, head), query-major, over all its sequences.  Runs end at multiples of 64 sequences.
 // One pass: running maximum and sum, the output rescaled only where a maximum moved by more than kMargin.  The weights are rounded
-// once to the input's 16 bits for their product with V, the sums of weights and of products are fp32: bf16 has fp32's range; fp16
-// ends at 2^-24, so its weights are held 2^kLift higher, and all down to 2^-21 of the largest are normal numbers.
+// to the input's 16 bits for their product with V, the sums of weights and of products are fp32: bf16 has fp32's range; fp16
+// ends at 2^-24, so its weights are held 2^kLift higher, and all down to 2^-21 of the largest are normal numbers.  With few rows,
+// where the matrix units wait for memory, what the rounding leaves off is multiplied as well, so that a weight is off by 2^-16 (fp16
+// 2^-22) of itself; with many rows, which they bound, that would be half as many products again, and a weight is off by 2^-8 (2^-11).
 #include "attn_tile.h"
 
 namespace aekv {
@@ -358,12 +360,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
     for (int t = 0; t < NT; ++t) take_queries(a, qb[t]);
     const int32_t q0 = cur.at.q0, n_rows = cur.at.n_rows, lk = cur.at.lk, row0 = cur.at.row0, u0 = cur.at.u0, u1 = cur.at.u1;
     float m[NT], l[NT];
-    f32x4_t O[NT][kMB];
+    f32x4_t O[NT][kMB], R[NT][kMB];  // R: by the weights' rests
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kNegInf, l[t] = 0.0f;
 #pragma unroll
-      for (int mb = 0; mb < kMB; ++mb) O[t][mb] = f32x4_t{};
+      for (int mb = 0; mb < kMB; ++mb) O[t][mb] = R[t][mb] = f32x4_t{};
     }
     auto step = [&](int32_t u, auto buf_c) __attribute__((always_inline)) {
       constexpr int buf = decltype(buf_c)::value;
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
       const int32_t at = (u << shift) + 32 * block;
       if (at >= lk || u >= u1) return;
       const uint8_t* vt = buf ? V1[wv] : V0[wv];
-      v8 pb[NT];
+      v8 pb[NT], pr[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         f32x4_t s[2];
@@ -403,7 +405,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
           const float to = top - E::kLift, r = moved ? __builtin_amdgcn_exp2f(m[t] - to) : 1.0f;
           l[t] *= r;
 #pragma unroll
-          for (int mb = 0; mb < kMB; ++mb) O[t][mb] *= r;
+          for (int mb = 0; mb < kMB; ++mb) O[t][mb] *= r, R[t][mb] *= r;
           m[t] = moved ? to : m[t];
         }
         float nm = m[t] == kNegInf ? 0.0f : -m[t], by = a.scale2;
@@ -423,14 +425,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
           p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], by, nm));
           l[t] += p[i];
         }
-        pb[t] = __builtin_bit_cast(v8, make_uint4(E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])));
+        uint32_t w[4], rest[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = E::pack(p[2 * i], p[2 * i + 1]);
+          rest[i] = E::pack(p[2 * i] - E::value(w[i] & 0xFFFFu), p[2 * i + 1] - E::value(w[i] >> 16));
+        }
+        pb[t] = __builtin_bit_cast(v8, make_uint4(w[0], w[1], w[2], w[3])), pr[t] = __builtin_bit_cast(v8, make_uint4(rest[0], rest[1], rest[2], rest[3]));
       }
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb) {
         const i16x4_t x = read_tr16(vt + (tA[0] ^ (mb << 5))), y = read_tr16(vt + (tA[1] ^ (mb << 5)));
         const v8 w = __builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) O[t][mb] = E::mma16(w, pb[t], O[t][mb]);
+        for (int t = 0; t < NT; ++t) O[t][mb] = E::mma16(w, pb[t], O[t][mb]), R[t][mb] = E::mma16(w, pr[t], R[t][mb]);
       }
     };
     int32_t u = u0;
@@ -441,6 +449,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void c
     } while (u < u1);
 
     load_queries(next.at);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int mb = 0; mb < kMB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[t][mb][i] += fabsf(R[t][mb][i]) < __builtin_inff() ? R[t][mb][i] : 0.0f;  // (an infinite value by a rest of 0 or less is none)
     // the waves' states through their own second buffers: row n16's four dims at 16 mb + 4 g, chunks swizzled by the row
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll

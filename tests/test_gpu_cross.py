@@ -203,6 +203,48 @@ def test_a_sequence_alone_and_among_others(dev, dtype, lq):
         R.within(l1, lse[rows].double().cpu(), 2 * lb[rows], "alone, lse")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,hk,dim,lq", [(4, 2, 64, 1), (12, 4, 128, 1), (12, 1, 64, 2), (8, 8, 128, 3)])
+def test_few_rows_weights_keep_their_bits(dev, dtype, H, hk, dim, lq):
+    """Values that nearly cancel: what is left is the difference of the weights.  With few rows a weight is its 16-bit rounding and the
+    rounded rest, off by the square of the half step u (fp16, held 2^7 higher than the largest, by 2^-32 of it at least):
+    |out - ref| <= u |ref| + (u^2 + 2 delta + (n + 16) 2^-24) sum_j p_j |v_j| + n 2^-32 max |v|."""
+    for n in (2, 6, 40, 300):
+        q = (0.2 * torch.randn(3 * lq, H, dim, device=dev, generator=_gen(dev, n))).to(dtype)
+        k = (0.2 * torch.randn(3 * n, hk, dim, device=dev, generator=_gen(dev, n + 1))).to(dtype)
+        v = torch.randn(3 * n // 2, hk, dim, device=dev, generator=_gen(dev, n + 2)).to(dtype)
+        v = torch.stack([v, -v], 1).flatten(0, 1)
+        cq, ck = _cu([lq] * 3), _cu([n] * 3)
+        out = cross_attention(q, k, v, _t(ck, dev), dim ** -0.5, cu_seqlens=_t(cq, dev))
+        want, bound, _, _ = C.cross_attention_ref(q.cpu(), k.cpu(), v.cpu(), cq, ck, None, dim ** -0.5)
+        plain, weighted = torch.zeros_like(bound), torch.zeros_like(bound)
+        u, d = R.U[dtype], dim ** -0.5
+        for b in range(3):
+            for h in range(H):
+                rows, keys = slice(cq[b], cq[b + 1]), slice(ck[b], ck[b + 1])
+                qq, kk, vv = q[rows, h].cpu().double(), k[keys, h // (H // hk)].cpu().double(), v[keys, h // (H // hk)].cpu().double()
+                logit = qq @ kk.T * d
+                delta = (d * (qq.abs() @ kk.abs().T) * (dim + 8) * 2.0 ** -24 + logit.abs() * 2.0 ** -21).amax(1, keepdim=True)
+                weighted[rows, h] = (u * u + 2 * delta + (n + 16) * 2.0 ** -24) * (torch.softmax(logit, 1) @ vv.abs()) + n * 2.0 ** -32 * vv.abs().max()
+                plain[rows, h] = u * want[rows, h].abs()
+        R.within(out, want, plain + weighted + R.TINY[dtype], "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,lq", [(64, 1), (64, 12), (128, 3), (128, 70)])
+def test_infinite_values_that_are_seen(dev, dtype, dim, lq):
+    """An infinite value gives infinities in its dim, a NaN gives NaN, and other dims do not see them."""
+    q = (0.3 * torch.randn(lq, 4, dim, device=dev, generator=_gen(dev, 0))).to(dtype)
+    k, v = (torch.randn(200, 2, dim, device=dev, generator=_gen(dev, i)).to(dtype) for i in (1, 2))
+    args = k, _t([0, 200], dev), dim ** -0.5
+    clean = cross_attention(q, args[0], v, *args[1:], cu_seqlens=_t([0, lq], dev))
+    v[150, 0, 7], v[30, 1, 9], v[199, 1, 11] = math.inf, -math.inf, NAN
+    out = cross_attention(q, args[0], v, *args[1:], cu_seqlens=_t([0, lq], dev))
+    assert (out[:, :2, 7] == math.inf).all() and (out[:, 2:, 9] == -math.inf).all() and out[:, 2:, 11].isnan().all()
+    out[:, :2, 7], out[:, 2:, 9], out[:, 2:, 11] = clean[:, :2, 7], clean[:, 2:, 9], clean[:, 2:, 11]
+    assert torch.equal(out, clean)
+
+
 def test_long_states_split_and_merged(dev):
     for lq, H, hk, n in ((1, 4, 1, 9001), (2, 2, 2, 5000), (50, 4, 4, 9001)):
         _check(dev, torch.bfloat16, 64, H, hk, [lq], [n], sink=True, seed=n)
