@@ -627,10 +627,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3
       for (int v = 0; v < 16; ++v) top = fmaxf(top, S[v]);
       const bool any = __builtin_amdgcn_ballot_w64(fmaf(top, a.scale2, -m) > kMargin + E::kLift) != 0;
       if (any) {
-        // (each row by itself: a row's bits do not depend on the others'; the difference, as m and a constant may round up)
-        top = fmaxf(top, xor_lane<32>(top)) * a.scale2;
-        const bool moved = top - m > kMargin + E::kLift;
-        const float to = top - E::kLift;
+        // (each row by itself, by the measure that brought the wave here: a row's bits do not depend on the others')
+        top = fmaxf(top, xor_lane<32>(top));
+        const bool moved = fmaf(top, a.scale2, -m) > kMargin + E::kLift;
+        const float to = top * a.scale2 - E::kLift;
         r = moved ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
         l *= r;
         m = moved ? to : m;

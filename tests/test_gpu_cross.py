@@ -203,6 +203,27 @@ def test_a_sequence_alone_and_among_others(dev, dtype, lq):
         R.within(l1, lse[rows].double().cpu(), 2 * lb[rows], "alone, lse")
 
 
+def test_a_rows_bits_do_not_depend_on_its_tiles_rows(dev):
+    """A row whose logits rise by the margin up to a rounding (their rounded difference passes it, the exact one, rounded, does not),
+    beside a row that rises far beyond it and beside one that does not: the same bits."""
+    for scale, t0, a, c, e in (("0x1.939af8p+0", 0.55078125, 155, 215, 2), ("0x1.87e506p+0", 1.3828125, 166, 247, 2), ("0x1.92c440p+0", 0.828125, 181, 197, 2), ("0x1.2356bep-1", 1.8515625, 190, 250, 3)):
+        q = torch.zeros(60, 1, 64, device=dev)
+        k = torch.zeros(64, 1, 64, device=dev)
+        v = torch.randn(64, 1, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+        q[:, 0, 2] = 1.0
+        k[:, 0, 2] = -torch.rand(64, device=dev, generator=_gen(dev, 1)) * 3 - 0.1  # the other logits
+        q[5, 0, 0], q[5, 0, 1] = 1.0, a / 128
+        k[3, 0, 0], k[3, 0, 2] = t0, 0.0                       # the first block's largest
+        k[40, 0, 1], k[40, 0, 2] = c / 128 * 2.0 ** (e - 1), 0.0  # the second's: a c 2^(e - 15)
+        outs = []
+        for far in (0.0, 50.0):
+            q[6, 0, 3], k[50, 0, 3] = far, 1.0
+            outs.append(cross_attention(q.bfloat16(), k.bfloat16(), v, _t([0, 64], dev), float.fromhex(scale), cu_seqlens=_t([0, 60], dev), return_lse=True))
+        assert not torch.equal(outs[0][0][6], outs[1][0][6])
+        for x, y in zip(*outs):
+            assert torch.equal(x[5], y[5])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("H,hk,dim,lq", [(4, 2, 64, 1), (12, 4, 128, 1), (12, 1, 64, 2), (8, 8, 128, 3)])
 def test_few_rows_weights_keep_their_bits(dev, dtype, H, hk, dim, lq):
