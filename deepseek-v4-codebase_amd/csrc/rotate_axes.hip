@@ -3,9 +3,9 @@
 // Pair i of R has frequency f_i and axis a_i.  Token n, at position p[a, n] on axis a, turns it by t = p[a_i, n] f_i:
 //   y1 = x1 cos t - x2 sin t,  y2 = x2 cos t + x1 sin t     (inverse: -t)
 // where (x1, x2) are the dims first + 2 i and first + 2 i + 1 (adjacent), or first + i and first + R + i (halves); other dims
-// stay as they are.  The angle is a product of an integer and an fp32 number, taken in fp64 and brought to [-pi, pi] there
-// (in fp32 it would be off by 2^-24 of itself, 0.01 at position 200000), cos and sin in fp32, the turned pair in fp32 with one
-// rounding to x's type.
+// stay as they are.  The angle is a product of an integer and an fp32 number, taken in fp64 (in fp32 it would be off by 2^-24
+// of itself, 0.01 at position 200000), as are its cos and sin, which are rounded to fp32; the turned pair is fp32 with one rounding
+// to x's type.
 //
 // A workgroup takes some tokens with all their heads, so that the heads share a token's cos and sin through LDS; its first
 // loads are under way while those are made.  A thread holds whole pairs: V neighbouring dims (adjacent), or V dims and their
@@ -89,14 +89,21 @@ struct Vec {
   }
 };
 
-// cos and sin of position * f
+// cos and sin of position * f: the angle less whole quarter turns, r, at most pi / 4, and the series of both, in fp64 and rounded
+// once, but for the terms from r^5 / 120 and r^6 / 720 on, at most 2^-8.6, which fp32 gives to 2^-30.  (A whole angle up to pi in
+// fp32 would be off by 2^-23; all terms in fp64 take a third more registers and a prompt's time from 57 to 63 us.)
 __device__ __forceinline__ float2 turn(double p, float f) {
-  constexpr double kTurns = 0.15915494309189535, kHi = 6.283185307179586, kLo = 2.4492935982947064e-16;  // 1 / 2 pi, 2 pi
-  const double a = p * static_cast<double>(f), n = rint(a * kTurns);
-  const float r = static_cast<float>(fma(-n, kLo, fma(-n, kHi, a)));
-  float2 cs;
-  sincosf(r, &cs.y, &cs.x);
-  return cs;
+  constexpr double kQuarters = 0.6366197723675814, kHi = 1.5707963267948966, kLo = 6.123233995736766e-17;  // 2 / pi, pi / 2
+  const double a = p * static_cast<double>(f), n = rint(a * kQuarters);
+  const double r = fma(-n, kLo, fma(-n, kHi, a)), x = r * r;
+  const float y = static_cast<float>(x);
+  const float s5 = fmaf(fmaf(fmaf(-1.0f / 39916800.0f, y, 1.0f / 362880.0f), y, -1.0f / 5040.0f), y, 1.0f / 120.0f) * y;
+  const float c6 = fmaf(fmaf(-1.0f / 3628800.0f, y, 1.0f / 40320.0f), y, -1.0f / 720.0f) * y;
+  const float s = static_cast<float>(fma(r * x, s5 - 1.0 / 6.0, r)), c = static_cast<float>(fma(fma(c6 + 1.0 / 24.0, x, -0.5), x, 1.0));
+  const double quarter = n - 4.0 * rint(0.25 * n);  // -2 .. 2
+  const bool odd = fabs(quarter) == 1.0, half = fabs(quarter) == 2.0;
+  const float cosine = odd ? s : c, sine = odd ? c : s;
+  return make_float2(half || quarter == 1.0 ? -cosine : cosine, half || quarter == -1.0 ? -sine : sine);
 }
 
 template <int DT, int V, bool HALVES>

@@ -387,7 +387,7 @@ int aekv_cross_attention(const void* q, const void* k, const void* v, int32_t dt
  * elements, d even, up to 1024, rows aligned to two elements.  Pair i < pairs of token n turns by
  * positions[axis[i] * pos_axis_stride + n * pos_token_stride] * inv_freq[i] (negative with inverse); it is dims first + 2 i and
  * first + 2 i + 1 (halves 0, first even) or first + i and first + pairs + i (halves 1, pairs even as well).  positions I32 or
- * I64; axis int32 [pairs], each below `axes`.  Angles in fp64, the rest in fp32, rounded once.  Other dims are copied; q_out
+ * I64; axis int32 [pairs], each below `axes`.  Angles in fp64, cosines, sines and the pair in fp32, rounded once.  Other dims are copied; q_out
  * and k_out may be q and k. */
 int aekv_rotate_axes(const void* q, const void* k, int32_t dtype, int64_t n, int32_t H, int32_t heads, int32_t d,
                      int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,

@@ -73,6 +73,28 @@ def test_far_positions(dev, dtype):
     _check(q, None, pos, rotary, axis)
 
 
+@pytest.mark.parametrize("pairs", ["adjacent", "halves"])
+def test_turns_in_fp32_are_off_by_their_roundings_alone(dev, pairs):
+    """Cosine and sine are 64-bit sums rounded to fp32 once, off by 2^-25 at most (they are below 1), but for terms of up to 2^-8.6 that
+    fp32 gives: their square of the angle, three steps of the series, its last product and the series' end are off by 2^-24 of them
+    each, 2^-30 in all.  Of a pair's two products one is rounded, by 2^-24 of itself, and the sum by 2^-24:
+    |y - ref| <= 2^-24 |y| + (|x1| + |x2|) (2^-25 + 2^-30 + 2^-24), and what the 64-bit angle leaves out is below 2^-10 of that.
+    An angle rounded to fp32 is off by up to 2^-23."""
+    axis = _axis(64, 2)
+    rotary = AxisRotary(rope_inv_freq(128, 10000.0, dev), axis, 128, pairs=pairs)
+    pos = torch.randint(-300000, 300000, (2, 3000), device=dev, generator=_gen(dev, 1))
+    q = torch.randn(3000, 2, 128, device=dev, generator=_gen(dev, 0))
+    q[1::3, :, ::2] = 0.0  # one of a pair alone
+    q[2::3, :, :64] = 0.0
+    for inverse in (False, True):
+        out = rotate_axes(q, None, pos, rotary, inverse=inverse)[0]
+        want, _ = C.rotate_ref(q.cpu(), pos.cpu(), rotary.inv_freq.cpu(), axis, 0, pairs == "halves", inverse)
+        x = q.cpu().double().abs()
+        both = x[..., ::2] + x[..., 1::2] if pairs == "adjacent" else x[..., :64] + x[..., 64:]
+        both = both.repeat_interleave(2, -1) if pairs == "adjacent" else torch.cat([both, both], -1)
+        R.within(out, want, (2.0 ** -24 * want.abs() + (1.5 * 2.0 ** -24 + 2.0 ** -30) * both) * (1 + 2.0 ** -10) + 2.0 ** -149, "turned")
+
+
 def test_in_place_views_and_strides(dev):
     axis = _axis(32, 3)
     for pairs in ("adjacent", "halves"):
