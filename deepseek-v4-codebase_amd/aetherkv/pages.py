@@ -64,8 +64,9 @@ class PagePool:
 
     @property
     def lacking(self) -> torch.Tensor:
-        """int32 [1]: pages that reserve could not give since it was last set to 0.  Their entries are -1, and what is written to
-        their slots is lost: look at it (once per step, with the tokens) and end or move a sequence in time."""
+        """int32 [1]: pages that reserve could not give since it was last set to 0.  Their entries are -1: what is written to their
+        slots is lost, and so are the tokens that a row had in a page it shared (the page's other holders keep them).  A later reserve
+        gives such an entry an empty page, not those tokens: the sequence has to end, or be filled again."""
         return self._lacking
 
     def unused(self) -> torch.Tensor:
@@ -93,8 +94,12 @@ class PagePool:
         Each entry of those slots' pages that holds none gets an unused page; one that holds a page which other entries hold too
         gets an unused page with a copy of it (if it has filled slots), unless the call gives pages to all those entries, of which
         the last (by row) keeps it.  Unused pages are taken from the lowest on, in the order of the entries.  first (default:
-        filled): zeros before evict_by_weight, which writes anywhere.  filled, wanted, first int32 [B].  Where the pool is out of
-        pages an entry becomes -1, and `lacking` counts it."""
+        filled): zeros before evict_by_weight, which writes anywhere.  filled, wanted, first int32 [B].
+
+        Where the pool is out of pages an entry becomes -1, `lacking` counts it, and what the entry shared is lost to its row.  That
+        does not happen where unused(), read with the tokens of the step before, is at least the number of entries that the call
+        covers (one per row for a step's token).  A row waits by wanted[b] <= first[b]: it takes no page and keeps what it shares, as
+        long as nothing is appended to it or evicted."""
         B, W = self._table(page_table)
         _one_device(self._index, page_table, filled, wanted, first, workspace)
         filled, wanted = _counts("filled", filled, B), _counts("wanted", wanted, B)

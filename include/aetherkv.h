@@ -407,7 +407,9 @@ size_t aekv_pool_workspace_size(int64_t B, int64_t max_pages, int64_t n_forks, i
 /* Slots first[b] .. wanted[b] - 1 (first NULL: filled) are about to be written: every entry of their pages that holds none
  * gets the lowest unused page, in the entries' order, and one whose page has other holders as well (refs > 1) too, with a copy
  * of the page where it has slots below filled[b]; if a page's holders are all among the call's entries, the last keeps it.
- * Without an unused page an entry becomes -1, and *lacking grows by 1.  marks: int32 [2, pages], zeros before and after. */
+ * Without an unused page an entry becomes -1, and *lacking grows by 1: it lets go of a page that it shared, whose tokens are lost
+ * to its row, and a later call gives it an empty page.  With as many unused pages as the call has entries that does not happen;
+ * a row with wanted[b] <= first[b] has none and keeps what it shares.  marks: int32 [2, pages], zeros before and after. */
 int aekv_pool_reserve(int32_t* table, int64_t B, int64_t max_pages, const int32_t* filled, const int32_t* wanted,
                       const int32_t* first, int32_t page_size, int32_t* refs, int32_t* marks, int32_t* lacking,
                       int64_t pages, const void* segments, int64_t n_segments, void* ws, size_t ws_bytes, void* stream);

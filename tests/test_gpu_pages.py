@@ -138,6 +138,35 @@ def test_more_than_the_pool_has(dev):
     b.compact()
 
 
+def test_what_a_short_pool_loses_and_what_waits(dev):
+    """A row that shares a filled page and gets none loses it, and a later reserve gives an empty page; rows that wait until the unused
+    pages cover the call's entries lose nothing."""
+    shared = [[0, 1, 2]] * 3
+    b = Both(dev, 4, 16, 3, 3)
+    b.reserve([0] * 3, [40, 0, 0])
+    b.fork([40, 0, 0], [0, 0], [1, 2])
+    assert b.rows == shared
+    b.reserve([40] * 3, [41] * 3)  # three entries, one unused page: the last keeps the shared one, the second has none
+    assert b.rows == [[0, 1, 3], [0, 1, -1], [0, 1, 2]] and b.pool.lacking.item() == 1 and b.pool.refs.tolist() == [3, 3, 1, 1]
+    b.release([0, 40, 41])
+    b.reserve([0, 40, 41], [0, 41, 42])
+    assert b.rows == [[-1] * 3, [0, 1, 3], [0, 1, 2]] and not b.model.copies  # (no copy of page 2: its tokens are not there)
+
+    b = Both(dev, 4, 16, 3, 3)
+    b.reserve([0] * 3, [40, 0, 0])
+    b.fork([40, 0, 0], [0, 0], [1, 2])
+    assert int(b.pool.unused()) == 1  # covers one entry: the others wait
+    b.reserve([40] * 3, [41, 40, 40])
+    assert b.rows == [[0, 1, 3], [0, 1, 2], [0, 1, 2]]
+    b.release([0, 40, 40])
+    assert int(b.pool.unused()) == 1
+    b.reserve([0, 40, 40], [0, 41, 40])
+    assert b.rows == [[-1] * 3, [0, 1, 3], [0, 1, 2]] and b.pool.lacking.item() == 0
+    b.release([0, 0, 40])
+    b.reserve([0, 0, 40], [0, 0, 0], first=[0] * 3)  # before an eviction: wanted at or below first waits as well
+    assert b.rows[2] == [0, 1, 2]
+
+
 def test_entries_outside_the_pool_and_odd_counts(dev):
     b = Both(dev, 20, 16, 3, 6)
     b.reserve([0, 0, 0], [50, 20, 96])
