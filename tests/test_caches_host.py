@@ -78,6 +78,13 @@ def test_cross_partial_rows_are_aligned(lib):
                         assert lib.aekv_cross_attention_workspace_size(B, E, nq, nk, H, hk, d) % 16 == 0, (B, E, nq, nk, H, hk, d)
 
 
+def test_cross_strides_that_no_second_row_needs(lib):
+    """One row of keys has no token stride: whatever stands there, the call goes on to its next check."""
+    for st in ((512, 128, 1 << 30, 128, 1 << 30, 128), (512, 128, -256, 128, 256, 128)):
+        assert _cross(lib, nk=2, st=st, ws=None) == L.ERR_UNSUPPORTED
+        assert _cross(lib, nk=1, st=st, ws=None) == L.ERR_WORKSPACE and _cross(lib, nk=0, st=st, ws=None) == L.ERR_WORKSPACE
+
+
 def test_rotate_refusals(lib):
     assert _rotate(lib, dtype=L.I32) == L.ERR_DTYPE and _rotate(lib, pdt=L.F32) == L.ERR_DTYPE
     assert _rotate(lib, n=-1) == L.ERR_SHAPE and _rotate(lib, H=0, hk=0) == L.ERR_SHAPE and _rotate(lib, H=-1) == L.ERR_SHAPE and _rotate(lib, axes=0) == L.ERR_SHAPE

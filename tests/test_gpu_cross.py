@@ -381,6 +381,19 @@ def test_offsets_past_32_bits_and_shared_strides(dev):
         cross_attention(q, wide, wide, _t([0, 3], dev), 0.1, cu_seqlens=cq)
 
 
+@pytest.mark.parametrize("lq", [1, 50])
+def test_one_state_out_of_a_wide_buffer(dev, lq):
+    """One row of keys and values, whose token stride is more than rows may lie apart."""
+    base = torch.randn(1 << 24, device=dev, generator=_gen(dev, 1)).bfloat16()
+    k, v = (base.as_strided((1, 2, 64), (1 << 24, 64, 1), at) for at in (0, 128))
+    q = torch.randn(lq, 4, 64, device=dev, generator=_gen(dev, 0)).bfloat16()
+    out = cross_attention(q, k, v, _t([0, 1], dev), 0.1, cu_seqlens=_t([0, lq], dev))
+    assert torch.equal(out, v.repeat_interleave(2, 1).expand(lq, 4, 64))  # (a weight of 1)
+    v[0, 1, 5] = math.inf
+    out = cross_attention(q, k, v, _t([0, 1], dev), 0.1, cu_seqlens=_t([0, lq], dev))
+    assert torch.equal(out, v.repeat_interleave(2, 1).expand(lq, 4, 64))
+
+
 def test_empty_calls(dev):
     q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=dev)
     k = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)
