@@ -60,6 +60,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
     q, (qt, qh, _) = _rows(q)
     k, (kt, kh, _) = _rows(k)
     v, (vt, vh, _) = _rows(v)
+    if (kt < D or vt < D) and M > 1:  # (rows that overlap: the kernels tell a sequence's end by where its last row ends)
+        k, v = k.contiguous(), v.contiguous()
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
     sk = None if sink is None else _sink_f32(sink, H)
     clear = 0
     if out is None:

@@ -853,7 +853,8 @@ extern "C" int aekv_cross_attention(const void* q, const void* k, const void* v,
     return fail(AEKV_ERR_UNSUPPORTED, "%s: B=%lld E=%lld n_q=%lld n_k=%lld H=%lld exceed the grid", who, (long long)B, (long long)E,
                 (long long)n_q, (long long)n_k, (long long)H);
   if (n_k < 2) k_token_stride = v_token_stride = d;  // (what no second row needs may be anything)
-  if (k_token_stride * 2 * 64 > 0x3fffffff || v_token_stride * 2 * 64 > 0x3fffffff || k_token_stride < 0 || v_token_stride < 0)
+  // (rows that overlap: the range that ends a sequence's last row would let parts of further ones through, by a weight of 0)
+  if (k_token_stride * 2 * 64 > 0x3fffffff || v_token_stride * 2 * 64 > 0x3fffffff || k_token_stride < d || v_token_stride < d)
     return fail(AEKV_ERR_UNSUPPORTED, "%s: token strides of %lld and %lld elements", who, (long long)k_token_stride, (long long)v_token_stride);
   const CrossPlan plan = plan_cross(B, E, n_q, n_k, H, heads, d);
   const size_t want = aekv_cross_attention_workspace_size(B, E, n_q, n_k, H, heads, d);

@@ -371,10 +371,11 @@ int aekv_prompt_attention(const void* q, const void* k, const void* v, int32_t d
                           int32_t clear_rest, void* ws, size_t ws_bytes, void* stream);
 
 /* Attention over all states of an encoder: q [n_q, H, d], k and v [n_k, heads, d] bf16 or fp16 (strides in elements, rows
- * 16-byte aligned), d = 64 or 128.  Sequence b holds queries cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (int32 [B + 1],
- * non-decreasing; NULL: query b, and n_q = B) and sees the keys cu_seqlens_k[e] .. cu_seqlens_k[e + 1] (int32 [E + 1]) of
- * e = states[b] (int32 [B]; NULL: b, and E = B); one outside 0 .. E - 1 has none.  out, lse, sink, clear_rest as in
- * aekv_prompt_attention.  Workspace: aekv_cross_attention_workspace_size bytes, 16-byte aligned; its contents never matter. */
+ * 16-byte aligned, tokens of k and v d elements apart or more), d = 64 or 128.  Sequence b holds queries cu_seqlens_q[b] ..
+ * cu_seqlens_q[b + 1] (int32 [B + 1], non-decreasing; NULL: query b, and n_q = B) and sees the keys cu_seqlens_k[e] ..
+ * cu_seqlens_k[e + 1] (int32 [E + 1]) of e = states[b] (int32 [B]; NULL: b, and E = B); one outside 0 .. E - 1 has none.  out,
+ * lse, sink, clear_rest as in aekv_prompt_attention.  Workspace: aekv_cross_attention_workspace_size bytes, 16-byte aligned; its
+ * contents never matter. */
 size_t aekv_cross_attention_workspace_size(int64_t B, int64_t E, int64_t n_q, int64_t n_k, int64_t H, int64_t heads, int32_t d);
 int aekv_cross_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t q_token_stride,
                          int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,

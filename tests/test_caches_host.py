@@ -78,6 +78,11 @@ def test_cross_partial_rows_are_aligned(lib):
                         assert lib.aekv_cross_attention_workspace_size(B, E, nq, nk, H, hk, d) % 16 == 0, (B, E, nq, nk, H, hk, d)
 
 
+def test_cross_rows_that_overlap_are_refused(lib):
+    for st in ((512, 128, 120, 128, 256, 128), (512, 128, 256, 128, 0, 128)):
+        assert _cross(lib, nk=2, st=st, ws=None) == L.ERR_UNSUPPORTED and "strides" in lib.aekv_last_error().decode()
+
+
 def test_cross_strides_that_no_second_row_needs(lib):
     """One row of keys has no token stride: whatever stands there, the call goes on to its next check."""
     for st in ((512, 128, 1 << 30, 128, 1 << 30, 128), (512, 128, -256, 128, 256, 128)):

@@ -394,6 +394,22 @@ def test_one_state_out_of_a_wide_buffer(dev, lq):
     assert torch.equal(out, v.repeat_interleave(2, 1).expand(lq, 4, 64))
 
 
+@pytest.mark.parametrize("lq", [1, 50])
+def test_rows_that_overlap(dev, lq):
+    """Keys and values whose rows are one and the same, or windows over one line: an infinite value stays in its own rows' dims."""
+    q = torch.randn(lq, 2, 64, device=dev, generator=_gen(dev, 0)).bfloat16() * 0.1
+    for step in (0, 8):
+        for n in (41, 33, 10):
+            line = torch.randn(64 + 8 * 40, device=dev, generator=_gen(dev, 1)).bfloat16()
+            k = (line * 0.1).as_strided((41, 1, 64), (step, 64, 1))
+            line[(n - 1) * step + 60] = math.inf  # dim 60 of the last row that is seen
+            v = line.as_strided((41, 1, 64), (step, 64, 1))
+            cu, cq = _t([0, n], dev), _t([0, lq], dev)
+            out = cross_attention(q, k, v, cu, 0.1, cu_seqlens=cq)
+            assert (out[..., 60] == math.inf).all() and torch.isfinite(out[..., [i for i in range(64) if i != 60]]).all()
+            assert torch.equal(out, cross_attention(q, k.contiguous(), v.contiguous(), cu, 0.1, cu_seqlens=cq))
+
+
 def test_empty_calls(dev):
     q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=dev)
     k = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev)
